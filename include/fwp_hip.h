@@ -420,6 +420,95 @@ int fwp_rec_bwd_static(const float *q_act, const float *k_act, const float *beta
                        float *gbx, float *gRq, float *gRk, float *gRv, float *grb, int N, int H,
                        int L, int D, int chunk, void *stream);
 
+/*
+ * The selective state space block: short causal convolution, selective scan, and the norms around a block.  No counterpart in the
+ * reference.  Rows may be fp32, fp16 or bf16 (`type`); parameters, states, sums and the saved buffers are fp32.
+ */
+enum { FWP_F32 = 0, FWP_F16 = 1, FWP_BF16 = 2 };
+
+/* [N,H,L,D] rows of such a type: element strides of the N, H and L axes, the last axis contiguous. */
+typedef struct fwp_rows {
+    const void *ptr;
+    int64_t sN, sH, sL;
+} fwp_rows;
+typedef struct fwp_out_rows {
+    void *ptr;
+    int64_t sN, sH, sL;
+} fwp_out_rows;
+
+/*
+ * Causal convolution of every channel with a filter of its own:
+ *   p[t] = bias + sum_j weight[j] x[t - K + 1 + j],  y = p, or p sigmoid(p) if `silu`
+ * x, y [N,H,L,D]; weight [H,D,K], bias [H,D] (NULL: 0), 1 <= K <= 8.  state [N,H,K-1,D] of x's type, contiguous, holds the rows
+ * before the first and is overwritten by the last K-1 rows (NULL: zeros, not kept).  lengths [N] (NULL: all are L; taken within
+ * 0 .. L): a sequence's steps from there on are not read, y is zero there, and the state is the one after its last step.
+ */
+typedef struct fwp_conv_args {
+    fwp_rows x;
+    const float *weight, *bias;
+    const int64_t *lengths;
+    int type, silu, N, H, L, D, K;
+} fwp_conv_args;
+int fwp_conv_fwd(const fwp_conv_args *a, void *state, fwp_out_rows y, void *stream);
+
+/* Its adjoint; state: the rows before the first as forward had them (NULL: zeros).  gx [N,H,L,D]; gweight [H,D,K] and gbias
+ * [H,D] together or NULL.  workspace: fwp_conv_workspace floats. */
+long long fwp_conv_workspace(int N, int H, int L, int D, int K);
+int fwp_conv_bwd(const fwp_conv_args *a, const void *state, fwp_rows grad_y, fwp_out_rows gx, float *gweight, float *gbias,
+                 float *workspace, void *stream);
+
+/*
+ * Selective scan: the sum rule with a decay, per step
+ *   dt = delta, or softplus(delta + delta_bias) if `softplus` (without it delta + delta_bias)
+ *   W[e][m] = exp(dt[m] A[e][m]) W[e][m] + dt[m] k[e] v[m]
+ *   o[m] = sum_e q[e] W[e][m] + D[m] v[m],  out = o, or o z sigmoid(z) where z is given
+ * q, k [N,H,L,E], E <= 64; v, delta, z, out [N,H,L,M]; A [H,E,M]; D, delta_bias [H,M] (NULL: 0); W [N,H,E,M] fp32 in/out (NULL:
+ * from zeros, not kept).  A should not be positive.  lengths as above.
+ * saved: NULL, or fwp_scan_saved_floats for a backward pass; workspace: fwp_scan_workspace(.., 0) floats.
+ */
+typedef struct fwp_scan_args {
+    fwp_rows q, k, v, delta, z; /* z.ptr NULL: no gate */
+    const float *A, *D, *delta_bias;
+    const int64_t *lengths;
+    int type, softplus, N, H, L, E, M;
+} fwp_scan_args;
+long long fwp_scan_saved_floats(int N, int H, int L, int E, int M);
+long long fwp_scan_workspace(int N, int H, int L, int E, int M, int backward);
+int fwp_scan_fwd(const fwp_scan_args *a, float *W, fwp_out_rows out, float *saved, float *workspace, void *stream);
+
+/* Its adjoint.  gq, gk [N,H,L,E]; gv, gdelta, gz [N,H,L,M] (gz with z only); gA [H,E,M]; gD, gdelta_bias [H,M].  q and k are
+ * not read.  workspace: fwp_scan_workspace(.., 1) floats. */
+int fwp_scan_bwd(const fwp_scan_args *a, const float *saved, fwp_rows grad_out, fwp_out_rows gq, fwp_out_rows gk, fwp_out_rows gv,
+                 fwp_out_rows gdelta, fwp_out_rows gz, float *gA, float *gD, float *gdelta_bias, float *workspace, void *stream);
+
+/*
+ * The norms around a block with its gate, scale and residual addition, over contiguous rows of `cols` <= 8192 elements:
+ *   u = norm(y) with after_weight and after_bias, or y where after_weight is NULL
+ *   r = x + scale act(gate) u          (scale [cols] NULL: 1; gate NULL: 1)
+ *   n = norm(r) with before_weight and before_bias (NULL before_weight: no n)
+ * norm: LayerNorm, or with `rms` x / sqrt(mean(x^2) + eps).  Biases may be NULL.  gate: [rows,cols], or [rows] if gate_rows; act is the
+ * sigmoid, FWP_ACT_SILU: gate sigmoid(gate), FWP_ACT_NONE: the gate itself.  y, gate and n are of `type`, x and r of `stream_type`
+ * (`type` or FWP_F32).  stats [rows,4]: saved for the adjoint, or NULL.
+ */
+enum { FWP_ACT_NONE = 0, FWP_ACT_SIGMOID = 1, FWP_ACT_SILU = 2 };
+typedef struct fwp_norm_args {
+    const void *y, *x, *gate;
+    const float *scale, *after_weight, *after_bias, *before_weight, *before_bias;
+    float eps;
+    int type, stream_type, rms, act, gate_rows, rows, cols;
+} fwp_norm_args;
+int fwp_residual_norm_fwd(const fwp_norm_args *a, void *r, void *n, float *stats, void *stream);
+
+/* Its adjoint: grad_r of `stream_type` and grad_n of `type` (NULL: zero), to gy, gx and ggate (like y, x, gate; ggate may be NULL),
+ * and to the parameters' gradients [cols] where those are not NULL.  workspace: fwp_residual_norm_workspace floats. */
+typedef struct fwp_norm_grads {
+    void *gy, *gx, *ggate;
+    float *gscale, *gafter_weight, *gafter_bias, *gbefore_weight, *gbefore_bias;
+} fwp_norm_grads;
+long long fwp_residual_norm_workspace(int rows, int cols);
+int fwp_residual_norm_bwd(const fwp_norm_args *a, const float *stats, const void *grad_r, const void *grad_n, const fwp_norm_grads *g,
+                          float *workspace, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -32,6 +32,30 @@ class Epilogue(ctypes.Structure):
                 ("colsum", ctypes.c_void_p), ("relu", ctypes.c_int)]
 
 
+class ConvArgs(ctypes.Structure):
+    """struct fwp_conv_args (rows and output rows have View's layout)."""
+    _fields_ = [("x", View), ("weight", ctypes.c_void_p), ("bias", ctypes.c_void_p), ("lengths", ctypes.c_void_p)] + \
+               [(n, ctypes.c_int) for n in ("type", "silu", "N", "H", "L", "D", "K")]
+
+
+class ScanArgs(ctypes.Structure):
+    """struct fwp_scan_args."""
+    _fields_ = [(n, View) for n in ("q", "k", "v", "delta", "z")] + \
+               [(n, ctypes.c_void_p) for n in ("A", "D", "delta_bias", "lengths")] + \
+               [(n, ctypes.c_int) for n in ("type", "softplus", "N", "H", "L", "E", "M")]
+
+
+class NormArgs(ctypes.Structure):
+    """struct fwp_norm_args."""
+    _fields_ = [(n, ctypes.c_void_p) for n in ("y", "x", "gate", "scale", "after_weight", "after_bias", "before_weight", "before_bias")] + \
+               [("eps", ctypes.c_float)] + [(n, ctypes.c_int) for n in ("type", "stream_type", "rms", "act", "gate_rows", "rows", "cols")]
+
+
+class NormGrads(ctypes.Structure):
+    """struct fwp_norm_grads."""
+    _fields_ = [(n, ctypes.c_void_p) for n in ("gy", "gx", "ggate", "gscale", "gafter_weight", "gafter_bias", "gbefore_weight", "gbefore_bias")]
+
+
 class FwpError(RuntimeError):
     pass
 
@@ -70,8 +94,15 @@ _MODEL_SIGNATURES = {
     "fwp_rows_matmul": [_P] * 3 + [ctypes.c_float] + [_P] * 4 + [_I, _P] + [_I] * 3 + [_P],
     "fwp_deltanet_step": [_P] * 4 + [_I] * 3 + [ctypes.c_float, _P],
     "fwp_embed": [_P] * 4 + [_I] * 3 + [_L, ctypes.c_float, ctypes.c_float, _P],
+    # the selective state space block (argument structures go by address)
+    "fwp_conv_fwd": [ctypes.POINTER(ConvArgs), _P, OutView, _P],
+    "fwp_conv_bwd": [ctypes.POINTER(ConvArgs), _P, _V, OutView] + [_P] * 4,
+    "fwp_scan_fwd": [ctypes.POINTER(ScanArgs), _P, OutView] + [_P] * 3,
+    "fwp_scan_bwd": [ctypes.POINTER(ScanArgs), _P, _V] + [OutView] * 5 + [_P] * 5,
+    "fwp_residual_norm_fwd": [ctypes.POINTER(NormArgs)] + [_P] * 4,
+    "fwp_residual_norm_bwd": [ctypes.POINTER(NormArgs)] + [_P] * 3 + [ctypes.POINTER(NormGrads)] + [_P] * 2,
 }
-_WORKSPACES = {"fwp_product_workspace": 3, "fwp_matmul_workspace": 3, "fwp_nll_workspace": 2, "fwp_layer_norm_workspace": 2}
+_WORKSPACES = {"fwp_conv_workspace": 5, "fwp_scan_saved_floats": 5, "fwp_scan_workspace": 6, "fwp_residual_norm_workspace": 2, "fwp_product_workspace": 3, "fwp_matmul_workspace": 3, "fwp_nll_workspace": 2, "fwp_layer_norm_workspace": 2}
 EXPORTS = sorted(list(_SIGNATURES) + list(_MODEL_SIGNATURES) + list(_WORKSPACES) + ["fwp_strerror", "fwp_query", "fwp_check_device", "fwp_config",
                                        "fwp_delta_ckpt_floats", "fwp_delta_segment_floats", "fwp_delta_bwd_segment_floats", "fwp_delta_kind", "fwp_delta_fwd_kind"])
 KIND_LDS, KIND_SCAN, KIND_CHUNKED, KIND_SPLIT, KIND_PHASE, KIND_STEP = 0, 1, 2, 3, 4, 5

@@ -679,6 +679,9 @@ void set_error_class(py::object cls) {
 }  // namespace
 
 void bind_blocks(py::module_ &m);       // fwp_torch_blocks.cpp
+#ifndef FWP_HOST_STUB
+void bind_scan(py::module_ &m);         // fwp_torch_scan.cpp
+#endif
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     py::register_exception_translator([](std::exception_ptr p) {
@@ -704,5 +707,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
           "rnn_out, cell_out = fast_lstm_v4(Zi, Ki, Vi, bi, Wi, Zu, Ku, Vu, bu, Wu, Zo, Ko, Vo, bo, Wo, h0, c0): "
           "Delta LSTM; the W, h0 and c0 are updated in place");
     bind_blocks(m);
+#ifndef FWP_HOST_STUB
+    bind_scan(m);
+#endif
     m.def("set_error_class", &set_error_class, "exception class raised for rejected calls");
 }
