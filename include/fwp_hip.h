@@ -463,7 +463,7 @@ int fwp_conv_bwd(const fwp_conv_args *a, const void *state, fwp_rows grad_y, fwp
  *   W[e][m] = exp(dt[m] A[e][m]) W[e][m] + dt[m] k[e] v[m]
  *   o[m] = sum_e q[e] W[e][m] + D[m] v[m],  out = o, or o z sigmoid(z) where z is given
  * q, k [N,H,L,E], E <= 64; v, delta, z, out [N,H,L,M]; A [H,E,M]; D, delta_bias [H,M] (NULL: 0); W [N,H,E,M] fp32 in/out (NULL:
- * from zeros, not kept).  A should not be positive.  lengths as above.
+ * from zeros, not kept).  A should not be positive.  lengths as above.  Steps of a view lie at most 2^25 elements apart.
  * saved: NULL, or fwp_scan_saved_floats for a backward pass; workspace: fwp_scan_workspace(.., 0) floats.
  */
 typedef struct fwp_scan_args {
@@ -476,8 +476,8 @@ long long fwp_scan_saved_floats(int N, int H, int L, int E, int M);
 long long fwp_scan_workspace(int N, int H, int L, int E, int M, int backward);
 int fwp_scan_fwd(const fwp_scan_args *a, float *W, fwp_out_rows out, float *saved, float *workspace, void *stream);
 
-/* Its adjoint.  gq, gk [N,H,L,E]; gv, gdelta, gz [N,H,L,M] (gz with z only); gA [H,E,M]; gD, gdelta_bias [H,M].  q and k are
- * not read.  workspace: fwp_scan_workspace(.., 1) floats. */
+/* Its adjoint.  gq, gk [N,H,L,E]; gv, gdelta, gz [N,H,L,M] (gz with z only); gA [H,E,M]; gD, gdelta_bias [H,M].
+ * workspace: fwp_scan_workspace(.., 1) floats. */
 int fwp_scan_bwd(const fwp_scan_args *a, const float *saved, fwp_rows grad_out, fwp_out_rows gq, fwp_out_rows gk, fwp_out_rows gv,
                  fwp_out_rows gdelta, fwp_out_rows gz, float *gA, float *gD, float *gdelta_bias, float *workspace, void *stream);
 

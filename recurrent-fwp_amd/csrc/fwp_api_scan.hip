@@ -21,6 +21,8 @@ int conv_check(const fwp_conv_args *a) {
     return rows_ok(a->x, a->type) ? 0 : FWP_E_NULL;
 }
 
+bool step_ok(int64_t sL) { return sL >= 0 && sL <= kScanMaxStep; }
+
 int scan_dims(int N, int H, int L, int E, int M) {
     return dims_ok(N, H, L) && E >= 1 && E <= kMaxKeys && M >= 1 && M <= kMaxChannels ? 0 : FWP_E_SHAPE;
 }
@@ -69,6 +71,8 @@ int fwp_scan_fwd(const fwp_scan_args *a, float *W, fwp_out_rows out, float *save
     for (const fwp_rows *v : {&a->q, &a->k, &a->v, &a->delta})
         if (!rows_ok(*v, a->type)) return FWP_E_NULL;
     if (!element_aligned(a->z.ptr, a->type) || !rows_ok(out, a->type) || !workspace) return FWP_E_NULL;
+    for (const int64_t sL : {a->q.sL, a->k.sL, a->v.sL, a->delta.sL, a->z.ptr ? a->z.sL : 0, out.sL})
+        if (!step_ok(sL)) return FWP_E_SHAPE;
     return scan_fwd(*a, W, out, saved, workspace, (hipStream_t)stream);
 }
 
@@ -76,11 +80,13 @@ int fwp_scan_bwd(const fwp_scan_args *a, const float *saved, fwp_rows grad_out, 
                  fwp_out_rows gdelta, fwp_out_rows gz, float *gA, float *gD, float *gdelta_bias, float *workspace, void *stream) {
     if (!a || !a->A || !saved || !gA || !gD || !gdelta_bias || !workspace) return FWP_E_NULL;
     if (!type_ok(a->type) || scan_dims(a->N, a->H, a->L, a->E, a->M)) return FWP_E_SHAPE;
-    for (const fwp_rows *v : {&a->v, &a->delta, (const fwp_rows *)&grad_out})
+    for (const fwp_rows *v : {&a->q, &a->k, &a->v, &a->delta, (const fwp_rows *)&grad_out})
         if (!rows_ok(*v, a->type)) return FWP_E_NULL;
     for (const fwp_out_rows *v : {&gq, &gk, &gv, &gdelta})
         if (!rows_ok(*v, a->type)) return FWP_E_NULL;
     if (a->z.ptr && (!element_aligned(a->z.ptr, a->type) || !rows_ok(gz, a->type))) return FWP_E_NULL;
+    for (const int64_t sL : {a->q.sL, a->k.sL, a->v.sL, a->delta.sL, grad_out.sL, gq.sL, gk.sL, gv.sL, gdelta.sL, a->z.ptr ? a->z.sL : 0, a->z.ptr ? gz.sL : 0})
+        if (!step_ok(sL)) return FWP_E_SHAPE;
     return scan_bwd(*a, saved, grad_out, gq, gk, gv, gdelta, gz, gA, gD, gdelta_bias, workspace, (hipStream_t)stream);
 }
 

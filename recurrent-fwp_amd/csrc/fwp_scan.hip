@@ -6,11 +6,10 @@
 //   g = dy q + c,  c (of the state before the step) = a g,  a = exp(dt A),  w = a W_before g
 //   gq = sum_m dy W    gk = sum_m g dt v    gv = dt sum_e g k + D dy    gdt = v sum_e g k + sum_e A w    gA = sum dt w    gD = sum dy v
 //
-// A workgroup takes 64 channels of one sequence and head: a lane is a channel, a wave four entries of the state (key rows), so
-// that k and q of a step are scalars for the wave (packed as fp32 beforehand, read through the scalar cache), a state and its
-// history stay in registers, and a sum over the channels is a sum over the lanes.  Steps go in tiles of kTile rows: each thread loads its
-// rows of v, delta, z once, works out dt and dt v, and puts them into LDS for all waves; the waves' parts of a sum over e meet in LDS
-// and the thread that loaded a row finishes it.
+// A workgroup takes 64 channels of one sequence and head: a lane is a channel, a wave four entries of the state (key rows), so that a
+// state and its history stay in registers, and a sum over the channels is a sum over the lanes.  Steps go in tiles of kTile rows: each thread
+// loads its rows of v, delta, z once, works out dt and dt v, and puts them into LDS for all waves, as k and q are; the waves' parts of a sum
+// over e meet in LDS and the thread that loaded a row finishes it.  The next tile's rows are on their way meanwhile.
 //
 // Few sequences and channels leave most of the chip idle, so a long sequence is cut into segments that run at the same time:
 // a first pass gives each segment's state from zeros and its sum of dt, a small kernel turns these into the state that each segment
@@ -26,72 +25,64 @@ namespace {
 
 constexpr int kRowMirror8 = 0x141;      // lane i of 8 gets lane 7 - i
 
-// For 1, 2, 4, 8 or 16 waves of four state rows each.  The widest states have half the tile: 16 waves leave 128 registers to a lane.
+// Waves of a workgroup and state rows of a wave (S).  Two rows a wave need half the registers of four, so that twice the waves are there to fill one another's
+// gaps: 32 x 1024 steps of 512 channels, 16 rows, forward + backward 125 + 344 us against 158 + 526 us with four.  At 32 rows sixteen waves of two
+// would not fit the LDS.  Fewer than four waves would load a tile's rows too slowly.
+int rows_of(int E) { return E <= 16 ? 2 : 4; }
+int waves_of(int E) { return E <= 8 ? 4 : E <= 32 ? 8 : 16; }
+// Steps of a tile, and from one saved state to the next.  Sixteen waves leave 128 registers to a lane, which must hold the history of a tile.
 constexpr int tile_of(int waves) { return waves == 16 ? 8 : 16; }
-int waves_of(int E) { return E <= 4 ? 1 : E <= 8 ? 2 : E <= 16 ? 4 : E <= 32 ? 8 : 16; }
-
-using scalar_float = const float __attribute__((address_space(4)));
 
 struct Dims {
     int N, H, L, E, M;
     int blocks_m;       // 64 channels each
     int segments, steps;      // per sequence, and steps of a segment (a multiple of the tile)
-    int padded;         // L rounded up to whole tiles: rows of the packed k and q
-    int tiles;
+    int tiles, padded;  // whole tiles of a sequence, and their steps
 };
 
 struct Plan : Dims {
-    int waves, tile;
-    int64_t heads, packed, states;      // N H; floats of packed k and q; floats of one set of states
+    int waves, rows, tile;
+    int64_t heads, states;      // N H; floats of one set of states
     Plan(int N_, int H_, int L_, int E_, int M_, bool backward) {
         N = N_, H = H_, L = L_, E = E_, M = M_;
-        waves = waves_of(E), tile = tile_of(waves);
+        rows = rows_of(E), waves = waves_of(E), tile = tile_of(waves);
         blocks_m = (M + 63) / 64;
         tiles = (L + tile - 1) / tile;
         padded = tiles * tile;
         heads = (int64_t)N * H;
-        packed = heads * waves * padded * 8;
         states = heads * E * M;
+        // Segments: with w of them the CUs have ceil(blocks w / 256) workgroups each, of 1 / w of the steps, and the pass before adds 0.7 (forward) and
+        // 0.2 (backward) of the work.  Workgroups that share a CU fill one another's gaps in the forward pass, where three fit: two take
+        // 1.36 times as long as one.  Measured, 256 workgroups cut into 1, 2, 4: 231, 282, 261 us and 587, 718, 718 us; 16 into
+        // 8, 16, 32, 64: 186, 116, 84, 85 us forward.  A segment has eight tiles at least, or the two launches more cost what it saves.
         const int64_t blocks = heads * blocks_m;
-        int64_t want = blocks >= 256 ? 1 : (512 + blocks - 1) / blocks;
-        want = std::max<int64_t>(1, std::min<int64_t>(want, tiles / 4));
-        const int per = (int)((tiles + want - 1) / want);      // tiles to a segment
-        segments = (tiles + per - 1) / per;
-        steps = per * tile;
-        (void)backward;
+        double best = 0;
+        segments = 1, steps = padded;
+        for (int w = 1; w <= 64 && (w == 1 || w <= tiles / 8); w++) {
+            const double turns = (double)((blocks * w + 255) / 256);
+            const double cost = (backward ? turns : turns > 1 ? 0.68 * turns : 1) / w * (w == 1 ? 1 : backward ? 1.2 : 1.7);
+            if (w > 1 && cost >= best) continue;
+            best = cost;
+            const int per = (tiles + w - 1) / w;
+            segments = (tiles + per - 1) / per, steps = per * tile;
+        }
     }
     int64_t grid() const { return heads * blocks_m * segments; }
     int64_t seg_states() const { return segments > 1 ? states * segments + heads * segments * M : 0; }      // the states and the sums of dt
 };
 
-// ------------------------------------------------------------------ k and q, packed
-
-// kq [heads][waves][padded][k0..k3 | q0..q3], zero where there is no such row, step or entry (so that whatever a padded row holds stays out)
-template <typename T>
-__global__ __launch_bounds__(256) void k_pack(fwp_rows q, fwp_rows k, const int64_t *__restrict__ lengths, float *__restrict__ kq,
-                                              int H, int L, int E, int padded, int chunks) {
-    const int64_t nh = blockIdx.x / chunks;
-    const int i = (blockIdx.x % chunks) * 256 + threadIdx.x, t = i / 8, j = i % 8, w = blockIdx.y, e = 4 * w + j % 4;
-    if (t >= padded) return;
-    const int n = (int)(nh / H), h = (int)(nh % H);
-    float x = 0.f;
-    if (e < E && t < length_of(lengths, n, L)) x = load(row<T>(j < 4 ? k : q, n, h, t) + e);
-    kq[(nh * gridDim.y + w) * padded * 8 + i] = x;
-}
-
 // ------------------------------------------------------------------ what the passes share
 
 struct Place {
-    int n, h, m, seg, wave, lane;
-    int64_t nh;
+    int n, h, m, mb, seg, wave, lane, nh;
     bool live;      // a channel that exists
     __device__ __forceinline__ Place(const Dims &d) {
-        int64_t b = blockIdx.x;
-        const int mb = (int)(b % d.blocks_m);
+        unsigned b = blockIdx.x;        // 32-bit divisions: those of 64 bits take a microsecond
+        mb = b % d.blocks_m;
         b /= d.blocks_m;
-        seg = (int)(b % d.segments);
+        seg = b % d.segments;
         nh = b / d.segments;
-        n = (int)(nh / d.H), h = (int)(nh % d.H);
+        n = nh / d.H, h = nh % d.H;
         wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x % 64;
         m = mb * 64 + lane;
         live = m < d.M;
@@ -101,27 +92,83 @@ struct Place {
 };
 
 // A log2(e) of the wave's four rows
-__device__ __forceinline__ void load_decays(float (&a)[4], const float *A, const Dims &d, const Place &p) {
+template <int S>
+__device__ __forceinline__ void load_decays(float (&a)[S], const float *A, const Dims &d, const Place &p) {
 #pragma unroll
-    for (int s = 0; s < 4; s++) {
-        const int e = 4 * p.wave + s;
+    for (int s = 0; s < S; s++) {
+        const int e = S * p.wave + s;
         a[s] = p.live && e < d.E ? A[p.state(d, p.h, e)] * kLog2e : 0.f;
     }
 }
-__device__ __forceinline__ void load_states(float (&x)[4], const float *from, int64_t at, const Dims &d, const Place &p) {
+template <int S>
+__device__ __forceinline__ void load_states(float (&x)[S], const float *from, int64_t at, const Dims &d, const Place &p) {
 #pragma unroll
-    for (int s = 0; s < 4; s++) {
-        const int e = 4 * p.wave + s;
+    for (int s = 0; s < S; s++) {
+        const int e = S * p.wave + s;
         x[s] = from && p.live && e < d.E ? from[p.state(d, at, e)] : 0.f;
     }
 }
-__device__ __forceinline__ void store_states(const float (&x)[4], float *to, int64_t at, const Dims &d, const Place &p) {
+template <int S>
+__device__ __forceinline__ void store_states(const float (&x)[S], float *to, int64_t at, const Dims &d, const Place &p) {
 #pragma unroll
-    for (int s = 0; s < 4; s++) {
-        const int e = 4 * p.wave + s;
+    for (int s = 0; s < S; s++) {
+        const int e = S * p.wave + s;
         if (p.live && e < d.E) to[p.state(d, at, e)] = x[s];
     }
 }
+
+// The rows of a tile in an [N,H,L,M] view, by the channel of the lane.  Addresses are a 64-bit base, the same for all lanes, that goes from tile to
+// tile, and 32-bit offsets in the tile (steps of up to kMaxStep elements).  Every lane loads: channels that do not exist read the last one, rows
+// behind the sequence its last row, and what they read is not used.  So no load waits behind a branch, and those of the next tile are on
+// their way while this one is worked on.
+template <typename T>
+struct Column {
+    char *base;
+    unsigned step, col;     // in bytes
+    template <typename V>
+    __device__ __forceinline__ Column(const V &v, const Place &at, const Dims &d, int t0)
+        : base((char *)v.ptr + (at.n * v.sN + at.h * v.sH + t0 * v.sL) * (int64_t)sizeof(T)), step((unsigned)v.sL * sizeof(T)),
+          col(min(at.m, d.M - 1) * (unsigned)sizeof(T)) {}
+    __device__ __forceinline__ T &operator[](int r) const { return *(T *)(base + (r * step + col)); }
+    __device__ __forceinline__ void go(int rows) { base += (int64_t)rows * step; }
+    // rows wave, wave + waves, .. as far as the last one that there is
+    template <typename U, int ROWS>
+    __device__ __forceinline__ void load(U (&to)[ROWS], int most, int wave, int waves) const {
+#pragma unroll
+        for (int j = 0; j < ROWS; j++) to[j] = (*this)[min(wave + waves * j, most)];
+    }
+};
+
+// A tile of k and q in LDS, [TILE][WAVES][S of k | S of q], or (PARTS 1) one of them, loaded the same way; zero where there is no
+// such entry or step (so that whatever a padded row holds stays out).
+template <typename T, int WAVES, int S, int TILE, int PARTS>
+struct Keys {
+    static constexpr int WIDTH = S * PARTS, ROW = WAVES * WIDTH, EACH = TILE * WIDTH > 64 ? TILE * WIDTH / 64 : 1, APART = 64 / WIDTH;
+    const char *p;
+    unsigned step;
+    int row, at;
+    bool in;
+    __device__ __forceinline__ Keys(const fwp_rows &k, const fwp_rows &q, const Place &w, const Dims &d, int t0) {
+        at = threadIdx.x % ROW, row = threadIdx.x / ROW;
+        const int e = at / WIDTH * S + at % S;
+        const bool is_k = at % WIDTH < S;
+        in = e < d.E;
+        const int64_t sL = is_k ? k.sL : q.sL;
+        p = (is_k ? (const char *)k.ptr + (w.n * k.sN + w.h * k.sH) * (int64_t)sizeof(T) : (const char *)q.ptr + (w.n * q.sN + w.h * q.sH) * (int64_t)sizeof(T)) +
+            (t0 * sL + min(e, d.E - 1)) * (int64_t)sizeof(T);
+        step = (unsigned)sL * sizeof(T);
+    }
+    __device__ __forceinline__ void go(int rows) { p += (int64_t)rows * step; }
+    __device__ __forceinline__ void load(T (&to)[EACH], int most) const {
+#pragma unroll
+        for (int j = 0; j < EACH; j++) to[j] = *(const T *)(p + min(row + APART * j, most) * step);
+    }
+    __device__ __forceinline__ void put(float (*to)[ROW], const T (&from)[EACH], int steps) const {
+#pragma unroll
+        for (int j = 0; j < EACH; j++)
+            if (row + APART * j < TILE) to[row + APART * j][at] = in && row + APART * j < steps ? (float)from[j] : 0.f;
+    }
+};
 
 // The parameters of a channel that the threads which load its rows need
 struct Channel {
@@ -136,79 +183,90 @@ struct Channel {
 // ------------------------------------------------------------------ forward
 
 // LOCAL: only the state after the segment, from zeros, and the segment's sum of dt; otherwise the scan
-template <typename T, int WAVES, bool LOCAL>
-__global__ __launch_bounds__(64 * WAVES) void k_scan_fwd(fwp_scan_args a, Dims d, const float *__restrict__ kq, const float *init, float *W,
-                                                         float *__restrict__ saved, float *__restrict__ sums, fwp_out_rows out) {
-    constexpr int TILE = tile_of(WAVES), ROWS = (TILE + WAVES - 1) / WAVES;
+template <typename T, int WAVES, int S, bool LOCAL>
+__global__ __launch_bounds__(64 * WAVES) void k_scan_fwd(fwp_scan_args a, Dims d, const float *init, float *W, float *__restrict__ saved,
+                                                         float *__restrict__ sums, fwp_out_rows out) {
+    constexpr int TILE = 16, ROWS = (TILE + WAVES - 1) / WAVES, KEEP = tile_of(WAVES);
+    using K = Keys<T, WAVES, S, TILE, LOCAL ? 1 : 2>;
+    __shared__ alignas(16) float kq[TILE][K::ROW];
     __shared__ float2 sx[TILE][64];                          // dt, dt v
     __shared__ float sy[LOCAL ? 1 : WAVES][TILE][64];        // the waves' parts of sum_e q W
     const Place p(d);
     const Channel ch(a, p);
-    const int len = length_of(a.lengths, p.n, d.L), first = p.seg * d.steps, end = min(first + d.steps, d.L);
-    float decay[4], state[4];
+    const int len = length_of(a.lengths, p.n, d.L), first = p.seg * d.steps, end = min(first + d.steps, d.L), last = min(end, len);
+    const bool gated = !LOCAL && a.z.ptr;
+    Column<const T> V(a.v, p, d, first), DT(a.delta, p, d, first), Z(gated ? a.z : a.v, p, d, first);
+    Column<T> O(LOCAL ? fwp_out_rows{(void *)a.v.ptr, 0, 0, 0} : out, p, d, first);
+    K keys(a.k, a.q, p, d, first);
+    float decay[S], state[S], sum = 0.f;
     load_decays(decay, a.A, d, p);
-    load_states(state, LOCAL ? nullptr : init, p.nh * d.segments + p.seg, d, p);
-    float sum = 0.f;
-    for (int t0 = first; t0 < end; t0 += TILE) {
-        if (t0 >= len) {        // behind the sequence
-            if constexpr (!LOCAL)
-#pragma unroll
-                for (int j = 0; j < ROWS; j++) {
-                    const int t = t0 + p.wave + WAVES * j;
-                    if (p.wave + WAVES * j < TILE && t < end && p.live) store(row<T>(out, p.n, p.h, t) + p.m, 0.f);
-                }
-            continue;
-        }
-        if constexpr (!LOCAL)
-            if (saved) store_states(state, saved, p.nh * d.tiles + t0 / TILE, d, p);
-        float v[ROWS];
+    load_states(state, LOCAL ? nullptr : init, (int64_t)p.nh * d.segments + p.seg, d, p);
+    T v[ROWS], dt[ROWS], z[ROWS], key[K::EACH];
+    // the rows of the tile that the columns are at, which starts at step t0
+    const auto fetch = [&](int t0) {
+        const int most = min(last - 1 - t0, TILE - 1);
+        V.load(v, most, p.wave, WAVES);
+        DT.load(dt, most, p.wave, WAVES);
+        if (gated) Z.load(z, most, p.wave, WAVES);
+        keys.load(key, most);
+        V.go(TILE), DT.go(TILE), Z.go(TILE), keys.go(TILE);
+    };
+    if (first < last) fetch(first);
+    for (int t0 = first; t0 < last; t0 += TILE) {
+        float dv[ROWS], gate[ROWS];       // D v and the gate of this thread's rows
 #pragma unroll
         for (int j = 0; j < ROWS; j++) {
-            const int r = p.wave + WAVES * j, t = t0 + r;
-            float dt = 0.f;
-            v[j] = 0.f;
-            if (r < TILE && t < len && p.live) {
-                v[j] = load(row<T>(a.v, p.n, p.h, t) + p.m);
-                dt = load(row<T>(a.delta, p.n, p.h, t) + p.m) + ch.bias;
-                if (a.softplus) dt = softplus(dt);
-            }
-            if (r < TILE) sx[r][p.lane] = make_float2(dt, dt * v[j]);
+            const int r = p.wave + WAVES * j;
+            const bool in = t0 + r < last && p.live;
+            float x = (float)dt[j] + ch.bias;
+            if (a.softplus) x = softplus(x);
+            x = in ? x : 0.f;
+            const float vs = in ? (float)v[j] : 0.f;
+            dv[j] = ch.D * vs;
+            gate[j] = gated ? silu((float)z[j], sigmoid((float)z[j])) : 1.f;
+            if (r < TILE) sx[r][p.lane] = make_float2(x, x * vs);
         }
+        keys.put(kq, key, last - t0);
         __syncthreads();
-        scalar_float *const ks = (scalar_float *)(kq + ((p.nh * WAVES + p.wave) * d.padded + t0) * 8);
+        if (t0 + TILE < last) fetch(t0 + TILE);
 #pragma unroll
         for (int r = 0; r < TILE; r++) {
+            if constexpr (!LOCAL)
+                if (r % KEEP == 0)
+                    if (saved && t0 + r < last) store_states(state, saved, (int64_t)p.nh * d.tiles + (t0 + r) / KEEP, d, p);
             const float2 x = sx[r][p.lane];
+            const float *const k = kq[r] + K::WIDTH * p.wave, *const q = k + S;
             float y = 0.f;
 #pragma unroll
-            for (int s = 0; s < 4; s++) {
-                state[s] = fmaf(__builtin_amdgcn_exp2f(x.x * decay[s]), state[s], x.y * ks[8 * r + s]);
-                if constexpr (!LOCAL) y = fmaf(ks[8 * r + 4 + s], state[s], y);
+            for (int s = 0; s < S; s++) {
+                state[s] = fmaf(__builtin_amdgcn_exp2f(x.x * decay[s]), state[s], x.y * k[s]);
+                if constexpr (!LOCAL) y = fmaf(q[s], state[s], y);
             }
             if constexpr (LOCAL) sum += x.x;
             else sy[p.wave][r][p.lane] = y;
         }
         __syncthreads();
-        if constexpr (!LOCAL)
+        if constexpr (!LOCAL) {
 #pragma unroll
             for (int j = 0; j < ROWS; j++) {
                 const int r = p.wave + WAVES * j, t = t0 + r;
-                if (r >= TILE || t >= end || !p.live) continue;
-                float o = ch.D * v[j];
+                if (r >= TILE) continue;
+                float o = dv[j];
 #pragma unroll
                 for (int w = 0; w < WAVES; w++) o += sy[w][r][p.lane];
-                if (a.z.ptr && t < len) {
-                    const float z = load(row<T>(a.z, p.n, p.h, t) + p.m);
-                    o *= silu(z, sigmoid(z));
-                }
-                store(row<T>(out, p.n, p.h, t) + p.m, t < len ? o : 0.f);
+                if (gated) o *= gate[j];
+                if (t < end && p.live) O[r] = (T)(t < len ? o : 0.f);
             }
+            O.go(TILE);
+        }
     }
     if constexpr (LOCAL) {
-        store_states(state, W, p.nh * d.segments + p.seg, d, p);
-        if (p.wave == 0 && p.live) sums[(p.nh * d.segments + p.seg) * d.M + p.m] = sum;
-    } else if (W) {
-        store_states(state, W, p.nh, d, p);     // one segment: the state that the call keeps
+        store_states(state, W, (int64_t)p.nh * d.segments + p.seg, d, p);
+        if (p.wave == 0 && p.live) sums[((int64_t)p.nh * d.segments + p.seg) * d.M + p.m] = sum;
+    } else {
+        if (W) store_states(state, W, p.nh, d, p);      // one segment: the state that the call keeps
+        for (int t = first + (max(last - first, 0) + TILE - 1) / TILE * TILE + p.wave; t < end; t += WAVES)      // tiles behind the sequence
+            if (p.live) *(row<T>(out, p.n, p.h, t) + p.m) = (T)0.f;
     }
 }
 
@@ -248,194 +306,268 @@ __global__ __launch_bounds__(256) void k_chain(const float *__restrict__ A, cons
 // ------------------------------------------------------------------ backward
 
 // The gradient of the state before the segment, from zeros behind it
-template <typename T, int WAVES>
-__global__ __launch_bounds__(64 * WAVES) void k_scan_bwd_local(fwp_scan_args a, Dims d, const float *__restrict__ kq, fwp_rows gout,
-                                                               float *__restrict__ own, float *__restrict__ sums) {
-    constexpr int TILE = tile_of(WAVES), ROWS = (TILE + WAVES - 1) / WAVES;
+template <typename T, int WAVES, int S>
+__global__ __launch_bounds__(64 * WAVES) void k_scan_bwd_local(fwp_scan_args a, Dims d, fwp_rows gout, float *__restrict__ own,
+                                                               float *__restrict__ sums) {
+    constexpr int TILE = 16, ROWS = (TILE + WAVES - 1) / WAVES;
+    using K = Keys<T, WAVES, S, TILE, 1>;
+    __shared__ alignas(16) float sq[TILE][K::ROW];
     __shared__ float2 sx[TILE][64];     // dt, dy
     const Place p(d);
     const Channel ch(a, p);
-    const int len = length_of(a.lengths, p.n, d.L), first = p.seg * d.steps, end = min(first + d.steps, d.L);
-    float decay[4], c[4] = {}, sum = 0.f;
+    const int len = length_of(a.lengths, p.n, d.L), first = p.seg * d.steps, end = min(first + d.steps, d.L), last = min(end, len);
+    const int top = first < last ? first + (last - first - 1) / TILE * TILE : first;
+    const bool gated = a.z.ptr != nullptr;
+    Column<const T> DT(a.delta, p, d, top), GO(gout, p, d, top), Z(gated ? a.z : a.v, p, d, top);
+    K keys(a.q, a.q, p, d, top);
+    float decay[S], c[S] = {}, sum = 0.f;
     load_decays(decay, a.A, d, p);
-    for (int t0 = first + (end - first - 1) / TILE * TILE; t0 >= first; t0 -= TILE) {
-        if (t0 >= len) continue;
+    T dt[ROWS], go[ROWS], z[ROWS], key[K::EACH];
+    const auto fetch = [&](int t0) {
+        const int most = min(last - 1 - t0, TILE - 1);
+        DT.load(dt, most, p.wave, WAVES);
+        GO.load(go, most, p.wave, WAVES);
+        if (gated) Z.load(z, most, p.wave, WAVES);
+        keys.load(key, most);
+        DT.go(-TILE), GO.go(-TILE), Z.go(-TILE), keys.go(-TILE);
+    };
+    if (first < last) fetch(top);
+    for (int t0 = top; t0 >= first && first < last; t0 -= TILE) {
 #pragma unroll
         for (int j = 0; j < ROWS; j++) {
-            const int r = p.wave + WAVES * j, t = t0 + r;
-            float dt = 0.f, dy = 0.f;
-            if (r < TILE && t < len && p.live) {
-                dy = load(row<T>(gout, p.n, p.h, t) + p.m);
-                dt = load(row<T>(a.delta, p.n, p.h, t) + p.m) + ch.bias;
-                if (a.softplus) dt = softplus(dt);
-                if (a.z.ptr) {
-                    const float z = load(row<T>(a.z, p.n, p.h, t) + p.m);
-                    dy *= silu(z, sigmoid(z));
-                }
-            }
-            if (r < TILE) sx[r][p.lane] = make_float2(dt, dy);
+            const int r = p.wave + WAVES * j;
+            const bool in = t0 + r < last && p.live;
+            float x = (float)dt[j] + ch.bias, dy = (float)go[j];
+            if (a.softplus) x = softplus(x);
+            if (gated) dy *= silu((float)z[j], sigmoid((float)z[j]));
+            if (r < TILE) sx[r][p.lane] = in ? make_float2(x, dy) : make_float2(0.f, 0.f);
         }
+        keys.put(sq, key, last - t0);
         __syncthreads();
-        scalar_float *const ks = (scalar_float *)(kq + ((p.nh * WAVES + p.wave) * d.padded + t0) * 8);
+        if (t0 > first) fetch(t0 - TILE);
 #pragma unroll
         for (int r = TILE - 1; r >= 0; r--) {
             const float2 x = sx[r][p.lane];
 #pragma unroll
-            for (int s = 0; s < 4; s++) c[s] = fmaf(x.y, ks[8 * r + 4 + s], c[s]) * __builtin_amdgcn_exp2f(x.x * decay[s]);
+            for (int s = 0; s < S; s++) c[s] = fmaf(x.y, sq[r][S * p.wave + s], c[s]) * __builtin_amdgcn_exp2f(x.x * decay[s]);
             sum += x.x;
         }
         __syncthreads();
     }
-    store_states(c, own, p.nh * d.segments + p.seg, d, p);
-    if (p.wave == 0 && p.live) sums[(p.nh * d.segments + p.seg) * d.M + p.m] = sum;
+    store_states(c, own, (int64_t)p.nh * d.segments + p.seg, d, p);
+    if (p.wave == 0 && p.live) sums[((int64_t)p.nh * d.segments + p.seg) * d.M + p.m] = sum;
 }
 
-// parts: [blocks_m][heads][padded][waves][gk0..gk3 | gq0..gq3], the sums over 64 channels
+// parts: [blocks_m][heads][padded][WAVES][S of gk | S of gq], the sums over 64 channels
 // params: [N segments][H][E + 2][M]: gA, gD, gdelta_bias of one segment
-template <typename T, int WAVES>
-__global__ __launch_bounds__(64 * WAVES) void k_scan_bwd(fwp_scan_args a, Dims d, const float *__restrict__ kq, const float *__restrict__ saved,
-                                                         const float *__restrict__ init, fwp_rows gout, fwp_out_rows gv, fwp_out_rows gdelta,
-                                                         fwp_out_rows gz, float *__restrict__ parts, float *__restrict__ params) {
+template <typename T, int WAVES, int S>
+__global__ __launch_bounds__(64 * WAVES, 2) void k_scan_bwd(fwp_scan_args a, Dims d, const float *__restrict__ saved, const float *__restrict__ init,
+                                                         fwp_rows gout, fwp_out_rows gv, fwp_out_rows gdelta, fwp_out_rows gz,
+                                                         float *__restrict__ parts, float *__restrict__ params) {
     constexpr int TILE = tile_of(WAVES), ROWS = (TILE + WAVES - 1) / WAVES;
-    __shared__ float2 sx[TILE][64];                      // dt, dt v
-    __shared__ float sg[TILE][64];                       // dy
+    using K = Keys<T, WAVES, S, TILE, 2>;
+    __shared__ alignas(16) float kqs[2][TILE][K::ROW];
+    __shared__ float2 sxs[2][TILE][64];                  // dt, dt v
+    __shared__ float sgs[2][TILE][64];                   // dy
     __shared__ float part[3][WAVES][TILE][64];           // the waves' parts of sum_e g k, sum_e A w (times log2 e), sum_e q W
     const Place p(d);
     const Channel ch(a, p);
-    const int len = length_of(a.lengths, p.n, d.L), first = p.seg * d.steps, end = min(first + d.steps, d.L);
-    float decay[4], c[4], gA[4] = {}, gD = 0.f, gbias = 0.f;
-    load_decays(decay, a.A, d, p);
-    load_states(c, init, p.nh * d.segments + p.seg, d, p);
-    for (int t0 = first + (end - first - 1) / TILE * TILE; t0 >= first; t0 -= TILE) {
-        if (t0 >= len) {
-#pragma unroll
-            for (int j = 0; j < ROWS; j++) {
-                const int t = t0 + p.wave + WAVES * j;
-                if (p.wave + WAVES * j >= TILE || t >= end || !p.live) continue;
-                store(row<T>(gv, p.n, p.h, t) + p.m, 0.f);
-                store(row<T>(gdelta, p.n, p.h, t) + p.m, 0.f);
-                if (a.z.ptr) store(row<T>(gz, p.n, p.h, t) + p.m, 0.f);
-            }
-            continue;
+    const int len = length_of(a.lengths, p.n, d.L), first = p.seg * d.steps, end = min(first + d.steps, d.L), last = min(end, len);
+    const int top = first < last ? first + (last - first - 1) / TILE * TILE : first - TILE;
+    const bool gated = a.z.ptr != nullptr;
+    Column<T> GV(gv, p, d, top), GD(gdelta, p, d, top), GZ(gated ? gz : gv, p, d, top);
+    // whole tiles behind the sequence
+    for (int t = top + TILE + p.wave; t < end; t += WAVES)
+        if (p.live) {
+            Column<T> gv0(gv, p, d, t), gd0(gdelta, p, d, t), gz0(gated ? gz : gv, p, d, t);
+            gv0[0] = gd0[0] = (T)0.f;
+            if (gated) gz0[0] = (T)0.f;
         }
-        float v[ROWS], pre[ROWS], go[ROWS], z[ROWS];
+    Column<const T> V(a.v, p, d, max(top, 0)), DT(a.delta, p, d, max(top, 0)), GO(gout, p, d, max(top, 0)), Z(gated ? a.z : a.v, p, d, max(top, 0));
+    K keys(a.k, a.q, p, d, max(top, 0));
+    float decay[S], c[S], gA[S] = {}, gD = 0.f, gbias = 0.f;
+    load_decays(decay, a.A, d, p);
+    load_states(c, init, (int64_t)p.nh * d.segments + p.seg, d, p);
+    T v[ROWS], dt[ROWS], go[ROWS], z[ROWS], key[K::EACH];
+    float next[S];
+    const auto fetch = [&](int t0) {
+        const int most = min(last - 1 - t0, TILE - 1);
+        V.load(v, most, p.wave, WAVES);
+        DT.load(dt, most, p.wave, WAVES);
+        GO.load(go, most, p.wave, WAVES);
+        if (gated) Z.load(z, most, p.wave, WAVES);
+        keys.load(key, most);
+        load_states(next, saved, (int64_t)p.nh * d.tiles + t0 / TILE, d, p);
+        V.go(-TILE), DT.go(-TILE), GO.go(-TILE), Z.go(-TILE), keys.go(-TILE);
+    };
+    float vs[ROWS], pre[ROWS], gos[ROWS], zs[ROWS], before0[S];
+    const auto stage = [&](int t0, int half) {
 #pragma unroll
         for (int j = 0; j < ROWS; j++) {
-            const int r = p.wave + WAVES * j, t = t0 + r;
-            float dt = 0.f, dy = 0.f;
-            v[j] = pre[j] = go[j] = z[j] = 0.f;
-            if (r < TILE && t < len && p.live) {
-                v[j] = load(row<T>(a.v, p.n, p.h, t) + p.m);
-                pre[j] = load(row<T>(a.delta, p.n, p.h, t) + p.m) + ch.bias;
-                dt = a.softplus ? softplus(pre[j]) : pre[j];
-                dy = go[j] = load(row<T>(gout, p.n, p.h, t) + p.m);
-                if (a.z.ptr) {
-                    z[j] = load(row<T>(a.z, p.n, p.h, t) + p.m);
-                    dy *= silu(z[j], sigmoid(z[j]));
-                }
+            const int r = p.wave + WAVES * j;
+            const bool in = t0 + r < last && p.live;
+            const float pre = (float)dt[j] + ch.bias, vs = in ? (float)v[j] : 0.f;
+            float x = a.softplus ? softplus(pre) : pre, dy = in ? (float)go[j] : 0.f;
+            x = in ? x : 0.f;
+            if (gated) {
+                const float z_ = in ? (float)z[j] : 0.f;
+                dy *= silu(z_, sigmoid(z_));
             }
-            if (r < TILE) sx[r][p.lane] = make_float2(dt, dt * v[j]), sg[r][p.lane] = dy;
+            if (r < TILE) sxs[half][r][p.lane] = make_float2(x, x * vs), sgs[half][r][p.lane] = dy;
         }
-        __syncthreads();
-        scalar_float *const ks = (scalar_float *)(kq + ((p.nh * WAVES + p.wave) * d.padded + t0) * 8);
-        float before[TILE + 1][4], al[TILE][4];      // the states before each step, and its decays
-        load_states(before[0], saved, p.nh * d.tiles + t0 / TILE, d, p);
+        keys.put(kqs[half], key, last - t0);
+    };
+    // what the last lines of a tile need of its rows
+    const auto keep = [&](int t0) {
+#pragma unroll
+        for (int j = 0; j < ROWS; j++) {
+            const bool in = t0 + p.wave + WAVES * j < last && p.live;
+            pre[j] = (float)dt[j] + ch.bias;
+            vs[j] = in ? (float)v[j] : 0.f;
+            gos[j] = in ? (float)go[j] : 0.f;
+            if (gated) zs[j] = in ? (float)z[j] : 0.f;
+        }
+#pragma unroll
+        for (int s = 0; s < S; s++) before0[s] = next[s];
+    };
+    if (first < last) {
+        fetch(top);
+        stage(top, 0);
+    }
+    int half = 0;
+    for (int t0 = top; t0 >= first; t0 -= TILE, half ^= 1) {
+        __syncthreads();        // this tile's rows are in LDS, and nobody reads `part` any more
+        const auto sx = sxs[half];
+        const auto sg = sgs[half];
+        const auto kq = kqs[half];
+        keep(t0);
+        if (t0 > first) fetch(t0 - TILE);
+        float before[TILE + 1][S], al[TILE][S];      // the states before each step, and its decays
+#pragma unroll
+        for (int s = 0; s < S; s++) before[0][s] = before0[s];
 #pragma unroll
         for (int r = 0; r < TILE; r++) {
             const float2 x = sx[r][p.lane];
+            const float *const k = kq[r] + K::WIDTH * p.wave, *const q = k + S;
             float y = 0.f;
 #pragma unroll
-            for (int s = 0; s < 4; s++) {
+            for (int s = 0; s < S; s++) {
                 al[r][s] = __builtin_amdgcn_exp2f(x.x * decay[s]);
-                before[r + 1][s] = fmaf(al[r][s], before[r][s], x.y * ks[8 * r + s]);
-                y = fmaf(ks[8 * r + 4 + s], before[r + 1][s], y);
+                before[r + 1][s] = fmaf(al[r][s], before[r][s], x.y * k[s]);
+                y = fmaf(q[s], before[r + 1][s], y);
             }
             part[2][p.wave][r][p.lane] = y;
         }
-        // One step back; what is summed over the channels comes out in `sums`: gk of the four rows, then gq
-        const auto back = [&](int r, float (&sums)[8]) {
+        float tile_gA[S] = {};      // a tile's share first: the sum over a sequence then has a sixteenth of the terms
+        // One step back; what is summed over the channels comes out in `sums`: gk of the wave's rows, then gq
+        constexpr int SUMS = 2 * S;
+        const auto back = [&](int r, float (&sums)[SUMS]) {
             const float2 x = sx[r][p.lane];
-            const float dy = sg[r][p.lane];
+            const float dy = sg[r][p.lane], *const k = kq[r] + K::WIDTH * p.wave, *const q = k + S;
             float read = 0.f, slope = 0.f;
 #pragma unroll
-            for (int s = 0; s < 4; s++) {
-                const float g = fmaf(dy, ks[8 * r + 4 + s], c[s]);
+            for (int s = 0; s < S; s++) {
+                const float g = fmaf(dy, q[s], c[s]);
                 sums[s] = g * x.y;
-                sums[4 + s] = dy * before[r + 1][s];
-                read = fmaf(g, ks[8 * r + s], read);
+                sums[S + s] = dy * before[r + 1][s];
+                read = fmaf(g, k[s], read);
                 c[s] = g * al[r][s];
                 const float w = c[s] * before[r][s];
                 slope = fmaf(w, decay[s], slope);
-                gA[s] = fmaf(w, x.x, gA[s]);
+                tile_gA[s] = fmaf(w, x.x, tile_gA[s]);
             }
             part[0][p.wave][r][p.lane] = read;
             part[1][p.wave][r][p.lane] = slope;
         };
-        // The sums over the lanes, halving what a lane holds as it goes: after eight steps lane l has the sum number l % 8 of the step whose bits
-        // 0, 1, 2 are l's bits 5, 4, 3.
-#pragma unroll
-        for (int r0 = TILE - 8; r0 >= 0; r0 -= 8) {
-            float eight[2][8];
+        // The sums over the lanes, halving what a lane holds as it goes, over 64 / SUMS steps (8 or 16): lane l then has the sum
+        // number l % SUMS of the step whose bits 0, 1, 2 (and 3) are l's bits 5, 4, 3 (and 2).
+        const bool b3 = p.lane & 8, b2 = p.lane & 4, b1 = p.lane & 2, b0 = p.lane & 1;
+        float *const to = parts + (((int64_t)p.mb * d.N * d.H + p.nh) * d.padded + t0) * WAVES * SUMS +
+                          ((p.lane >> 5 & 1) + 2 * (p.lane >> 4 & 1) + 4 * (p.lane >> 3 & 1) + (S == 2 ? 8 * (p.lane >> 2 & 1) : 0)) * WAVES * SUMS +
+                          p.wave * SUMS + p.lane % SUMS;
+        const auto eight_back = [&](int r0, float (&x)[SUMS]) {
+            float eight[2][SUMS];
 #pragma unroll
             for (int q2 = 1; q2 >= 0; q2--) {
-                float four[2][8];
+                float four[2][SUMS];
 #pragma unroll
                 for (int q1 = 1; q1 >= 0; q1--) {
-                    float odd[8], even[8];
+                    float odd[SUMS], even[SUMS];
                     back(r0 + 4 * q2 + 2 * q1 + 1, odd);
                     back(r0 + 4 * q2 + 2 * q1, even);
 #pragma unroll
-                    for (int i = 0; i < 8; i++) {
+                    for (int i = 0; i < SUMS; i++) {
                         swap32(even[i], odd[i]);
                         four[q1][i] = even[i] + odd[i];
                     }
                 }
 #pragma unroll
-                for (int i = 0; i < 8; i++) {
+                for (int i = 0; i < SUMS; i++) {
                     swap16(four[0][i], four[1][i]);
                     eight[q2][i] = pinned(four[0][i] + four[1][i]);
                 }
             }
-            const bool b3 = p.lane & 8, b2 = p.lane & 4, b1 = p.lane & 2, b0 = p.lane & 1;
-            float x[8];
 #pragma unroll
-            for (int i = 0; i < 8; i++) x[i] = pinned((b3 ? eight[1][i] : eight[0][i]) + dpp<kRowRor8>(b3 ? eight[0][i] : eight[1][i]));
-#pragma unroll
-            for (int i = 0; i < 4; i++) x[i] = pinned((b2 ? x[i + 4] : x[i]) + dpp<kRowMirror8>(b2 ? x[i] : x[i + 4]));
+            for (int i = 0; i < SUMS; i++) x[i] = pinned((b3 ? eight[1][i] : eight[0][i]) + dpp<kRowRor8>(b3 ? eight[0][i] : eight[1][i]));
+        };
+        const auto four_lanes = [&](float (&x)[4]) {
 #pragma unroll
             for (int i = 0; i < 2; i++) x[i] = pinned((b1 ? x[i + 2] : x[i]) + dpp<kQuadXor2>(b1 ? x[i] : x[i + 2]));
-            x[0] = pinned((b0 ? x[1] : x[0]) + dpp<kQuadXor1>(b0 ? x[0] : x[1]));
-            const int t = t0 + r0 + (p.lane >> 5 & 1) + 2 * (p.lane >> 4 & 1) + 4 * (p.lane >> 3 & 1);
-            const int64_t mb = blockIdx.x % d.blocks_m;
-            parts[(((mb * d.N * d.H + p.nh) * d.padded + t) * WAVES + p.wave) * 8 + p.lane % 8] = x[0];
+            return pinned((b0 ? x[1] : x[0]) + dpp<kQuadXor1>(b0 ? x[0] : x[1]));
+        };
+        if constexpr (S == 4) {
+#pragma unroll
+            for (int r0 = TILE - 8; r0 >= 0; r0 -= 8) {
+                float x[8], y[4];
+                eight_back(r0, x);
+#pragma unroll
+                for (int i = 0; i < 4; i++) y[i] = pinned((b2 ? x[i + 4] : x[i]) + dpp<kRowMirror8>(b2 ? x[i] : x[i + 4]));
+                to[r0 * WAVES * SUMS] = four_lanes(y);
+            }
+        } else {
+            float hi[4], lo[4], y[4];
+            eight_back(8, hi);
+            eight_back(0, lo);
+#pragma unroll
+            for (int i = 0; i < 4; i++) y[i] = pinned((b2 ? hi[i] : lo[i]) + dpp<kRowMirror8>(b2 ? lo[i] : hi[i]));
+            *to = four_lanes(y);
         }
+#pragma unroll
+        for (int s = 0; s < S; s++) gA[s] += tile_gA[s];
+        if (t0 > first) stage(t0 - TILE, half ^ 1);
         __syncthreads();
+        float tile_gD = 0.f, tile_gbias = 0.f;
 #pragma unroll
         for (int j = 0; j < ROWS; j++) {
             const int r = p.wave + WAVES * j, t = t0 + r;
-            if (r >= TILE || t >= end || !p.live) continue;
-            float read = 0.f, slope = 0.f, o = ch.D * v[j];
+            if (r >= TILE) continue;
+            float read = 0.f, slope = 0.f, o = ch.D * vs[j];
 #pragma unroll
             for (int w = 0; w < WAVES; w++) {
                 read += part[0][w][r][p.lane];
                 slope += part[1][w][r][p.lane];
                 o += part[2][w][r][p.lane];
             }
-            const float dt = sx[r][p.lane].x, dy = sg[r][p.lane];
-            float gdt = fmaf(v[j], read, kLn2 * slope);
+            const float x = sx[r][p.lane].x, dy = sg[r][p.lane];
+            float gdt = fmaf(vs[j], read, kLn2 * slope);
             if (a.softplus) gdt *= sigmoid(pre[j]);
             const bool in = t < len;
-            store(row<T>(gv, p.n, p.h, t) + p.m, in ? fmaf(dt, read, ch.D * dy) : 0.f);
-            store(row<T>(gdelta, p.n, p.h, t) + p.m, in ? gdt : 0.f);
-            if (a.z.ptr) store(row<T>(gz, p.n, p.h, t) + p.m, in ? go[j] * o * silu_slope(z[j], sigmoid(z[j])) : 0.f);
-            if (in) gD = fmaf(dy, v[j], gD), gbias += gdt;
+            gdt = in ? gdt : 0.f;
+            if (t < end && p.live) {
+                GV[r] = (T)(in ? fmaf(x, read, ch.D * dy) : 0.f);
+                GD[r] = (T)gdt;
+                if (gated) GZ[r] = (T)(in ? gos[j] * o * silu_slope(zs[j], sigmoid(zs[j])) : 0.f);
+            }
+            if (in) tile_gD = fmaf(dy, vs[j], tile_gD), tile_gbias += gdt;
         }
-        __syncthreads();        // the next tile overwrites what this one's last rows are read from
+        GV.go(-TILE), GD.go(-TILE), GZ.go(-TILE);
+        gD += tile_gD, gbias += tile_gbias;
     }
+    __syncthreads();
     float *const to = params + ((int64_t)(p.n * d.segments + p.seg) * d.H + p.h) * (d.E + 2) * d.M + p.m;
 #pragma unroll
-    for (int s = 0; s < 4; s++)
-        if (p.live && 4 * p.wave + s < d.E) to[(int64_t)(4 * p.wave + s) * d.M] = gA[s];
+    for (int s = 0; s < S; s++)
+        if (p.live && S * p.wave + s < d.E) to[(int64_t)(S * p.wave + s) * d.M] = gA[s];
     // the waves' rows of a channel
     part[0][p.wave][0][p.lane] = gD;
     part[1][p.wave][0][p.lane] = gbias;
@@ -452,18 +584,18 @@ template <typename T>
 __global__ __launch_bounds__(256) void k_scan_finish(const float *__restrict__ parts, const float *__restrict__ params, fwp_out_rows gq,
                                                      fwp_out_rows gk, float *__restrict__ gA, float *__restrict__ gD,
                                                      float *__restrict__ gbias, const int64_t *__restrict__ lengths, Dims d, int waves,
-                                                     int64_t row_blocks) {
+                                                     int S, int64_t row_blocks) {
     if (blockIdx.x < row_blocks) {
-        const int width = waves * 8;
+        const int width = waves * 2 * S;
         const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, heads = (int64_t)d.N * d.H;
         const int64_t nh = i / ((int64_t)d.L * width), rest = i % ((int64_t)d.L * width);
-        const int t = (int)(rest / width), j = (int)(rest % width), e = j / 8 * 4 + j % 4;
+        const int t = (int)(rest / width), j = (int)(rest % width), e = j / (2 * S) * S + j % S;
         if (nh >= heads || e >= d.E) return;
         const int n = (int)(nh / d.H), h = (int)(nh % d.H);
         float x = 0.f;
         if (t < length_of(lengths, n, d.L))
             for (int mb = 0; mb < d.blocks_m; mb++) x += parts[((mb * heads + nh) * d.padded + t) * width + j];
-        store(row<T>(j % 8 < 4 ? gk : gq, n, h, t) + e, x);
+        store(row<T>(j % (2 * S) < S ? gk : gq, n, h, t) + e, x);
         return;
     }
     // 64 columns and four slices of the sequences and segments to a workgroup
@@ -530,15 +662,14 @@ __global__ __launch_bounds__(256) void k_scan_step(fwp_scan_args a, float *__res
 
 // ------------------------------------------------------------------ launches
 
+// f(WAVES, S)
 template <typename F>
-void by_waves(int waves, F f) {
-    switch (waves) {
-        case 1: f(std::integral_constant<int, 1>()); break;
-        case 2: f(std::integral_constant<int, 2>()); break;
-        case 4: f(std::integral_constant<int, 4>()); break;
-        case 8: f(std::integral_constant<int, 8>()); break;
-        default: f(std::integral_constant<int, 16>()); break;
-    }
+void by_waves(const Plan &p, F f) {
+    using std::integral_constant;
+    if (p.waves == 4) f(integral_constant<int, 4>(), integral_constant<int, 2>());
+    else if (p.waves == 16) f(integral_constant<int, 16>(), integral_constant<int, 4>());
+    else if (p.rows == 2) f(integral_constant<int, 8>(), integral_constant<int, 2>());
+    else f(integral_constant<int, 8>(), integral_constant<int, 4>());
 }
 
 constexpr int64_t kMaxBlocks = (int64_t(1) << 31) - 1;
@@ -547,13 +678,13 @@ constexpr int64_t kMaxBlocks = (int64_t(1) << 31) - 1;
 
 int64_t scan_saved_floats(int N, int H, int L, int E, int M) {
     const Plan p(N, H, L, E, M, false);
-    return p.packed + p.states * p.tiles;
+    return p.states * p.tiles;
 }
 
 int64_t scan_workspace(int N, int H, int L, int E, int M, bool backward) {
     const Plan p(N, H, L, E, M, backward);
-    if (!backward) return p.packed + p.seg_states();
-    return p.blocks_m * p.heads * p.padded * p.waves * 8 + (int64_t)N * p.segments * H * (E + 2) * M + p.seg_states();
+    if (!backward) return p.seg_states();
+    return p.blocks_m * p.heads * p.padded * p.waves * 2 * p.rows + (int64_t)N * p.segments * H * (E + 2) * M + p.seg_states();
 }
 
 int scan_fwd(const fwp_scan_args &a, float *W, fwp_out_rows out, float *saved, float *workspace, hipStream_t s) {
@@ -564,24 +695,20 @@ int scan_fwd(const fwp_scan_args &a, float *W, fwp_out_rows out, float *saved, f
         return (int)hipGetLastError();
     }
     const Plan p(a.N, a.H, a.L, a.E, a.M, false);
-    const int chunks = (int)(((int64_t)p.padded * 8 + 255) / 256);
-    if (p.grid() > kMaxBlocks || p.heads * chunks > kMaxBlocks || (p.states + 255) / 256 > kMaxBlocks) return FWP_E_SHAPE;
-    float *const kq = saved ? saved : workspace, *const ckpt = saved ? saved + p.packed : nullptr, *const seg = workspace + (saved ? 0 : p.packed),
-                *const sums = seg + p.states * p.segments;
+    if (p.grid() > kMaxBlocks || (p.states + 255) / 256 > kMaxBlocks) return FWP_E_SHAPE;
+    float *const seg = workspace, *const sums = seg + p.states * p.segments;
     const Dims d = p;
     by_type(a.type, [&](auto t) {
         using T = decltype(t);
-        hipLaunchKernelGGL((k_pack<T>), dim3((unsigned)(p.heads * chunks), p.waves), dim3(256), 0, s, a.q, a.k, a.lengths, kq, a.H, a.L, a.E,
-                           p.padded, chunks);
-        by_waves(p.waves, [&](auto w) {
-            constexpr int WAVES = decltype(w)::value;
+        by_waves(p, [&](auto w, auto r) {
+            constexpr int WAVES = decltype(w)::value, S = decltype(r)::value;
             const dim3 grid((unsigned)p.grid()), block(64 * WAVES);
             if (p.segments > 1) {
-                hipLaunchKernelGGL((k_scan_fwd<T, WAVES, true>), grid, block, 0, s, a, d, kq, nullptr, seg, nullptr, sums, out);
+                hipLaunchKernelGGL((k_scan_fwd<T, WAVES, S, true>), grid, block, 0, s, a, d, nullptr, seg, nullptr, sums, out);
                 hipLaunchKernelGGL((k_chain<false>), dim3((unsigned)((p.states + 255) / 256)), dim3(256), 0, s, a.A, sums, seg, W, W, d);
             }
-            hipLaunchKernelGGL((k_scan_fwd<T, WAVES, false>), grid, block, 0, s, a, d, kq, p.segments > 1 ? seg : W,
-                               p.segments > 1 ? nullptr : W, ckpt, nullptr, out);
+            hipLaunchKernelGGL((k_scan_fwd<T, WAVES, S, false>), grid, block, 0, s, a, d, p.segments > 1 ? seg : W,
+                               p.segments > 1 ? nullptr : W, saved, nullptr, out);
         });
     });
     return (int)hipGetLastError();
@@ -590,29 +717,28 @@ int scan_fwd(const fwp_scan_args &a, float *W, fwp_out_rows out, float *saved, f
 int scan_bwd(const fwp_scan_args &a, const float *saved, fwp_rows gout, fwp_out_rows gq, fwp_out_rows gk, fwp_out_rows gv,
              fwp_out_rows gdelta, fwp_out_rows gz, float *gA, float *gD, float *gdelta_bias, float *workspace, hipStream_t s) {
     const Plan p(a.N, a.H, a.L, a.E, a.M, true);
-    const int64_t row_blocks = (p.heads * a.L * p.waves * 8 + 255) / 256,
+    const int64_t row_blocks = (p.heads * a.L * p.waves * 2 * p.rows + 255) / 256,
                   param_blocks = ((int64_t)a.H * (a.E + 2) * a.M + 63) / 64;
     if (p.grid() > kMaxBlocks || row_blocks + param_blocks > kMaxBlocks || (p.states + 255) / 256 > kMaxBlocks ||
         (int64_t)a.N * p.segments > kMaxBlocks)
         return FWP_E_SHAPE;
-    const float *const kq = saved, *const ckpt = saved + p.packed;
-    float *const parts = workspace, *const params = parts + p.blocks_m * p.heads * p.padded * p.waves * 8,
+    float *const parts = workspace, *const params = parts + p.blocks_m * p.heads * p.padded * p.waves * 2 * p.rows,
                 *const seg = params + (int64_t)a.N * p.segments * a.H * (a.E + 2) * a.M, *const sums = seg + p.states * p.segments;
     const Dims d = p;
     by_type(a.type, [&](auto t) {
         using T = decltype(t);
-        by_waves(p.waves, [&](auto w) {
-            constexpr int WAVES = decltype(w)::value;
+        by_waves(p, [&](auto w, auto r) {
+            constexpr int WAVES = decltype(w)::value, S = decltype(r)::value;
             const dim3 grid((unsigned)p.grid()), block(64 * WAVES);
             if (p.segments > 1) {
-                hipLaunchKernelGGL((k_scan_bwd_local<T, WAVES>), grid, block, 0, s, a, d, kq, gout, seg, sums);
+                hipLaunchKernelGGL((k_scan_bwd_local<T, WAVES, S>), grid, block, 0, s, a, d, gout, seg, sums);
                 hipLaunchKernelGGL((k_chain<true>), dim3((unsigned)((p.states + 255) / 256)), dim3(256), 0, s, a.A, sums, seg, nullptr, nullptr, d);
             }
-            hipLaunchKernelGGL((k_scan_bwd<T, WAVES>), grid, block, 0, s, a, d, kq, ckpt, p.segments > 1 ? seg : nullptr, gout, gv, gdelta, gz,
-                               parts, params);
+            hipLaunchKernelGGL((k_scan_bwd<T, WAVES, S>), grid, block, 0, s, a, d, saved, p.segments > 1 ? seg : nullptr, gout, gv, gdelta, gz, parts,
+                               params);
         });
         hipLaunchKernelGGL((k_scan_finish<T>), dim3((unsigned)(row_blocks + param_blocks)), dim3(256), 0, s, parts, params, gq, gk, gA, gD,
-                           gdelta_bias, a.lengths, d, p.waves, row_blocks);
+                           gdelta_bias, a.lengths, d, p.waves, p.rows, row_blocks);
     });
     return (int)hipGetLastError();
 }

@@ -50,26 +50,29 @@ at::Tensor lengths_of(const at::Tensor &t, int64_t N) {
     return t.contiguous();
 }
 
-// [N,H,L,D] rows whose last axis is contiguous; a copy where it is not
-at::Tensor rows_of(const at::Tensor &t) { return !t.defined() || t.size(3) == 1 || t.stride(3) == 1 ? t : t.contiguous(); }
+constexpr int64_t kMaxStep = 1 << 25;      // elements between the steps of a view that the scan takes
+
+// [N,H,L,D] rows whose last axis is contiguous; a copy where it is not, and of rows too far apart
+at::Tensor rows_of(const at::Tensor &t, int64_t most = std::numeric_limits<int64_t>::max()) {
+    if (!t.defined() || ((t.size(3) == 1 || t.stride(3) == 1) && (t.size(2) == 1 || t.stride(2) <= most))) return t;
+    return t.clone(at::MemoryFormat::Contiguous);
+}
 
 fwp_rows view(const at::Tensor &t) {
-    return t.defined() ? fwp_rows{t.const_data_ptr(), t.stride(0), t.stride(1), t.stride(2)} : fwp_rows{};
+    return t.defined() ? fwp_rows{t.const_data_ptr(), t.stride(0), t.stride(1), t.size(2) > 1 ? t.stride(2) : 0} : fwp_rows{};
 }
 fwp_out_rows out_view(const at::Tensor &t) {
-    return t.defined() ? fwp_out_rows{t.data_ptr(), t.stride(0), t.stride(1), t.stride(2)} : fwp_out_rows{};
+    return t.defined() ? fwp_out_rows{t.data_ptr(), t.stride(0), t.stride(1), t.size(2) > 1 ? t.stride(2) : 0} : fwp_out_rows{};
 }
 
 // Do these rows lie with the steps outermost, as a layer's permuted views do?  Results take the order of the rows they belong to.
 bool steps_lead(const at::Tensor &t) {
     const int64_t N = t.size(0), H = t.size(1), L = t.size(2);
-    return L > 1 && (N > 1 || H > 1) && (N == 1 || t.stride(2) > t.stride(0)) && (H == 1 || t.stride(2) > t.stride(1));
-}
-at::Tensor empty_rows(int64_t N, int64_t H, int64_t L, int64_t D, bool lead, const at::TensorOptions &opts) {
-    return lead ? at::empty({L, N, H, D}, opts).permute({1, 2, 0, 3}) : at::empty({N, H, L, D}, opts);
+    return L > 1 && (N > 1 || H > 1) && N * H * t.size(3) <= kMaxStep && (N == 1 || t.stride(2) > t.stride(0)) && (H == 1 || t.stride(2) > t.stride(1));
 }
 at::Tensor empty_rows(const at::Tensor &like) {
-    return empty_rows(like.size(0), like.size(1), like.size(2), like.size(3), steps_lead(like), like.options());
+    const int64_t N = like.size(0), H = like.size(1), L = like.size(2), D = like.size(3);
+    return steps_lead(like) ? at::empty({L, N, H, D}, like.options()).permute({1, 2, 0, 3}) : at::empty({N, H, L, D}, like.options());
 }
 
 const float *floats(const at::Tensor &t) { return t.defined() ? t.const_data_ptr<float>() : nullptr; }
@@ -215,7 +218,8 @@ struct ScanFn : torch::autograd::Function<ScanFn> {
             fail("W must be a contiguous fp32 [N,H,E,M] tensor");
         require_device(q_in);
         same_device(q_in, {k_in, v_in, delta_in, A, D, z_, bias, W, lengths});
-        const at::Tensor q = rows_of(q_in), k = rows_of(k_in), v = rows_of(v_in), delta = rows_of(delta_in), z = rows_of(z_), out = empty_rows(v);
+        const at::Tensor q = rows_of(q_in, kMaxStep), k = rows_of(k_in, kMaxStep), v = rows_of(v_in, kMaxStep), delta = rows_of(delta_in, kMaxStep),
+                         z = rows_of(z_, kMaxStep), out = empty_rows(v);
         fwp_scan_args a = args(v, delta, z, A, D, bias, lengths, softplus);
         a.q = view(q), a.k = view(k);
         LaunchGuard guard(q);
@@ -225,10 +229,7 @@ struct ScanFn : torch::autograd::Function<ScanFn> {
         check(fwp_scan_fwd(&a, floats_out(W), out_view(out), floats_out(saved), work.data_ptr<float>(), stream_of(q)), "fwp_scan_fwd");
         overwritten(W);
         if (ctx) {
-            // q and k are in `saved`, as the kernels read them
-            ctx->save_for_backward({v, delta, z, A, D, bias, lengths, saved});
-            ctx->saved_data["q_lead"] = steps_lead(q);
-            ctx->saved_data["k_lead"] = steps_lead(k);
+            ctx->save_for_backward({v, delta, z, A, D, bias, lengths, saved, q, k});
             ctx->saved_data["softplus"] = softplus;
             ctx->set_materialize_grads(false);
         }
@@ -240,11 +241,11 @@ struct ScanFn : torch::autograd::Function<ScanFn> {
         once_only();
         const auto s = ctx->get_saved_variables();
         const at::Tensor &v = s[0], &delta = s[1], &z = s[2], &A = s[3], &D = s[4], &bias = s[5], &lengths = s[6], &saved = s[7];
-        const at::Tensor g = rows_of(grads[0]);
-        const fwp_scan_args a = args(v, delta, z, A, D, bias, lengths, ctx->saved_data["softplus"].toBool());
+        const at::Tensor g = rows_of(grads[0], kMaxStep);
+        fwp_scan_args a = args(v, delta, z, A, D, bias, lengths, ctx->saved_data["softplus"].toBool());
+        a.q = view(s[8]), a.k = view(s[9]);
         LaunchGuard guard(v);
-        const at::Tensor gq = empty_rows(a.N, a.H, a.L, a.E, ctx->saved_data["q_lead"].toBool(), v.options()),
-                         gk = empty_rows(a.N, a.H, a.L, a.E, ctx->saved_data["k_lead"].toBool(), v.options()), gv = empty_rows(v), gdelta = empty_rows(delta),
+        const at::Tensor gq = empty_rows(s[8]), gk = empty_rows(s[9]), gv = empty_rows(v), gdelta = empty_rows(delta),
                          gz = z.defined() ? empty_rows(z) : at::Tensor(), gA = at::empty_like(A), gD = at::empty({a.H, a.M}, A.options()),
                          gbias = at::empty({a.H, a.M}, A.options()), work = scratch(fwp_scan_workspace(a.N, a.H, a.L, a.E, a.M, 1), v);
         check(fwp_scan_bwd(&a, floats(saved), view(g), out_view(gq), out_view(gk), out_view(gv), out_view(gdelta), out_view(gz), floats_out(gA),
