@@ -70,7 +70,7 @@ int fwp_scan_fwd(const fwp_scan_args *a, float *W, fwp_out_rows out, float *save
     if (!type_ok(a->type) || scan_dims(a->N, a->H, a->L, a->E, a->M)) return FWP_E_SHAPE;
     for (const fwp_rows *v : {&a->q, &a->k, &a->v, &a->delta})
         if (!rows_ok(*v, a->type)) return FWP_E_NULL;
-    if (!element_aligned(a->z.ptr, a->type) || !rows_ok(out, a->type) || !workspace) return FWP_E_NULL;
+    if (!element_aligned(a->z.ptr, a->type) || !rows_ok(out, a->type)) return FWP_E_NULL;
     for (const int64_t sL : {a->q.sL, a->k.sL, a->v.sL, a->delta.sL, a->z.ptr ? a->z.sL : 0, out.sL})
         if (!step_ok(sL)) return FWP_E_SHAPE;
     return scan_fwd(*a, W, out, saved, workspace, (hipStream_t)stream);

@@ -41,8 +41,9 @@ __device__ __forceinline__ float silu(float x, float s) { return s == 0.f ? 0.f 
 
 // log(1 + exp(x)) = max(x, 0) + log1p(u), u = exp(-|x|) in (0, 1], and log1p(u) = 2 atanh(s) with s = u / (2 + u) <= 1/3:
 // s times a polynomial in s^2 (Chebyshev over [0, 1/9], 4e-9 off), so that small results keep their relative precision.
-__device__ __forceinline__ float softplus(float x) {
-    const float u = exp_of(-fabsf(x)), s = u * __builtin_amdgcn_rcpf(2.f + u), y = s * s;
+__device__ __forceinline__ float softplus(float x, float &u) {
+    u = exp_of(-fabsf(x));
+    const float s = u * __builtin_amdgcn_rcpf(2.f + u), y = s * s;
     float p = 0.1408732831478119f;
     p = fmaf(p, y, 0.1398070901632309f);
     p = fmaf(p, y, 0.20012426376342773f);
@@ -50,6 +51,12 @@ __device__ __forceinline__ float softplus(float x) {
     p = fmaf(p, y, 1.f);
     return fmaf(2.f * s, p, x < 0.f ? 0.f : x);      // NaN stays
 }
+__device__ __forceinline__ float softplus(float x) {
+    float u;
+    return softplus(x, u);
+}
+// its slope, the sigmoid, from the same u
+__device__ __forceinline__ float softplus_slope(float x, float u) { return (x < 0.f ? u : 1.f) * __builtin_amdgcn_rcpf(1.f + u); }
 
 // The steps of sequence n that count
 __device__ __forceinline__ int length_of(const int64_t *lengths, int n, int L) {

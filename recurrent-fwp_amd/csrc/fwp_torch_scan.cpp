@@ -225,8 +225,9 @@ struct ScanFn : torch::autograd::Function<ScanFn> {
         LaunchGuard guard(q);
         at::Tensor saved;
         if (ctx) saved = scratch(fwp_scan_saved_floats(a.N, a.H, a.L, a.E, a.M), v);
-        const at::Tensor work = scratch(fwp_scan_workspace(a.N, a.H, a.L, a.E, a.M, 0), v);
-        check(fwp_scan_fwd(&a, floats_out(W), out_view(out), floats_out(saved), work.data_ptr<float>(), stream_of(q)), "fwp_scan_fwd");
+        at::Tensor work;
+        if (const int64_t n = a.L == 1 ? 0 : fwp_scan_workspace(a.N, a.H, a.L, a.E, a.M, 0)) work = scratch(n, v);
+        check(fwp_scan_fwd(&a, floats_out(W), out_view(out), floats_out(saved), floats_out(work), stream_of(q)), "fwp_scan_fwd");
         overwritten(W);
         if (ctx) {
             ctx->save_for_backward({v, delta, z, A, D, bias, lengths, saved, q, k});

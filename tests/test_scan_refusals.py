@@ -85,7 +85,8 @@ def test_c_entry_points_refuse_before_any_launch(fwp):
     scan = lambda **k: ctypes.byref(L.ScanArgs(**{**dict(q=v, k=v, v=v, delta=v, A=4096, type=2, N=2, H=1, L=5, E=16, M=8), **k}))
     assert lib.fwp_scan_fwd(scan(q=null), p, out, p, p, None) == E_NULL
     assert lib.fwp_scan_fwd(scan(A=0), p, out, p, p, None) == E_NULL
-    assert lib.fwp_scan_fwd(scan(), p, out, p, None, None) == E_NULL                           # no workspace
+    assert lib.fwp_scan_workspace(2, 1, 5, 16, 8, 0) == 0 and lib.fwp_scan_workspace(1, 1, 8192, 16, 8, 0) > 0
+    assert lib.fwp_scan_fwd(scan(L=8192), p, out, p, None, None) == E_NULL                     # no workspace for its segments
     for bad in (dict(E=65), dict(E=0), dict(M=0), dict(L=0), dict(type=-1)):
         assert lib.fwp_scan_fwd(scan(**bad), p, out, p, p, None) == E_SHAPE, bad
     assert lib.fwp_scan_bwd(scan(), None, v, out, out, out, out, none, p, p, p, p, None) == E_NULL
