@@ -15,6 +15,7 @@ from torch.utils._device import DeviceContext
 
 from . import _lib
 from .fast_weight import _fwp_torch, fast_weight_delta
+from .selective_scan import causal_conv, residual_norm, selective_scan
 
 
 def _untouched(m, cls):
@@ -334,3 +335,87 @@ class DeltaNetDecoderLayer(nn.Module):
             out, new_mem = out
             return self.pos_ff(out), new_mem
         return self.pos_ff(out)
+
+
+class SelectiveScanLayer(nn.Module):
+    """The mixer of a selective state space block, beside :class:`DeltaNetLayer`: ``h`` is ``[len, bsz, d_model]``, one projection gives the
+    values and their gate (``expand * d_model`` channels each), the values go through a :func:`causal_conv` of ``taps`` taps, another
+    projection of the result gives q and k (``n_state`` each, shared by all channels) and the step sizes by way of ``rank`` numbers, and
+    :func:`selective_scan` and a projection back follow.  No norm and no residual: those are the block's.
+
+    ``mems`` is the pair (``W[bsz, 1, n_state, channels]``, the convolution's last rows ``[bsz, 1, taps - 1, channels]``); with
+    ``carry_over_fast_weight`` the call returns ``(output, mems)``.  ``lengths`` (int64 ``[bsz]``) marks a padded batch.  No counterpart in the reference.
+    """
+
+    def __init__(self, d_model, n_state=16, taps=4, expand=2, rank=None, dropout=0.0):
+        super().__init__()
+        self.d_model, self.n_state, self.taps, self.channels = d_model, n_state, taps, expand * d_model
+        self.rank = rank or -(-d_model // 16)
+        self.in_net = Linear(d_model, 2 * self.channels)
+        self.conv_weight = nn.Parameter(torch.empty(1, self.channels, taps))
+        self.conv_bias = nn.Parameter(torch.empty(1, self.channels))
+        self.step_net = Linear(self.channels, self.rank + 2 * n_state)
+        self.delta_net = nn.Linear(self.rank, self.channels, bias=False)
+        self.delta_bias = nn.Parameter(torch.empty(1, self.channels))
+        self.log_decay = nn.Parameter(torch.empty(1, n_state, self.channels))
+        self.skip = nn.Parameter(torch.empty(1, self.channels))
+        self.o_net = Linear(self.channels, d_model)
+        self.drop = nn.Dropout(dropout)
+        self.reset_scan_parameters()
+
+    def reset_scan_parameters(self):
+        """Decays of 1 .. n_state at step size 1, step sizes spread from 0.001 to 0.1 over the channels."""
+        with torch.no_grad():
+            self.conv_weight.uniform_(-1, 1).mul_(self.taps ** -0.5)
+            self.conv_bias.zero_()
+            self.log_decay.copy_(torch.arange(1.0, self.n_state + 1, device=self.log_decay.device).log()[None, :, None].expand_as(self.log_decay))
+            self.skip.fill_(1.0)
+            step = torch.logspace(-3, -1, self.channels, device=self.delta_bias.device)
+            self.delta_bias.copy_(step + torch.log(-torch.expm1(-step)))
+
+    def forward(self, h, attn_mask=None, mems=None, carry_over_fast_weight=False, lengths=None):
+        if mems is not None and not carry_over_fast_weight:
+            raise ValueError("mems are only meaningful with carry_over_fast_weight=True")
+        slen, bsz, _ = h.shape
+        rows = lambda t: t.view(slen, bsz, 1, -1).permute(1, 2, 0, 3)       # [bsz, 1, slen, .], the steps outermost in memory
+        steps = lambda t: t.permute(2, 0, 1, 3).reshape(slen, bsz, -1)      # and back, a view
+        x, z = (rows(t) for t in self.in_net(h).split(self.channels, -1))
+        if not carry_over_fast_weight:
+            W = state = None
+        elif mems is None:
+            W = torch.zeros(bsz, 1, self.n_state, self.channels, device=h.device)
+            state = torch.zeros(bsz, 1, self.taps - 1, self.channels, device=h.device, dtype=x.dtype)
+        else:       # the last batch of an epoch may be smaller than the carried state
+            W, state = mems[0][:bsz].clone(), mems[1][:bsz].to(x.dtype, copy=True)
+        v = causal_conv(x, self.conv_weight, self.conv_bias, state, silu=True, lengths=lengths)
+        rank, q, k = self.step_net(steps(v)).split((self.rank, self.n_state, self.n_state), -1)
+        out = selective_scan(rows(q), rows(k), v, rows(self.delta_net(rank)), -torch.exp(self.log_decay), W, D=self.skip, Z=z,
+                             delta_bias=self.delta_bias, softplus=True, lengths=lengths)
+        out = self.drop(self.o_net(steps(out)))
+        return (out, (W, state)) if carry_over_fast_weight else out
+
+
+class SelectiveScanDecoderLayer(nn.Module):
+    """A :class:`SelectiveScanLayer` and the feed-forward block behind it on a residual stream: norm, mixer, norm and scale on its output, and
+    the same around the feed-forward block; :func:`residual_norm` is what lies between and behind the two.  Constructor and call as
+    :class:`DeltaNetDecoderLayer`'s, whose place it takes in :class:`DeltaNetLM`; heads do not count here (q and k are shared by all
+    channels), and norms come before a block whatever ``pre_lnorm``."""
+
+    def __init__(self, n_head, d_model, d_head, d_inner, dropout=0.0, dropatt=0.0, pre_lnorm=True, layer_id=None, num_layer=None,
+                 fast_weight_op=None, n_state=16, taps=4):
+        super().__init__()
+        if fast_weight_op is not None:
+            raise ValueError("a selective scan layer has its own operator")
+        self.dec_attn = SelectiveScanLayer(d_model, n_state, taps, dropout=dropout)
+        self.norm_in, self.norm_mid = nn.LayerNorm(d_model), nn.LayerNorm(d_model)
+        self.norm_attn, self.norm_ff = nn.LayerNorm(d_model), nn.LayerNorm(d_model)
+        self.scale_attn, self.scale_ff = nn.Parameter(torch.ones(d_model)), nn.Parameter(torch.ones(d_model))
+        self.ff = nn.Sequential(Linear(d_model, d_inner), nn.ReLU(), nn.Dropout(dropout), Linear(d_inner, d_model), nn.Dropout(dropout))
+
+    def forward(self, dec_inp, dec_attn_mask=None, mems=None, carry_over_fast_weight=False, lengths=None):
+        pair = lambda norm: (norm.weight, norm.bias)
+        out = self.dec_attn(_layer_norm(self.norm_in, dec_inp), mems=mems, carry_over_fast_weight=carry_over_fast_weight, lengths=lengths)
+        out, mems = out if carry_over_fast_weight else (out, None)
+        r, n = residual_norm(out, dec_inp, after=pair(self.norm_attn), scale=self.scale_attn, before=pair(self.norm_mid), eps=self.norm_mid.eps)
+        r, _ = residual_norm(self.ff(n), r, after=pair(self.norm_ff), scale=self.scale_ff, eps=self.norm_ff.eps)
+        return (r, mems) if carry_over_fast_weight else r

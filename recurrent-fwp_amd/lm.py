@@ -54,20 +54,21 @@ class DeltaNetLM(nn.Module):
     """``forward(data, target, *mems, carry_over_fast_weight=False)`` with ``data`` and
     ``target`` of shape ``[len, bsz]`` (int64) returns ``[loss]`` or, when the fast
     weights are carried, ``[loss, mem_0, ..., mem_{n_layer-1}]``; ``loss`` is
-    ``[len, bsz]`` and each ``mem_i`` is the pair ``(W[bsz,H,D,D], None)`` the layers take.
+    ``[len, bsz]`` and each ``mem_i`` is the pair ``(W[bsz,H,D,D], None)`` the layers take.  ``decoder_layer`` replaces the
+    layers' class (``SelectiveScanDecoderLayer``, whose ``mem_i`` are its own pairs).
     """
 
     def __init__(self, n_token, n_layer, n_head, d_model, d_head, d_inner, dropout=0.0,
                  dropatt=0.0, pre_lnorm=False, tie_weight=True, clamp_len=-1, init_std=0.02,
-                 fast_weight_op=None):
+                 fast_weight_op=None, decoder_layer=DeltaNetDecoderLayer):
         super().__init__()
         self.n_token, self.n_layer, self.d_model, self.clamp_len = n_token, n_layer, d_model, clamp_len
         self.word_emb = _WordEmbedding(n_token, d_model)
         self.pos_emb = PositionalEmbedding(d_model)
         self.drop = nn.Dropout(dropout)
         self.layers = nn.ModuleList([
-            DeltaNetDecoderLayer(n_head, d_model, d_head, d_inner, dropout, dropatt, pre_lnorm,
-                                 layer_id=i, num_layer=n_layer, fast_weight_op=fast_weight_op)
+            decoder_layer(n_head, d_model, d_head, d_inner, dropout, dropatt, pre_lnorm,
+                          layer_id=i, num_layer=n_layer, fast_weight_op=fast_weight_op)
             for i in range(n_layer)])
         self.crit = _TiedSoftmaxLoss(n_token, d_model)
         self.reset_parameters(init_std)
