@@ -41,7 +41,11 @@ def selective_scan(Q, K, V, delta, A, W=None, D=None, Z=None, delta_bias=None, s
 
 def _weights(norm):
     """(weight, bias) of a norm given as a weight, as such a pair, or not at all."""
-    return tuple(norm) if isinstance(norm, (tuple, list)) else (norm, None)
+    if not isinstance(norm, (tuple, list)):
+        return norm, None
+    if len(norm) != 2:
+        raise _lib.FwpError("a norm is its weight or the pair (weight, bias)")
+    return norm
 
 
 def residual_norm(y, x, after=None, gate=None, scale=None, before=None, eps=1e-5, rms=False, activation=None):
@@ -51,9 +55,8 @@ def residual_norm(y, x, after=None, gate=None, scale=None, before=None, eps=1e-5
     y, x ``[..., cols]``, cols up to 8192; x may be fp32 beside narrower rows, and r has its type.  ``after`` and ``before``: a weight ``[cols]`` or a pair
     (weight, bias), ``None``: no norm there.  The norms are LayerNorms, with ``rms`` divisions by the root mean square.  gate ``[..., cols]`` or
     ``[..., 1]`` through ``activation`` (``None``, ``"sigmoid"``, ``"silu"``); scale ``[cols]``.  Gradients flow to every tensor."""
-    if activation not in _ACTIVATIONS:
+    act = _ACTIVATIONS.get(activation)
+    if act is None:
         raise _lib.FwpError(f"activation must be None, 'sigmoid' or 'silu', got {activation!r}")
-    pairs = [_weights(norm) for norm in (after, before)]
-    if any(len(pair) != 2 for pair in pairs):
-        raise _lib.FwpError("a norm is its weight or the pair (weight, bias)")
-    return _native().residual_norm(y, x, gate, scale, *pairs[0], *pairs[1], eps, rms, _ACTIVATIONS[activation])
+    (aw, ab), (bw, bb) = _weights(after), _weights(before)
+    return _native().residual_norm(y, x, gate, scale, aw, ab, bw, bb, eps, rms, act)
