@@ -14,7 +14,6 @@ namespace fwp {
 namespace {
 
 constexpr int kThreads = 256, kAhead = 8;
-constexpr int64_t kMaxBlocks = (int64_t(1) << 31) - 1;
 
 // How rows lie: kWhole, four channels at a time, aligned for that everywhere; kRagged, any width from four on and any place: the same loads without the
 // alignment, and the thread that the row's end cuts reads its last four and moves them up; kTiny, one channel to a thread.
@@ -325,7 +324,7 @@ void by_kind(const fwp_conv_args &a, int lie, F f) {
 int conv_fwd(const fwp_conv_args &a, void *state, fwp_out_rows y, hipStream_t s) {
     const int lie = lie_of(a, {a.x, {y.ptr, y.sN, y.sH, y.sL}}, state);
     const Tiling g(a.N, a.H, a.L, a.D, a.K, width_of(lie), false);
-    if (g.grid(a.N, a.H) > kMaxBlocks) return FWP_E_SHAPE;
+    if (!fits_launch(g.grid(a.N, a.H), kThreads)) return FWP_E_SHAPE;
     const dim3 grid((unsigned)g.grid(a.N, a.H));
     by_kind(a, lie, [&](auto t, auto k, auto l) {
         using T = decltype(t);
@@ -343,7 +342,7 @@ int conv_bwd(const fwp_conv_args &a, const void *state, fwp_rows gy, fwp_out_row
     const int lie = lie_of(a, {a.x, gy, {gx.ptr, gx.sN, gx.sH, gx.sL}}, state);
     const Tiling g(a.N, a.H, a.L, a.D, a.K, width_of(lie), true);
     const int64_t param_blocks = ((int64_t)a.H * (a.K + 1) * a.D + 15) / 16;
-    if (g.grid(a.N, a.H) > kMaxBlocks || param_blocks > kMaxBlocks) return FWP_E_SHAPE;
+    if (!fits_launch(g.grid(a.N, a.H), kThreads) || !fits_launch(param_blocks, 1024)) return FWP_E_SHAPE;
     const dim3 grid((unsigned)g.grid(a.N, a.H));
     by_kind(a, lie, [&](auto t, auto k, auto l) {
         using T = decltype(t);

@@ -58,6 +58,13 @@ __device__ __forceinline__ float softplus(float x) {
 // its slope, the sigmoid, from the same u
 __device__ __forceinline__ float softplus_slope(float x, float u) { return (x < 0.f ? u : 1.f) * __builtin_amdgcn_rcpf(1.f + u); }
 
+// An infinite decay as the largest finite one: exp(dt A) is 0 (or infinite) all the same for every dt from 1e-36 on, and 1, not NaN, for the dt of zero that rows
+// behind a sequence have.
+__device__ __forceinline__ float within_range(float x) {
+    constexpr float most = 3.402823466e38f;
+    return x < -most ? -most : x > most ? most : x;      // NaN stays
+}
+
 // The steps of sequence n that count
 __device__ __forceinline__ int length_of(const int64_t *lengths, int n, int L) {
     if (!lengths) return L;
@@ -79,6 +86,9 @@ int conv_fwd(const fwp_conv_args &a, void *state, fwp_out_rows y, hipStream_t s)
 int64_t conv_workspace(int N, int H, int L, int D, int K);
 int conv_bwd(const fwp_conv_args &a, const void *state, fwp_rows gy, fwp_out_rows gx, float *gweight, float *gbias, float *workspace,
              hipStream_t s);
+
+// A launch has fewer than 2^32 threads.
+inline bool fits_launch(int64_t blocks, int threads) { return blocks <= (int64_t(1) << 32) / threads - 1; }
 
 // Elements between the steps of a view that the scan takes: sixteen steps and a row then lie within 32 bits of bytes.
 constexpr int64_t kScanMaxStep = 1 << 25;

@@ -20,7 +20,6 @@ namespace fwp {
 namespace {
 
 constexpr int kParams = 5;
-constexpr int64_t kMaxBlocks = (int64_t(1) << 31) - 1;
 
 template <typename T>
 struct alignas(4 * sizeof(T)) Four {
@@ -227,7 +226,7 @@ __global__ __launch_bounds__(threads_of(WAVES)) void k_rnorm_fwd(fwp_norm_args a
         sr = statistics<LIE, WAVES, NV>(r, a.rms, a.cols, a.eps, lane, sh, turn);
 #pragma unroll
         for (int i = 0; i < NV; i++) {
-                float w[4], b[4], o[4];
+            float w[4], b[4], o[4];
             param4<LIE, WAVES>(w, a.before_weight, 1.f, lane, i, a.cols);
             param4<LIE, WAVES>(b, a.before_bias, 0.f, lane, i, a.cols);
 #pragma unroll
@@ -403,7 +402,7 @@ __global__ __launch_bounds__(threads_of(WAVES)) void k_rnorm_bwd(fwp_norm_args a
         for (int i = 0; i < NV; i++) {
             float o[4];
 #pragma unroll
-            for (int k = 0; k < 4; k++) o[k] = st.y * fmaf(-y.x[i][k], n1, h.x[i][k] - n0);
+            for (int k = 0; k < 4; k++) o[k] = after ? st.y * fmaf(-y.x[i][k], n1, h.x[i][k] - n0) : h.x[i][k];      // without a norm, not infinity times zero
             store4<LIE, WAVES>(gy + at, o, lane, i, a.cols);
         }
     }
@@ -523,18 +522,24 @@ int64_t residual_norm_workspace(int rows, int cols) { return (int64_t)blocks_of(
 int residual_norm_fwd(const fwp_norm_args &a, void *r, void *n, float *stats, hipStream_t s) {
     const bool whole = whole_rows(a, {a.y, a.gate_rows ? nullptr : a.gate, n}, {a.x, r},
                                   {a.scale, a.after_weight, a.after_bias, a.before_weight, a.before_bias});
+    int rc = 0;
     by_types(a, [&](auto t, auto st) {
         using T = decltype(t);
         using S = decltype(st);
         by_width(a.cols, [&](auto w, auto v) {
             constexpr int WAVES = decltype(w)::value, NV = decltype(v)::value;
-            const dim3 grid((unsigned)(((int64_t)a.rows + rows_at_once(WAVES) - 1) / rows_at_once(WAVES))), block(threads_of(WAVES));
+            const int64_t blocks = ((int64_t)a.rows + rows_at_once(WAVES) - 1) / rows_at_once(WAVES);
+            if (!fits_launch(blocks, threads_of(WAVES))) {
+                rc = FWP_E_SHAPE;
+                return;
+            }
+            const dim3 grid((unsigned)blocks), block(threads_of(WAVES));
             if (whole) hipLaunchKernelGGL((k_rnorm_fwd<T, S, WAVES, NV, kWhole>), grid, block, 0, s, a, (S *)r, (T *)n, stats);
             else if (a.cols >= 4) hipLaunchKernelGGL((k_rnorm_fwd<T, S, WAVES, NV, kRagged>), grid, block, 0, s, a, (S *)r, (T *)n, stats);
             else hipLaunchKernelGGL((k_rnorm_fwd<T, S, 1, 1, kTiny>), grid, block, 0, s, a, (S *)r, (T *)n, stats);
         });
     });
-    return (int)hipGetLastError();
+    return rc ? rc : (int)hipGetLastError();
 }
 
 int residual_norm_bwd(const fwp_norm_args &a, const float *stats, const void *gr, const void *gn, const fwp_norm_grads &g, float *workspace,

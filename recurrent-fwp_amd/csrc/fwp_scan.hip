@@ -19,6 +19,7 @@
 #include "fwp_wave.hpp"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace fwp {
 namespace {
@@ -97,7 +98,7 @@ __device__ __forceinline__ void load_decays(float (&a)[S], const float *A, const
 #pragma unroll
     for (int s = 0; s < S; s++) {
         const int e = S * p.wave + s;
-        a[s] = p.live && e < d.E ? A[p.state(d, p.h, e)] * kLog2e : 0.f;
+        a[s] = p.live && e < d.E ? within_range(A[p.state(d, p.h, e)] * kLog2e) : 0.f;
     }
 }
 template <int S>
@@ -170,20 +171,37 @@ struct Keys {
     }
 };
 
+// Where a state has fewer rows than the waves (not FULL), the others hold zeros, whatever values meet their k and q of zero: an infinite value then
+// gives infinity, not infinity times zero.  2 us of 47 (30 x 8 heads of 391 steps, 11 x 49); the adjoint, where it would be 12 of 120, goes without: gradients that meet
+// an infinity may be NaN.
+template <int S, bool FULL>
+struct Existing {
+    int mask[S];
+    __device__ __forceinline__ Existing(const Dims &d, const Place &p) {
+#pragma unroll
+        for (int s = 0; s < S; s++) mask[s] = __builtin_amdgcn_readfirstlane(S * p.wave + s < d.E ? -1 : 0);
+    }
+    __device__ __forceinline__ float operator()(float x, int s) const { return FULL ? x : __int_as_float(__float_as_int(x) & mask[s]); }
+};
+
 // The parameters of a channel that the threads which load its rows need
 struct Channel {
     float D, bias;
+    int has_D;
     __device__ __forceinline__ Channel(const fwp_scan_args &a, const Place &p) {
         const int64_t at = (int64_t)p.h * a.M + p.m;
         D = p.live && a.D ? a.D[at] : 0.f;
         bias = p.live && a.delta_bias ? a.delta_bias[at] : 0.f;
+        has_D = __builtin_amdgcn_readfirstlane(a.D ? -1 : 0);
     }
+    // D x, or 0 for any x without D
+    __device__ __forceinline__ float skip(float x) const { return D * __int_as_float(__float_as_int(x) & has_D); }
 };
 
 // ------------------------------------------------------------------ forward
 
-// LOCAL: only the state after the segment, from zeros, and the segment's sum of dt; otherwise the scan
-template <typename T, int WAVES, int S, bool LOCAL>
+// LOCAL: only the state after the segment, from zeros, and the segment's sum of dt; otherwise the scan.  FULL: every row of every wave is one of the state's.
+template <typename T, int WAVES, int S, bool LOCAL, bool FULL>
 __global__ __launch_bounds__(64 * WAVES) void k_scan_fwd(fwp_scan_args a, Dims d, const float *init, float *W, float *__restrict__ saved,
                                                          float *__restrict__ sums, fwp_out_rows out) {
     constexpr int TILE = 16, ROWS = (TILE + WAVES - 1) / WAVES, KEEP = tile_of(WAVES);
@@ -198,6 +216,7 @@ __global__ __launch_bounds__(64 * WAVES) void k_scan_fwd(fwp_scan_args a, Dims d
     Column<const T> V(a.v, p, d, first), DT(a.delta, p, d, first), Z(gated ? a.z : a.v, p, d, first);
     Column<T> O(LOCAL ? fwp_out_rows{(void *)a.v.ptr, 0, 0, 0} : out, p, d, first);
     K keys(a.k, a.q, p, d, first);
+    const Existing<S, FULL> keep(d, p);
     float decay[S], state[S], sum = 0.f;
     load_decays(decay, a.A, d, p);
     load_states(state, LOCAL ? nullptr : init, (int64_t)p.nh * d.segments + p.seg, d, p);
@@ -222,7 +241,7 @@ __global__ __launch_bounds__(64 * WAVES) void k_scan_fwd(fwp_scan_args a, Dims d
             if (a.softplus) x = softplus(x);
             x = in ? x : 0.f;
             const float vs = in ? (float)v[j] : 0.f;
-            dv[j] = ch.D * vs;
+            dv[j] = ch.skip(vs);
             gate[j] = gated ? silu((float)z[j], sigmoid((float)z[j])) : 1.f;
             if (r < TILE) sx[r][p.lane] = make_float2(x, x * vs);
         }
@@ -239,7 +258,7 @@ __global__ __launch_bounds__(64 * WAVES) void k_scan_fwd(fwp_scan_args a, Dims d
             float y = 0.f;
 #pragma unroll
             for (int s = 0; s < S; s++) {
-                state[s] = fmaf(__builtin_amdgcn_exp2f(x.x * decay[s]), state[s], x.y * k[s]);
+                state[s] = keep(fmaf(__builtin_amdgcn_exp2f(x.x * decay[s]), state[s], x.y * k[s]), s);
                 if constexpr (!LOCAL) y = fmaf(q[s], state[s], y);
             }
             if constexpr (LOCAL) sum += x.x;
@@ -279,7 +298,7 @@ __global__ __launch_bounds__(256) void k_chain(const float *__restrict__ A, cons
     if (i >= (int64_t)d.N * d.H * per) return;
     const int64_t nh = i / per, em = i % per;
     const int m = (int)(em % d.M);
-    const float half = 0.5f * kLog2e * A[(nh % d.H) * per + em];
+    const float half = within_range(0.5f * kLog2e * A[(nh % d.H) * per + em]);
     float x = W_in ? W_in[i] : 0.f;
     constexpr int AHEAD = 8;
     for (int s0 = 0; s0 < d.segments; s0 += AHEAD) {
@@ -297,7 +316,7 @@ __global__ __launch_bounds__(256) void k_chain(const float *__restrict__ A, cons
             const int seg = REVERSE ? d.segments - 1 - (s0 + j) : s0 + j;
             own[(nh * d.segments + seg) * per + em] = x;
             const float e = __builtin_amdgcn_exp2f(half * dt[j]);
-            x = fmaf(e, e * x, o[j]);
+            x = x == 0.f ? o[j] : fmaf(e, e * x, o[j]);       // nothing grows out of nothing, however large exp(A sum dt)
         }
     }
     if (W_out) W_out[i] = x;
@@ -669,7 +688,7 @@ __global__ __launch_bounds__(256) void k_scan_step(fwp_scan_args a, float *__res
 #pragma unroll
             for (int i = 0; i < V; i++) {
                 const float x = dt[i] * v[i] * ks[j];
-                st[j].x[i] = w ? fmaf(exp_of(dt[i] * al[j].x[i]), st[j].x[i], x) : x;
+                st[j].x[i] = w ? fmaf(exp_of(dt[i] * within_range(al[j].x[i])), st[j].x[i], x) : x;
                 y.x[i] = fmaf(qs[j], st[j].x[i], y.x[i]);
             }
             if (w && live) *reinterpret_cast<Floats<V> *>(w + e * rows) = st[j];
@@ -701,8 +720,6 @@ void by_waves(const Plan &p, F f) {
     else f(integral_constant<int, 8>(), integral_constant<int, 4>());
 }
 
-constexpr int64_t kMaxBlocks = (int64_t(1) << 31) - 1;
-
 }  // namespace
 
 int64_t scan_saved_floats(int N, int H, int L, int E, int M) {
@@ -722,7 +739,7 @@ int scan_fwd(const fwp_scan_args &a, float *W, fwp_out_rows out, float *saved, f
                           (int64_t)a.N * a.H * a.M >= 1 << 18;
         const int across = four ? 256 : 64;
         const int64_t grid = (int64_t)a.N * a.H * ((a.M + across - 1) / across);
-        if (grid > kMaxBlocks) return FWP_E_SHAPE;
+        if (!fits_launch(grid, 256)) return FWP_E_SHAPE;
         by_type(a.type, [&](auto t) {
             using T = decltype(t);
             if (four) hipLaunchKernelGGL((k_scan_step<T, 4>), dim3((unsigned)grid), dim3(256), 0, s, a, W, out);
@@ -731,7 +748,7 @@ int scan_fwd(const fwp_scan_args &a, float *W, fwp_out_rows out, float *saved, f
         return (int)hipGetLastError();
     }
     const Plan p(a.N, a.H, a.L, a.E, a.M, false);
-    if (p.grid() > kMaxBlocks || (p.states + 255) / 256 > kMaxBlocks) return FWP_E_SHAPE;
+    if (!fits_launch(p.grid(), 64 * p.waves) || (p.segments > 1 && !fits_launch((p.states + 255) / 256, 256))) return FWP_E_SHAPE;
     if (p.segments > 1 && !workspace) return FWP_E_NULL;
     float *const seg = workspace, *const sums = seg + p.states * p.segments;
     const Dims d = p;
@@ -741,11 +758,15 @@ int scan_fwd(const fwp_scan_args &a, float *W, fwp_out_rows out, float *saved, f
             constexpr int WAVES = decltype(w)::value, S = decltype(r)::value;
             const dim3 grid((unsigned)p.grid()), block(64 * WAVES);
             if (p.segments > 1) {
-                hipLaunchKernelGGL((k_scan_fwd<T, WAVES, S, true>), grid, block, 0, s, a, d, nullptr, seg, nullptr, sums, out);
+                hipLaunchKernelGGL((k_scan_fwd<T, WAVES, S, true, true>), grid, block, 0, s, a, d, nullptr, seg, nullptr, sums, out);
                 hipLaunchKernelGGL((k_chain<false>), dim3((unsigned)((p.states + 255) / 256)), dim3(256), 0, s, a.A, sums, seg, W, W, d);
             }
-            hipLaunchKernelGGL((k_scan_fwd<T, WAVES, S, false>), grid, block, 0, s, a, d, p.segments > 1 ? seg : W,
-                               p.segments > 1 ? nullptr : W, saved, nullptr, out);
+            const auto scan = [&](auto full) {
+                hipLaunchKernelGGL((k_scan_fwd<T, WAVES, S, false, decltype(full)::value>), grid, block, 0, s, a, d, p.segments > 1 ? seg : W,
+                                   p.segments > 1 ? nullptr : W, saved, nullptr, out);
+            };
+            if (p.E == WAVES * S) scan(std::true_type());
+            else scan(std::false_type());
         });
     });
     return (int)hipGetLastError();
@@ -756,8 +777,8 @@ int scan_bwd(const fwp_scan_args &a, const float *saved, fwp_rows gout, fwp_out_
     const Plan p(a.N, a.H, a.L, a.E, a.M, true);
     const int64_t row_blocks = (p.heads * a.L * p.waves * 2 * p.rows + 255) / 256,
                   param_blocks = ((int64_t)a.H * (a.E + 2) * a.M + 63) / 64;
-    if (p.grid() > kMaxBlocks || row_blocks + param_blocks > kMaxBlocks || (p.states + 255) / 256 > kMaxBlocks ||
-        (int64_t)a.N * p.segments > kMaxBlocks)
+    if (!fits_launch(p.grid(), 64 * p.waves) || !fits_launch(row_blocks + param_blocks, 256) ||
+        (p.segments > 1 && !fits_launch((p.states + 255) / 256, 256)))
         return FWP_E_SHAPE;
     float *const parts = workspace, *const params = parts + p.blocks_m * p.heads * p.padded * p.waves * 2 * p.rows,
                 *const seg = params + (int64_t)a.N * p.segments * a.H * (a.E + 2) * a.M, *const sums = seg + p.states * p.segments;

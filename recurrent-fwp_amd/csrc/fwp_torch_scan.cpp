@@ -295,8 +295,8 @@ struct ResidualNormFn : torch::autograd::Function<ResidualNormFn> {
         const at::Tensor g = given(gate_in);
         if (y_in.dim() < 1 || x_in.sizes() != y_in.sizes()) misfit("x", x_in, "the shape of y");
         const int64_t cols = y_in.size(-1);
-        require_sizes({cols, y_in.numel()});
-        require_sizes({y_in.numel() / cols});
+        require_sizes({cols});
+        require_sizes({y_in.numel() / cols});      // rows; their elements may be more
         if (cols > 8192) fail("rows of at most 8192 columns, got " + std::to_string(cols));
         type_of(y_in, "y");
         if (x_in.scalar_type() != y_in.scalar_type() && x_in.scalar_type() != at::kFloat) fail("x must be fp32 or have the type of y");

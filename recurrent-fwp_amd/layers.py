@@ -383,7 +383,7 @@ class SelectiveScanLayer(nn.Module):
         if not carry_over_fast_weight:
             W = state = None
         elif mems is None:
-            W = torch.zeros(bsz, 1, self.n_state, self.channels, device=h.device)
+            W = torch.zeros(bsz, 1, self.n_state, self.channels, device=h.device, dtype=torch.float32)
             state = torch.zeros(bsz, 1, self.taps - 1, self.channels, device=h.device, dtype=x.dtype)
         else:       # the last batch of an epoch may be smaller than the carried state
             W, state = mems[0][:bsz].clone(), mems[1][:bsz].to(x.dtype, copy=True)

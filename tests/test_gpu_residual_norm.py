@@ -118,8 +118,8 @@ def test_only_one_of_the_results_is_used(fwp):
 
 
 def test_rows_that_are_not_contiguous_or_aligned(fwp):
-    """Views are the same call as their copies.  Rows and parameters at four bytes from a boundary are read element by element, and their sums are added in
-    another order: each result is within the 128 roundings of its terms, so two of them are within twice that of one another.  The terms of n are at most
+    """Views are the same call as their copies.  Rows and parameters at four bytes from a boundary are
+    read by other loads: each result is within the 128 roundings of its terms, so two of them are within twice that of one another.  The terms of n are at most
     8 here (r below 16 times the spread), those of r 32."""
     g = torch.Generator().manual_seed(1)
     wide = torch.randn(40, 6, 130, generator=g).cuda()
@@ -146,6 +146,42 @@ def test_constant_rows_and_large_means(fwp):
     r, _ = fwp.residual_norm(y, torch.zeros(3, 512).cuda(), after=w)
     want = F.residual_norm(F.double(y), torch.zeros(3, 512, dtype=torch.float64), F.double(w))[0]
     assert float((F.double(r) - want).abs().max()) <= (4096 + 64) * F.EPS32      # the mean is off by a rounding of 4096, the spread is about 5
+
+
+def test_infinite_rows_that_a_gate_masks(fwp):
+    """Without a norm on y the gradients do not pass y's values: where an infinite one is masked away by the caller, gy is as for any other."""
+    g = torch.Generator().manual_seed(4)
+    y, x, gate, gr = (torch.randn(6, 300, generator=g).cuda() for _ in range(4))
+    scale = torch.randn(300, generator=g).cuda()
+    masked = torch.zeros(6, 300, dtype=torch.bool).cuda()
+    masked[1, 7] = masked[4, 299] = masked[5, 0] = True
+    gr = gr.masked_fill(masked, 0)
+    seen = []
+    for fill in (0.0, float("inf"), float("nan")):
+        leaves = [y.masked_fill(masked, fill).requires_grad_(), x.clone().requires_grad_()]
+        r, _ = fwp.residual_norm(leaves[0], leaves[1], gate=gate, scale=scale, activation="sigmoid")
+        seen.append(torch.autograd.grad(r, leaves, gr))
+    for other in seen[1:]:
+        assert all(torch.equal(a, b) for a, b in zip(seen[0], other))
+    assert torch.equal(seen[0][1], gr)
+
+
+def test_more_than_two_to_the_31_elements(fwp):
+    """The last rows of a tensor whose offsets pass 32 bits are as those of a small one."""
+    rows, cols = (1 << 18) + 5, 8192
+    g = torch.Generator().manual_seed(5)
+    few = [torch.randn(4, cols, generator=g).to(torch.bfloat16).cuda() for _ in range(4)]
+    w = torch.randn(cols, generator=g).cuda()
+    y, x, gr, gn = (torch.zeros(rows, cols, dtype=torch.bfloat16, device="cuda") for _ in range(4))
+    for big, small in zip((y, x, gr, gn), few):
+        big[:2], big[-2:] = small[:2], small[2:]
+    results = []
+    for y_, x_, gr_, gn_ in ((y, x, gr, gn), few):
+        y_, x_ = y_.requires_grad_(), x_.requires_grad_()
+        r, n = fwp.residual_norm(y_, x_, after=w, before=w, rms=True)
+        results.append([r.detach(), n.detach(), *torch.autograd.grad([r, n], [y_, x_], [gr_, gn_])])
+    for a, b in zip(*results):
+        assert torch.equal(a[:2], b[:2]) and torch.equal(a[-2:], b[2:])
 
 
 def test_a_captured_step_beside_eager_work(fwp):

@@ -238,6 +238,113 @@ def test_infinities_and_nan_go_where_they_belong(fwp):
     assert torch.equal(slope.flatten().cpu(), torch.tensor([0.0, 1.0, 0.0, 1.0]))
 
 
+def test_infinite_values_without_a_skip(fwp):
+    """No D is no term at all, not zero times the value."""
+    t = {k: torch.rand(1, 1, 30, n, generator=torch.Generator().manual_seed(7)).cuda() + 0.1 for k, n in (("Q", 5), ("K", 5), ("V", 3), ("delta", 3))}
+    t["V"][0, 0, 10, 1] = float("inf")
+    out = fwp.selective_scan(**t, A=-torch.ones(1, 5, 3).cuda())
+    want = torch.zeros(30, 3, dtype=torch.bool).cuda()
+    want[10:, 1] = True
+    assert torch.equal(torch.isposinf(out[0, 0]), want) and not torch.isnan(out).any()
+
+
+@pytest.mark.parametrize("E,L", [(4, 1), (4, 300), (16, 300), (40, 700)])
+def test_entries_that_forget_at_once(fwp, E, L):
+    """A decay of minus infinity is exp(..) = 0 for every step that there is and changes nothing behind a sequence's end: the formula with -1e30, whose
+    products with the steps (above 1e-3) are as far below the smallest exponent."""
+    g = torch.Generator().manual_seed(E + L)
+    t = scan_inputs(g, torch.float32, 3, 1, L, E, 20, "plain", True, True)
+    forgets = (torch.rand(1, E, 20, generator=g) < 0.3).cuda()
+    n = torch.tensor([L, L // 2, 0]).cuda()
+    want, size = (formulas({**t, "A": t["A"].masked_fill(forgets, -1e30)}, True, n, absolute=a) for a in (False, True))
+    W = t["W"].clone()
+    t["A"] = t["A"].masked_fill(forgets, float("-inf"))
+    with torch.no_grad():
+        out = fwp.selective_scan(**t, softplus=True, lengths=n)
+    check(out, want[0], size[0], 4 * L + E + 64, "out", torch.float32)
+    check(t["W"], want[1], size[1], 4 * L + E + 64, "W", torch.float32)
+    names = ["Q", "K", "V", "delta", "A", "D", "Z", "delta_bias"]
+    for k in names:
+        t[k] = t[k].detach().requires_grad_()
+    out = fwp.selective_scan(**{**t, "W": W}, softplus=True, lengths=n)
+    grads = torch.autograd.grad(out, [t[k] for k in names], torch.ones_like(out))
+    assert all(torch.isfinite(x).all() for x in grads) and not grads[4][forgets].any()
+
+
+def test_growth_of_nothing(fwp):
+    """Steps below zero make the state grow, here by exp(256) and more over a part of the sequence that is worked on by itself: a state of zero stays one."""
+    g = torch.Generator().manual_seed(14)
+    L, E, M = 2048, 4, 8
+    t = scan_inputs(g, torch.float32, 1, 1, L, E, M, "plain", False, True)
+    t["A"], t["delta_bias"], t["delta"] = -torch.ones(1, E, M).cuda(), None, torch.full((1, 1, L, M), -2.0).cuda()
+    t["V"][:, :, :-5] = 0
+    go = randn(g, 1, 1, L, M).cuda()
+    go[:, :, 3:-5] = 0
+    want, size = formulas(t, False, None, go), formulas(t, False, None, go, absolute=True)
+    names = ["Q", "K", "V", "delta", "A", "D", "Z"]
+    go[:, :, -5:] = 0       # whose gradient would grow without bound on the way back
+    want = want[:2] + formulas(t, False, None, go)[2:]
+    size = size[:2] + formulas(t, False, None, go, absolute=True)[2:]
+    for k in names:
+        t[k] = t[k].detach().requires_grad_()
+    out = fwp.selective_scan(**t)
+    check(out, want[0], size[0], 4 * 5 + E + 64, "out", torch.float32)      # five steps from the first value on
+    for k, got, i in zip(names, torch.autograd.grad(out, [t[k] for k in names], go), range(2, 9)):
+        check(got, want[i], size[i], 8 * 5 + 2 * E + M + 128, "gradient of " + k, torch.float32)
+
+
+def test_any_of_the_gradients_alone(fwp):
+    g = torch.Generator().manual_seed(15)
+    t = scan_inputs(g, torch.float32, 2, 1, 50, 16, 40, "steps", False, True)
+    t["w"], t["b"] = randn(g, 1, 40, 4).cuda(), randn(g, 1, 40).cuda()
+    go = randn(g, 2, 1, 50, 40).cuda()
+    names = ["Q", "K", "V", "delta", "A", "D", "Z", "delta_bias", "w", "b"]
+
+    def gradients(of):
+        u = {k: x if x is None else x.detach().requires_grad_(k in of) for k, x in t.items()}
+        w, b = u.pop("w"), u.pop("b")
+        out = fwp.selective_scan(**{**u, "V": fwp.causal_conv(u["V"], w, b, silu=True)}, softplus=True)
+        return torch.autograd.grad(out, [{**u, "w": w, "b": b}[k] for k in of], go)
+
+    for k, want in zip(names, gradients(names)):
+        assert torch.equal(gradients([k])[0], want), k
+
+
+def test_rows_shared_by_heads(fwp):
+    """One q and k for all heads, as views that repeat them: their gradients are the sums over the heads (two roundings)."""
+    g = torch.Generator().manual_seed(16)
+    t = scan_inputs(g, torch.float32, 2, 3, 60, 16, 30, "plain", False, True)
+    q, k = randn(g, 2, 1, 60, 16).cuda().requires_grad_(), randn(g, 2, 1, 60, 16).cuda().requires_grad_()
+    go = randn(g, 2, 3, 60, 30).cuda()
+    each = [x.detach().repeat(1, 3, 1, 1).requires_grad_() for x in (q, k)]
+    a = fwp.selective_scan(**{**t, "Q": q.expand(2, 3, 60, 16), "K": k.expand(2, 3, 60, 16)}, softplus=True)
+    b = fwp.selective_scan(**{**t, "Q": each[0], "K": each[1]}, softplus=True)
+    assert torch.equal(a, b)
+    for got, want in zip(torch.autograd.grad(a, [q, k], go), torch.autograd.grad(b, each, go)):
+        assert float(((got - want.sum(1, keepdim=True)).abs() - 4 * F.EPS32 * want.abs().sum(1, keepdim=True)).max()) <= 0
+
+
+def test_in_inference_mode(fwp):
+    g = torch.Generator().manual_seed(17)
+    t = scan_inputs(g, torch.bfloat16, 2, 1, 30, 16, 64, "steps", True, True)
+    w, state = randn(g, 1, 64, 4).cuda(), torch.zeros(2, 1, 3, 64, dtype=torch.bfloat16).cuda()
+
+    def block(u, state):
+        v = fwp.causal_conv(u["V"], w, None, state, silu=True)
+        out = fwp.selective_scan(**{**u, "V": v}, softplus=True)
+        return [out, *(x for x in fwp.residual_norm(out, u["Z"], after=w[0, :, 0], before=w[0, :, 1]) if x is not None), u["W"], state]
+
+    with torch.no_grad():
+        want = block({**t, "W": t["W"].clone()}, state.clone())
+    W0 = t["W"].clone()
+    with torch.inference_mode():        # states made here and outside
+        inside = block({**t, "W": t["W"].clone()}, state.clone())
+        outside = block(t, state)
+    for a, b, c in zip(want, inside, outside):
+        assert torch.equal(a, b) and torch.equal(a, c)
+    assert not torch.equal(W0, t["W"])
+
+
 def test_the_same_call_gives_the_same_bits(fwp):
     g = torch.Generator().manual_seed(8)
     t = scan_inputs(g, torch.bfloat16, 3, 1, 400, 16, 200, "steps", False, True)

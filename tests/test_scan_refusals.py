@@ -101,6 +101,13 @@ def test_c_entry_points_refuse_before_any_launch(fwp):
         assert lib.fwp_residual_norm_fwd(norm(**bad), p, p, None, None) == E_SHAPE, bad
     assert lib.fwp_residual_norm_bwd(norm(), None, p, p, ctypes.byref(L.NormGrads(gy=4096, gx=4096)), p, None) == E_NULL
     assert lib.fwp_residual_norm_workspace(4, 8193) == E_SHAPE
+    # 2^32 threads are more than a launch has: 256 or 512 to a sequence (or four rows), 32 numbers of gq and gk to a step
+    assert lib.fwp_conv_fwd(conv(N=1 << 24, L=1), p, out, None) == E_SHAPE
+    assert lib.fwp_conv_bwd(conv(N=1 << 24), p, v, out, p, p, p, None) == E_SHAPE
+    assert lib.fwp_scan_fwd(scan(N=1 << 24, L=1), p, out, None, None, None) == E_SHAPE
+    assert lib.fwp_scan_fwd(scan(N=1 << 23), p, out, p, p, None) == E_SHAPE
+    assert lib.fwp_scan_bwd(scan(N=1 << 15, L=1 << 13), p, v, out, out, out, out, none, p, p, p, p, None) == E_SHAPE
+    assert lib.fwp_residual_norm_fwd(norm(rows=1 << 26), p, p, None, None) == E_SHAPE
 
 
 def test_formulas_against_differences():
