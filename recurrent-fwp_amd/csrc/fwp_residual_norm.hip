@@ -9,7 +9,8 @@
 // A row is read once and stays in registers: one wave to a row of up to 1024 columns, 4, 8 or 16 waves to wider ones, four neighbouring
 // columns a lane and turn.  Means and variances (of the differences from the mean) are sums over the lanes by DPP and row exchanges, and over waves by way
 // of LDS.  The backward pass forms r again from y, x and the gate; its workgroups go over many rows and keep the column sums in registers, and a
-// second kernel adds the workgroups' sums in a fixed order.  Bound by memory.
+// second kernel adds the workgroups' sums in a fixed order.  Bound by memory: 32768 x 256 fp32 with a gate, forward 33 us (168 MB, 5.1 TB/s), adjoint 51 (268 MB, 5.2 TB/s)
+// and its sums 5; 16384 x 4096 bf16 on an fp32 stream, RMS, 144 us (0.81 GB, 5.6 TB/s), 225-249 (1.2 GB, 4.8-5.4 TB/s) and 8.
 #include "fwp_elements.hpp"
 #include "fwp_wave.hpp"
 
