@@ -21,8 +21,8 @@
 // the slots of four), a quarter of the rest the sums over the lanes, the other half the softplus, the gate and their slopes.  The vector pipes are at work 56 % of the
 // forward and 69 % of the adjoint's time, with two waves a SIMD (the adjoint's LDS leaves no room for more), LDS another 12-14 %.  Without the sums over the lanes the
 // adjoint's 603 us were 543, without softplus and gate 509, with one wave's part instead of eight's 568, without exponentials 583, without k and q from LDS 555.
-// Not kept: k and q by scalar loads (297 us forward, 186 from LDS at that stage), tiles of 8 steps with one barrier (149 us against 125) or of 32 (128), k and
-// q held in registers between the adjoint's two sweeps (585 against 596 us, spills at 32 rows).
+// Not kept: k and q by scalar loads (297 us forward, 186 from LDS at that stage), tiles of 8 steps with one barrier (149 us against 125) or of 32 (128), one barrier
+// and all of a tile's LDS twice (158 against 140 us), steps and values held in registers between the adjoint's two sweeps as k and q are (no change).
 //
 // One long prompt, 8192 steps of 1024 channels, bf16, 32 segments: 33 + 7 + 47 us.
 #include "fwp_elements.hpp"
@@ -474,12 +474,19 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_scan_bwd(fwp_scan_args a, Dim
         turn();
         if (t0 > first) fetch(t0 - TILE);
         float before[TILE + 1][S], al[TILE][S];      // the states before each step, and its decays
+        // k and q of the tile for the way back as well, where the registers are there for it (two rows a wave: 551 us against 568, 8 x 2048 steps of 2048
+        // channels; four rows spill 115 registers)
+        constexpr bool HELD = S == 2;
+        float kq_held[HELD ? TILE : 1][2 * S];
 #pragma unroll
         for (int s = 0; s < S; s++) before[0][s] = before0[s];
 #pragma unroll
         for (int r = 0; r < TILE; r++) {
             const float2 x = sx[r][p.lane];
-            const float *const k = kq[r] + K::WIDTH * p.wave, *const q = k + S;
+            if constexpr (HELD)
+#pragma unroll
+                for (int i = 0; i < 2 * S; i++) kq_held[r][i] = kq[r][K::WIDTH * p.wave + i];
+            const float *const k = HELD ? kq_held[HELD ? r : 0] : kq[r] + K::WIDTH * p.wave, *const q = k + S;
             float y = 0.f;
 #pragma unroll
             for (int s = 0; s < S; s++) {
@@ -494,7 +501,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_scan_bwd(fwp_scan_args a, Dim
         constexpr int SUMS = 2 * S;
         const auto back = [&](int r, float (&sums)[SUMS]) {
             const float2 x = sx[r][p.lane];
-            const float dy = sg[r][p.lane], *const k = kq[r] + K::WIDTH * p.wave, *const q = k + S;
+            const float dy = sg[r][p.lane], *const k = HELD ? kq_held[HELD ? r : 0] : kq[r] + K::WIDTH * p.wave, *const q = k + S;
             float read = 0.f, slope = 0.f;
 #pragma unroll
             for (int s = 0; s < S; s++) {
