@@ -39,10 +39,12 @@ constexpr int kRowMirror8 = 0x141;      // lane i of 8 gets lane 7 - i
 // Waves of a workgroup and state rows of a wave (S).  Two rows a wave need half the registers of four, so that twice the waves are there to fill one another's
 // gaps: 32 x 1024 steps of 512 channels, 16 rows, forward + backward 125 + 344 us against 158 + 526 us with four.  At 32 rows sixteen waves of two
 // would not fit the LDS.  Fewer than four waves would load a tile's rows too slowly.
-int rows_of(int E) { return E <= 16 ? 2 : 4; }
-int waves_of(int E) { return E <= 8 ? 4 : E <= 32 ? 8 : 16; }
-// Steps of a tile, and from one saved state to the next.  Sixteen waves leave 128 registers to a lane, which must hold the history of a tile.
-constexpr int tile_of(int waves) { return waves == 16 ? 8 : 16; }
+// Beyond 32 rows sixteen waves of four go forward, and eight of eight back, since sixteen leave 128 registers to a lane and a tile's history does not fit them
+// (32 x 1024 steps of 512 channels, 64 rows: 2441 us, and 913 with eight).
+int rows_of(int E, bool backward) { return E <= 16 ? 2 : E <= 32 || !backward ? 4 : 8; }
+int waves_of(int E, bool backward) { return E <= 8 ? 4 : E <= 32 || backward ? 8 : 16; }
+// Steps from one saved state to the next, and of the adjoint's tiles, whose states a wave holds in registers
+constexpr int tile_of(int rows, int waves) { return rows * waves > 32 ? 8 : 16; }
 
 struct Dims {
     int N, H, L, E, M;
@@ -56,7 +58,7 @@ struct Plan : Dims {
     int64_t heads, states;      // N H; floats of one set of states
     Plan(int N_, int H_, int L_, int E_, int M_, bool backward) {
         N = N_, H = H_, L = L_, E = E_, M = M_;
-        rows = rows_of(E), waves = waves_of(E), tile = tile_of(waves);
+        rows = rows_of(E, backward), waves = waves_of(E, backward), tile = tile_of(rows, waves);
         blocks_m = (M + 63) / 64;
         tiles = (L + tile - 1) / tile;
         padded = tiles * tile;
@@ -66,12 +68,16 @@ struct Plan : Dims {
         // 0.2 (backward) of the work.  Workgroups that share a CU fill one another's gaps in the forward pass, where three fit: two take
         // 1.36 times as long as one.  Measured, 256 workgroups cut into 1, 2, 4: 231, 282, 261 us and 587, 718, 718 us; 16 into
         // 8, 16, 32, 64: 186, 116, 84, 85 us forward.  A segment has eight tiles at least, or the two launches more cost what it saves.
+        // Workgroups of four waves (up to 8 rows) leave more of a CU idle, forward and backward: two take 1.2 times as long as one, eight 3.5 times, and the pass before 0.4 of the
+        // adjoint.  128 workgroups (1024 steps) cut into 1, 2, 4, 8: 118, 103, 68, 55 and 268, 190, 125, 126 us; 256: 124, 127, 103, 96 and 288, 245, 243, 254;
+        // 512: 152, 188, 176, 171 and 350, 434, 435, 465.
         const int64_t blocks = heads * blocks_m;
         double best = 0;
         segments = 1, steps = padded;
         for (int w = 1; w <= 64 && (w == 1 || w <= tiles / 8); w++) {
             const double turns = (double)((blocks * w + 255) / 256);
-            const double cost = (backward ? turns : turns > 1 ? 0.68 * turns : 1) / w * (w == 1 ? 1 : backward ? 1.2 : 1.7);
+            const double side_by_side = waves == 4 ? (backward ? 0.6 * turns : 0.35 + 0.42 * turns) : backward ? turns : 0.68 * turns;
+            const double cost = (turns > 1 ? side_by_side : 1) / w * (w == 1 ? 1 : !backward ? 1.7 : waves == 4 ? 1.4 : 1.2);
             if (w > 1 && cost >= best) continue;
             best = cost;
             const int per = (tiles + w - 1) / w;
@@ -214,7 +220,7 @@ struct Channel {
 template <typename T, int WAVES, int S, bool LOCAL, bool FULL>
 __global__ __launch_bounds__(64 * WAVES) void k_scan_fwd(fwp_scan_args a, Dims d, const float *init, float *W, float *__restrict__ saved,
                                                          float *__restrict__ sums, fwp_out_rows out) {
-    constexpr int TILE = 16, ROWS = (TILE + WAVES - 1) / WAVES, KEEP = tile_of(WAVES);
+    constexpr int TILE = 16, ROWS = (TILE + WAVES - 1) / WAVES, KEEP = tile_of(S, WAVES);
     using K = Keys<T, WAVES, S, TILE, LOCAL ? 1 : 2>;
     __shared__ alignas(16) float kq[TILE][K::ROW];
     __shared__ float2 sx[TILE][64];                          // dt, dt v
@@ -393,7 +399,7 @@ template <typename T, int WAVES, int S>
 __global__ __launch_bounds__(64 * WAVES, 2) void k_scan_bwd(fwp_scan_args a, Dims d, const float *__restrict__ saved, const float *__restrict__ init,
                                                          fwp_rows gout, fwp_out_rows gv, fwp_out_rows gdelta, fwp_out_rows gz,
                                                          float *__restrict__ parts, float *__restrict__ params) {
-    constexpr int TILE = tile_of(WAVES), ROWS = (TILE + WAVES - 1) / WAVES;
+    constexpr int TILE = tile_of(S, WAVES), ROWS = (TILE + WAVES - 1) / WAVES;
     using K = Keys<T, WAVES, S, TILE, 2>;
     __shared__ alignas(16) float kqs[2][TILE][K::ROW];
     __shared__ float2 sxs[2][TILE][64];                  // dt, dt v
@@ -473,7 +479,8 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_scan_bwd(fwp_scan_args a, Dim
         const auto kq = kqs[half];
         turn();
         if (t0 > first) fetch(t0 - TILE);
-        float before[TILE + 1][S], al[TILE][S];      // the states before each step, and its decays
+        constexpr bool AGAIN = S == 8;               // no registers for them: formed again on the way back
+        float before[TILE + 1][S], al[AGAIN ? 1 : TILE][S];      // the states before each step, and its decays
         // k and q of the tile for the way back as well, where the registers are there for it (two rows a wave: 551 us against 568, 8 x 2048 steps of 2048
         // channels; four rows spill 115 registers)
         constexpr bool HELD = S == 2;
@@ -490,8 +497,9 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_scan_bwd(fwp_scan_args a, Dim
             float y = 0.f;
 #pragma unroll
             for (int s = 0; s < S; s++) {
-                al[r][s] = __builtin_amdgcn_exp2f(x.x * decay[s]);
-                before[r + 1][s] = fmaf(al[r][s], before[r][s], x.y * k[s]);
+                const float e = __builtin_amdgcn_exp2f(x.x * decay[s]);
+                if constexpr (!AGAIN) al[r][s] = e;
+                before[r + 1][s] = fmaf(e, before[r][s], x.y * k[s]);
                 y = fmaf(q[s], before[r + 1][s], y);
             }
             part[2][p.wave][r][p.lane] = y;
@@ -509,7 +517,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_scan_bwd(fwp_scan_args a, Dim
                 sums[s] = g * x.y;
                 sums[S + s] = dy * before[r + 1][s];
                 read = fmaf(g, k[s], read);
-                c[s] = g * al[r][s];
+                c[s] = g * (AGAIN ? __builtin_amdgcn_exp2f(x.x * decay[s]) : al[AGAIN ? 0 : r][s]);
                 const float w = c[s] * before[r][s];
                 slope = fmaf(w, decay[s], slope);
                 tile_gA[s] = fmaf(w, x.x, tile_gA[s]);
@@ -517,34 +525,35 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_scan_bwd(fwp_scan_args a, Dim
             part[0][p.wave][r][p.lane] = read;
             part[1][p.wave][r][p.lane] = slope;
         };
-        // The sums over the lanes, halving what a lane holds as it goes, over 64 / SUMS steps (8 or 16): lane l then has the sum
-        // number l % SUMS of the step whose bits 0, 1, 2 (and 3) are l's bits 5, 4, 3 (and 2).
+        // The sums over the lanes, halving what a lane holds as it goes, over 64 / SUMS steps (4, 8 or 16): lane l then has the sum
+        // number l % SUMS of the step whose bits 0, 1 (2, and 3) are l's bits 5, 4 (3, and 2).
         const bool b3 = p.lane & 8, b2 = p.lane & 4, b1 = p.lane & 2, b0 = p.lane & 1;
         float *const to = parts + (((int64_t)p.mb * d.N * d.H + p.nh) * d.padded + t0) * WAVES * SUMS +
-                          ((p.lane >> 5 & 1) + 2 * (p.lane >> 4 & 1) + 4 * (p.lane >> 3 & 1) + (S == 2 ? 8 * (p.lane >> 2 & 1) : 0)) * WAVES * SUMS +
+                          ((p.lane >> 5 & 1) + 2 * (p.lane >> 4 & 1) + (S <= 4 ? 4 * (p.lane >> 3 & 1) : 0) + (S == 2 ? 8 * (p.lane >> 2 & 1) : 0)) * WAVES * SUMS +
                           p.wave * SUMS + p.lane % SUMS;
-        const auto eight_back = [&](int r0, float (&x)[SUMS]) {
-            float eight[2][SUMS];
+        const auto four_back = [&](int r0, float (&x)[SUMS]) {
+            float two[2][SUMS];
 #pragma unroll
-            for (int q2 = 1; q2 >= 0; q2--) {
-                float four[2][SUMS];
-#pragma unroll
-                for (int q1 = 1; q1 >= 0; q1--) {
-                    float odd[SUMS], even[SUMS];
-                    back(r0 + 4 * q2 + 2 * q1 + 1, odd);
-                    back(r0 + 4 * q2 + 2 * q1, even);
-#pragma unroll
-                    for (int i = 0; i < SUMS; i++) {
-                        swap32(even[i], odd[i]);
-                        four[q1][i] = even[i] + odd[i];
-                    }
-                }
+            for (int q1 = 1; q1 >= 0; q1--) {
+                float odd[SUMS], even[SUMS];
+                back(r0 + 2 * q1 + 1, odd);
+                back(r0 + 2 * q1, even);
 #pragma unroll
                 for (int i = 0; i < SUMS; i++) {
-                    swap16(four[0][i], four[1][i]);
-                    eight[q2][i] = pinned(four[0][i] + four[1][i]);
+                    swap32(even[i], odd[i]);
+                    two[q1][i] = even[i] + odd[i];
                 }
             }
+#pragma unroll
+            for (int i = 0; i < SUMS; i++) {
+                swap16(two[0][i], two[1][i]);
+                x[i] = pinned(two[0][i] + two[1][i]);
+            }
+        };
+        const auto eight_back = [&](int r0, float (&x)[SUMS]) {
+            float eight[2][SUMS];
+            four_back(r0 + 4, eight[1]);
+            four_back(r0, eight[0]);
 #pragma unroll
             for (int i = 0; i < SUMS; i++) x[i] = pinned((b3 ? eight[1][i] : eight[0][i]) + dpp<kRowRor8>(b3 ? eight[0][i] : eight[1][i]));
         };
@@ -553,7 +562,18 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_scan_bwd(fwp_scan_args a, Dim
             for (int i = 0; i < 2; i++) x[i] = pinned((b1 ? x[i + 2] : x[i]) + dpp<kQuadXor2>(b1 ? x[i] : x[i + 2]));
             return pinned((b0 ? x[1] : x[0]) + dpp<kQuadXor1>(b0 ? x[0] : x[1]));
         };
-        if constexpr (S == 4) {
+        if constexpr (S == 8) {
+#pragma unroll
+            for (int r0 = TILE - 4; r0 >= 0; r0 -= 4) {
+                float x[SUMS], y[8], u[4];
+                four_back(r0, x);
+#pragma unroll
+                for (int i = 0; i < 8; i++) y[i] = pinned((b3 ? x[i + 8] : x[i]) + dpp<kRowRor8>(b3 ? x[i] : x[i + 8]));
+#pragma unroll
+                for (int i = 0; i < 4; i++) u[i] = pinned((b2 ? y[i + 4] : y[i]) + dpp<kRowMirror8>(b2 ? y[i] : y[i + 4]));
+                to[r0 * WAVES * SUMS] = four_lanes(u);
+            }
+        } else if constexpr (S == 4) {
 #pragma unroll
             for (int r0 = TILE - 8; r0 >= 0; r0 -= 8) {
                 float x[8], y[4];
@@ -728,11 +748,11 @@ __global__ __launch_bounds__(256) void k_scan_step(fwp_scan_args a, float *__res
 // ------------------------------------------------------------------ launches
 
 // f(WAVES, S)
-template <typename F>
+template <bool BACKWARD, typename F>
 void by_waves(const Plan &p, F f) {
     using std::integral_constant;
     if (p.waves == 4) f(integral_constant<int, 4>(), integral_constant<int, 2>());
-    else if (p.waves == 16) f(integral_constant<int, 16>(), integral_constant<int, 4>());
+    else if (p.E > 32) f(integral_constant<int, BACKWARD ? 8 : 16>(), integral_constant<int, BACKWARD ? 8 : 4>());
     else if (p.rows == 2) f(integral_constant<int, 8>(), integral_constant<int, 2>());
     else f(integral_constant<int, 8>(), integral_constant<int, 4>());
 }
@@ -771,7 +791,7 @@ int scan_fwd(const fwp_scan_args &a, float *W, fwp_out_rows out, float *saved, f
     const Dims d = p;
     by_type(a.type, [&](auto t) {
         using T = decltype(t);
-        by_waves(p, [&](auto w, auto r) {
+        by_waves<false>(p, [&](auto w, auto r) {
             constexpr int WAVES = decltype(w)::value, S = decltype(r)::value;
             const dim3 grid((unsigned)p.grid()), block(64 * WAVES);
             if (p.segments > 1) {
@@ -802,7 +822,7 @@ int scan_bwd(const fwp_scan_args &a, const float *saved, fwp_rows gout, fwp_out_
     const Dims d = p;
     by_type(a.type, [&](auto t) {
         using T = decltype(t);
-        by_waves(p, [&](auto w, auto r) {
+        by_waves<true>(p, [&](auto w, auto r) {
             constexpr int WAVES = decltype(w)::value, S = decltype(r)::value;
             const dim3 grid((unsigned)p.grid()), block(64 * WAVES);
             if (p.segments > 1) {

@@ -93,7 +93,8 @@ SCAN = [  # N, H, L, E, M, layout, ragged, carried, gated
     (4, 1, 33, 8, 70, "plain", True, True, True), (1, 1, 200, 16, 64, "steps", False, True, True), (5, 2, 131, 11, 49, "slice", True, False, False),
     (2, 1, 70, 32, 33, "strided", True, True, True), (2, 1, 41, 17, 64, "plain", False, False, True), (1, 2, 100, 64, 20, "steps", False, True, True),
     (3, 1, 24, 33, 66, "plain", True, True, False), (2, 1, 40, 16, 32, "same", False, False, True), (1, 1, 700, 2, 3, "plain", False, True, True),
-    (3, 1, 513, 16, 5, "steps", True, True, True),
+    (3, 1, 513, 16, 5, "steps", True, True, True), (4, 1, 150, 64, 70, "slice", True, True, True), (2, 2, 61, 49, 64, "steps", False, True, False),
+    (2, 1, 600, 8, 130, "plain", True, True, True),
 ]
 
 
