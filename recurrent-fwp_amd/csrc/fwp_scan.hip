@@ -641,26 +641,30 @@ template <typename T>
 __global__ __launch_bounds__(256) void k_scan_finish(const float *__restrict__ parts, const float *__restrict__ params, fwp_out_rows gq,
                                                      fwp_out_rows gk, float *__restrict__ gA, float *__restrict__ gD,
                                                      float *__restrict__ gbias, const int64_t *__restrict__ lengths, Dims d, int waves,
-                                                     int S, int64_t row_blocks) {
-    if (blockIdx.x < row_blocks) {
-        const int width = waves * 2 * S;
-        const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, heads = (int64_t)d.N * d.H;
-        const int64_t nh = i / ((int64_t)d.L * width), rest = i % ((int64_t)d.L * width);
-        const int t = (int)(rest / width), j = (int)(rest % width), e = j / (2 * S) * S + j % S;
+                                                     int S, unsigned param_blocks) {
+    if (blockIdx.x >= param_blocks) {       // the parameters' first: they take longer
+        const unsigned width = waves * 2 * S, heads = (unsigned)d.N * d.H, i = (blockIdx.x - param_blocks) * 256 + threadIdx.x;      // a launch's threads fit 32 bits
+        const unsigned row_of = i / width, j = i % width, nh = row_of / d.L, t = row_of % d.L;
+        const int e = (int)(j / (2 * S) * S + j % S);
         if (nh >= heads || e >= d.E) return;
         const int n = (int)(nh / d.H), h = (int)(nh % d.H);
         float x = 0.f;
-        if (t < length_of(lengths, n, d.L))
-            for (int mb = 0; mb < d.blocks_m; mb++) x += parts[((mb * heads + nh) * d.padded + t) * width + j];
+        if ((int)t < length_of(lengths, n, d.L)) {
+            const float *from = parts + ((int64_t)nh * d.padded + t) * width + j;
+            const int64_t step = (int64_t)heads * d.padded * width;
+#pragma unroll 8
+            for (int mb = 0; mb < d.blocks_m; mb++) x += from[mb * step];
+        }
         store(row<T>(j % (2 * S) < S ? gk : gq, n, h, t) + e, x);
         return;
     }
     // 64 columns and four slices of the sequences and segments to a workgroup
     __shared__ float sh[4][64];
-    const int64_t per = (int64_t)d.H * (d.E + 2) * d.M, i = (blockIdx.x - row_blocks) * 64 + threadIdx.x % 64;
+    const int64_t per = (int64_t)d.H * (d.E + 2) * d.M, i = (int64_t)blockIdx.x * 64 + threadIdx.x % 64;
     const int slice = threadIdx.x / 64, terms = d.N * d.segments;
     float x = 0.f;
     if (i < per)
+#pragma unroll 8
         for (int k = slice; k < terms; k += 4) x += params[k * per + i];
     sh[slice][threadIdx.x % 64] = x;
     __syncthreads();
@@ -833,7 +837,7 @@ int scan_bwd(const fwp_scan_args &a, const float *saved, fwp_rows gout, fwp_out_
                                params);
         });
         hipLaunchKernelGGL((k_scan_finish<T>), dim3((unsigned)(row_blocks + param_blocks)), dim3(256), 0, s, parts, params, gq, gk, gA, gD,
-                           gdelta_bias, a.lengths, d, p.waves, p.rows, row_blocks);
+                           gdelta_bias, a.lengths, d, p.waves, p.rows, (unsigned)param_blocks);
     });
     return (int)hipGetLastError();
 }
