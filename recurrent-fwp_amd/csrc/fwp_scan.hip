@@ -16,11 +16,11 @@
 // starts from (the decay over a segment is exp(A sum dt), whatever its length), and the second pass is the scan itself.  That doubles the
 // exponentials, and instructions are what bounds these kernels, so a call that fills the chip is not cut.
 //
-// Measured, 32 sequences x 1024 steps of 512 channels, 16 rows, fp32: forward 136 us, adjoint 333, its sums 15; their bytes would take 51 and 84 at 5 TB/s.  8 x 2048 steps of 2048
-// channels, bf16: 235-245, 565-590, 20 us.  An entry and step costs 8 vector instructions forward, 24 backward: 5 and 13 are the recurrences (the exponential takes
+// Measured, 32 sequences x 1024 steps of 512 channels, 16 rows, fp32: forward 128 us, adjoint 300-320, its sums 10; their bytes would take 51 and 84 at 5 TB/s.  8 x 2048 steps of
+// 2048 channels, bf16: 236, 551, 17 us.  An entry and step costs 8 vector instructions forward, 24 backward: 5 and 13 are the recurrences (the exponential takes
 // the slots of four), a quarter of the rest the sums over the lanes, the other half the softplus, the gate and their slopes.  The vector pipes are at work 56 % of the
-// forward and 69 % of the adjoint's time, with two waves a SIMD (the adjoint's LDS leaves no room for more), LDS another 12-14 %.  Without the sums over the lanes the
-// adjoint's 603 us were 543, without softplus and gate 509, with one wave's part instead of eight's 568, without exponentials 583, without k and q from LDS 555.
+// forward and 71 % of the adjoint's time, with two waves a SIMD (the adjoint's LDS leaves no room for more), LDS another 12-13 %.  Without the sums over the lanes the
+// adjoint's 603 us of an earlier stage were 543, without softplus and gate 509, with one wave's part instead of eight's 568, without exponentials 583, without k and q from LDS 555.
 // Not kept: k and q by scalar loads (297 us forward, 186 from LDS at that stage), tiles of 8 steps with one barrier (149 us against 125) or of 32 (128), one barrier
 // and all of a tile's LDS twice (158 against 140 us), steps and values held in registers between the adjoint's two sweeps as k and q are (no change).
 //

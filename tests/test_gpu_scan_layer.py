@@ -60,7 +60,7 @@ def test_the_block_and_its_gradients(fwp, T, B, ragged):
     tol = 64 * (4 * T + 400) * F.EPS32
     for name, a, b in zip(["out", "h"] + [k for k, _ in m.named_parameters()], [got, *grads], [want, *want_grads]):
         # a parameter's gradient adds up the tokens' shares
-        scale = float(b.abs().max()) + (1e-3 if name in ("out", "h") else 1e-3 * (T * B) ** 0.5)
+        scale = float(b.detach().abs().max()) + (1e-3 if name in ("out", "h") else 1e-3 * (T * B) ** 0.5)
         assert float((F.double(a) - b).abs().max()) <= tol * scale, name
 
 
