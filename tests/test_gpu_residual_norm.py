@@ -148,6 +148,26 @@ def test_constant_rows_and_large_means(fwp):
     assert float((F.double(r) - want).abs().max()) <= (4096 + 64) * F.EPS32      # the mean is off by a rounding of 4096, the spread is about 5
 
 
+def test_parameters_gradients_are_tensors_of_their_own(fwp):
+    """They share memory, not a byte of it: accumulated, cleared and changed one by one."""
+    g = torch.Generator().manual_seed(6)
+    y, x = torch.randn(9, 131, generator=g).cuda(), torch.randn(9, 131, generator=g).cuda()
+    params = [torch.randn(131, generator=g).cuda().requires_grad_() for _ in range(5)]
+
+    def backward():
+        r, n = fwp.residual_norm(y, x, after=(params[0], params[1]), scale=params[2], before=(params[3], params[4]))
+        (r * x + n * y).sum().backward()
+
+    backward()
+    once = [p.grad.clone() for p in params]
+    backward()
+    for p, a in zip(params, once):
+        assert p.grad.is_contiguous() and torch.equal(p.grad, a + a)
+    for i, p in enumerate(params):
+        p.grad.fill_(float(i))
+    assert all(bool((p.grad == float(i)).all()) for i, p in enumerate(params))
+
+
 def test_infinite_rows_that_a_gate_masks(fwp):
     """Without a norm on y the gradients do not pass y's values: where an infinite one is masked away by the caller, gy is as for any other."""
     g = torch.Generator().manual_seed(4)
