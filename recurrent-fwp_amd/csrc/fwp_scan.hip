@@ -6,7 +6,7 @@
 //   g = dy q + c,  c (of the state before the step) = a g,  a = exp(dt A),  w = a W_before g
 //   gq = sum_m dy W    gk = sum_m g dt v    gv = dt sum_e g k + D dy    gdt = v sum_e g k + sum_e A w    gA = sum dt w    gD = sum dy v
 //
-// A workgroup takes 64 channels of one sequence and head: a lane is a channel, a wave two or four entries of the state (key rows), so that a
+// A workgroup takes 64 channels of one sequence and head: a lane is a channel, a wave two, four or eight entries of the state (key rows), so that a
 // state and its history stay in registers, and a sum over the channels is a sum over the lanes.  Steps go in tiles of 16 (8 for 16 waves) rows: each thread
 // loads its rows of v, delta, z once, works out dt and dt v, and puts them into LDS for all waves, as k and q are; the waves' parts of a sum
 // over e meet in LDS and the thread that loaded a row finishes it.  The next tile's rows are on their way meanwhile.
