@@ -38,9 +38,10 @@ constexpr int kRowMirror8 = 0x141;      // lane i of 8 gets lane 7 - i
 
 // Waves of a workgroup and state rows of a wave (S).  Two rows a wave need half the registers of four, so that twice the waves are there to fill one another's
 // gaps: 32 x 1024 steps of 512 channels, 16 rows, forward + backward 125 + 344 us against 158 + 526 us with four.  At 32 rows sixteen waves of two
-// would not fit the LDS.  Fewer than four waves would load a tile's rows too slowly.
+// would not fit the LDS of the adjoint; forward they take 139 us against 151 with 256 workgroups and 275 against 229 with 512.  Fewer than four waves would load a tile's rows too slowly.
 // Beyond 32 rows sixteen waves of four go forward, and eight of eight back, since sixteen leave 128 registers to a lane and a tile's history does not fit them
 // (32 x 1024 steps of 512 channels, 64 rows: 2441 us, and 913 with eight).
+// Sixteen waves of one row forward at 16 rows: 147 us against 127 with 256 workgroups, 256 against 157 with 512 (twice the parts of sum_e q W through LDS).
 int rows_of(int E, bool backward) { return E <= 16 ? 2 : E <= 32 || !backward ? 4 : 8; }
 int waves_of(int E, bool backward) { return E <= 8 ? 4 : E <= 32 || backward ? 8 : 16; }
 // Steps from one saved state to the next, and of the adjoint's tiles, whose states a wave holds in registers
