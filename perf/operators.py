@@ -12,7 +12,6 @@ scan, and the norms around a block with its gate, scale and residual addition.
 A case's mode: "train" (forward and backward of one call), "forward" (a prompt: nothing recorded, the state kept), "step" (one
 token per sequence, the state advanced in place).
 """
-import functools
 import importlib
 import math
 
@@ -295,14 +294,9 @@ def _plain_norm(s):
 
 # ------------------------------------------------------------------ the framework's operators
 
-@functools.cache
-def _framework():
-    """Imported once, as a program does."""
-    return importlib.import_module("recurrent-fwp_amd")
-
-
 def _own(s):
-    fwp, case = _framework(), s["case"]
+    fwp = importlib.import_module("recurrent-fwp_amd")
+    case = s["case"]
     if case["op"] == "conv":
         return (fwp.causal_conv(s["x"], s["weight"], s["bias"], s["state"], silu=case["silu"], lengths=s["lengths"]),)
     if case["op"] == "scan":
