@@ -2,7 +2,7 @@
 // scan, and the norms around a block with its gate, scale and residual addition.  Host code only.
 //
 // Arguments are checked against one another before the device is, and a rejected call has changed nothing.  States are updated in place and get no
-// gradient, as in the fast-weight operators; gradients cannot be differentiated again.
+// gradient, as in the fast-weight operators; gradients cannot be differentiated again, and there is no forward-mode derivative.
 #include "fwp_torch.hpp"
 
 #include <torch/csrc/autograd/variable.h>
@@ -122,6 +122,12 @@ bool records(std::initializer_list<const at::Tensor *> ts) {
     return false;
 }
 
+// A tangent of forward-mode differentiation would be lost without a word: its tensor need not require a gradient.
+void no_tangents(std::initializer_list<const at::Tensor *> ts) {
+    for (const at::Tensor *t : ts)
+        if (t->defined() && t->_fw_grad(0).defined()) fail("this operator has no forward-mode derivative: a tensor of the call has a tangent");
+}
+
 // ------------------------------------------------------------------ short causal convolution
 
 struct ConvFn : torch::autograd::Function<ConvFn> {
@@ -196,7 +202,8 @@ struct ConvFn : torch::autograd::Function<ConvFn> {
 };
 
 at::Tensor causal_conv(const at::Tensor &x, const at::Tensor &w, const Optional &b, const Optional &state, bool silu, const Optional &lengths) {
-    const at::Tensor bias = given(b);
+    const at::Tensor bias = given(b), state_ = given(state);
+    no_tangents({&x, &w, &bias, &state_});
     if (records({&x, &w, &bias})) return ConvFn::apply(x, w, b, state, lengths, silu);
     at::AutoDispatchBelowADInplaceOrView below;
     return ConvFn::forward(nullptr, x, w, b, state, lengths, silu);
@@ -282,7 +289,8 @@ struct ScanFn : torch::autograd::Function<ScanFn> {
 
 at::Tensor selective_scan(const at::Tensor &q, const at::Tensor &k, const at::Tensor &v, const at::Tensor &delta, const at::Tensor &A,
                           const Optional &W, const Optional &D, const Optional &z, const Optional &bias, bool softplus, const Optional &lengths) {
-    const at::Tensor D_ = given(D), z_ = given(z), bias_ = given(bias);
+    const at::Tensor D_ = given(D), z_ = given(z), bias_ = given(bias), W_ = given(W);
+    no_tangents({&q, &k, &v, &delta, &A, &W_, &D_, &z_, &bias_});
     if (records({&q, &k, &v, &delta, &A, &D_, &z_, &bias_})) return ScanFn::apply(q, k, v, delta, A, D, z, bias, W, lengths, softplus);
     at::AutoDispatchBelowADInplaceOrView below;
     return ScanFn::forward(nullptr, q, k, v, delta, A, D, z, bias, W, lengths, softplus);
@@ -389,6 +397,7 @@ std::pair<at::Tensor, Optional> residual_norm(const at::Tensor &y, const at::Ten
                                               int64_t act) {
     const at::Tensor g = given(gate), sc = given(scale), t0 = given(aw), t1 = given(ab), t2 = given(bw), t3 = given(bb);
     variable_list out;
+    no_tangents({&y, &x, &g, &sc, &t0, &t1, &t2, &t3});
     if (records({&y, &x, &g, &sc, &t0, &t1, &t2, &t3})) {
         out = ResidualNormFn::apply(y, x, gate, scale, aw, ab, bw, bb, eps, rms, act);
     } else {

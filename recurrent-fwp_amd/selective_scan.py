@@ -6,7 +6,8 @@ Rows (``X``, ``Q``, ``K``, ``V``, ``delta``, ``Z``, ``y``, ``x``, ``gate``) are 
 are fp32.  Views are read in place as long as their last axis is contiguous, and results take the memory order of the rows they belong to (steps outermost
 for the permuted views that a layer hands over).  ``lengths`` (int64 ``[N]``, on the GPU, values beyond ``0 .. L`` are cut to it) marks a padded batch: the rows of sequence ``n``
 from ``lengths[n]`` on are not read, whatever they hold, their results and gradients are zero, and its states are those after its last row.
-States are updated in place and get no gradient; gradients cannot be differentiated again.  Anything else raises ``FwpError``.
+States are updated in place and get no gradient; gradients cannot be differentiated again, and tensors with a tangent
+(forward-mode differentiation) are refused.  Anything else raises ``FwpError``.
 """
 from . import _lib
 from .fast_weight import _fwp_torch
