@@ -397,9 +397,9 @@ class SelectiveScanLayer(nn.Module):
 
 class SelectiveScanDecoderLayer(nn.Module):
     """A :class:`SelectiveScanLayer` and the feed-forward block behind it on a residual stream: norm, mixer, norm and scale on its output, and
-    the same around the feed-forward block; :func:`residual_norm` is what lies between and behind the two.  Constructor and call as
-    :class:`DeltaNetDecoderLayer`'s, whose place it takes in :class:`DeltaNetLM`; heads do not count here (q and k are shared by all
-    channels), and norms come before a block whatever ``pre_lnorm``."""
+    the same around the feed-forward block; :func:`residual_norm` is what lies between and behind the two, but for a norm that was replaced or
+    hooked to, which is called.  Constructor and call as :class:`DeltaNetDecoderLayer`'s, whose place it takes in :class:`DeltaNetLM`; heads do not
+    count here (q and k are shared by all channels), ``dropatt`` has nothing to drop, and norms come before a block whatever ``pre_lnorm``."""
 
     def __init__(self, n_head, d_model, d_head, d_inner, dropout=0.0, dropatt=0.0, pre_lnorm=True, layer_id=None, num_layer=None,
                  fast_weight_op=None, n_state=16, taps=4):
@@ -413,9 +413,29 @@ class SelectiveScanDecoderLayer(nn.Module):
         self.ff = nn.Sequential(Linear(d_model, d_inner), nn.ReLU(), nn.Dropout(dropout), Linear(d_inner, d_model), nn.Dropout(dropout))
 
     def forward(self, dec_inp, dec_attn_mask=None, mems=None, carry_over_fast_weight=False, lengths=None):
-        pair = lambda norm: (norm.weight, norm.bias)
         out = self.dec_attn(_layer_norm(self.norm_in, dec_inp), mems=mems, carry_over_fast_weight=carry_over_fast_weight, lengths=lengths)
         out, mems = out if carry_over_fast_weight else (out, None)
-        r, n = residual_norm(out, dec_inp, after=pair(self.norm_attn), scale=self.scale_attn, before=pair(self.norm_mid), eps=self.norm_mid.eps)
-        r, _ = residual_norm(self.ff(n), r, after=pair(self.norm_ff), scale=self.scale_ff, eps=self.norm_ff.eps)
+        r, n = _around(out, dec_inp, self.norm_attn, self.scale_attn, self.norm_mid)
+        r, _ = _around(self.ff(n), r, self.norm_ff, self.scale_ff)
         return (r, mems) if carry_over_fast_weight else r
+
+
+def _fuses(norm, cols):
+    """Is this norm what :func:`residual_norm` computes: a LayerNorm over the last axis with a weight, that nothing watches?"""
+    return (_untouched(norm, nn.LayerNorm) and not torch.nn.modules.module._has_any_global_hook() and norm.normalized_shape == (cols,)
+            and norm.weight is not None)
+
+
+def _around(y, x, after, scale, before=None):
+    """``r = x + scale after(y)`` and ``before(r)`` (or ``None``) in one operator, but for the norms that it would pass by, which are called."""
+    cols = y.shape[-1]
+    pair = lambda norm: (norm.weight, norm.bias)
+    inside, eps = {}, 1e-5
+    if _fuses(after, cols):
+        inside["after"], eps = pair(after), after.eps
+    else:
+        y = _layer_norm(after, y)
+    if before is not None and _fuses(before, cols) and ("after" not in inside or before.eps == eps):
+        inside["before"], eps = pair(before), before.eps
+    r, n = residual_norm(y, x, scale=scale, eps=eps, **inside)
+    return r, n if before is None or "before" in inside else _layer_norm(before, r)
