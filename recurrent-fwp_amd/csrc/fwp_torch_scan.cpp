@@ -85,21 +85,8 @@ at::Tensor scratch(int64_t n, const at::Tensor &t) {
     return at::empty({std::max<int64_t>(n, 1)}, fp32(t));
 }
 
-// The gradients of a call's parameters in one allocation: each is a tensor of its own on the shared storage, which costs a tenth of an allocation.
-struct Gradients {
-    at::Tensor all;
-    int64_t at = 0;
-    Gradients(int64_t floats, const at::Tensor &by) : all(at::empty({floats}, fp32(by))) {}
-    static int64_t room(const at::Tensor &t) { return t.defined() ? (t.numel() + 3) & ~int64_t(3) : 0; }
-    at::Tensor take(at::IntArrayRef sizes) {
-        const at::Tensor t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(all.storage()), all.key_set(), all.dtype());
-        t.unsafeGetTensorImpl()->set_storage_offset(at);
-        t.unsafeGetTensorImpl()->set_sizes_contiguous(sizes);
-        at += room(t);
-        return t;
-    }
-    at::Tensor like(const at::Tensor &t) { return t.defined() ? take(t.sizes()) : t; }
-};
+// Room for a tensor of its own like this one, where there is one
+at::Tensor room_like(const at::Tensor &t) { return t.defined() ? at::empty(t.sizes(), t.options()) : t; }
 
 void require_sizes(std::initializer_list<int64_t> sizes) {
     for (const int64_t n : sizes)
@@ -188,10 +175,7 @@ struct ConvFn : torch::autograd::Function<ConvFn> {
         LaunchGuard guard(x);
         const at::Tensor gx = empty_rows(x), work = scratch(fwp_conv_workspace(a.N, a.H, a.L, a.D, a.K), x);
         at::Tensor gw, gb;
-        if (ctx->saved_data["params"].toBool()) {
-            Gradients params(Gradients::room(w) + ((int64_t)a.H * a.D + 3), w);
-            gw = params.like(w), gb = params.take({a.H, a.D});
-        }
+        if (ctx->saved_data["params"].toBool()) gw = room_like(w), gb = at::empty({a.H, a.D}, w.options());
         check(fwp_conv_bwd(&a, before.defined() && a.K > 1 ? before.const_data_ptr() : nullptr, view(g), out_view(gx), floats_out(gw),
                            floats_out(gb), work.data_ptr<float>(), stream_of(x)),
               "fwp_conv_bwd");
@@ -274,8 +258,7 @@ struct ScanFn : torch::autograd::Function<ScanFn> {
         LaunchGuard guard(v);
         const at::Tensor gq = empty_rows(s[8]), gk = empty_rows(s[9]), gv = empty_rows(v), gdelta = empty_rows(delta),
                          gz = z.defined() ? empty_rows(z) : at::Tensor(), work = scratch(fwp_scan_workspace(a.N, a.H, a.L, a.E, a.M, 1), v);
-        Gradients params(Gradients::room(A) + 2 * ((int64_t)a.H * a.M + 3), A);
-        const at::Tensor gA = params.like(A), gD = params.take({a.H, a.M}), gbias = params.take({a.H, a.M});
+        const at::Tensor gA = room_like(A), gD = at::empty({a.H, a.M}, A.options()), gbias = at::empty({a.H, a.M}, A.options());
         check(fwp_scan_bwd(&a, floats(saved), view(g), out_view(gq), out_view(gk), out_view(gv), out_view(gdelta), out_view(gz), floats_out(gA),
                            floats_out(gD), floats_out(gbias), work.data_ptr<float>(), stream_of(v)),
               "fwp_scan_bwd");
@@ -368,15 +351,9 @@ struct ResidualNormFn : torch::autograd::Function<ResidualNormFn> {
         const fwp_norm_args a =
             args(y, x, gate, scale, aw, ab, bw, bb, ctx->saved_data["eps"].toDouble(), ctx->saved_data["rms"].toBool(), ctx->saved_data["act"].toInt());
         LaunchGuard guard(y);
-        const auto like = [](const at::Tensor &t) { return t.defined() ? at::empty(t.sizes(), t.options()) : t; };
-        res[0] = like(y), res[1] = like(x);
-        int64_t room = 0;
-        for (const at::Tensor *t : {&scale, &aw, &ab, &bw, &bb}) room += Gradients::room(*t);
-        if (room) {
-            Gradients params(room, y);
-            res[3] = params.like(scale), res[4] = params.like(aw), res[5] = params.like(ab), res[6] = params.like(bw), res[7] = params.like(bb);
-        }
-        if (ctx->saved_data["gate"].toBool()) res[2] = like(gate);
+        res[0] = room_like(y), res[1] = room_like(x);
+        if (ctx->saved_data["gate"].toBool()) res[2] = room_like(gate);
+        res[3] = room_like(scale), res[4] = room_like(aw), res[5] = room_like(ab), res[6] = room_like(bw), res[7] = room_like(bb);
         const at::Tensor work = scratch(fwp_residual_norm_workspace(a.rows, a.cols), y);
         fwp_norm_grads g{};
         g.gy = res[0].data_ptr();
