@@ -307,7 +307,8 @@ __global__ __launch_bounds__(64 * WAVES) void k_scan_fwd(fwp_scan_args a, Dims d
 }
 
 // From each segment's own state (or gradient) to the one it starts from: after a segment x becomes exp(A sum dt) x + own.  The
-// exponential is applied as two halves, which reach twice as far before one of them is infinite.
+// exponential is applied as two halves, which reach twice as far before one of them is infinite.  An infinite x stays infinite as step by step,
+// also where exp(A sum dt) is zero: unless the steps' decays cannot all be above zero (2^-126 each).
 template <bool REVERSE>
 __global__ __launch_bounds__(256) void k_chain(const float *__restrict__ A, const float *__restrict__ sums, float *__restrict__ own,
                                                const float *W_in, float *W_out, Dims d) {
@@ -332,7 +333,9 @@ __global__ __launch_bounds__(256) void k_chain(const float *__restrict__ A, cons
             if (s0 + j >= d.segments) continue;
             const int seg = REVERSE ? d.segments - 1 - (s0 + j) : s0 + j;
             own[(nh * d.segments + seg) * per + em] = x;
-            const float e = __builtin_amdgcn_exp2f(half * dt[j]);
+            const float exponent = half * dt[j];
+            float e = __builtin_amdgcn_exp2f(exponent);
+            if (fabsf(x) == __builtin_inff() && exponent >= -63.f * d.steps) e = fmaxf(e, 1.17549435e-38f);
             x = x == 0.f ? o[j] : fmaf(e, e * x, o[j]);       // nothing grows out of nothing, however large exp(A sum dt)
         }
     }
