@@ -463,9 +463,10 @@ int fwp_conv_bwd(const fwp_conv_args *a, const void *state, fwp_rows grad_y, fwp
  *   W[e][m] = exp(dt[m] A[e][m]) W[e][m] + dt[m] k[e] v[m]
  *   o[m] = sum_e q[e] W[e][m] + D[m] v[m],  out = o, or o z sigmoid(z) where z is given
  * q, k [N,H,L,E], E <= 64; v, delta, z, out [N,H,L,M]; A [H,E,M]; D, delta_bias [H,M] (NULL: 0); W [N,H,E,M] fp32 in/out (NULL:
- * from zeros, not kept).  A should not be positive.  lengths as above.  Steps of a view lie at most 2^25 elements apart.
+ * from zeros, not kept).  A should not be positive.  lengths as above.  Steps of a view lie at most FWP_SCAN_MAX_STEP elements apart.
  * saved: NULL, or fwp_scan_saved_floats for a backward pass; workspace: fwp_scan_workspace(.., 0) floats (NULL if that is 0).
  */
+#define FWP_SCAN_MAX_STEP (1 << 25)
 typedef struct fwp_scan_args {
     fwp_rows q, k, v, delta, z; /* z.ptr NULL: no gate */
     const float *A, *D, *delta_bias;

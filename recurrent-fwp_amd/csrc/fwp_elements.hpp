@@ -91,7 +91,7 @@ int conv_bwd(const fwp_conv_args &a, const void *state, fwp_rows gy, fwp_out_row
 inline bool fits_launch(int64_t blocks, int threads) { return blocks <= (int64_t(1) << 32) / threads - 1; }
 
 // Elements between the steps of a view that the scan takes: sixteen steps and a row then lie within 32 bits of bytes.
-constexpr int64_t kScanMaxStep = 1 << 25;
+constexpr int64_t kScanMaxStep = FWP_SCAN_MAX_STEP;
 int64_t scan_saved_floats(int N, int H, int L, int E, int M);
 int64_t scan_workspace(int N, int H, int L, int E, int M, bool backward);
 int scan_fwd(const fwp_scan_args &a, float *W, fwp_out_rows out, float *saved, float *workspace, hipStream_t s);

@@ -473,7 +473,8 @@ void by_width(int cols, F f) {
 }
 
 // The adjoint's, with the columns' sums in registers: 4096 columns took 230 us with eight columns a lane and 472 with four (16384 rows, bf16, RMS), since
-// sixteen waves leave 128 registers to a lane, which then spills; 8192 columns 976 us that way
+// sixteen waves leave 128 registers to a lane, which then spills; 8192 columns 976 us that way.  Sixteen columns a lane (beyond 4096) need more than the 256
+// registers there are all the same: with biases 2 to 18 of them go to scratch where rows are aligned, 23 to 25 where they are not; without biases none.
 template <typename F>
 void by_width_bwd(int cols, F f) {
     using std::integral_constant;

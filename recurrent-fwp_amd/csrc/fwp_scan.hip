@@ -109,7 +109,7 @@ struct Place {
     __device__ __forceinline__ int64_t state(const Dims &d, int64_t at, int e) const { return (at * d.E + e) * d.M + m; }
 };
 
-// A log2(e) of the wave's four rows
+// A log2(e) of the wave's S rows
 template <int S>
 __device__ __forceinline__ void load_decays(float (&a)[S], const float *A, const Dims &d, const Place &p) {
 #pragma unroll
@@ -136,7 +136,7 @@ __device__ __forceinline__ void store_states(const float (&x)[S], float *to, int
 }
 
 // The rows of a tile in an [N,H,L,M] view, by the channel of the lane.  Addresses are a 64-bit base, the same for all lanes, that goes from tile to
-// tile, and 32-bit offsets in the tile (steps of up to kMaxStep elements).  Every lane loads: channels that do not exist read the last one, rows
+// tile, and 32-bit offsets in the tile (steps of up to kScanMaxStep elements).  Every lane loads: channels that do not exist read the last one, rows
 // behind the sequence its last row, and what they read is not used.  So no load waits behind a branch, and those of the next tile are on
 // their way while this one is worked on.
 template <typename T>

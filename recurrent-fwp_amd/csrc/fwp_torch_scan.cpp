@@ -50,7 +50,7 @@ at::Tensor lengths_of(const at::Tensor &t, int64_t N) {
     return t.contiguous();
 }
 
-constexpr int64_t kMaxStep = 1 << 25;      // elements between the steps of a view that the scan takes
+constexpr int64_t kMaxStep = FWP_SCAN_MAX_STEP;
 
 // [N,H,L,D] rows whose last axis is contiguous; a copy where it is not, and of rows too far apart
 at::Tensor rows_of(const at::Tensor &t, int64_t most = std::numeric_limits<int64_t>::max()) {

@@ -101,7 +101,7 @@ ROWS = [  # as test_gpu_residual_norm's
     ((9001, 200), False, "full", "sigmoid", True, 2, 2), ((5003, 255), True, "one", "silu", True, 1, 1), ((4501, 500), False, "full", "silu", True, 2, 2),
     ((1101, 800), False, "one", None, True, 2, 2), ((1030, 1999), True, "full", "sigmoid", True, 1, 1), ((601, 2560), True, "full", "silu", True, 1, 1),
     ((600, 4095), False, "full", "sigmoid", True, 2, 2), ((601, 4100), False, "full", None, True, 2, 2), ((300, 4099), True, "one", "sigmoid", True, 1, 1),
-    ((530, 8192), True, "full", "silu", True, 1, 1),
+    ((530, 8192), True, "full", "silu", True, 1, 1), ((9001, 3), False, "full", "sigmoid", True, 2, 2),
 ]
 
 
@@ -112,3 +112,41 @@ def test_more_rows_than_workgroups(fwp, monkeypatch, shape, rms, gating, act, sc
     real = norms.check
     monkeypatch.setattr(norms, "check", lambda got, want, size, dtype, what, more=0: real(got, want, size, dtype, what, min(more, 64)))
     norms.test_rows(fwp, shape, rms, gating, act, scaled, after, before, dtype, stream)
+
+
+@pytest.mark.parametrize("E", [4, 16, 40])
+def test_steps_far_apart_in_place(fwp, E):
+    """Steps just within what is read in place: a tile's offsets pass 2^31 bytes, a sequence's 2^32.  The same numbers as from copies, forward and backward."""
+    N, L, M = 2, 41, 8
+    g = torch.Generator().manual_seed(E)
+    wide = torch.empty(L, (1 << 25) - 7, dtype=torch.float32, device="cuda")      # 5.5 GB
+    at = wide.shape[1] - N * (3 * M + 2 * E) - 3
+    block = wide[:, at:at + N * (3 * M + 2 * E)].view(L, N, 1, 3 * M + 2 * E)
+    block.copy_(scans.randn(g, L, N, 1, 3 * M + 2 * E))
+    views = [t.permute(1, 2, 0, 3) for t in block.split([M, M, M, E, E], -1)]
+    A, go = -torch.rand(1, E, M, generator=g).cuda(), scans.randn(g, N, 1, L, M).cuda()
+    seen = []
+    for rows in (views, [t.contiguous() for t in views]):
+        v, delta, z, q, k = (t.detach().requires_grad_() for t in rows)
+        A_ = A.clone().requires_grad_()
+        out = fwp.selective_scan(q, k, v, delta, A_, Z=z, softplus=True)
+        seen.append([out, *torch.autograd.grad(out, [q, k, v, delta, z, A_], go)])
+    assert all(torch.equal(a, b) for a, b in zip(*seen))
+
+
+def test_very_many_sequences(fwp):
+    """70000 of them, with the formula for every one."""
+    N, L, E, M = 70000, 3, 4, 5
+    g = torch.Generator().manual_seed(2)
+    t = scans.scan_inputs(g, torch.float32, N, 1, L, E, M, "plain", True, True)
+    go = scans.randn(g, N, 1, L, M).cuda()
+    want, size = scans.formulas(t, True, None, go), scans.formulas(t, True, None, go, absolute=True)
+    names = ["Q", "K", "V", "delta", "A", "D", "Z", "delta_bias"]
+    for k in names:
+        t[k] = t[k].detach().requires_grad_()
+    out = fwp.selective_scan(**t, softplus=True)
+    scans.check(out, want[0], size[0], 4 * L + E + 64, "out", torch.float32)
+    scans.check(t["W"], want[1], size[1], 4 * L + E + 64, "W", torch.float32)
+    # a parameter's gradient adds up every fourth of the sequences' sums: 17500, and three more
+    for k, got, i in zip(names, torch.autograd.grad(out, [t[k] for k in names], go), range(2, 10)):
+        scans.check(got, want[i], size[i], 8 * L + 2 * E + M + 128 + (17504 if k in ("A", "D", "delta_bias") else 0), "gradient of " + k, torch.float32)
