@@ -17,7 +17,7 @@
 // exponentials, and instructions are what bounds these kernels, so a call that fills the chip is not cut.
 //
 // Measured, 32 sequences x 1024 steps of 512 channels, 16 rows, fp32: forward 128 us, adjoint 300-320, its sums 10; their bytes would take 51 and 84 at 5 TB/s.  8 x 2048 steps of
-// 2048 channels, bf16: 236, 551, 17 us.  An entry and step costs 8 vector instructions forward, 24 backward: 5 and 13 are the recurrences (the exponential takes
+// 2048 channels, bf16: 236-244, 551-568, 17 us.  An entry and step costs 8 vector instructions forward, 24 backward: 5 and 13 are the recurrences (the exponential takes
 // the slots of four), a quarter of the rest the sums over the lanes, the other half the softplus, the gate and their slopes.  The vector pipes are at work 56 % of the
 // forward and 71 % of the adjoint's time, with two waves a SIMD (the adjoint's LDS leaves no room for more), LDS another 12-13 %.  Without the sums over the lanes the
 // adjoint's 603 us of an earlier stage were 543, without softplus and gate 509, with one wave's part instead of eight's 568, without exponentials 583, without k and q from LDS 555.
