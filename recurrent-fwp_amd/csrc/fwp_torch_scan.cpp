@@ -35,12 +35,15 @@ void same_type(const at::Tensor &t, const at::Tensor &like, const char *name) {
     if (t.defined() && t.scalar_type() != like.scalar_type()) fail(std::string(name) + " must have the type of the other rows");
 }
 
+// Contiguous, and with the values that its memory holds: a view with its sign still to be changed (the imaginary part of a conjugate) is a copy too
+at::Tensor plain(const at::Tensor &t) { return !t.defined() ? t : t.is_neg() ? t.resolve_neg().contiguous() : t.contiguous(); }
+
 // A parameter: fp32, of this shape, contiguous (a copy if it is not)
 at::Tensor parameter(const at::Tensor &t, at::IntArrayRef shape, const char *name, const char *wanted) {
     if (!t.defined()) return t;
     if (t.scalar_type() != at::kFloat) fail(std::string(name) + " must be fp32");
     if (t.sizes() != shape) misfit(name, t, wanted);
-    return t.contiguous();
+    return plain(t);
 }
 
 // lengths [N]: int64
@@ -54,7 +57,7 @@ constexpr int64_t kMaxStep = FWP_SCAN_MAX_STEP;
 
 // [N,H,L,D] rows whose last axis is contiguous; a copy where it is not, and of rows too far apart
 at::Tensor rows_of(const at::Tensor &t, int64_t most = std::numeric_limits<int64_t>::max()) {
-    if (!t.defined() || ((t.size(3) == 1 || t.stride(3) == 1) && (t.size(2) == 1 || t.stride(2) <= most))) return t;
+    if (!t.defined() || (!t.is_neg() && (t.size(3) == 1 || t.stride(3) == 1) && (t.size(2) == 1 || t.stride(2) <= most))) return t;
     return t.clone(at::MemoryFormat::Contiguous);
 }
 
@@ -144,7 +147,7 @@ struct ConvFn : torch::autograd::Function<ConvFn> {
         if (state.defined()) {
             if (!same_shape(state, {N, H, K - 1, D})) misfit("state", state, "[N,H,K-1,D]");
             same_type(state, x_in, "state");
-            if (!state.is_contiguous()) fail("state must be contiguous");
+            if (!state.is_contiguous() || state.is_neg()) fail("state must be contiguous");
         }
         require_device(x_in);
         same_device(x_in, {w, b, state, lengths});
@@ -224,7 +227,7 @@ struct ScanFn : torch::autograd::Function<ScanFn> {
         if (z_.defined() && !same_shape(z_, {N, H, L, M})) misfit("Z", z_, "[N,H,L,M] as V is");
         const at::Tensor A = parameter(A_in, {H, E, M}, "A", "[H,E,M]"), D = parameter(given(D_in), {H, M}, "D", "[H,M]"),
                          bias = parameter(given(bias_in), {H, M}, "delta_bias", "[H,M]"), lengths = lengths_of(given(lengths_in), N);
-        if (W.defined() && (!same_shape(W, {N, H, E, M}) || !W.is_contiguous() || W.scalar_type() != at::kFloat))
+        if (W.defined() && (!same_shape(W, {N, H, E, M}) || !W.is_contiguous() || W.is_neg() || W.scalar_type() != at::kFloat))
             fail("W must be a contiguous fp32 [N,H,E,M] tensor");
         require_device(q_in);
         same_device(q_in, {k_in, v_in, delta_in, A, D, z_, bias, W, lengths});
@@ -323,7 +326,7 @@ struct ResidualNormFn : torch::autograd::Function<ResidualNormFn> {
         if ((ab.defined() && !aw.defined()) || (bb.defined() && !bw.defined())) fail("a norm's bias without its weight");
         require_device(y_in);
         same_device(y_in, {x_in, g, scale, aw, ab, bw, bb});
-        const at::Tensor y = y_in.contiguous(), x = x_in.contiguous(), gate = g.defined() ? g.contiguous() : g, r = at::empty(x.sizes(), x.options());
+        const at::Tensor y = plain(y_in), x = plain(x_in), gate = plain(g), r = at::empty(x.sizes(), x.options());
         at::Tensor n, stats;
         if (bw.defined()) n = at::empty(y.sizes(), y.options());
         const fwp_norm_args a = args(y, x, gate, scale, aw, ab, bw, bb, eps, rms, act);
@@ -347,7 +350,7 @@ struct ResidualNormFn : torch::autograd::Function<ResidualNormFn> {
         once_only();
         const auto s = ctx->get_saved_variables();
         const at::Tensor &y = s[0], &x = s[1], &gate = s[2], &scale = s[3], &aw = s[4], &ab = s[5], &bw = s[6], &bb = s[7], &stats = s[8];
-        const at::Tensor gr = gr_in.defined() ? gr_in.contiguous() : gr_in, gn = gn_in.defined() ? gn_in.contiguous() : gn_in;
+        const at::Tensor gr = plain(gr_in), gn = plain(gn_in);
         const fwp_norm_args a =
             args(y, x, gate, scale, aw, ab, bw, bb, ctx->saved_data["eps"].toDouble(), ctx->saved_data["rms"].toBool(), ctx->saved_data["act"].toInt());
         LaunchGuard guard(y);
