@@ -123,3 +123,21 @@ def test_an_untouched_layer_takes_two_operators(fwp, monkeypatch, device):
     monkeypatch.setattr(layers, "residual_norm", lambda *a, **k: (calls.append(k), real(*a, **k))[1])
     m(torch.randn(5, 2, COLS, device=device))
     assert [("after" in k, "before" in k) for k in calls] == [(True, True), (True, False)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("change", ["norm_attn hook", "norm_mid eps", "norm_ff rms", "norm_mid identity"])
+def test_under_autocast(fwp, change, dtype):
+    """About sixteen roundings of the narrow type lie on the way: the products' operands and results, and those of the residual norms beside them."""
+    m = layer_of(fwp)
+    ref = copy.deepcopy(m)
+    CHANGES[change](m), CHANGES[change](ref)
+    h = torch.randn(7, 3, COLS)
+    want = by_modules(ref.double(), h.double())
+    m = m.cuda()
+    with torch.autocast("cuda", dtype):
+        got = m(h.cuda())
+    got.square().mean().backward()
+    assert got.dtype is torch.float32 and float((got.cpu().double() - want).norm()) <= 16 * F.half_step(dtype) * float(want.norm())
+    assert all(p.grad is not None and torch.isfinite(p.grad).all() for p in m.parameters())
