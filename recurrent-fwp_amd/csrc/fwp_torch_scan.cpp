@@ -112,6 +112,12 @@ bool records(std::initializer_list<const at::Tensor *> ts) {
     return false;
 }
 
+// Autograd refuses to keep an inference tensor, but only once the call is done and a state has gone on: refused before that.
+void may_be_kept(std::initializer_list<at::Tensor> ts) {
+    for (const at::Tensor &t : ts)
+        if (t.defined() && t.is_inference()) fail("an inference tensor cannot be kept for a backward pass: clone it outside inference mode");
+}
+
 // A tangent of forward-mode differentiation would be lost without a word: its tensor need not require a gradient.
 void no_tangents(std::initializer_list<const at::Tensor *> ts) {
     for (const at::Tensor *t : ts)
@@ -152,6 +158,7 @@ struct ConvFn : torch::autograd::Function<ConvFn> {
         require_device(x_in);
         same_device(x_in, {w, b, state, lengths});
         const at::Tensor x = rows_of(x_in), y = empty_rows(x);
+        if (ctx) may_be_kept({x, w, b, lengths});
         at::Tensor before;
         if (ctx && state.defined()) before = state.detach().clone();
         {
@@ -235,6 +242,7 @@ struct ScanFn : torch::autograd::Function<ScanFn> {
                          z = rows_of(z_, kMaxStep), out = empty_rows(v);
         fwp_scan_args a = args(v, delta, z, A, D, bias, lengths, softplus);
         a.q = view(q), a.k = view(k);
+        if (ctx) may_be_kept({v, delta, z, A, D, bias, lengths, q, k});
         LaunchGuard guard(q);
         at::Tensor saved;
         if (ctx) saved = scratch(fwp_scan_saved_floats(a.N, a.H, a.L, a.E, a.M), v);
