@@ -510,6 +510,64 @@ long long fwp_residual_norm_workspace(int rows, int cols);
 int fwp_residual_norm_bwd(const fwp_norm_args *a, const float *stats, const void *grad_r, const void *grad_n, const fwp_norm_grads *g,
                           float *workspace, void *stream);
 
+/*
+ * The sum rule with a decay for each head, per step
+ *   W[e][m] = exp(g) W[e][m] + k[e] v[m],  o[m] = scale sum_e q[e] W[e][m]
+ * q [N,HQ,L,E], k [N,HK,L,E], v [N,HV,L,M], o [N,H,L,M]; HQ, HK and HV divide H, and head h takes the rows of head h / (H / HQ) and so on.  E <= 128.
+ * g: fp32 at n dN + h dH + t dL, not positive; -inf empties the state.  per_head: g is of a head (dN and dL are 0), and so is its gradient.  lengths as
+ * above.  W [N,H,E,M] fp32 in/out (NULL: from zeros, not kept).  saved: NULL, or fwp_decayed_sum_saved_floats, 16-byte aligned, for a backward pass;
+ * workspace: fwp_decayed_sum_workspace(.., 0) floats, 16-byte aligned (NULL if that is 0).
+ */
+typedef struct fwp_dsum_args {
+    fwp_rows q, k, v;
+    const float *decay;
+    int64_t dN, dH, dL;
+    const int64_t *lengths;
+    float scale;
+    int type, per_head, N, H, L, E, M, HQ, HK, HV;
+} fwp_dsum_args;
+long long fwp_decayed_sum_saved_floats(int type, int N, int H, int L, int E, int M);
+long long fwp_decayed_sum_workspace(const fwp_dsum_args *a, int backward);
+int fwp_decayed_sum_fwd(const fwp_dsum_args *a, float *W, fwp_out_rows out, float *saved, float *workspace, void *stream);
+
+/* Its adjoint: gq, gk, gv like q, k, v; gdecay [H] if per_head, else [N,H,L].  workspace: fwp_decayed_sum_workspace(.., 1) floats, 16-byte aligned. */
+int fwp_decayed_sum_bwd(const fwp_dsum_args *a, const float *saved, fwp_rows grad_out, fwp_out_rows gq, fwp_out_rows gk, fwp_out_rows gv,
+                        float *gdecay, float *workspace, void *stream);
+
+/*
+ * Rotary positions of the rows of q [N,HQ,L,D] and k [N,HK,L,D] (k.ptr NULL: none), to oq and ok: the first 2 `pairs` channels turn,
+ *   (a, b) -> scale (a cos - b sin, a sin + b cos),  angle = position * frequencies[i]
+ * a and b being channels i and i + pairs, or 2i and 2i + 1 if `interleaved`; the others are copied.  The position of step t of sequence n is t, plus
+ * positions[n] where `positions` is [N], or positions[n][t] where each_step says that it is [N,L]; NULL: t.  frequencies [pairs] fp64, radians.  inverse: by minus the
+ * angle, which is the adjoint.  lengths as above: rows behind a sequence become zero.  Input and output may be the same rows.
+ */
+typedef struct fwp_rotary_args {
+    fwp_rows q, k;
+    const double *frequencies;
+    const int64_t *positions, *lengths;
+    float scale;
+    int type, interleaved, inverse, each_step, N, HQ, HK, L, D, pairs;
+} fwp_rotary_args;
+int fwp_rotary(const fwp_rotary_args *a, fwp_out_rows oq, fwp_out_rows ok, void *stream);
+
+/*
+ * Norm of groups of channels: every row's `groups` groups of `size` channels (size <= 1024, groups * size <= 65536), contiguous rows,
+ *   u = norm(group) weight + bias (either NULL: without it),  y = act(gate) u, or act(u) where gate is NULL
+ * norm as above; act: FWP_ACT_*.  x, gate, y of `type`; weight, bias [groups * size].
+ */
+typedef struct fwp_group_norm_args {
+    const void *x, *gate;
+    const float *weight, *bias;
+    float eps;
+    int type, rms, act, rows, groups, size;
+} fwp_group_norm_args;
+int fwp_group_norm_fwd(const fwp_group_norm_args *a, void *y, void *stream);
+
+/* Its adjoint: gx and ggate like x (ggate NULL without a gate), gweight and gbias [groups * size] or NULL.  workspace: fwp_group_norm_workspace floats. */
+long long fwp_group_norm_workspace(int type, int rows, int groups, int size);
+int fwp_group_norm_bwd(const fwp_group_norm_args *a, const void *grad_y, void *gx, void *ggate, float *gweight, float *gbias, float *workspace,
+                       void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -13,12 +13,14 @@ from .fast_lstm_v4 import FastLSTMv4, fast_lstm_v4
 from .fast_weight_rnn_v2 import FastRNNv2, fast_rnn_v2
 from .rec_update_fwm_tanh import FastWeightRecUpdateTanh, rec_update_fwm_tanh
 from .selective_scan import causal_conv, residual_norm, selective_scan
+from .decayed_sum import decayed_sum, group_norm, rotary, rotary_frequencies
 from .layers import (DeltaNetDecoderLayer, DeltaNetLayer, DeltaNetPrep, PositionalEmbedding, PositionwiseFF, SelectiveScanDecoderLayer,
                      SelectiveScanLayer)
 from .lm import DeltaNetLM
 
 __all__ = ["DeltaFastWeight", "fast_weight_delta", "FastWeightSum", "fast_weight_sum", "FastRNNv2", "fast_rnn_v2",
            "FastLSTMv4", "fast_lstm_v4",
-           "FastWeightRecUpdateTanh", "rec_update_fwm_tanh", "causal_conv", "selective_scan", "residual_norm", "DeltaNetLayer", "DeltaNetPrep",
+           "FastWeightRecUpdateTanh", "rec_update_fwm_tanh", "causal_conv", "selective_scan", "residual_norm", "decayed_sum", "rotary",
+           "rotary_frequencies", "group_norm", "DeltaNetLayer", "DeltaNetPrep",
            "DeltaNetDecoderLayer", "PositionwiseFF", "PositionalEmbedding", "SelectiveScanLayer", "SelectiveScanDecoderLayer",
            "DeltaNetLM"]

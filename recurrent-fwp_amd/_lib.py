@@ -56,6 +56,25 @@ class NormGrads(ctypes.Structure):
     _fields_ = [(n, ctypes.c_void_p) for n in ("gy", "gx", "ggate", "gscale", "gafter_weight", "gafter_bias", "gbefore_weight", "gbefore_bias")]
 
 
+class DecayedSumArgs(ctypes.Structure):
+    """struct fwp_dsum_args."""
+    _fields_ = [(n, View) for n in ("q", "k", "v")] + [("decay", ctypes.c_void_p)] + [(n, ctypes.c_int64) for n in ("dN", "dH", "dL")] + \
+               [("lengths", ctypes.c_void_p), ("scale", ctypes.c_float)] + \
+               [(n, ctypes.c_int) for n in ("type", "per_head", "N", "H", "L", "E", "M", "HQ", "HK", "HV")]
+
+
+class RotaryArgs(ctypes.Structure):
+    """struct fwp_rotary_args."""
+    _fields_ = [(n, View) for n in ("q", "k")] + [(n, ctypes.c_void_p) for n in ("frequencies", "positions", "lengths")] + [("scale", ctypes.c_float)] + \
+               [(n, ctypes.c_int) for n in ("type", "interleaved", "inverse", "each_step", "N", "HQ", "HK", "L", "D", "pairs")]
+
+
+class GroupNormArgs(ctypes.Structure):
+    """struct fwp_group_norm_args."""
+    _fields_ = [(n, ctypes.c_void_p) for n in ("x", "gate", "weight", "bias")] + [("eps", ctypes.c_float)] + \
+               [(n, ctypes.c_int) for n in ("type", "rms", "act", "rows", "groups", "size")]
+
+
 class FwpError(RuntimeError):
     pass
 
@@ -101,8 +120,15 @@ _MODEL_SIGNATURES = {
     "fwp_scan_bwd": [ctypes.POINTER(ScanArgs), _P, _V] + [OutView] * 5 + [_P] * 5,
     "fwp_residual_norm_fwd": [ctypes.POINTER(NormArgs)] + [_P] * 4,
     "fwp_residual_norm_bwd": [ctypes.POINTER(NormArgs)] + [_P] * 3 + [ctypes.POINTER(NormGrads)] + [_P] * 2,
+    # the decayed sum rule's block
+    "fwp_decayed_sum_workspace": [ctypes.POINTER(DecayedSumArgs), _I],
+    "fwp_decayed_sum_fwd": [ctypes.POINTER(DecayedSumArgs), _P, OutView] + [_P] * 3,
+    "fwp_decayed_sum_bwd": [ctypes.POINTER(DecayedSumArgs), _P, _V] + [OutView] * 3 + [_P] * 3,
+    "fwp_rotary": [ctypes.POINTER(RotaryArgs), OutView, OutView, _P],
+    "fwp_group_norm_fwd": [ctypes.POINTER(GroupNormArgs)] + [_P] * 2,
+    "fwp_group_norm_bwd": [ctypes.POINTER(GroupNormArgs)] + [_P] * 7,
 }
-_WORKSPACES = {"fwp_conv_workspace": 5, "fwp_scan_saved_floats": 5, "fwp_scan_workspace": 6, "fwp_residual_norm_workspace": 2, "fwp_product_workspace": 3, "fwp_matmul_workspace": 3, "fwp_nll_workspace": 2, "fwp_layer_norm_workspace": 2}
+_WORKSPACES = {"fwp_decayed_sum_saved_floats": 6, "fwp_group_norm_workspace": 4, "fwp_conv_workspace": 5, "fwp_scan_saved_floats": 5, "fwp_scan_workspace": 6, "fwp_residual_norm_workspace": 2, "fwp_product_workspace": 3, "fwp_matmul_workspace": 3, "fwp_nll_workspace": 2, "fwp_layer_norm_workspace": 2}
 EXPORTS = sorted(list(_SIGNATURES) + list(_MODEL_SIGNATURES) + list(_WORKSPACES) + ["fwp_strerror", "fwp_query", "fwp_check_device", "fwp_config",
                                        "fwp_delta_ckpt_floats", "fwp_delta_segment_floats", "fwp_delta_bwd_segment_floats", "fwp_delta_kind", "fwp_delta_fwd_kind"])
 KIND_LDS, KIND_SCAN, KIND_CHUNKED, KIND_SPLIT, KIND_PHASE, KIND_STEP = 0, 1, 2, 3, 4, 5
@@ -143,6 +169,8 @@ def lib():
             if hasattr(handle, name):
                 getattr(handle, name).argtypes = [ctypes.c_int] * n
                 getattr(handle, name).restype = ctypes.c_longlong
+        if hasattr(handle, "fwp_decayed_sum_workspace"):
+            handle.fwp_decayed_sum_workspace.restype = ctypes.c_longlong
         handle.fwp_delta_kind.argtypes = [_I] + [_V] * 4 + [_I] * 5
         handle.fwp_delta_kind.restype = ctypes.c_int
         handle.fwp_delta_fwd_kind.argtypes = [_V] * 4 + [OutView] + [_I] * 6

@@ -1,0 +1,289 @@
+// The decayed sum rule: how a call is cut into workgroups, what joins its parts, and single steps.
+#include <algorithm>
+#include <type_traits>
+
+#include "fwp_dsum.hpp"
+
+namespace fwp {
+namespace {
+
+// What the segments leave, joined in order: every segment's first state from the one before it.  Slot s of `ends` holds what segment s - 1 leaves when it
+// starts from zero, and then the state that segment s starts from; BACKWARD: of segment s + 1, from the last to the first.  One thread a number of the state;
+// the slots of eight segments are loaded at once.
+template <bool BACKWARD>
+__global__ __launch_bounds__(256) void k_dsum_join(float *ends, const float *factors, const float *from, int E, int M, int Ep, int Mp, int segments) {
+    const int cells = Ep * Mp, blocks = cells / 256, cell = blockIdx.x % blocks * 256 + threadIdx.x;      // at least 32 x 32 of them
+    const int64_t head = blockIdx.x / blocks;
+    float *at = ends + head * segments * cells + cell;
+    const float *f = factors + head * segments;
+    float cur = 0.f;
+    if (!BACKWARD && from) {
+        const int e = cell / Mp, m = cell % Mp;
+        if (e < E && m < M) cur = from[(head * E + e) * M + m];
+    }
+    at[(int64_t)(BACKWARD ? segments - 1 : 0) * cells] = cur;
+    for (int s0 = 1; s0 < segments; s0 += 8) {
+        float x[8], y[8];
+#pragma unroll
+        for (int i = 0; i < 8; i++)
+            if (s0 + i < segments) {
+                const int slot = BACKWARD ? segments - 1 - (s0 + i) : s0 + i;
+                x[i] = at[(int64_t)slot * cells];
+                y[i] = f[BACKWARD ? slot + 1 : slot - 1];
+            }
+#pragma unroll
+        for (int i = 0; i < 8; i++)
+            if (s0 + i < segments) {
+                const int slot = BACKWARD ? segments - 1 - (s0 + i) : s0 + i;
+                cur = fmaf(y[i], cur, x[i]);
+                at[(int64_t)slot * cells] = cur;
+            }
+    }
+}
+
+// rows [N,G,L,D] of type T as the sum of `parts` fp32 tensors of that shape, in their order
+template <typename T>
+__global__ __launch_bounds__(256) void k_sum_parts(const float *x, fwp_out_rows out, int parts, int64_t total, int G, int L, int D) {
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
+        float s = 0.f;
+        for (int p = 0; p < parts; p++) s += x[p * total + i];
+        const int d = i % D;
+        int64_t r = i / D;
+        const int64_t t = r % L;
+        r /= L;
+        store(row<T>(out, r / G, r % G, t) + d, s);
+    }
+}
+
+// [H] = sums over n and the parts of each head of x [N,H,parts], one workgroup a head
+__global__ __launch_bounds__(256) void k_sum_heads(const float *x, float *out, int N, int H, int parts) {
+    __shared__ float part[4];
+    const int h = blockIdx.x;
+    float s = 0.f;
+    for (int64_t i = threadIdx.x; i < (int64_t)N * parts; i += 256) s += x[(i / parts * H + h) * parts + i % parts];
+#pragma unroll
+    for (int off = 1; off < 64; off *= 2) s += __shfl_xor(s, off);
+    if (threadIdx.x % 64 == 0) part[threadIdx.x / 64] = s;
+    __syncthreads();
+    if (threadIdx.x == 0) out[h] = (part[0] + part[1]) + (part[2] + part[3]);
+}
+
+// One step: S = exp(g) S + k (x) v, o = scale S^T q.  Bound by the state, which is read and written once: a lane holds four columns of R rows, all loaded before
+// any is used; X lanes lie side by side on a row.
+template <typename T, int R>
+__global__ __launch_bounds__(256) void k_dsum_step(const DsumWalk a, int X, int blocks) {
+    __shared__ float part[4][128 + 4];
+    const int tid = threadIdx.x, x = tid % X, y = tid / X, Y = 256 / X;
+    const int head = blockIdx.x / blocks, block = blockIdx.x % blocks, h = head % a.H, n = head / a.H, m = (block * X + x) * 4;
+    const T *q = row<T>(a.q, n, h / (a.H / a.HQ), 0), *k = row<T>(a.k, n, h / (a.H / a.HK), 0), *v = row<T>(a.v, n, h / (a.H / a.HV), 0);
+    T *out = row<T>(a.out, n, h, 0);
+    const bool counts = length_of(a.lengths, n, 1) > 0;
+    if (!counts) {
+        if (y == 0)
+            for (int i = 0; i < 4; i++)
+                if (m + i < a.M) out[m + i] = (T)0.f;
+        return;
+    }
+    struct __attribute__((packed, aligned(4))) Four { float x[4]; };
+    const float *from = a.from ? a.from + ((int64_t)n * a.H + h) * a.E * a.M : nullptr;
+    const bool whole = m + 4 <= a.M;
+    float S[R][4], kv[R], qv[R], vv[4], o[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int r = 0; r < R; r++) {
+        const int e = y + r * Y;
+        kv[r] = e < a.E ? (float)k[e] : 0.f, qv[r] = e < a.E ? (float)q[e] : 0.f;
+        if (from && e < a.E && whole) {
+            const Four s = *reinterpret_cast<const Four *>(from + (int64_t)e * a.M + m);
+#pragma unroll
+            for (int i = 0; i < 4; i++) S[r][i] = s.x[i];
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; i++) S[r][i] = from && e < a.E && m + i < a.M ? from[(int64_t)e * a.M + m + i] : 0.f;
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; i++) vv[i] = m + i < a.M ? (float)v[m + i] : 0.f;
+    const float decay = exp_of(a.decay[n * a.dN + h * a.dH]);
+#pragma unroll
+    for (int r = 0; r < R; r++) {
+        const int e = y + r * Y;
+        Four s;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            s.x[i] = fmaf(kv[r], vv[i], decay * S[r][i]);
+            if (e < a.E) o[i] = fmaf(qv[r], s.x[i], o[i]);
+        }
+        if (!a.to || e >= a.E) continue;
+        float *to = a.to + (((int64_t)n * a.H + h) * a.E + e) * a.M + m;
+        if (whole) *reinterpret_cast<Four *>(to) = s;
+        else
+            for (int i = 0; i < 4; i++)
+                if (m + i < a.M) to[i] = s.x[i];
+    }
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+        for (int off = X; off < 64; off *= 2) o[i] += __shfl_xor(o[i], off);
+    const int wave = tid / 64, lane = tid % 64;
+    if (lane < X) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) part[wave][4 * lane + i] = o[i];
+    }
+    __syncthreads();
+    if (tid < 4 * X && block * X * 4 + tid < a.M)
+        store(out + block * X * 4 + tid, a.scale * ((part[0][tid] + part[1][tid]) + (part[2][tid] + part[3][tid])));
+}
+
+struct Plan {
+    int Ep, MS, Mp, slices, chunk, chunks, segments, per;
+    int64_t heads, cells, ends;      // ends: floats of the segments' states and factors
+};
+
+// Segments: enough workgroups that every CU has several, none shorter than four chunks.
+Plan plan_of(int type, int N, int H, int L, int E, int M) {
+    Plan p{};
+    p.Ep = E <= 32 ? 32 : E <= 64 ? 64 : 128;
+    p.MS = M <= 32 ? 32 : M <= 64 ? 64 : 128;
+    p.slices = (M + p.MS - 1) / p.MS;
+    p.Mp = p.slices * p.MS;
+    p.chunk = type == FWP_BF16 ? kChunkOf<bf16_t> : type == FWP_F16 ? kChunkOf<half_t> : kChunkOf<float>;
+    p.chunks = (L + p.chunk - 1) / p.chunk;
+    p.heads = (int64_t)N * H;
+    const int64_t units = p.heads * p.slices, wanted = 256 * 32 / (p.MS / 16);
+    const int64_t most = std::max(1, p.chunks / 4);
+    const int64_t segments = std::min(most, std::max<int64_t>(1, (wanted + units - 1) / units));
+    p.per = (int)((p.chunks + segments - 1) / segments);
+    p.segments = (p.chunks + p.per - 1) / p.per;
+    p.cells = (int64_t)p.Ep * p.Mp;
+    p.ends = p.segments > 1 ? p.heads * p.segments * (p.cells + 1) : 0;
+    return p;
+}
+
+int64_t padded(int64_t n) { return (n + 3) & ~int64_t(3); }
+
+struct BackwardRoom {
+    int64_t q, k, v, decay, total;
+};
+BackwardRoom backward_room(const fwp_dsum_args &a, const Plan &p) {
+    BackwardRoom r{};
+    const int64_t rows = p.heads * a.L;
+    r.q = a.HQ < a.H || p.slices > 1 ? rows * p.slices * a.E : 0;
+    r.k = a.HK < a.H || p.slices > 1 ? rows * p.slices * a.E : 0;
+    r.v = a.HV < a.H ? rows * a.M : 0;
+    r.decay = a.per_head ? p.heads * p.slices * p.segments : p.slices > 1 ? rows * p.slices : 0;
+    r.total = padded(p.ends) + padded(r.q) + padded(r.k) + padded(r.v) + padded(r.decay);
+    return r;
+}
+
+DsumWalk walk_of(const fwp_dsum_args &a, const Plan &p) {
+    DsumWalk w{};
+    w.q = a.q, w.k = a.k, w.v = a.v;
+    w.decay = a.decay, w.dN = a.dN, w.dH = a.dH, w.dL = a.dL;
+    w.lengths = a.lengths;
+    w.scale = a.scale;
+    w.N = a.N, w.H = a.H, w.L = a.L, w.E = a.E, w.M = a.M, w.HQ = a.HQ, w.HK = a.HK, w.HV = a.HV;
+    w.Mp = p.Mp, w.slices = p.slices, w.segments = p.segments, w.per = p.per;
+    w.sum_decay = a.per_head;
+    return w;
+}
+
+int launch(int which, const fwp_dsum_args &a, const Plan &p, const DsumWalk &w, int segments, hipStream_t s) {
+    const int64_t blocks = p.heads * p.slices * segments;
+    if (!fits_launch(blocks, 4 * p.MS) || !fits_launch(p.heads * (p.cells / 256), 256)) return FWP_E_SHAPE;
+    bool done = false;
+    by_type(a.type, [&](auto t) { done = dsum_launch<decltype(t)>(which, w, p.Ep, p.MS, (unsigned)blocks, s); });
+    return done ? 0 : FWP_E_SHAPE;
+}
+
+template <typename T>
+int launch_step(const DsumWalk &w, hipStream_t s) {
+    const int columns = (w.M + 3) / 4;
+    int X = 1;
+    while (X < columns && X < 32) X *= 2;
+    const int rows = (w.E + 256 / X - 1) / (256 / X);
+    const int blocks = (columns + X - 1) / X;
+    const int64_t grid = (int64_t)blocks * w.N * w.H;
+    if (!fits_launch(grid, 256)) return FWP_E_SHAPE;
+    if (rows <= 1) k_dsum_step<T, 1><<<(unsigned)grid, 256, 0, s>>>(w, X, blocks);
+    else if (rows <= 2) k_dsum_step<T, 2><<<(unsigned)grid, 256, 0, s>>>(w, X, blocks);
+    else if (rows <= 4) k_dsum_step<T, 4><<<(unsigned)grid, 256, 0, s>>>(w, X, blocks);
+    else if (rows <= 8) k_dsum_step<T, 8><<<(unsigned)grid, 256, 0, s>>>(w, X, blocks);
+    else k_dsum_step<T, 16><<<(unsigned)grid, 256, 0, s>>>(w, X, blocks);
+    return (int)hipGetLastError();
+}
+
+}  // namespace
+
+int64_t dsum_saved_floats(int type, int N, int H, int L, int E, int M) {
+    const Plan p = plan_of(type, N, H, L, E, M);
+    return p.heads * p.chunks * p.cells;
+}
+
+int64_t dsum_workspace(const fwp_dsum_args &a, bool backward) {
+    const Plan p = plan_of(a.type, a.N, a.H, a.L, a.E, a.M);
+    return backward ? backward_room(a, p).total : p.ends;
+}
+
+int dsum_fwd(const fwp_dsum_args &a, float *W, fwp_out_rows out, float *saved, float *workspace, hipStream_t s) {
+    const Plan p = plan_of(a.type, a.N, a.H, a.L, a.E, a.M);
+    DsumWalk w = walk_of(a, p);
+    w.out = out;
+    w.from = w.to = W;
+    w.saved = saved;
+    if (a.L == 1 && !saved) {
+        int rc = FWP_E_SHAPE;
+        by_type(a.type, [&](auto t) { rc = launch_step<decltype(t)>(w, s); });
+        return rc;
+    }
+    if (p.segments > 1) {
+        if (!workspace) return FWP_E_NULL;
+        w.ends = workspace;
+        w.factors = workspace + p.heads * p.segments * p.cells;
+        if (int rc = launch(kDsumForwardEnds, a, p, w, p.segments - 1, s)) return rc;
+        k_dsum_join<false><<<(unsigned)(p.heads * (p.cells / 256)), 256, 0, s>>>(w.ends, w.factors, W, a.E, a.M, p.Ep, p.Mp, p.segments);
+    }
+    if (int rc = launch(kDsumForward, a, p, w, p.segments, s)) return rc;
+    return (int)hipGetLastError();
+}
+
+int dsum_bwd(const fwp_dsum_args &a, const float *saved, fwp_rows gout, fwp_out_rows gq, fwp_out_rows gk, fwp_out_rows gv, float *gdecay,
+             float *workspace, hipStream_t s) {
+    const Plan p = plan_of(a.type, a.N, a.H, a.L, a.E, a.M);
+    const BackwardRoom room = backward_room(a, p);
+    DsumWalk w = walk_of(a, p);
+    w.go = gout;
+    w.gq = gq, w.gk = gk, w.gv = gv;
+    w.saved = const_cast<float *>(saved);
+    float *at = workspace;
+    const auto take = [&](int64_t n) {
+        float *r = n ? at : nullptr;
+        at += padded(n);
+        return r;
+    };
+    w.ends = take(p.ends);
+    w.factors = w.ends ? w.ends + p.heads * p.segments * p.cells : nullptr;
+    w.pq = take(room.q), w.pk = take(room.k), w.pv = take(room.v);
+    float *parts = take(room.decay);
+    w.gdecay = parts ? parts : gdecay;
+    if (p.segments > 1) {
+        if (int rc = launch(kDsumBackwardEnds, a, p, w, p.segments - 1, s)) return rc;
+        k_dsum_join<true><<<(unsigned)(p.heads * (p.cells / 256)), 256, 0, s>>>(w.ends, w.factors, nullptr, a.E, a.M, p.Ep, p.Mp, p.segments);
+    }
+    if (int rc = launch(kDsumBackward, a, p, w, p.segments, s)) return rc;
+    const auto blocks = [](int64_t n) { return (unsigned)std::min<int64_t>((n + 255) / 256, 4096); };
+    by_type(a.type, [&](auto t) {
+        using T = decltype(t);
+        const int64_t nq = (int64_t)a.N * a.HQ * a.L * a.E, nk = (int64_t)a.N * a.HK * a.L * a.E, nv = (int64_t)a.N * a.HV * a.L * a.M;
+        if (w.pq) k_sum_parts<T><<<blocks(nq), 256, 0, s>>>(w.pq, gq, a.H / a.HQ * p.slices, nq, a.HQ, a.L, a.E);
+        if (w.pk) k_sum_parts<T><<<blocks(nk), 256, 0, s>>>(w.pk, gk, a.H / a.HK * p.slices, nk, a.HK, a.L, a.E);
+        if (w.pv) k_sum_parts<T><<<blocks(nv), 256, 0, s>>>(w.pv, gv, a.H / a.HV, nv, a.HV, a.L, a.M);
+    });
+    if (a.per_head) {
+        k_sum_heads<<<a.H, 256, 0, s>>>(parts, gdecay, a.N, a.H, p.slices * p.segments);
+    } else if (parts) {
+        const int64_t n = p.heads * a.L;
+        k_sum_parts<float><<<blocks(n), 256, 0, s>>>(parts, fwp_out_rows{gdecay, (int64_t)a.H * a.L, a.L, 1}, p.slices, n, a.H, a.L, 1);
+    }
+    return (int)hipGetLastError();
+}
+
+}  // namespace fwp

@@ -1,0 +1,816 @@
+// The sum rule with a decay for each head, in chunks on the matrix cores.
+//
+//   S_t = a_t S_{t-1} + k_t (x) v_t,  o_t = scale S_t^T q_t,  a_t = exp(g_t), g_t of a head or of a step of a head
+//
+// Over a chunk of C steps with b_t = g_1 + .. + g_t, S the state before it and G the adjoint of the state behind it (both without `scale`):
+//
+//   P_ts = exp(b_t - b_s) q_t . k_s (s <= t)       o  = scale (P V + exp(b) Q S)         S' = exp(b_C) S + K^T (exp(b_C - b) V)
+//   R_ts = exp(b_t - b_s) do_t . v_s (s <= t)      dq = scale (R K + exp(b) dO S^T)      dk = scale (R^T Q + exp(b_C - b) V G^T)
+//   G'   = exp(b_C) G + Q^T (exp(b) dO)            dv = scale (P^T dO + exp(b_C - b) K G)
+//   dg_t = sum_{s >= t in the chunk} (q_s . dq_s - k_s . dk_s) + scale <G, S'>
+//
+// Every factor is exp of a difference that is itself a sum of decays, at most 1 where they are not positive.  The sums b are made in 64 bits and kept as a
+// pair of floats: behind a step of strong decay, differences of small ones would otherwise have lost their digits.  The inner product <G, S'> at every
+// chunk's end keeps the decays' gradients from being differences of sums over the whole sequence.
+//
+// A workgroup owns a sequence's head and a slice of its value columns, and walks over the chunks of a segment with the state in registers:
+// a wave holds all key rows of MW x 16 columns.  A sequence is cut into segments where there are too few of them to fill the GPU: a first kernel walks over each
+// but the last from zero, a second one joins what they leave, and the walk proper starts every segment from its own state.
+#pragma once
+#include "fwp_parts.hpp"
+
+namespace fwp {
+
+template <typename T>
+constexpr int kChunkOf = sizeof(T) == 2 && kPartsOf<T> == 1 ? 64 : 32;
+// Orders of the products that end in results: of fewer bits than fp32, 2^-16 of a term is far below their rounding
+template <typename T>
+constexpr int kOrdersOf = sizeof(T) == 2 ? 2 : 3;
+constexpr int kWide = 3;      // orders of what ends in fp32: the state, its adjoint, the decays' gradients
+
+struct DsumWalk {
+    fwp_rows q, k, v, go;
+    fwp_out_rows out, gq, gk, gv;      // gq, gk, gv: used where the partial buffers are NULL
+    const float *decay;
+    int64_t dN, dH, dL;
+    const int64_t *lengths;
+    const float *from;                 // the state a sequence starts from (NULL: zeros), [N,H,E,M]
+    float *to;                         // the state after the last step (NULL: not kept)
+    float *saved;                      // [N,H,chunks,Ep,Mp]: the states before each chunk
+    float *ends, *factors;             // [N,H,segments,Ep,Mp], [N,H,segments]
+    float *pq, *pk, *pv;               // partial gradients [parts][N,G,L,E|M]
+    float *gdecay;                     // [slices][N,H,L], or [N,H,slices,segments] where a head has one decay
+    float scale;
+    int N, H, L, E, M, HQ, HK, HV, Mp, slices, segments, per;      // per: chunks of a segment
+    int sum_decay;
+};
+
+// Workgroups b, b + 8, .. run on one XCD: neighbours in the order of the work, which share rows, get numbers that lie 8 apart.
+__device__ __forceinline__ int64_t by_xcd(int64_t b, int64_t n) {
+    const int64_t whole = n / 8 * 8;
+    return b < whole ? b % 8 * (n / 8) + b / 8 : b;
+}
+
+template <int C>
+struct alignas(16) Decays {
+    float hi[C], lo[C], into[C], rest[C];
+    float whole, pad[3];
+
+    // One wave: the sums over a chunk of its steps' decays, lane t those up to step t.  A decay below -1e5 is 0 all the same.
+    __device__ __forceinline__ double sum(float g, int lane) {
+        constexpr float least = -1e5f;
+        double x = (double)(g < least ? least : g) * 1.4426950408889634074;
+#pragma unroll
+        for (int off = 1; off < C; off *= 2) {
+            const double y = __shfl_up(x, off);
+            if (lane >= off) x += y;
+        }
+        const double total = __shfl(x, C - 1);
+        if (lane < C) {
+            const float h = (float)x;
+            hi[lane] = h;
+            lo[lane] = (float)(x - (double)h);
+            into[lane] = __builtin_amdgcn_exp2f(h);
+            rest[lane] = __builtin_amdgcn_exp2f((float)(total - x));
+        }
+        if (lane == 0) whole = __builtin_amdgcn_exp2f((float)total);
+        return total;
+    }
+    // exp(b_t - b_s) for the four steps s ..; 0 where s > t
+    __device__ __forceinline__ v4f between(int t, int s) const {
+        const v4f h = *reinterpret_cast<const v4f *>(&hi[s]), l = *reinterpret_cast<const v4f *>(&lo[s]);
+        const float ht = hi[t], lt = lo[t];
+        v4f f;
+#pragma unroll
+        for (int i = 0; i < 4; i++) f[i] = s + i <= t ? __builtin_amdgcn_exp2f((ht - h[i]) + (lt - l[i])) : 0.f;
+        return f;
+    }
+};
+
+// W consecutive numbers of a row whose element `col` is the first, columns below `cols` only
+template <typename T, int W>
+__device__ __forceinline__ void store_some(T *at, int col, int cols, const float (&x)[W]) {
+    if (col + W <= cols) {
+        struct __attribute__((packed, aligned(sizeof(T)))) Any { T x[W]; };
+        Any a;
+#pragma unroll
+        for (int i = 0; i < W; i++) a.x[i] = (T)x[i];
+        *reinterpret_cast<Any *>(at + col) = a;
+    } else {
+#pragma unroll
+        for (int i = 0; i < W; i++)
+            if (col + i < cols) at[col + i] = (T)x[i];
+    }
+}
+
+// ------------------------------------------------------------------ forward
+
+template <typename T, int NE, int NW, int MW>
+struct DsumForward {
+    static constexpr int C = kChunkOf<T>, P = kPartsOf<T>, O = kOrdersOf<T>, E = 16 * NE, MS = 16 * MW * NW, kThreads = 64 * NW;
+    static constexpr int NB = NE / 2, SB = C / 32, TT = C / 16;
+    struct Shared {
+        Tile<C, E, P> q, k;
+        Tile<C, MS, P> v;
+        Tile<C, C, O> p;
+        Decays<C> d[2];
+    };
+    struct Ends {
+        Tile<C, E, P> k;
+        Tile<C, MS, P> v;
+        Decays<C> d[2];
+    };
+};
+
+// ENDS: the state that a segment leaves when it starts from zero, and the segment's whole decay; nothing else.
+template <typename T, int NE, int NW, int MW, bool ENDS>
+__global__ __launch_bounds__(64 * NW) void k_dsum_fwd(const DsumWalk a) {
+    using F = DsumForward<T, NE, NW, MW>;
+    constexpr int C = F::C, P = F::P, O = F::O, E = F::E, MS = F::MS, NB = F::NB, SB = F::SB, TT = F::TT;
+    __shared__ std::conditional_t<ENDS, typename F::Ends, typename F::Shared> sh;
+    const int tid = threadIdx.x, lane = tid % 64, wave = tid / 64, g = lane / 16, c = lane % 16;
+
+    const int segments = ENDS ? a.segments - 1 : a.segments;
+    int64_t w = by_xcd(blockIdx.x, gridDim.x);
+    const int slice = w % a.slices;
+    w /= a.slices;
+    const int seg = w % segments;
+    w /= segments;
+    const int h = w % a.H, n = w / a.H;
+
+    const int len = length_of(a.lengths, n, a.L), chunks = (a.L + C - 1) / C, live = (len + C - 1) / C;
+    const int first = seg * a.per, last = min(first + a.per, chunks), stop = min(last, live);
+    const int hq = h / (a.H / a.HQ), hk = h / (a.H / a.HK), hv = h / (a.H / a.HV), m0 = slice * MS, mcols = min(a.M - m0, MS), mw = wave * 16 * MW;
+    const T *qb = row<T>(a.q, n, hq, 0), *kb = row<T>(a.k, n, hk, 0), *vb = row<T>(a.v, n, hv, 0) + m0;
+    const float *gb = a.decay + n * a.dN + h * a.dH;
+    T *ob = nullptr;
+    if constexpr (!ENDS) ob = row<T>(a.out, n, h, 0) + m0;
+
+    v4f S[NB][2][MW];
+    const int64_t head = (int64_t)n * a.H + h;
+    {
+        const float *from = nullptr;
+        int64_t stride = a.M;
+        int rows = a.E, cols = a.M;
+        if (!ENDS) {
+            if (a.segments > 1) from = a.ends + (head * a.segments + seg) * E * a.Mp, stride = a.Mp, rows = E, cols = a.Mp;
+            else if (a.from) from = a.from + head * a.E * a.M;
+        }
+#pragma unroll
+        for (int b = 0; b < NB; b++)
+#pragma unroll
+            for (int u = 0; u < 2; u++)
+#pragma unroll
+                for (int j = 0; j < MW; j++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        const int e = 32 * b + 8 * g + 4 * u + i, m = m0 + mw + place(MW, c, j);
+                        S[b][u][j][i] = from && e < rows && m < cols ? from[e * stride + m] : 0.f;
+                    }
+    }
+    if constexpr (!ENDS) {      // tiles of P above the diagonal stay zero
+        for (int i = tid; i < (int)(sizeof(sh.p) / 16); i += 64 * NW) reinterpret_cast<v4f *>(&sh.p)[i] = v4f{0, 0, 0, 0};
+    }
+
+    Stage<T, C, E, 64 * NW> sq, sk;
+    Stage<T, C, MS, 64 * NW> sv;
+    double total = 0;
+    float gnext = 0;
+    const auto fetch = [&](int chunk) {
+        const int64_t t0 = (int64_t)chunk * C;
+        const int rows = len - (int)t0;
+        if constexpr (!ENDS) sq.load(qb + t0 * a.q.sL, a.q.sL, rows, a.E, tid);
+        sk.load(kb + t0 * a.k.sL, a.k.sL, rows, a.E, tid);
+        sv.load(vb + t0 * a.v.sL, a.v.sL, rows, mcols, tid);
+        if (wave == NW - 1) gnext = lane < C && lane < rows ? gb[(t0 + lane) * a.dL] : 0.f;
+    };
+    if (first < stop) {
+        fetch(first);
+        if (wave == NW - 1) total += sh.d[first & 1].sum(gnext, lane);
+    }
+    for (int chunk = first; chunk < stop; chunk++) {
+        if constexpr (!ENDS) sq.put(sh.q, tid);
+        sk.put(sh.k, tid);
+        sv.put(sh.v, tid);
+        lds_barrier();
+        const Decays<C> &d = sh.d[chunk & 1];
+        if (chunk + 1 < stop) fetch(chunk + 1);
+
+        v4f acc[TT][MW];
+        if constexpr (!ENDS) {
+            if (a.saved) {
+                float *at = a.saved + (head * chunks + chunk) * E * a.Mp + m0 + mw;
+#pragma unroll
+                for (int b = 0; b < NB; b++)
+#pragma unroll
+                    for (int u = 0; u < 2; u++)
+#pragma unroll
+                        for (int j = 0; j < MW; j++)
+#pragma unroll
+                            for (int i = 0; i < 4; i++) at[(32 * b + 8 * g + 4 * u + i) * a.Mp + place(MW, c, j)] = S[b][u][j][i];
+            }
+            // P, a 16 x 16 tile of it at a time
+            for (int tile = wave; tile < TT * (TT + 1) / 2; tile += NW) {
+                int I = 0, J = tile;
+                while (J > I) J -= ++I;
+                v4f p = {0, 0, 0, 0};
+#pragma unroll
+                for (int b = 0; b < NB; b++) p = product<O>(sh.k.rows(16 * J, 32 * b, g, c), sh.q.rows(16 * I, 32 * b, g, c), p);
+                const int t = 16 * I + c, s = 16 * J + 4 * g;
+                const v4f f = d.between(t, s);
+                float x[4];
+#pragma unroll
+                for (int i = 0; i < 4; i++) x[i] = s + i <= t ? p[i] * f[i] : 0.f;      // a product beyond the diagonal may be infinite
+                v4b parts[O];
+                split<O, 4>(x, parts);
+#pragma unroll
+                for (int o = 0; o < O; o++) sh.p.put4(o, t, s, parts[o]);
+            }
+            // what the queries read from the state
+#pragma unroll
+            for (int I = 0; I < TT; I++)
+#pragma unroll
+                for (int j = 0; j < MW; j++) acc[I][j] = v4f{0, 0, 0, 0};
+#pragma unroll
+            for (int b = 0; b < NB; b++) {
+                Frag<O> s[MW];
+#pragma unroll
+                for (int j = 0; j < MW; j++) s[j] = split8<O>(S[b][0][j], S[b][1][j]);
+#pragma unroll
+                for (int I = 0; I < TT; I++) {
+                    const Frag<P> q = sh.q.rows(16 * I, 32 * b, g, c);
+#pragma unroll
+                    for (int j = 0; j < MW; j++) acc[I][j] = product<O>(s[j], q, acc[I][j]);
+                }
+            }
+#pragma unroll
+            for (int I = 0; I < TT; I++) {
+                const float f = d.into[16 * I + c];
+#pragma unroll
+                for (int j = 0; j < MW; j++) acc[I][j] *= f;
+            }
+            lds_barrier();
+        }
+#pragma unroll
+        for (int b = 0; b < NB; b++)
+#pragma unroll
+            for (int u = 0; u < 2; u++)
+#pragma unroll
+                for (int j = 0; j < MW; j++) S[b][u][j] *= d.whole;
+#pragma unroll
+        for (int sb = 0; sb < SB; sb++) {
+            Frag<kWide> vs[MW];
+            const v4f r0 = *reinterpret_cast<const v4f *>(&d.rest[32 * sb + 8 * g]), r1 = *reinterpret_cast<const v4f *>(&d.rest[32 * sb + 8 * g + 4]);
+#pragma unroll
+            for (int j = 0; j < MW; j++) {
+                const Frag<P> v = sh.v.template columns<MW>(mw, j, 32 * sb, g, c);
+                if constexpr (!ENDS) {
+#pragma unroll
+                    for (int I = 2 * sb; I < TT; I++) acc[I][j] = product<O>(v, sh.p.rows(16 * I, 32 * sb, g, c), acc[I][j]);
+                }
+                float x[8];
+                join8(v, x);
+#pragma unroll
+                for (int i = 0; i < 4; i++) x[i] *= r0[i], x[i + 4] *= r1[i];
+                vs[j] = split8<kWide>(x);
+            }
+#pragma unroll
+            for (int b = 0; b < NB; b++)
+#pragma unroll
+                for (int u = 0; u < 2; u++) {
+                    const Frag<P> k = sh.k.template columns<2>(32 * b, u, 32 * sb, g, c);
+#pragma unroll
+                    for (int j = 0; j < MW; j++) S[b][u][j] = product<kWide>(k, vs[j], S[b][u][j]);
+                }
+        }
+        if constexpr (!ENDS) {
+#pragma unroll
+            for (int I = 0; I < TT; I++) {
+                const int t = chunk * C + 16 * I + c;
+                if (t >= a.L) continue;
+                float x[4 * MW];
+#pragma unroll
+                for (int j = 0; j < MW; j++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) x[4 * j + i] = t < len ? acc[I][j][i] * a.scale : 0.f;
+                store_some<T, 4 * MW>(ob + t * a.out.sL, mw + 4 * MW * g, mcols, x);
+            }
+        }
+        if (chunk + 1 < stop && wave == NW - 1) total += sh.d[(chunk + 1) & 1].sum(gnext, lane);
+        lds_barrier();
+    }
+
+    if constexpr (ENDS) {
+        float *at = a.ends + (head * a.segments + seg + 1) * E * a.Mp + m0 + mw;
+#pragma unroll
+        for (int b = 0; b < NB; b++)
+#pragma unroll
+            for (int u = 0; u < 2; u++)
+#pragma unroll
+                for (int j = 0; j < MW; j++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) at[(32 * b + 8 * g + 4 * u + i) * a.Mp + place(MW, c, j)] = S[b][u][j][i];
+        if (tid == 64 * (NW - 1) && slice == 0) a.factors[head * a.segments + seg] = __builtin_amdgcn_exp2f((float)total);
+    } else {
+        // rows behind the sequence
+        for (int64_t i = (int64_t)max(stop, first) * C * MS + tid; i < (int64_t)min(last * C, a.L) * MS; i += 64 * NW) {
+            const int64_t t = i / MS;
+            const int m = i % MS;
+            if (m < mcols) ob[t * a.out.sL + m] = (T)0.f;
+        }
+        if (a.to && last == chunks) {
+            float *to = a.to + head * a.E * a.M;
+#pragma unroll
+            for (int b = 0; b < NB; b++)
+#pragma unroll
+                for (int u = 0; u < 2; u++)
+#pragma unroll
+                    for (int j = 0; j < MW; j++)
+#pragma unroll
+                        for (int i = 0; i < 4; i++) {
+                            const int e = 32 * b + 8 * g + 4 * u + i, m = m0 + mw + place(MW, c, j);
+                            if (e < a.E && m < a.M) to[(int64_t)e * a.M + m] = S[b][u][j][i];
+                        }
+        }
+    }
+}
+
+// ------------------------------------------------------------------ backward
+
+template <typename T, int NE, int NW, int MW>
+struct DsumBackward {
+    static constexpr int C = kChunkOf<T>, P = kPartsOf<T>, O = kOrdersOf<T>, E = 16 * NE, MS = 16 * MW * NW, kThreads = 64 * NW;
+    static constexpr int NB = NE / 2, SB = C / 32, TT = C / 16, MB = (MW * NW + 1) / 2;
+    static constexpr int EW = NE >= NW ? NE / NW : 1;      // key tiles of a wave
+    struct Shared {
+        Tile<C, E, P> q, k;
+        Tile<C, 32 * MB, P> v, go;
+        Tile<C, C, O> p;
+        Tile<C, C, kWide> r;
+        Decays<C> d[2];
+        float sums[NW][C], inner[NW];
+    };
+    struct Ends {
+        Tile<C, E, P> q;
+        Tile<C, MS, P> go;
+        Decays<C> d[2];
+    };
+};
+
+// The adjoint of a segment's first state when that of its last one is zero, and the segment's whole decay.
+template <typename T, int NE, int NW, int MW>
+__global__ __launch_bounds__(64 * NW) void k_dsum_bwd_ends(const DsumWalk a) {
+    using F = DsumBackward<T, NE, NW, MW>;
+    constexpr int C = F::C, P = F::P, E = F::E, MS = F::MS, NB = F::NB, SB = F::SB;
+    __shared__ typename F::Ends sh;
+    const int tid = threadIdx.x, lane = tid % 64, wave = tid / 64, g = lane / 16, c = lane % 16;
+    int64_t w = by_xcd(blockIdx.x, gridDim.x);
+    const int slice = w % a.slices;
+    w /= a.slices;
+    const int seg = w % (a.segments - 1) + 1;
+    w /= a.segments - 1;
+    const int h = w % a.H, n = w / a.H;
+    const int len = length_of(a.lengths, n, a.L), chunks = (a.L + C - 1) / C, live = (len + C - 1) / C;
+    const int first = seg * a.per, stop = min(min(first + a.per, chunks), live);
+    const int hq = h / (a.H / a.HQ), m0 = slice * MS, mcols = min(a.M - m0, MS), mw = wave * 16 * MW;
+    const T *qb = row<T>(a.q, n, hq, 0), *db = row<T>(a.go, n, h, 0) + m0;
+    const float *gb = a.decay + n * a.dN + h * a.dH;
+    const int64_t head = (int64_t)n * a.H + h;
+    v4f G[NB][2][MW];
+#pragma unroll
+    for (int b = 0; b < NB; b++)
+#pragma unroll
+        for (int u = 0; u < 2; u++)
+#pragma unroll
+            for (int j = 0; j < MW; j++) G[b][u][j] = v4f{0, 0, 0, 0};
+    Stage<T, C, E, 64 * NW> sq;
+    Stage<T, C, MS, 64 * NW> sd;
+    double total = 0;
+    float gnext = 0;
+    const auto fetch = [&](int chunk) {
+        const int64_t t0 = (int64_t)chunk * C;
+        const int rows = len - (int)t0;
+        sq.load(qb + t0 * a.q.sL, a.q.sL, rows, a.E, tid);
+        sd.load(db + t0 * a.go.sL, a.go.sL, rows, mcols, tid);
+        if (wave == NW - 1) gnext = lane < C && lane < rows ? gb[(t0 + lane) * a.dL] : 0.f;
+    };
+    if (first < stop) {
+        fetch(stop - 1);
+        if (wave == NW - 1) total += sh.d[(stop - 1) & 1].sum(gnext, lane);
+    }
+    for (int chunk = stop - 1; chunk >= first; chunk--) {
+        sq.put(sh.q, tid);
+        sd.put(sh.go, tid);
+        lds_barrier();
+        const Decays<C> &d = sh.d[chunk & 1];
+        if (chunk > first) fetch(chunk - 1);
+#pragma unroll
+        for (int b = 0; b < NB; b++)
+#pragma unroll
+            for (int u = 0; u < 2; u++)
+#pragma unroll
+                for (int j = 0; j < MW; j++) G[b][u][j] *= d.whole;
+#pragma unroll
+        for (int tb = 0; tb < SB; tb++) {
+            const v4f f0 = *reinterpret_cast<const v4f *>(&d.into[32 * tb + 8 * g]), f1 = *reinterpret_cast<const v4f *>(&d.into[32 * tb + 8 * g + 4]);
+            Frag<kWide> ds[MW];
+#pragma unroll
+            for (int j = 0; j < MW; j++) {
+                float x[8];
+                join8(sh.go.template columns<MW>(mw, j, 32 * tb, g, c), x);
+#pragma unroll
+                for (int i = 0; i < 4; i++) x[i] *= f0[i], x[i + 4] *= f1[i];
+                ds[j] = split8<kWide>(x);
+            }
+#pragma unroll
+            for (int b = 0; b < NB; b++)
+#pragma unroll
+                for (int u = 0; u < 2; u++) {
+                    const Frag<P> q = sh.q.template columns<2>(32 * b, u, 32 * tb, g, c);
+#pragma unroll
+                    for (int j = 0; j < MW; j++) G[b][u][j] = product<kWide>(q, ds[j], G[b][u][j]);
+                }
+        }
+        if (chunk > first && wave == NW - 1) total += sh.d[(chunk - 1) & 1].sum(gnext, lane);
+        lds_barrier();
+    }
+    float *at = a.ends + (head * a.segments + seg - 1) * E * a.Mp + m0 + mw;
+#pragma unroll
+    for (int b = 0; b < NB; b++)
+#pragma unroll
+        for (int u = 0; u < 2; u++)
+#pragma unroll
+            for (int j = 0; j < MW; j++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) at[(32 * b + 8 * g + 4 * u + i) * a.Mp + place(MW, c, j)] = G[b][u][j][i];
+    if (tid == 64 * (NW - 1) && slice == 0) a.factors[head * a.segments + seg] = __builtin_amdgcn_exp2f((float)total);
+}
+
+template <typename T, int NE, int NW, int MW>
+__global__ __launch_bounds__(64 * NW) void k_dsum_bwd(const DsumWalk a) {
+    using F = DsumBackward<T, NE, NW, MW>;
+    constexpr int C = F::C, P = F::P, O = F::O, E = F::E, MS = F::MS, NB = F::NB, SB = F::SB, TT = F::TT, MB = F::MB, EW = F::EW;
+    __shared__ typename F::Shared sh;
+    const int tid = threadIdx.x, lane = tid % 64, wave = tid / 64, g = lane / 16, c = lane % 16;
+    int64_t w = by_xcd(blockIdx.x, gridDim.x);
+    const int slice = w % a.slices;
+    w /= a.slices;
+    const int seg = w % a.segments;
+    w /= a.segments;
+    const int h = w % a.H, n = w / a.H;
+    const int len = length_of(a.lengths, n, a.L), chunks = (a.L + C - 1) / C, live = (len + C - 1) / C;
+    const int first = seg * a.per, last = min(first + a.per, chunks), stop = min(last, live);
+    const int rq = a.H / a.HQ, rk = a.H / a.HK, rv = a.H / a.HV, m0 = slice * MS, mcols = min(a.M - m0, MS), mw = wave * 16 * MW, ew = wave * 16 * EW;
+    const bool keys = ew < E;      // has this wave key rows of its own?
+    const T *qb = row<T>(a.q, n, h / rq, 0), *kb = row<T>(a.k, n, h / rk, 0), *vb = row<T>(a.v, n, h / rv, 0) + m0, *db = row<T>(a.go, n, h, 0) + m0;
+    const float *gb = a.decay + n * a.dN + h * a.dH;
+    const int64_t head = (int64_t)n * a.H + h;
+
+    // G: all key rows of this wave's value columns.  H: the same numbers, all value columns of its key rows, transposed.
+    v4f G[NB][2][MW], H[MB][2][EW];
+    {
+        const float *from = a.segments > 1 && seg + 1 < a.segments ? a.ends + (head * a.segments + seg) * E * a.Mp + m0 : nullptr;
+#pragma unroll
+        for (int b = 0; b < NB; b++)
+#pragma unroll
+            for (int u = 0; u < 2; u++)
+#pragma unroll
+                for (int j = 0; j < MW; j++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) G[b][u][j][i] = from ? from[(32 * b + 8 * g + 4 * u + i) * a.Mp + mw + place(MW, c, j)] : 0.f;
+#pragma unroll
+        for (int b = 0; b < MB; b++)
+#pragma unroll
+            for (int u = 0; u < 2; u++)
+#pragma unroll
+                for (int j = 0; j < EW; j++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        const int m = 32 * b + 8 * g + 4 * u + i;
+                        H[b][u][j][i] = from && keys && m < MS ? from[(ew + place(EW, c, j)) * a.Mp + m] : 0.f;
+                    }
+    }
+    for (int i = tid; i < (int)(sizeof(sh.p) / 16); i += 64 * NW) reinterpret_cast<v4f *>(&sh.p)[i] = v4f{0, 0, 0, 0};
+    for (int i = tid; i < (int)(sizeof(sh.r) / 16); i += 64 * NW) reinterpret_cast<v4f *>(&sh.r)[i] = v4f{0, 0, 0, 0};
+
+    // what this wave reads of a chunk's first state, by key rows
+    const auto before = [&](int chunk, int b, int j, float (&x)[8]) {
+        const int m = 32 * b + 8 * g;
+        if (keys && m < MS) {
+            const float *at = a.saved + ((head * chunks + chunk) * E + ew + place(EW, c, j)) * a.Mp + m0 + m;
+            const float4 lo = *reinterpret_cast<const float4 *>(at), hi = *reinterpret_cast<const float4 *>(at + 4);
+            x[0] = lo.x, x[1] = lo.y, x[2] = lo.z, x[3] = lo.w, x[4] = hi.x, x[5] = hi.y, x[6] = hi.z, x[7] = hi.w;
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; i++) x[i] = 0.f;
+        }
+    };
+    // <H, the first state of `chunk`>, this wave's part
+    const auto inner = [&](int chunk) {
+        float s = 0.f;
+#pragma unroll
+        for (int b = 0; b < MB; b++)
+#pragma unroll
+            for (int j = 0; j < EW; j++) {
+                float x[8];
+                before(chunk, b, j, x);
+#pragma unroll
+                for (int i = 0; i < 4; i++) s = fmaf(x[i], H[b][0][j][i], s), s = fmaf(x[i + 4], H[b][1][j][i], s);
+            }
+#pragma unroll
+        for (int off = 1; off < 64; off *= 2) s += __shfl_xor(s, off);
+        return s;
+    };
+
+    Stage<T, C, E, 64 * NW> sq, sk;
+    Stage<T, C, 32 * MB, 64 * NW> sv, sd;
+    float gnext = 0, all = 0;
+    const auto fetch = [&](int chunk) {
+        const int64_t t0 = (int64_t)chunk * C;
+        const int rows = len - (int)t0;
+        sq.load(qb + t0 * a.q.sL, a.q.sL, rows, a.E, tid);
+        sk.load(kb + t0 * a.k.sL, a.k.sL, rows, a.E, tid);
+        sv.load(vb + t0 * a.v.sL, a.v.sL, rows, mcols, tid);
+        sd.load(db + t0 * a.go.sL, a.go.sL, rows, mcols, tid);
+        if (wave == NW - 1) gnext = lane < C && lane < rows ? gb[(t0 + lane) * a.dL] : 0.f;
+    };
+    if (first < stop) {
+        fetch(stop - 1);
+        if (wave == NW - 1) sh.d[(stop - 1) & 1].sum(gnext, lane);
+    }
+    // the inner product at the segment's end, with the next segment's first state; behind the last chunk the adjoint is zero
+    float x_end = stop == last && stop < live ? inner(stop) : 0.f;
+
+    for (int chunk = stop - 1; chunk >= first; chunk--) {
+        sq.put(sh.q, tid);
+        sk.put(sh.k, tid);
+        sv.put(sh.v, tid);
+        sd.put(sh.go, tid);
+        if (lane == 0) sh.inner[wave] = x_end;
+        lds_barrier();
+        const Decays<C> &d = sh.d[chunk & 1];
+        if (chunk > first) fetch(chunk - 1);
+
+        for (int tile = wave; tile < TT * (TT + 1) / 2; tile += NW) {
+            int I = 0, J = tile;
+            while (J > I) J -= ++I;
+            v4f p = {0, 0, 0, 0}, r = {0, 0, 0, 0};
+#pragma unroll
+            for (int b = 0; b < NB; b++) p = product<O>(sh.k.rows(16 * J, 32 * b, g, c), sh.q.rows(16 * I, 32 * b, g, c), p);
+#pragma unroll
+            for (int b = 0; b < MB; b++) r = product<kWide>(sh.v.rows(16 * J, 32 * b, g, c), sh.go.rows(16 * I, 32 * b, g, c), r);
+            const int t = 16 * I + c, s = 16 * J + 4 * g;
+            const v4f f = d.between(t, s);
+            float x[4], y[4];
+#pragma unroll
+            for (int i = 0; i < 4; i++) x[i] = s + i <= t ? p[i] * f[i] : 0.f, y[i] = s + i <= t ? r[i] * f[i] : 0.f;
+            v4b parts[O], wide[kWide];
+            split<O, 4>(x, parts);
+            split<kWide, 4>(y, wide);
+#pragma unroll
+            for (int o = 0; o < O; o++) sh.p.put4(o, t, s, parts[o]);
+#pragma unroll
+            for (int o = 0; o < kWide; o++) sh.r.put4(o, t, s, wide[o]);
+        }
+
+        v4f dq[TT][EW], dk[TT][EW], dv[TT][MW];
+#pragma unroll
+        for (int I = 0; I < TT; I++) {
+#pragma unroll
+            for (int j = 0; j < EW; j++) dq[I][j] = dk[I][j] = v4f{0, 0, 0, 0};
+#pragma unroll
+            for (int j = 0; j < MW; j++) dv[I][j] = v4f{0, 0, 0, 0};
+        }
+        // through the states before and behind the chunk
+        if (keys) {
+#pragma unroll
+            for (int b = 0; b < MB; b++) {
+                Frag<kWide> s[EW], ht[EW];
+#pragma unroll
+                for (int j = 0; j < EW; j++) {
+                    float x[8];
+                    before(chunk, b, j, x);
+                    s[j] = split8<kWide>(x);
+                    ht[j] = split8<kWide>(H[b][0][j], H[b][1][j]);
+                }
+#pragma unroll
+                for (int I = 0; I < TT; I++) {
+                    const Frag<P> go = sh.go.rows(16 * I, 32 * b, g, c), v = sh.v.rows(16 * I, 32 * b, g, c);
+#pragma unroll
+                    for (int j = 0; j < EW; j++) dq[I][j] = product<kWide>(s[j], go, dq[I][j]), dk[I][j] = product<kWide>(ht[j], v, dk[I][j]);
+                }
+            }
+        }
+#pragma unroll
+        for (int b = 0; b < NB; b++) {
+            Frag<O> s[MW];
+#pragma unroll
+            for (int j = 0; j < MW; j++) s[j] = split8<O>(G[b][0][j], G[b][1][j]);
+#pragma unroll
+            for (int I = 0; I < TT; I++) {
+                const Frag<P> k = sh.k.rows(16 * I, 32 * b, g, c);
+#pragma unroll
+                for (int j = 0; j < MW; j++) dv[I][j] = product<O>(s[j], k, dv[I][j]);
+            }
+        }
+#pragma unroll
+        for (int I = 0; I < TT; I++) {
+            const float into = d.into[16 * I + c], rest = d.rest[16 * I + c];
+#pragma unroll
+            for (int j = 0; j < EW; j++) dq[I][j] *= into, dk[I][j] *= rest;
+#pragma unroll
+            for (int j = 0; j < MW; j++) dv[I][j] *= rest;
+        }
+        lds_barrier();
+
+        // within the chunk, and the adjoint of the state before it
+#pragma unroll
+        for (int b = 0; b < NB; b++)
+#pragma unroll
+            for (int u = 0; u < 2; u++)
+#pragma unroll
+                for (int j = 0; j < MW; j++) G[b][u][j] *= d.whole;
+#pragma unroll
+        for (int b = 0; b < MB; b++)
+#pragma unroll
+            for (int u = 0; u < 2; u++)
+#pragma unroll
+                for (int j = 0; j < EW; j++) H[b][u][j] *= d.whole;
+#pragma unroll
+        for (int sb = 0; sb < SB; sb++) {
+            const v4f f0 = *reinterpret_cast<const v4f *>(&d.into[32 * sb + 8 * g]), f1 = *reinterpret_cast<const v4f *>(&d.into[32 * sb + 8 * g + 4]);
+            if (keys) {
+                Frag<kWide> qs[EW];
+#pragma unroll
+                for (int j = 0; j < EW; j++) {
+                    const Frag<P> k = sh.k.template columns<EW>(ew, j, 32 * sb, g, c), q = sh.q.template columns<EW>(ew, j, 32 * sb, g, c);
+#pragma unroll
+                    for (int I = 2 * sb; I < TT; I++) dq[I][j] = product<kWide>(k, sh.r.rows(16 * I, 32 * sb, g, c), dq[I][j]);
+#pragma unroll
+                    for (int I = 0; I < 2 * sb + 2; I++) dk[I][j] = product<kWide>(q, sh.r.template columns<1>(16 * I, 0, 32 * sb, g, c), dk[I][j]);
+                    float x[8];
+                    join8(q, x);
+#pragma unroll
+                    for (int i = 0; i < 4; i++) x[i] *= f0[i], x[i + 4] *= f1[i];
+                    qs[j] = split8<kWide>(x);
+                }
+#pragma unroll
+                for (int b = 0; b < MB; b++)
+#pragma unroll
+                    for (int u = 0; u < 2; u++) {
+                        const Frag<P> go = sh.go.template columns<2>(32 * b, u, 32 * sb, g, c);
+#pragma unroll
+                        for (int j = 0; j < EW; j++) H[b][u][j] = product<kWide>(go, qs[j], H[b][u][j]);
+                    }
+            }
+            Frag<kWide> ds[MW];
+#pragma unroll
+            for (int j = 0; j < MW; j++) {
+                const Frag<P> go = sh.go.template columns<MW>(mw, j, 32 * sb, g, c);
+#pragma unroll
+                for (int I = 0; I < 2 * sb + 2; I++) dv[I][j] = product<O>(go, sh.p.template columns<1>(16 * I, 0, 32 * sb, g, c), dv[I][j]);
+                float x[8];
+                join8(go, x);
+#pragma unroll
+                for (int i = 0; i < 4; i++) x[i] *= f0[i], x[i + 4] *= f1[i];
+                ds[j] = split8<kWide>(x);
+            }
+#pragma unroll
+            for (int b = 0; b < NB; b++)
+#pragma unroll
+                for (int u = 0; u < 2; u++) {
+                    const Frag<P> q = sh.q.template columns<2>(32 * b, u, 32 * sb, g, c);
+#pragma unroll
+                    for (int j = 0; j < MW; j++) G[b][u][j] = product<kWide>(q, ds[j], G[b][u][j]);
+                }
+        }
+
+        // results, and the rows' part of the decays' gradients
+#pragma unroll
+        for (int I = 0; I < TT; I++) {
+            const int r = 16 * I + c, t = chunk * C + r;
+            float u = 0.f;
+            if (keys) {
+                float xq[4 * EW], xk[4 * EW];
+#pragma unroll
+                for (int j = 0; j < EW; j++) {
+                    const v4f q = sh.q.four(r, ew + 4 * EW * g + 4 * j), k = sh.k.four(r, ew + 4 * EW * g + 4 * j);
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        u = fmaf(q[i], dq[I][j][i], u), u = fmaf(-k[i], dk[I][j][i], u);
+                        xq[4 * j + i] = t < len ? dq[I][j][i] * a.scale : 0.f, xk[4 * j + i] = t < len ? dk[I][j][i] * a.scale : 0.f;
+                    }
+                }
+                if (t < a.L) {
+                    const int col = ew + 4 * EW * g;
+                    if (a.pq) store_some<float, 4 * EW>(a.pq + ((((int64_t)(h % rq) * a.slices + slice) * a.N + n) * a.HQ + h / rq) * a.L * a.E + (int64_t)t * a.E, col, a.E, xq);
+                    else store_some<T, 4 * EW>(row<T>(a.gq, n, h, t), col, a.E, xq);
+                    if (a.pk) store_some<float, 4 * EW>(a.pk + ((((int64_t)(h % rk) * a.slices + slice) * a.N + n) * a.HK + h / rk) * a.L * a.E + (int64_t)t * a.E, col, a.E, xk);
+                    else store_some<T, 4 * EW>(row<T>(a.gk, n, h, t), col, a.E, xk);
+                }
+            }
+            u += __shfl_xor(u, 16);
+            u += __shfl_xor(u, 32);
+            if (g == 0) sh.sums[wave][r] = u;
+            if (t < a.L) {
+                float xv[4 * MW];
+#pragma unroll
+                for (int j = 0; j < MW; j++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) xv[4 * j + i] = t < len ? dv[I][j][i] * a.scale : 0.f;
+                const int col = mw + 4 * MW * g;
+                if (a.pv) store_some<float, 4 * MW>(a.pv + (((int64_t)(h % rv) * a.N + n) * a.HV + h / rv) * a.L * a.M + (int64_t)t * a.M + m0, col, mcols, xv);
+                else store_some<T, 4 * MW>(row<T>(a.gv, n, h, t) + m0, col, mcols, xv);
+            }
+        }
+        x_end = chunk > first ? inner(chunk) : 0.f;      // for the chunk before this one
+        if (chunk > first && wave == NW - 1) sh.d[(chunk - 1) & 1].sum(gnext, lane);
+        lds_barrier();
+        if (wave == 0) {
+            float s = 0.f, x = 0.f;
+            if (lane < C)
+#pragma unroll
+                for (int i = 0; i < NW; i++) s += sh.sums[i][lane];
+#pragma unroll
+            for (int i = 0; i < NW; i++) x += sh.inner[i];
+#pragma unroll
+            for (int off = 1; off < C; off *= 2) {
+                const float y = __shfl_down(s, off);
+                if (lane + off < C) s += y;
+            }
+            const int t = chunk * C + lane;
+            const bool counts = lane < C && t < len;
+            s = counts ? (s + x) * a.scale : 0.f;
+            if (a.sum_decay) all += s;
+            else if (lane < C && t < a.L) a.gdecay[(((int64_t)slice * a.N + n) * a.H + h) * a.L + t] = s;
+        }
+        lds_barrier();
+    }
+
+    // rows behind the sequence
+    const int64_t t0 = (int64_t)max(stop, first) * C, t1 = min((int64_t)last * C, (int64_t)a.L);
+    for (int64_t i = t0 * E + tid; i < t1 * E; i += 64 * NW) {
+        const int64_t t = i / E;
+        const int e = i % E;
+        if (e >= a.E) continue;
+        if (a.pq) a.pq[((((int64_t)(h % rq) * a.slices + slice) * a.N + n) * a.HQ + h / rq) * a.L * a.E + t * a.E + e] = 0.f;
+        else row<T>(a.gq, n, h, t)[e] = (T)0.f;
+        if (a.pk) a.pk[((((int64_t)(h % rk) * a.slices + slice) * a.N + n) * a.HK + h / rk) * a.L * a.E + t * a.E + e] = 0.f;
+        else row<T>(a.gk, n, h, t)[e] = (T)0.f;
+    }
+    for (int64_t i = t0 * MS + tid; i < t1 * MS; i += 64 * NW) {
+        const int64_t t = i / MS;
+        const int m = i % MS;
+        if (m >= mcols) continue;
+        if (a.pv) a.pv[(((int64_t)(h % rv) * a.N + n) * a.HV + h / rv) * a.L * a.M + t * a.M + m0 + m] = 0.f;
+        else (row<T>(a.gv, n, h, t) + m0)[m] = (T)0.f;
+    }
+    if (a.sum_decay) {
+        if (wave == 0) {
+#pragma unroll
+            for (int off = 1; off < 64; off *= 2) all += __shfl_xor(all, off);
+            if (lane == 0) a.gdecay[(head * a.slices + slice) * a.segments + seg] = all;
+        }
+    } else {
+        for (int64_t t = t0 + tid; t < t1; t += 64 * NW) a.gdecay[(((int64_t)slice * a.N + n) * a.H + h) * a.L + t] = 0.f;
+    }
+}
+
+// ------------------------------------------------------------------ launches
+
+enum { kDsumForward, kDsumForwardEnds, kDsumBackward, kDsumBackwardEnds };
+
+// Launches one of the four for states of Ep keys and slices of MS value columns; false: there is no such kernel.
+template <typename T>
+bool dsum_launch(int which, const DsumWalk &a, int Ep, int MS, unsigned blocks, hipStream_t s);
+
+template <typename T, int NE, int NW, int MW>
+void dsum_launch_one(int which, const DsumWalk &a, unsigned blocks, hipStream_t s) {
+    const dim3 grid(blocks), block(64 * NW);
+    switch (which) {
+        case kDsumForward: k_dsum_fwd<T, NE, NW, MW, false><<<grid, block, 0, s>>>(a); break;
+        case kDsumForwardEnds: k_dsum_fwd<T, NE, NW, MW, true><<<grid, block, 0, s>>>(a); break;
+        case kDsumBackward: k_dsum_bwd<T, NE, NW, MW><<<grid, block, 0, s>>>(a); break;
+        default: k_dsum_bwd_ends<T, NE, NW, MW><<<grid, block, 0, s>>>(a); break;
+    }
+}
+
+template <typename T, int NE>
+bool dsum_launch_keys(int which, const DsumWalk &a, int MS, unsigned blocks, hipStream_t s) {
+    if (MS == 32) dsum_launch_one<T, NE, 2, 1>(which, a, blocks, s);
+    else if (MS == 64) dsum_launch_one<T, NE, 4, 1>(which, a, blocks, s);
+    else if (MS == 128) dsum_launch_one<T, NE, 8, 1>(which, a, blocks, s);
+    else return false;
+    return true;
+}
+
+#define FWP_DSUM_INSTANCES(T)                                                                              \
+    template <>                                                                                            \
+    bool dsum_launch<T>(int which, const DsumWalk &a, int Ep, int MS, unsigned blocks, hipStream_t s) {    \
+        if (Ep == 32) return dsum_launch_keys<T, 2>(which, a, MS, blocks, s);                              \
+        if (Ep == 64) return dsum_launch_keys<T, 4>(which, a, MS, blocks, s);                              \
+        if (Ep == 128) return dsum_launch_keys<T, 8>(which, a, MS, blocks, s);                             \
+        return false;                                                                                      \
+    }
+
+}  // namespace fwp

@@ -98,6 +98,18 @@ int scan_fwd(const fwp_scan_args &a, float *W, fwp_out_rows out, float *saved, f
 int scan_bwd(const fwp_scan_args &a, const float *saved, fwp_rows gout, fwp_out_rows gq, fwp_out_rows gk, fwp_out_rows gv,
              fwp_out_rows gdelta, fwp_out_rows gz, float *gA, float *gD, float *gdelta_bias, float *workspace, hipStream_t s);
 
+int64_t dsum_saved_floats(int type, int N, int H, int L, int E, int M);
+int64_t dsum_workspace(const fwp_dsum_args &a, bool backward);
+int dsum_fwd(const fwp_dsum_args &a, float *W, fwp_out_rows out, float *saved, float *workspace, hipStream_t s);
+int dsum_bwd(const fwp_dsum_args &a, const float *saved, fwp_rows gout, fwp_out_rows gq, fwp_out_rows gk, fwp_out_rows gv, float *gdecay,
+             float *workspace, hipStream_t s);
+
+int rotary(const fwp_rotary_args &a, fwp_out_rows oq, fwp_out_rows ok, hipStream_t s);
+
+int64_t group_norm_workspace(int type, int rows, int groups, int size);
+int group_norm_fwd(const fwp_group_norm_args &a, void *y, hipStream_t s);
+int group_norm_bwd(const fwp_group_norm_args &a, const void *gy, void *gx, void *ggate, float *gweight, float *gbias, float *workspace, hipStream_t s);
+
 int64_t residual_norm_workspace(int rows, int cols);
 int residual_norm_fwd(const fwp_norm_args &a, void *r, void *n, float *stats, hipStream_t s);
 int residual_norm_bwd(const fwp_norm_args &a, const float *stats, const void *gr, const void *gn, const fwp_norm_grads &g,

@@ -1,0 +1,174 @@
+// Tiles of rows in LDS as sums of bfloat16 parts, and products of such sums on the matrix cores.
+//
+// An fp32 number is the sum of three bfloat16 numbers (8 significant bits each), an fp16 number that of two, and a product of two sums
+// keeps the pairs of parts whose orders add up to less than a stated number: three orders leave out 2^-24 of a product, two 2^-16.  The 16-bit
+// products run at 16 times the rate of v_mfma_f32_16x16x4_f32, so six of them are 2.7 times as fast as one fp32 product, and every type takes
+// the same path.
+//
+// Fragments of v_mfma_f32_16x16x32_bf16, lane l = 16 g + c: an operand holds, for its row (A) or column (B) c, the summation indexes 8 g .. 8 g + 7; a
+// result holds rows 4 g .. 4 g + 3 of column c.  Two results whose rows stand for the indexes 8 g + i and 8 g + 4 + i are therefore an operand of the next
+// product as they are: nothing moves between lanes.  place() gives such an order to the 16 rows of each of `tiles` results.
+#pragma once
+#include <type_traits>
+
+#include "fwp_elements.hpp"
+#include "fwp_mfma.hpp"
+
+namespace fwp {
+
+typedef __bf16 v8b __attribute__((ext_vector_type(8)));
+typedef __bf16 v4b __attribute__((ext_vector_type(4)));
+typedef short v4h __attribute__((ext_vector_type(4)));
+
+// bfloat16 parts that hold a row element of this type whole
+template <typename T>
+constexpr int kPartsOf = std::is_same_v<T, bf16_t> ? 1 : std::is_same_v<T, half_t> ? 2 : 3;
+
+template <int P>
+struct Frag {
+    v8b p[P];
+};
+
+// x[i] as the sum of P parts: each takes what the ones before it left.  The rounding of a part to nearest is exact to 2^-9 of what was left.
+template <int P, int W, typename V>
+__device__ __forceinline__ void split(const float (&x)[W], V (&out)[P]) {
+    float left[W];
+#pragma unroll
+    for (int i = 0; i < W; i++) left[i] = x[i];
+#pragma unroll
+    for (int p = 0; p < P; p++)
+#pragma unroll
+        for (int i = 0; i < W; i++) {
+            const __bf16 part = (__bf16)left[i];
+            out[p][i] = part;
+            if (p + 1 < P) left[i] -= (float)part;
+        }
+}
+
+template <int P>
+__device__ __forceinline__ Frag<P> split8(const float (&x)[8]) {
+    Frag<P> f;
+    split<P, 8>(x, f.p);
+    return f;
+}
+
+template <int P>
+__device__ __forceinline__ Frag<P> split8(const v4f &lo, const v4f &hi) {
+    const float x[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+    return split8<P>(x);
+}
+
+template <int P>
+__device__ __forceinline__ void join8(const Frag<P> &f, float (&x)[8]) {
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        x[i] = (float)f.p[P - 1][i];
+#pragma unroll
+        for (int p = P - 2; p >= 0; p--) x[i] += (float)f.p[p][i];
+    }
+}
+
+// acc + A B over 32 summation indexes, pairs of parts of orders below ORDERS
+template <int ORDERS, int PA, int PB>
+__device__ __forceinline__ v4f product(const Frag<PA> &a, const Frag<PB> &b, v4f acc) {
+#pragma unroll
+    for (int i = 0; i < PA; i++)
+#pragma unroll
+        for (int j = 0; j < PB; j++)
+            if (i + j < ORDERS) acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.p[i], b.p[j], acc, 0, 0, 0);
+    return acc;
+}
+
+// Row (or column) a of the j-th of `tiles` results that lie side by side: four consecutive numbers a lane, 4 * tiles in a row of them.
+__device__ __forceinline__ constexpr int place(int tiles, int a, int j) { return 4 * tiles * (a / 4) + 4 * j + a % 4; }
+
+// R rows of W elements as P parts; rows are 16 bytes longer than their elements, which spreads 16 rows over the banks.
+template <int R, int W, int P>
+struct alignas(16) Tile {
+    static constexpr int kStride = W + 8, kPart = R * kStride;
+    __bf16 x[P * kPart];
+
+    __device__ __forceinline__ void put(int p, int r, int col, const v8b &v) { *reinterpret_cast<v8b *>(&x[p * kPart + r * kStride + col]) = v; }
+    __device__ __forceinline__ void put4(int p, int r, int col, const v4b &v) { *reinterpret_cast<v4b *>(&x[p * kPart + r * kStride + col]) = v; }
+
+    // rows r0 .. r0 + 15 against columns k0 .. k0 + 31 as they lie
+    __device__ __forceinline__ Frag<P> rows(int r0, int k0, int g, int c) const {
+        Frag<P> f;
+#pragma unroll
+        for (int p = 0; p < P; p++) f.p[p] = *reinterpret_cast<const v8b *>(&x[p * kPart + (r0 + c) * kStride + k0 + 8 * g]);
+        return f;
+    }
+    // columns c0 + place(tiles, c, j) against rows k0 .. k0 + 31.  ds_read_b64_tr_b16: each lane names four elements, the 16 lanes of a group four
+    // rows of 16, and lane c of the group gets the four rows' c-th.
+    template <int TILES>
+    __device__ __forceinline__ Frag<P> columns(int c0, int j, int k0, int g, int c) const {
+        typedef __attribute__((address_space(3))) v4h *lds4;
+        Frag<P> f;
+#pragma unroll
+        for (int p = 0; p < P; p++) {
+            const __bf16 *at = &x[p * kPart + (k0 + 8 * g + c / 4) * kStride + c0 + 4 * TILES * (c % 4) + 4 * j];
+            const v4h lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)at), hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(at + 4 * kStride));
+            const v4b l = __builtin_bit_cast(v4b, lo), h = __builtin_bit_cast(v4b, hi);
+            f.p[p] = v8b{l[0], l[1], l[2], l[3], h[0], h[1], h[2], h[3]};
+        }
+        return f;
+    }
+    // four elements of a row, summed up again
+    __device__ __forceinline__ v4f four(int r, int col) const {
+        v4f s = {0, 0, 0, 0};
+#pragma unroll
+        for (int p = P - 1; p >= 0; p--) {
+            const v4b v = *reinterpret_cast<const v4b *>(&x[p * kPart + r * kStride + col]);
+#pragma unroll
+            for (int i = 0; i < 4; i++) s[i] += (float)v[i];
+        }
+        return s;
+    }
+};
+
+// Eight elements of a row at any alignment: the hardware loads and stores 16 bytes at element addresses.
+template <typename T>
+struct alignas(sizeof(T)) Eight {
+    T x[8];
+};
+
+// A block of R rows of up to W elements on its way from memory to a Tile: load() starts the loads, put() converts and writes what they brought.
+// Rows from `rows` on and columns from `cols` on are zero and not read.
+template <typename T, int R, int W, int THREADS>
+struct Stage {
+    static constexpr int kRow = W / 8, kVecs = R * kRow, kPer = (kVecs + THREADS - 1) / THREADS;
+    T x[kPer][8];
+
+    __device__ __forceinline__ void load(const T *base, int64_t stride, int rows, int cols, int tid) {
+#pragma unroll
+        for (int i = 0; i < kPer; i++) {
+            const int v = tid + i * THREADS, r = v / kRow, col = v % kRow * 8;
+            const T *at = base + r * stride + col;
+            if (r < rows && col + 8 <= cols) {
+                struct __attribute__((packed, aligned(sizeof(T)))) Any { T x[8]; };
+                const Any a = *reinterpret_cast<const Any *>(at);
+#pragma unroll
+                for (int e = 0; e < 8; e++) x[i][e] = a.x[e];
+            } else {
+#pragma unroll
+                for (int e = 0; e < 8; e++) x[i][e] = r < rows && col + e < cols ? at[e] : (T)0.f;
+            }
+        }
+    }
+    template <int P>
+    __device__ __forceinline__ void put(Tile<R, W, P> &t, int tid) const {
+#pragma unroll
+        for (int i = 0; i < kPer; i++) {
+            const int v = tid + i * THREADS, r = v / kRow, col = v % kRow * 8;
+            if (kVecs % THREADS && v >= kVecs) continue;
+            float f[8];
+#pragma unroll
+            for (int e = 0; e < 8; e++) f[e] = (float)x[i][e];
+            const Frag<P> s = split8<P>(f);
+#pragma unroll
+            for (int p = 0; p < P; p++) t.put(p, r, col, s.p[p]);
+        }
+    }
+};
+
+}  // namespace fwp

@@ -681,6 +681,7 @@ void set_error_class(py::object cls) {
 void bind_blocks(py::module_ &m);       // fwp_torch_blocks.cpp
 #ifndef FWP_HOST_STUB
 void bind_scan(py::module_ &m);         // fwp_torch_scan.cpp
+void bind_decay(py::module_ &m);        // fwp_torch_decay.cpp
 #endif
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -709,6 +710,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     bind_blocks(m);
 #ifndef FWP_HOST_STUB
     bind_scan(m);
+    bind_decay(m);
 #endif
     m.def("set_error_class", &set_error_class, "exception class raised for rejected calls");
 }
