@@ -138,22 +138,39 @@ struct Plan {
     int64_t heads, cells, ends;      // ends: floats of the segments' states and factors
 };
 
-// Segments: enough workgroups that every CU has several, none shorter than four chunks.
-Plan plan_of(int type, int N, int H, int L, int E, int M) {
+int resident_of(int type, int which, int Ep, int MS) {
+    int n = 1;
+    by_type(type, [&](auto t) { n = dsum_launch<decltype(t)>(which, nullptr, Ep, MS, 0, nullptr); });
+    return std::max(n, 1);
+}
+
+// How a pass is cut.  Segments by a model of its time in chunks of the walk, which goes in rounds of as many workgroups as the GPU holds, each as long as its
+// chunks and the way into them.  Cutting sequences adds the walk that finds the segments' states: a chunk of it is 0.45 of a chunk forward and 0.3 backward where it
+// fills the GPU, and half of that at least; and joining them.  8 x 16 sequences of 64 chunks, 64 x 64 bf16: 6 segments forward 32 + 6 + 100 us, 8 are
+// 34 + 7 + 124; 4 segments backward 34 + 6 + 214, 8 are 36 + 7 + 228.
+Plan plan_of(int type, int N, int H, int L, int E, int M, bool backward) {
     Plan p{};
     p.Ep = E <= 32 ? 32 : E <= 64 ? 64 : 128;
     p.MS = M <= 32 ? 32 : M <= 64 ? 64 : 128;
     p.slices = (M + p.MS - 1) / p.MS;
     p.Mp = p.slices * p.MS;
-    p.chunk = type == FWP_BF16 ? kChunkOf<bf16_t> : type == FWP_F16 ? kChunkOf<half_t> : kChunkOf<float>;
+    by_type(type, [&](auto t) { p.chunk = kChunkOf<decltype(t)>; });
     p.chunks = (L + p.chunk - 1) / p.chunk;
     p.heads = (int64_t)N * H;
-    const int64_t units = p.heads * p.slices, wanted = 256 * 32 / (p.MS / 16);
-    const int64_t most = std::max(1, p.chunks / 4);
-    const int64_t segments = std::min(most, std::max<int64_t>(1, (wanted + units - 1) / units));
-    p.per = (int)((p.chunks + segments - 1) / segments);
-    p.segments = (p.chunks + p.per - 1) / p.per;
     p.cells = (int64_t)p.Ep * p.Mp;
+    const int64_t units = p.heads * p.slices, walks = 256 * resident_of(type, backward ? kDsumBackward : kDsumForward, p.Ep, p.MS),
+                  ends = 256 * resident_of(type, backward ? kDsumBackwardEnds : kDsumForwardEnds, p.Ep, p.MS);
+    const auto rounds = [](int64_t blocks, int64_t held) { return (double)((blocks + held - 1) / held); };
+    double best = 0;
+    for (int64_t s = 1; s <= std::max(1, p.chunks / 2) && (s == 1 || units * (s - 1) < 4 * walks); s++) {
+        const int64_t per = (p.chunks + s - 1) / s, segments = (p.chunks + per - 1) / per;
+        double time = rounds(units * segments, walks) * (per + 0.6);
+        if (segments > 1) {
+            const double blocks = (double)units * (segments - 1);
+            time += (per + 1) * (backward ? 0.3 : 0.45) * std::max(0.5 * rounds(units * (segments - 1), ends), blocks / ends) + 0.6 + 0.03 * segments;
+        }
+        if (s == 1 || time < best) best = time, p.per = (int)per, p.segments = (int)segments;
+    }
     p.ends = p.segments > 1 ? p.heads * p.segments * (p.cells + 1) : 0;
     return p;
 }
@@ -190,7 +207,7 @@ int launch(int which, const fwp_dsum_args &a, const Plan &p, const DsumWalk &w, 
     const int64_t blocks = p.heads * p.slices * segments;
     if (!fits_launch(blocks, 4 * p.MS) || !fits_launch(p.heads * (p.cells / 256), 256)) return FWP_E_SHAPE;
     bool done = false;
-    by_type(a.type, [&](auto t) { done = dsum_launch<decltype(t)>(which, w, p.Ep, p.MS, (unsigned)blocks, s); });
+    by_type(a.type, [&](auto t) { done = dsum_launch<decltype(t)>(which, &w, p.Ep, p.MS, (unsigned)blocks, s) > 0; });
     return done ? 0 : FWP_E_SHAPE;
 }
 
@@ -214,17 +231,17 @@ int launch_step(const DsumWalk &w, hipStream_t s) {
 }  // namespace
 
 int64_t dsum_saved_floats(int type, int N, int H, int L, int E, int M) {
-    const Plan p = plan_of(type, N, H, L, E, M);
+    const Plan p = plan_of(type, N, H, L, E, M, false);
     return p.heads * p.chunks * p.cells;
 }
 
 int64_t dsum_workspace(const fwp_dsum_args &a, bool backward) {
-    const Plan p = plan_of(a.type, a.N, a.H, a.L, a.E, a.M);
+    const Plan p = plan_of(a.type, a.N, a.H, a.L, a.E, a.M, backward);
     return backward ? backward_room(a, p).total : p.ends;
 }
 
 int dsum_fwd(const fwp_dsum_args &a, float *W, fwp_out_rows out, float *saved, float *workspace, hipStream_t s) {
-    const Plan p = plan_of(a.type, a.N, a.H, a.L, a.E, a.M);
+    const Plan p = plan_of(a.type, a.N, a.H, a.L, a.E, a.M, false);
     DsumWalk w = walk_of(a, p);
     w.out = out;
     w.from = w.to = W;
@@ -247,7 +264,7 @@ int dsum_fwd(const fwp_dsum_args &a, float *W, fwp_out_rows out, float *saved, f
 
 int dsum_bwd(const fwp_dsum_args &a, const float *saved, fwp_rows gout, fwp_out_rows gq, fwp_out_rows gk, fwp_out_rows gv, float *gdecay,
              float *workspace, hipStream_t s) {
-    const Plan p = plan_of(a.type, a.N, a.H, a.L, a.E, a.M);
+    const Plan p = plan_of(a.type, a.N, a.H, a.L, a.E, a.M, true);
     const BackwardRoom room = backward_room(a, p);
     DsumWalk w = walk_of(a, p);
     w.go = gout;

@@ -18,15 +18,22 @@
 // but the last from zero, a second one joins what they leave, and the walk proper starts every segment from its own state.
 #pragma once
 #include "fwp_parts.hpp"
+#include "fwp_wave.hpp"
 
 namespace fwp {
 
 template <typename T>
-constexpr int kChunkOf = sizeof(T) == 2 && kPartsOf<T> == 1 ? 64 : 32;
-// Orders of the products that end in results: of fewer bits than fp32, 2^-16 of a term is far below their rounding
-template <typename T>
-constexpr int kOrdersOf = sizeof(T) == 2 ? 2 : 3;
-constexpr int kWide = 3;      // orders of what ends in fp32: the state, its adjoint, the decays' gradients
+constexpr int kChunkOf = std::is_same_v<T, bf16_t> ? 64 : 32;
+// Parts of rows of type T and of what is made of them: numbers that end in results of fewer bits than fp32 keep 2^-16, far below their rounding,
+// those that end in the state, its adjoint and the decays' gradients 2^-24.
+#ifndef PLAIN_NE
+#define PLAIN_NE 2
+#endif
+template <typename T, int NE>
+struct Parts {
+    static constexpr bool kWhole = std::is_same_v<T, float> && NE <= PLAIN_NE;
+    static constexpr int P = kWhole ? kPlain : kPartsOf<T>, O = kWhole ? kPlain : sizeof(T) == 2 ? 2 : 3, X = kWhole ? kPlain : 3;
+};
 
 struct DsumWalk {
     fwp_rows q, k, v, go;
@@ -45,7 +52,8 @@ struct DsumWalk {
     int sum_decay;
 };
 
-// Workgroups b, b + 8, .. run on one XCD: neighbours in the order of the work, which share rows, get numbers that lie 8 apart.
+// Workgroups b, b + 8, .. run on one XCD: neighbours in the order of the work get numbers that lie 8 apart.  Slices and heads come first in that order: they share
+// rows, or read rows that lie side by side where steps are outermost, at about the same time.
 __device__ __forceinline__ int64_t by_xcd(int64_t b, int64_t n) {
     const int64_t whole = n / 8 * 8;
     return b < whole ? b % 8 * (n / 8) + b / 8 : b;
@@ -60,12 +68,14 @@ struct alignas(16) Decays {
     __device__ __forceinline__ double sum(float g, int lane) {
         constexpr float least = -1e5f;
         double x = (double)(g < least ? least : g) * 1.4426950408889634074;
-#pragma unroll
-        for (int off = 1; off < C; off *= 2) {
-            const double y = __shfl_up(x, off);
-            if (lane >= off) x += y;
-        }
-        const double total = __shfl(x, C - 1);
+        x += shifted<0x111, 0xf>(x);      // row_shr:1, 2, 4, 8
+        x += shifted<0x112, 0xf>(x);
+        x += shifted<0x114, 0xf>(x);
+        x += shifted<0x118, 0xf>(x);
+        x += shifted<kRowBcast15, 0xa>(x);
+        x += shifted<kRowBcast31, 0xc>(x);
+        const double total = __builtin_bit_cast(double, (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)__builtin_bit_cast(uint64_t, x), 63) |
+                                                            (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(__builtin_bit_cast(uint64_t, x) >> 32), 63) << 32);
         if (lane < C) {
             const float h = (float)x;
             hi[lane] = h;
@@ -75,6 +85,13 @@ struct alignas(16) Decays {
         }
         if (lane == 0) whole = __builtin_amdgcn_exp2f((float)total);
         return total;
+    }
+    // x of another lane of the wave, 0 where there is none
+    template <int CTRL, int ROWS>
+    static __device__ __forceinline__ double shifted(double x) {
+        const uint64_t u = __builtin_bit_cast(uint64_t, x);
+        const uint32_t l = __builtin_amdgcn_update_dpp(0, (int)u, CTRL, ROWS, 0xf, true), h = __builtin_amdgcn_update_dpp(0, (int)(u >> 32), CTRL, ROWS, 0xf, true);
+        return __builtin_bit_cast(double, (uint64_t)h << 32 | l);
     }
     // exp(b_t - b_s) for the four steps s ..; 0 where s > t
     __device__ __forceinline__ v4f between(int t, int s) const {
@@ -87,27 +104,71 @@ struct alignas(16) Decays {
     }
 };
 
-// W consecutive numbers of a row whose element `col` is the first, columns below `cols` only
+// Sums over the four groups of 16 lanes, and over the lanes of a group, in every lane
+__device__ __forceinline__ float over_groups(float x) {
+    float y = x;
+    swap16(x, y);
+    x += y, y = x;
+    swap32(x, y);
+    return x + y;
+}
+__device__ __forceinline__ float over_sixteen(float x) {
+    x += dpp<kQuadXor1>(x);
+    x += dpp<kQuadXor2>(x);
+    x += dpp<kRowRor4>(x);
+    return x + dpp<kRowRor8>(x);
+}
+
+// A number that is the same all along, but not to the compiler: what follows from it is worked out where it is needed, instead of being kept in scalar registers that run out.
+__device__ __forceinline__ int opaque(int x) {
+    asm volatile("" : "+s"(x));
+    return x;
+}
+
+// W consecutive numbers of a row, in stores of up to 16 bytes at an element's address
 template <typename T, int W>
-__device__ __forceinline__ void store_some(T *at, int col, int cols, const float (&x)[W]) {
-    if (col + W <= cols) {
-        struct __attribute__((packed, aligned(sizeof(T)))) Any { T x[W]; };
-        Any a;
+__device__ __forceinline__ void store_whole(T *at, const float (&x)[W]) {
+    constexpr int kWords = sizeof(T) * W / 4, kStep = kWords < 4 ? kWords : 4;
+    typedef uint32_t Words __attribute__((ext_vector_type(kStep)));
+    struct __attribute__((packed, aligned(sizeof(T)))) Anywhere { Words w; };
+    struct Row { T x[W]; } row;
+    struct Split { Words w[kWords / kStep]; };
 #pragma unroll
-        for (int i = 0; i < W; i++) a.x[i] = (T)x[i];
-        *reinterpret_cast<Any *>(at + col) = a;
-    } else {
+    for (int i = 0; i < W; i++) row.x[i] = (T)x[i];
+    const Split split = __builtin_bit_cast(Split, row);
 #pragma unroll
-        for (int i = 0; i < W; i++)
-            if (col + i < cols) at[col + i] = (T)x[i];
+    for (int i = 0; i < kWords / kStep; i++) reinterpret_cast<Anywhere *>(at)[i].w = split.w[i];
+}
+// A chunk's results, columns col .. of rows 16 I + c.  base: its first row, the same for all lanes; C rows lie within 32 bits of bytes.  live: the chunk's rows that count, the others become zero; there: those that are
+// there at all.  cols: this lane's columns that are there, of 4 J.
+template <typename T, int C, int J>
+__device__ __forceinline__ void store_rows(T *base, int stride, int col, const v4f (&acc)[C / 16][J], float scale, int live, int there, bool whole, int cols, int c) {
+#pragma unroll
+    for (int I = 0; I < C / 16; I++) {
+        float x[4 * J];
+#pragma unroll
+        for (int j = 0; j < J; j++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) x[4 * j + i] = acc[I][j][i] * scale;
+        T *to = from(base, (uint32_t)(16 * I + c) * (uint32_t)stride + (uint32_t)col);
+        if (whole) {
+            store_whole<T, 4 * J>(to, x);
+        } else if (16 * I + c < there) {
+#pragma unroll
+            for (int i = 0; i < 4 * J; i++)
+                if (i < cols) to[i] = (T)(16 * I + c < live ? x[i] : 0.f);
+        }
     }
 }
+
+// Workgroups of a kernel that a CU holds at once: 160 KB of LDS, and registers for `waves` on each of four SIMDs, which the kernel's launch bounds ask for
+constexpr int resident(size_t lds, int waves, int NW) { return (int)(160 * 1024 / lds) < 4 * waves / NW ? (int)(160 * 1024 / lds) : 4 * waves / NW; }
 
 // ------------------------------------------------------------------ forward
 
 template <typename T, int NE, int NW, int MW>
 struct DsumForward {
-    static constexpr int C = kChunkOf<T>, P = kPartsOf<T>, O = kOrdersOf<T>, E = 16 * NE, MS = 16 * MW * NW, kThreads = 64 * NW;
+    static constexpr int C = kChunkOf<T>, P = Parts<T, NE>::P, O = Parts<T, NE>::O, X = Parts<T, NE>::X, E = 16 * NE, MS = 16 * MW * NW, kThreads = 64 * NW;
     static constexpr int NB = NE / 2, SB = C / 32, TT = C / 16;
     struct Shared {
         Tile<C, E, P> q, k;
@@ -120,23 +181,23 @@ struct DsumForward {
         Tile<C, MS, P> v;
         Decays<C> d[2];
     };
+    static constexpr int kWaves = P == kPlain ? 4 : NE <= 4 ? 3 : 2, kEndWaves = NE <= 4 ? 4 : 3;
 };
 
 // ENDS: the state that a segment leaves when it starts from zero, and the segment's whole decay; nothing else.
 template <typename T, int NE, int NW, int MW, bool ENDS>
-__global__ __launch_bounds__(64 * NW) void k_dsum_fwd(const DsumWalk a) {
+__global__ __launch_bounds__(64 * NW, (ENDS ? DsumForward<T, NE, NW, MW>::kEndWaves : DsumForward<T, NE, NW, MW>::kWaves)) void k_dsum_fwd(const DsumWalk a) {
     using F = DsumForward<T, NE, NW, MW>;
-    constexpr int C = F::C, P = F::P, O = F::O, E = F::E, MS = F::MS, NB = F::NB, SB = F::SB, TT = F::TT;
+    constexpr int C = F::C, P = F::P, O = F::O, X = F::X, E = F::E, MS = F::MS, NB = F::NB, SB = F::SB, TT = F::TT;
     __shared__ std::conditional_t<ENDS, typename F::Ends, typename F::Shared> sh;
     const int tid = threadIdx.x, lane = tid % 64, wave = tid / 64, g = lane / 16, c = lane % 16;
 
-    const int segments = ENDS ? a.segments - 1 : a.segments;
     int64_t w = by_xcd(blockIdx.x, gridDim.x);
     const int slice = w % a.slices;
     w /= a.slices;
-    const int seg = w % segments;
-    w /= segments;
-    const int h = w % a.H, n = w / a.H;
+    const int h = w % a.H;
+    w /= a.H;
+    const int n = w % a.N, seg = w / a.N;
 
     const int len = length_of(a.lengths, n, a.L), chunks = (a.L + C - 1) / C, live = (len + C - 1) / C;
     const int first = seg * a.per, last = min(first + a.per, chunks), stop = min(last, live);
@@ -179,27 +240,38 @@ __global__ __launch_bounds__(64 * NW) void k_dsum_fwd(const DsumWalk a) {
     const auto fetch = [&](int chunk) {
         const int64_t t0 = (int64_t)chunk * C;
         const int rows = len - (int)t0;
-        if constexpr (!ENDS) sq.load(qb + t0 * a.q.sL, a.q.sL, rows, a.E, tid);
-        sk.load(kb + t0 * a.k.sL, a.k.sL, rows, a.E, tid);
-        sv.load(vb + t0 * a.v.sL, a.v.sL, rows, mcols, tid);
-        if (wave == NW - 1) gnext = lane < C && lane < rows ? gb[(t0 + lane) * a.dL] : 0.f;
+        if constexpr (!ENDS) sq.load(qb + t0 * a.q.sL, (int)a.q.sL, rows, a.E, tid);
+        sk.load(kb + t0 * a.k.sL, (int)a.k.sL, rows, a.E, tid);
+        sv.load(vb + t0 * a.v.sL, (int)a.v.sL, rows, mcols, tid);
     };
+    // the last wave, which has the fewest tiles of P, sums up the next chunk's decays
+    const auto fetch_decay = [&](int chunk) { gnext = gb[min((int64_t)chunk * C + lane, (int64_t)len - 1) * a.dL]; };
+    const auto sum_decay = [&](int chunk) { total += sh.d[chunk & 1].sum(lane < C && chunk * C + lane < len ? gnext : 0.f, lane); };
     if (first < stop) {
+        if (wave == NW - 1) fetch_decay(first);
         fetch(first);
-        if (wave == NW - 1) total += sh.d[first & 1].sum(gnext, lane);
+        if (wave == NW - 1) {
+            sum_decay(first);
+            if (first + 1 < stop) fetch_decay(first + 1);
+        }
     }
     for (int chunk = first; chunk < stop; chunk++) {
-        if constexpr (!ENDS) sq.put(sh.q, tid);
-        sk.put(sh.k, tid);
-        sv.put(sh.v, tid);
+        const int rows = len - chunk * C, keys = opaque(a.E), values = opaque(mcols);
+        if constexpr (!ENDS) sq.put(sh.q, rows, keys, tid);
+        sk.put(sh.k, rows, keys, tid);
+        sv.put(sh.v, rows, values, tid);
         lds_barrier();
         const Decays<C> &d = sh.d[chunk & 1];
+        if (wave == NW - 1 && chunk + 1 < stop) {
+            sum_decay(chunk + 1);
+            if (chunk + 2 < stop) fetch_decay(chunk + 2);
+        }
         if (chunk + 1 < stop) fetch(chunk + 1);
 
         v4f acc[TT][MW];
         if constexpr (!ENDS) {
             if (a.saved) {
-                float *at = a.saved + (head * chunks + chunk) * E * a.Mp + m0 + mw;
+                float *at = a.saved + (head * chunks + chunk) * E * a.Mp + m0;
 #pragma unroll
                 for (int b = 0; b < NB; b++)
 #pragma unroll
@@ -207,7 +279,7 @@ __global__ __launch_bounds__(64 * NW) void k_dsum_fwd(const DsumWalk a) {
 #pragma unroll
                         for (int j = 0; j < MW; j++)
 #pragma unroll
-                            for (int i = 0; i < 4; i++) at[(32 * b + 8 * g + 4 * u + i) * a.Mp + place(MW, c, j)] = S[b][u][j][i];
+                            for (int i = 0; i < 4; i++) *from(at, (uint32_t)(32 * b + 8 * g + 4 * u + i) * (uint32_t)a.Mp + mw + place(MW, c, j)) = S[b][u][j][i];
             }
             // P, a 16 x 16 tile of it at a time
             for (int tile = wave; tile < TT * (TT + 1) / 2; tile += NW) {
@@ -221,10 +293,7 @@ __global__ __launch_bounds__(64 * NW) void k_dsum_fwd(const DsumWalk a) {
                 float x[4];
 #pragma unroll
                 for (int i = 0; i < 4; i++) x[i] = s + i <= t ? p[i] * f[i] : 0.f;      // a product beyond the diagonal may be infinite
-                v4b parts[O];
-                split<O, 4>(x, parts);
-#pragma unroll
-                for (int o = 0; o < O; o++) sh.p.put4(o, t, s, parts[o]);
+                sh.p.put4(t, s, x);
             }
             // what the queries read from the state
 #pragma unroll
@@ -259,7 +328,7 @@ __global__ __launch_bounds__(64 * NW) void k_dsum_fwd(const DsumWalk a) {
                 for (int j = 0; j < MW; j++) S[b][u][j] *= d.whole;
 #pragma unroll
         for (int sb = 0; sb < SB; sb++) {
-            Frag<kWide> vs[MW];
+            Frag<X> vs[MW];
             const v4f r0 = *reinterpret_cast<const v4f *>(&d.rest[32 * sb + 8 * g]), r1 = *reinterpret_cast<const v4f *>(&d.rest[32 * sb + 8 * g + 4]);
 #pragma unroll
             for (int j = 0; j < MW; j++) {
@@ -272,7 +341,7 @@ __global__ __launch_bounds__(64 * NW) void k_dsum_fwd(const DsumWalk a) {
                 join8(v, x);
 #pragma unroll
                 for (int i = 0; i < 4; i++) x[i] *= r0[i], x[i + 4] *= r1[i];
-                vs[j] = split8<kWide>(x);
+                vs[j] = split8<X>(x);
             }
 #pragma unroll
             for (int b = 0; b < NB; b++)
@@ -280,23 +349,13 @@ __global__ __launch_bounds__(64 * NW) void k_dsum_fwd(const DsumWalk a) {
                 for (int u = 0; u < 2; u++) {
                     const Frag<P> k = sh.k.template columns<2>(32 * b, u, 32 * sb, g, c);
 #pragma unroll
-                    for (int j = 0; j < MW; j++) S[b][u][j] = product<kWide>(k, vs[j], S[b][u][j]);
+                    for (int j = 0; j < MW; j++) S[b][u][j] = product<X>(k, vs[j], S[b][u][j]);
                 }
         }
         if constexpr (!ENDS) {
-#pragma unroll
-            for (int I = 0; I < TT; I++) {
-                const int t = chunk * C + 16 * I + c;
-                if (t >= a.L) continue;
-                float x[4 * MW];
-#pragma unroll
-                for (int j = 0; j < MW; j++)
-#pragma unroll
-                    for (int i = 0; i < 4; i++) x[4 * j + i] = t < len ? acc[I][j][i] * a.scale : 0.f;
-                store_some<T, 4 * MW>(ob + t * a.out.sL, mw + 4 * MW * g, mcols, x);
-            }
+            const int col = mw + 4 * MW * g;
+            store_rows<T, C, MW>(ob + (int64_t)chunk * C * a.out.sL, (int)a.out.sL, col, acc, a.scale, rows, a.L - chunk * C, rows >= C && values == MS, values - col, c);
         }
-        if (chunk + 1 < stop && wave == NW - 1) total += sh.d[(chunk + 1) & 1].sum(gnext, lane);
         lds_barrier();
     }
 
@@ -339,37 +398,38 @@ __global__ __launch_bounds__(64 * NW) void k_dsum_fwd(const DsumWalk a) {
 
 template <typename T, int NE, int NW, int MW>
 struct DsumBackward {
-    static constexpr int C = kChunkOf<T>, P = kPartsOf<T>, O = kOrdersOf<T>, E = 16 * NE, MS = 16 * MW * NW, kThreads = 64 * NW;
-    static constexpr int NB = NE / 2, SB = C / 32, TT = C / 16, MB = (MW * NW + 1) / 2;
+    static constexpr int C = kChunkOf<T>, P = Parts<T, NE>::P, O = Parts<T, NE>::O, X = Parts<T, NE>::X, E = 16 * NE, MS = 16 * MW * NW, kThreads = 64 * NW;
+    static constexpr int NB = NE / 2, SB = C / 32, TT = C / 16, MB = MW * NW / 2;      // an even number of waves
     static constexpr int EW = NE >= NW ? NE / NW : 1;      // key tiles of a wave
     struct Shared {
         Tile<C, E, P> q, k;
-        Tile<C, 32 * MB, P> v, go;
+        Tile<C, MS, P> v, go;
         Tile<C, C, O> p;
-        Tile<C, C, kWide> r;
+        Tile<C, C, O> r;
         Decays<C> d[2];
-        float sums[NW][C], inner[NW];
+        float sums[2][NW][C], within[2][TT + 1][C], inner[2][NW];
     };
     struct Ends {
         Tile<C, E, P> q;
         Tile<C, MS, P> go;
         Decays<C> d[2];
     };
+    static constexpr int kWaves = P == kPlain && NW <= 4 ? 3 : NE <= 4 || NW == 8 ? 2 : 1, kEndWaves = NE <= 4 ? 4 : 3;
 };
 
 // The adjoint of a segment's first state when that of its last one is zero, and the segment's whole decay.
 template <typename T, int NE, int NW, int MW>
-__global__ __launch_bounds__(64 * NW) void k_dsum_bwd_ends(const DsumWalk a) {
+__global__ __launch_bounds__(64 * NW, (DsumBackward<T, NE, NW, MW>::kEndWaves)) void k_dsum_bwd_ends(const DsumWalk a) {
     using F = DsumBackward<T, NE, NW, MW>;
-    constexpr int C = F::C, P = F::P, E = F::E, MS = F::MS, NB = F::NB, SB = F::SB;
+    constexpr int C = F::C, P = F::P, X = F::X, E = F::E, MS = F::MS, NB = F::NB, SB = F::SB;
     __shared__ typename F::Ends sh;
     const int tid = threadIdx.x, lane = tid % 64, wave = tid / 64, g = lane / 16, c = lane % 16;
     int64_t w = by_xcd(blockIdx.x, gridDim.x);
     const int slice = w % a.slices;
     w /= a.slices;
-    const int seg = w % (a.segments - 1) + 1;
-    w /= a.segments - 1;
-    const int h = w % a.H, n = w / a.H;
+    const int h = w % a.H;
+    w /= a.H;
+    const int n = w % a.N, seg = w / a.N + 1;
     const int len = length_of(a.lengths, n, a.L), chunks = (a.L + C - 1) / C, live = (len + C - 1) / C;
     const int first = seg * a.per, stop = min(min(first + a.per, chunks), live);
     const int hq = h / (a.H / a.HQ), m0 = slice * MS, mcols = min(a.M - m0, MS), mw = wave * 16 * MW;
@@ -390,19 +450,29 @@ __global__ __launch_bounds__(64 * NW) void k_dsum_bwd_ends(const DsumWalk a) {
     const auto fetch = [&](int chunk) {
         const int64_t t0 = (int64_t)chunk * C;
         const int rows = len - (int)t0;
-        sq.load(qb + t0 * a.q.sL, a.q.sL, rows, a.E, tid);
-        sd.load(db + t0 * a.go.sL, a.go.sL, rows, mcols, tid);
-        if (wave == NW - 1) gnext = lane < C && lane < rows ? gb[(t0 + lane) * a.dL] : 0.f;
+        sq.load(qb + t0 * a.q.sL, (int)a.q.sL, rows, a.E, tid);
+        sd.load(db + t0 * a.go.sL, (int)a.go.sL, rows, mcols, tid);
     };
+    const auto fetch_decay = [&](int chunk) { gnext = gb[min((int64_t)chunk * C + lane, (int64_t)len - 1) * a.dL]; };
+    const auto sum_decay = [&](int chunk) { total += sh.d[chunk & 1].sum(lane < C && chunk * C + lane < len ? gnext : 0.f, lane); };
     if (first < stop) {
+        if (wave == NW - 1) fetch_decay(stop - 1);
         fetch(stop - 1);
-        if (wave == NW - 1) total += sh.d[(stop - 1) & 1].sum(gnext, lane);
+        if (wave == NW - 1) {
+            sum_decay(stop - 1);
+            if (stop - 1 > first) fetch_decay(stop - 2);
+        }
     }
     for (int chunk = stop - 1; chunk >= first; chunk--) {
-        sq.put(sh.q, tid);
-        sd.put(sh.go, tid);
+        const int rows = len - chunk * C;
+        sq.put(sh.q, rows, opaque(a.E), tid);
+        sd.put(sh.go, rows, opaque(mcols), tid);
         lds_barrier();
         const Decays<C> &d = sh.d[chunk & 1];
+        if (wave == NW - 1 && chunk > first) {
+            sum_decay(chunk - 1);
+            if (chunk - 1 > first) fetch_decay(chunk - 2);
+        }
         if (chunk > first) fetch(chunk - 1);
 #pragma unroll
         for (int b = 0; b < NB; b++)
@@ -413,14 +483,14 @@ __global__ __launch_bounds__(64 * NW) void k_dsum_bwd_ends(const DsumWalk a) {
 #pragma unroll
         for (int tb = 0; tb < SB; tb++) {
             const v4f f0 = *reinterpret_cast<const v4f *>(&d.into[32 * tb + 8 * g]), f1 = *reinterpret_cast<const v4f *>(&d.into[32 * tb + 8 * g + 4]);
-            Frag<kWide> ds[MW];
+            Frag<X> ds[MW];
 #pragma unroll
             for (int j = 0; j < MW; j++) {
                 float x[8];
                 join8(sh.go.template columns<MW>(mw, j, 32 * tb, g, c), x);
 #pragma unroll
                 for (int i = 0; i < 4; i++) x[i] *= f0[i], x[i + 4] *= f1[i];
-                ds[j] = split8<kWide>(x);
+                ds[j] = split8<X>(x);
             }
 #pragma unroll
             for (int b = 0; b < NB; b++)
@@ -428,10 +498,9 @@ __global__ __launch_bounds__(64 * NW) void k_dsum_bwd_ends(const DsumWalk a) {
                 for (int u = 0; u < 2; u++) {
                     const Frag<P> q = sh.q.template columns<2>(32 * b, u, 32 * tb, g, c);
 #pragma unroll
-                    for (int j = 0; j < MW; j++) G[b][u][j] = product<kWide>(q, ds[j], G[b][u][j]);
+                    for (int j = 0; j < MW; j++) G[b][u][j] = product<X>(q, ds[j], G[b][u][j]);
                 }
         }
-        if (chunk > first && wave == NW - 1) total += sh.d[(chunk - 1) & 1].sum(gnext, lane);
         lds_barrier();
     }
     float *at = a.ends + (head * a.segments + seg - 1) * E * a.Mp + m0 + mw;
@@ -447,17 +516,17 @@ __global__ __launch_bounds__(64 * NW) void k_dsum_bwd_ends(const DsumWalk a) {
 }
 
 template <typename T, int NE, int NW, int MW>
-__global__ __launch_bounds__(64 * NW) void k_dsum_bwd(const DsumWalk a) {
+__global__ __launch_bounds__(64 * NW, (DsumBackward<T, NE, NW, MW>::kWaves)) void k_dsum_bwd(const DsumWalk a) {
     using F = DsumBackward<T, NE, NW, MW>;
-    constexpr int C = F::C, P = F::P, O = F::O, E = F::E, MS = F::MS, NB = F::NB, SB = F::SB, TT = F::TT, MB = F::MB, EW = F::EW;
+    constexpr int C = F::C, P = F::P, O = F::O, X = F::X, E = F::E, MS = F::MS, NB = F::NB, SB = F::SB, TT = F::TT, MB = F::MB, EW = F::EW;
     __shared__ typename F::Shared sh;
     const int tid = threadIdx.x, lane = tid % 64, wave = tid / 64, g = lane / 16, c = lane % 16;
     int64_t w = by_xcd(blockIdx.x, gridDim.x);
     const int slice = w % a.slices;
     w /= a.slices;
-    const int seg = w % a.segments;
-    w /= a.segments;
-    const int h = w % a.H, n = w / a.H;
+    const int h = w % a.H;
+    w /= a.H;
+    const int n = w % a.N, seg = w / a.N;
     const int len = length_of(a.lengths, n, a.L), chunks = (a.L + C - 1) / C, live = (len + C - 1) / C;
     const int first = seg * a.per, last = min(first + a.per, chunks), stop = min(last, live);
     const int rq = a.H / a.HQ, rk = a.H / a.HK, rv = a.H / a.HV, m0 = slice * MS, mcols = min(a.M - m0, MS), mw = wave * 16 * MW, ew = wave * 16 * EW;
@@ -465,6 +534,12 @@ __global__ __launch_bounds__(64 * NW) void k_dsum_bwd(const DsumWalk a) {
     const T *qb = row<T>(a.q, n, h / rq, 0), *kb = row<T>(a.k, n, h / rk, 0), *vb = row<T>(a.v, n, h / rv, 0) + m0, *db = row<T>(a.go, n, h, 0) + m0;
     const float *gb = a.decay + n * a.dN + h * a.dH;
     const int64_t head = (int64_t)n * a.H + h;
+
+    // where this head's gradients go: rows of their own, or its part of a sum
+    float *const pq = a.pq + ((((int64_t)(h % rq) * a.slices + slice) * a.N + n) * a.HQ + h / rq) * a.L * a.E;
+    float *const pk = a.pk + ((((int64_t)(h % rk) * a.slices + slice) * a.N + n) * a.HK + h / rk) * a.L * a.E;
+    float *const pv = a.pv + (((int64_t)(h % rv) * a.N + n) * a.HV + h / rv) * a.L * a.M + m0;
+    T *const gq = row<T>(a.gq, n, h, 0), *const gk = row<T>(a.gk, n, h, 0), *const gv = row<T>(a.gv, n, h, 0) + m0;
 
     // G: all key rows of this wave's value columns.  H: the same numbers, all value columns of its key rows, transposed.
     v4f G[NB][2][MW], H[MB][2][EW];
@@ -487,7 +562,7 @@ __global__ __launch_bounds__(64 * NW) void k_dsum_bwd(const DsumWalk a) {
 #pragma unroll
                     for (int i = 0; i < 4; i++) {
                         const int m = 32 * b + 8 * g + 4 * u + i;
-                        H[b][u][j][i] = from && keys && m < MS ? from[(ew + place(EW, c, j)) * a.Mp + m] : 0.f;
+                        H[b][u][j][i] = from && keys ? from[(ew + place(EW, c, j)) * a.Mp + m] : 0.f;
                     }
     }
     for (int i = tid; i < (int)(sizeof(sh.p) / 16); i += 64 * NW) reinterpret_cast<v4f *>(&sh.p)[i] = v4f{0, 0, 0, 0};
@@ -495,82 +570,119 @@ __global__ __launch_bounds__(64 * NW) void k_dsum_bwd(const DsumWalk a) {
 
     // what this wave reads of a chunk's first state, by key rows
     const auto before = [&](int chunk, int b, int j, float (&x)[8]) {
-        const int m = 32 * b + 8 * g;
-        if (keys && m < MS) {
-            const float *at = a.saved + ((head * chunks + chunk) * E + ew + place(EW, c, j)) * a.Mp + m0 + m;
-            const float4 lo = *reinterpret_cast<const float4 *>(at), hi = *reinterpret_cast<const float4 *>(at + 4);
-            x[0] = lo.x, x[1] = lo.y, x[2] = lo.z, x[3] = lo.w, x[4] = hi.x, x[5] = hi.y, x[6] = hi.z, x[7] = hi.w;
-        } else {
-#pragma unroll
-            for (int i = 0; i < 8; i++) x[i] = 0.f;
-        }
+        const float *at = from((const float *)a.saved + (head * chunks + chunk) * E * a.Mp + m0, (uint32_t)((keys ? ew : 0) + place(EW, c, j)) * (uint32_t)a.Mp + 32 * b + 8 * g);
+        const float4 lo = *reinterpret_cast<const float4 *>(at), hi = *reinterpret_cast<const float4 *>(at + 4);
+        x[0] = lo.x, x[1] = lo.y, x[2] = lo.z, x[3] = lo.w, x[4] = hi.x, x[5] = hi.y, x[6] = hi.z, x[7] = hi.w;
     };
-    // <H, the first state of `chunk`>, this wave's part
-    const auto inner = [&](int chunk) {
+    // <H, S>, this wave's part
+    const auto inner = [&](const float(&S)[MB][EW][8]) {
         float s = 0.f;
 #pragma unroll
         for (int b = 0; b < MB; b++)
 #pragma unroll
-            for (int j = 0; j < EW; j++) {
-                float x[8];
-                before(chunk, b, j, x);
+            for (int j = 0; j < EW; j++)
 #pragma unroll
-                for (int i = 0; i < 4; i++) s = fmaf(x[i], H[b][0][j][i], s), s = fmaf(x[i + 4], H[b][1][j][i], s);
-            }
-#pragma unroll
-        for (int off = 1; off < 64; off *= 2) s += __shfl_xor(s, off);
-        return s;
+                for (int i = 0; i < 4; i++) s = fmaf(S[b][j][i], H[b][0][j][i], s), s = fmaf(S[b][j][i + 4], H[b][1][j][i], s);
+        return over_groups(over_sixteen(s));
     };
 
     Stage<T, C, E, 64 * NW> sq, sk;
-    Stage<T, C, 32 * MB, 64 * NW> sv, sd;
+    Stage<T, C, MS, 64 * NW> sv, sd;
     float gnext = 0, all = 0;
     const auto fetch = [&](int chunk) {
         const int64_t t0 = (int64_t)chunk * C;
         const int rows = len - (int)t0;
-        sq.load(qb + t0 * a.q.sL, a.q.sL, rows, a.E, tid);
-        sk.load(kb + t0 * a.k.sL, a.k.sL, rows, a.E, tid);
-        sv.load(vb + t0 * a.v.sL, a.v.sL, rows, mcols, tid);
-        sd.load(db + t0 * a.go.sL, a.go.sL, rows, mcols, tid);
-        if (wave == NW - 1) gnext = lane < C && lane < rows ? gb[(t0 + lane) * a.dL] : 0.f;
+        sq.load(qb + t0 * a.q.sL, (int)a.q.sL, rows, a.E, tid);
+        sk.load(kb + t0 * a.k.sL, (int)a.k.sL, rows, a.E, tid);
+        sv.load(vb + t0 * a.v.sL, (int)a.v.sL, rows, mcols, tid);
+        sd.load(db + t0 * a.go.sL, (int)a.go.sL, rows, mcols, tid);
     };
+    const auto fetch_decay = [&](int chunk) { gnext = gb[min((int64_t)chunk * C + lane, (int64_t)len - 1) * a.dL]; };
+    const auto sum_decay = [&](int chunk) { sh.d[chunk & 1].sum(lane < C && chunk * C + lane < len ? gnext : 0.f, lane); };
     if (first < stop) {
+        if (wave == NW - 1) fetch_decay(stop - 1);
         fetch(stop - 1);
-        if (wave == NW - 1) sh.d[(stop - 1) & 1].sum(gnext, lane);
+        if (wave == NW - 1) {
+            sum_decay(stop - 1);
+            if (stop - 1 > first) fetch_decay(stop - 2);
+        }
     }
     // the inner product at the segment's end, with the next segment's first state; behind the last chunk the adjoint is zero
-    float x_end = stop == last && stop < live ? inner(stop) : 0.f;
+    float x_end = 0.f;
+    if (stop == last && stop < live) {
+        float S[MB][EW][8];
+#pragma unroll
+        for (int b = 0; b < MB; b++)
+#pragma unroll
+            for (int j = 0; j < EW; j++) before(stop, b, j, S[b][j]);
+        x_end = inner(S);
+    }
+
+    // the decays' gradients of the chunk behind this one, from what the waves have left in LDS
+    const auto decay_gradients = [&](int chunk) {
+        float s = 0.f, x = 0.f;
+#pragma unroll
+        for (int i = 0; i < NW; i++) s += sh.sums[chunk & 1][i][lane % C], x += sh.inner[chunk & 1][i];
+#pragma unroll
+        for (int i = 0; i <= TT; i++) s += sh.within[chunk & 1][i][lane % C];
+        if (lane >= C) s = 0.f;
+#pragma unroll
+        for (int off = 1; off < C; off *= 2) {
+            const float y = __shfl_down(s, off);
+            if (lane + off < C) s += y;
+        }
+        const int t = chunk * C + lane;
+        s = lane < C && t < len ? (s + x) * a.scale : 0.f;
+        if (a.sum_decay) all += s;
+        else if (lane < C && t < a.L) a.gdecay[(((int64_t)slice * a.N + n) * a.H + h) * a.L + t] = s;
+    };
 
     for (int chunk = stop - 1; chunk >= first; chunk--) {
-        sq.put(sh.q, tid);
-        sk.put(sh.k, tid);
-        sv.put(sh.v, tid);
-        sd.put(sh.go, tid);
-        if (lane == 0) sh.inner[wave] = x_end;
+        const int rows = len - chunk * C, wide = opaque(a.E), values = opaque(mcols);
+        sq.put(sh.q, rows, wide, tid);
+        sk.put(sh.k, rows, wide, tid);
+        sv.put(sh.v, rows, values, tid);
+        sd.put(sh.go, rows, values, tid);
+        if (lane == 0) sh.inner[chunk & 1][wave] = x_end;
         lds_barrier();
         const Decays<C> &d = sh.d[chunk & 1];
+        float S[MB][EW][8];
+#pragma unroll
+        for (int b = 0; b < MB; b++)
+#pragma unroll
+            for (int j = 0; j < EW; j++) before(chunk, b, j, S[b][j]);
+        if (wave == NW - 1 && chunk > first) {
+            sum_decay(chunk - 1);
+            if (chunk - 1 > first) fetch_decay(chunk - 2);
+        }
         if (chunk > first) fetch(chunk - 1);
+        if (wave == NW - 2 && chunk + 1 < stop) decay_gradients(chunk + 1);
 
         for (int tile = wave; tile < TT * (TT + 1) / 2; tile += NW) {
             int I = 0, J = tile;
             while (J > I) J -= ++I;
             v4f p = {0, 0, 0, 0}, r = {0, 0, 0, 0};
 #pragma unroll
-            for (int b = 0; b < NB; b++) p = product<O>(sh.k.rows(16 * J, 32 * b, g, c), sh.q.rows(16 * I, 32 * b, g, c), p);
+            for (int b = 0; b < NB; b++) p = product<X>(sh.k.rows(16 * J, 32 * b, g, c), sh.q.rows(16 * I, 32 * b, g, c), p);
 #pragma unroll
-            for (int b = 0; b < MB; b++) r = product<kWide>(sh.v.rows(16 * J, 32 * b, g, c), sh.go.rows(16 * I, 32 * b, g, c), r);
+            for (int b = 0; b < MB; b++) r = product<X>(sh.v.rows(16 * J, 32 * b, g, c), sh.go.rows(16 * I, 32 * b, g, c), r);
             const int t = 16 * I + c, s = 16 * J + 4 * g;
             const v4f f = d.between(t, s);
-            float x[4], y[4];
+            float x[4], y[4], u = 0.f, z[4];
 #pragma unroll
-            for (int i = 0; i < 4; i++) x[i] = s + i <= t ? p[i] * f[i] : 0.f, y[i] = s + i <= t ? r[i] * f[i] : 0.f;
-            v4b parts[O], wide[kWide];
-            split<O, 4>(x, parts);
-            split<kWide, 4>(y, wide);
+            for (int i = 0; i < 4; i++) {
+                x[i] = s + i <= t ? p[i] * f[i] : 0.f, y[i] = s + i <= t ? r[i] * f[i] : 0.f;
+                z[i] = s + i < t ? x[i] * r[i] : 0.f;
+                u += z[i];
+            }
+            // what step t reads of what step s wrote counts for the decays between them: sums over s for every t, and over t for every s
+            u = over_groups(u);
 #pragma unroll
-            for (int o = 0; o < O; o++) sh.p.put4(o, t, s, parts[o]);
-#pragma unroll
-            for (int o = 0; o < kWide; o++) sh.r.put4(o, t, s, wide[o]);
+            for (int i = 0; i < 4; i++) z[i] = over_sixteen(z[i]);
+            if (g == 0) sh.within[chunk & 1][J][t] = u;
+            if (c == 0) *reinterpret_cast<v4f *>(&sh.within[chunk & 1][I == J ? TT : I][s]) = v4f{-z[0], -z[1], -z[2], -z[3]};
+            sh.p.put4(t, s, x);
+            sh.r.put4(t, s, y);
         }
 
         v4f dq[TT][EW], dk[TT][EW], dv[TT][MW];
@@ -585,19 +697,17 @@ __global__ __launch_bounds__(64 * NW) void k_dsum_bwd(const DsumWalk a) {
         if (keys) {
 #pragma unroll
             for (int b = 0; b < MB; b++) {
-                Frag<kWide> s[EW], ht[EW];
+                Frag<X> s[EW], ht[EW];
 #pragma unroll
                 for (int j = 0; j < EW; j++) {
-                    float x[8];
-                    before(chunk, b, j, x);
-                    s[j] = split8<kWide>(x);
-                    ht[j] = split8<kWide>(H[b][0][j], H[b][1][j]);
+                    s[j] = split8<X>(S[b][j]);
+                    ht[j] = split8<X>(H[b][0][j], H[b][1][j]);
                 }
 #pragma unroll
                 for (int I = 0; I < TT; I++) {
                     const Frag<P> go = sh.go.rows(16 * I, 32 * b, g, c), v = sh.v.rows(16 * I, 32 * b, g, c);
 #pragma unroll
-                    for (int j = 0; j < EW; j++) dq[I][j] = product<kWide>(s[j], go, dq[I][j]), dk[I][j] = product<kWide>(ht[j], v, dk[I][j]);
+                    for (int j = 0; j < EW; j++) dq[I][j] = product<X>(s[j], go, dq[I][j]), dk[I][j] = product<X>(ht[j], v, dk[I][j]);
                 }
             }
         }
@@ -615,9 +725,20 @@ __global__ __launch_bounds__(64 * NW) void k_dsum_bwd(const DsumWalk a) {
         }
 #pragma unroll
         for (int I = 0; I < TT; I++) {
-            const float into = d.into[16 * I + c], rest = d.rest[16 * I + c];
+            const int r = 16 * I + c;
+            const float into = d.into[r], rest = d.rest[r];
+            float u = 0.f;
 #pragma unroll
-            for (int j = 0; j < EW; j++) dq[I][j] *= into, dk[I][j] *= rest;
+            for (int j = 0; j < EW; j++) {
+                dq[I][j] *= into, dk[I][j] *= rest;
+                if (keys) {
+                    const v4f q = sh.q.four(r, ew + 4 * EW * g + 4 * j), k = sh.k.four(r, ew + 4 * EW * g + 4 * j);
+#pragma unroll
+                    for (int i = 0; i < 4; i++) u = fmaf(q[i], dq[I][j][i], u), u = fmaf(-k[i], dk[I][j][i], u);
+                }
+            }
+            u = over_groups(u);
+            if (g == 0) sh.sums[chunk & 1][wave][r] = u;
 #pragma unroll
             for (int j = 0; j < MW; j++) dv[I][j] *= rest;
         }
@@ -640,19 +761,19 @@ __global__ __launch_bounds__(64 * NW) void k_dsum_bwd(const DsumWalk a) {
         for (int sb = 0; sb < SB; sb++) {
             const v4f f0 = *reinterpret_cast<const v4f *>(&d.into[32 * sb + 8 * g]), f1 = *reinterpret_cast<const v4f *>(&d.into[32 * sb + 8 * g + 4]);
             if (keys) {
-                Frag<kWide> qs[EW];
+                Frag<X> qs[EW];
 #pragma unroll
                 for (int j = 0; j < EW; j++) {
                     const Frag<P> k = sh.k.template columns<EW>(ew, j, 32 * sb, g, c), q = sh.q.template columns<EW>(ew, j, 32 * sb, g, c);
 #pragma unroll
-                    for (int I = 2 * sb; I < TT; I++) dq[I][j] = product<kWide>(k, sh.r.rows(16 * I, 32 * sb, g, c), dq[I][j]);
+                    for (int I = 2 * sb; I < TT; I++) dq[I][j] = product<O>(k, sh.r.rows(16 * I, 32 * sb, g, c), dq[I][j]);
 #pragma unroll
-                    for (int I = 0; I < 2 * sb + 2; I++) dk[I][j] = product<kWide>(q, sh.r.template columns<1>(16 * I, 0, 32 * sb, g, c), dk[I][j]);
+                    for (int I = 0; I < 2 * sb + 2; I++) dk[I][j] = product<O>(q, sh.r.template columns<1>(16 * I, 0, 32 * sb, g, c), dk[I][j]);
                     float x[8];
                     join8(q, x);
 #pragma unroll
                     for (int i = 0; i < 4; i++) x[i] *= f0[i], x[i + 4] *= f1[i];
-                    qs[j] = split8<kWide>(x);
+                    qs[j] = split8<X>(x);
                 }
 #pragma unroll
                 for (int b = 0; b < MB; b++)
@@ -660,10 +781,10 @@ __global__ __launch_bounds__(64 * NW) void k_dsum_bwd(const DsumWalk a) {
                     for (int u = 0; u < 2; u++) {
                         const Frag<P> go = sh.go.template columns<2>(32 * b, u, 32 * sb, g, c);
 #pragma unroll
-                        for (int j = 0; j < EW; j++) H[b][u][j] = product<kWide>(go, qs[j], H[b][u][j]);
+                        for (int j = 0; j < EW; j++) H[b][u][j] = product<X>(go, qs[j], H[b][u][j]);
                     }
             }
-            Frag<kWide> ds[MW];
+            Frag<X> ds[MW];
 #pragma unroll
             for (int j = 0; j < MW; j++) {
                 const Frag<P> go = sh.go.template columns<MW>(mw, j, 32 * sb, g, c);
@@ -673,7 +794,7 @@ __global__ __launch_bounds__(64 * NW) void k_dsum_bwd(const DsumWalk a) {
                 join8(go, x);
 #pragma unroll
                 for (int i = 0; i < 4; i++) x[i] *= f0[i], x[i + 4] *= f1[i];
-                ds[j] = split8<kWide>(x);
+                ds[j] = split8<X>(x);
             }
 #pragma unroll
             for (int b = 0; b < NB; b++)
@@ -681,71 +802,29 @@ __global__ __launch_bounds__(64 * NW) void k_dsum_bwd(const DsumWalk a) {
                 for (int u = 0; u < 2; u++) {
                     const Frag<P> q = sh.q.template columns<2>(32 * b, u, 32 * sb, g, c);
 #pragma unroll
-                    for (int j = 0; j < MW; j++) G[b][u][j] = product<kWide>(q, ds[j], G[b][u][j]);
+                    for (int j = 0; j < MW; j++) G[b][u][j] = product<X>(q, ds[j], G[b][u][j]);
                 }
         }
 
-        // results, and the rows' part of the decays' gradients
-#pragma unroll
-        for (int I = 0; I < TT; I++) {
-            const int r = 16 * I + c, t = chunk * C + r;
-            float u = 0.f;
-            if (keys) {
-                float xq[4 * EW], xk[4 * EW];
-#pragma unroll
-                for (int j = 0; j < EW; j++) {
-                    const v4f q = sh.q.four(r, ew + 4 * EW * g + 4 * j), k = sh.k.four(r, ew + 4 * EW * g + 4 * j);
-#pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        u = fmaf(q[i], dq[I][j][i], u), u = fmaf(-k[i], dk[I][j][i], u);
-                        xq[4 * j + i] = t < len ? dq[I][j][i] * a.scale : 0.f, xk[4 * j + i] = t < len ? dk[I][j][i] * a.scale : 0.f;
-                    }
-                }
-                if (t < a.L) {
-                    const int col = ew + 4 * EW * g;
-                    if (a.pq) store_some<float, 4 * EW>(a.pq + ((((int64_t)(h % rq) * a.slices + slice) * a.N + n) * a.HQ + h / rq) * a.L * a.E + (int64_t)t * a.E, col, a.E, xq);
-                    else store_some<T, 4 * EW>(row<T>(a.gq, n, h, t), col, a.E, xq);
-                    if (a.pk) store_some<float, 4 * EW>(a.pk + ((((int64_t)(h % rk) * a.slices + slice) * a.N + n) * a.HK + h / rk) * a.L * a.E + (int64_t)t * a.E, col, a.E, xk);
-                    else store_some<T, 4 * EW>(row<T>(a.gk, n, h, t), col, a.E, xk);
-                }
-            }
-            u += __shfl_xor(u, 16);
-            u += __shfl_xor(u, 32);
-            if (g == 0) sh.sums[wave][r] = u;
-            if (t < a.L) {
-                float xv[4 * MW];
-#pragma unroll
-                for (int j = 0; j < MW; j++)
-#pragma unroll
-                    for (int i = 0; i < 4; i++) xv[4 * j + i] = t < len ? dv[I][j][i] * a.scale : 0.f;
-                const int col = mw + 4 * MW * g;
-                if (a.pv) store_some<float, 4 * MW>(a.pv + (((int64_t)(h % rv) * a.N + n) * a.HV + h / rv) * a.L * a.M + (int64_t)t * a.M + m0, col, mcols, xv);
-                else store_some<T, 4 * MW>(row<T>(a.gv, n, h, t) + m0, col, mcols, xv);
-            }
+        const int there = a.L - chunk * C;
+        if (keys) {
+            const int col = ew + 4 * EW * g;
+            const bool whole = rows >= C && wide == E;
+            if (a.pq) store_rows<float, C, EW>(pq + (int64_t)chunk * C * wide, wide, col, dq, a.scale, rows, there, whole, wide - col, c);
+            else store_rows<T, C, EW>(gq + (int64_t)chunk * C * a.gq.sL, (int)a.gq.sL, col, dq, a.scale, rows, there, whole, wide - col, c);
+            if (a.pk) store_rows<float, C, EW>(pk + (int64_t)chunk * C * wide, wide, col, dk, a.scale, rows, there, whole, wide - col, c);
+            else store_rows<T, C, EW>(gk + (int64_t)chunk * C * a.gk.sL, (int)a.gk.sL, col, dk, a.scale, rows, there, whole, wide - col, c);
         }
-        x_end = chunk > first ? inner(chunk) : 0.f;      // for the chunk before this one
-        if (chunk > first && wave == NW - 1) sh.d[(chunk - 1) & 1].sum(gnext, lane);
-        lds_barrier();
-        if (wave == 0) {
-            float s = 0.f, x = 0.f;
-            if (lane < C)
-#pragma unroll
-                for (int i = 0; i < NW; i++) s += sh.sums[i][lane];
-#pragma unroll
-            for (int i = 0; i < NW; i++) x += sh.inner[i];
-#pragma unroll
-            for (int off = 1; off < C; off *= 2) {
-                const float y = __shfl_down(s, off);
-                if (lane + off < C) s += y;
-            }
-            const int t = chunk * C + lane;
-            const bool counts = lane < C && t < len;
-            s = counts ? (s + x) * a.scale : 0.f;
-            if (a.sum_decay) all += s;
-            else if (lane < C && t < a.L) a.gdecay[(((int64_t)slice * a.N + n) * a.H + h) * a.L + t] = s;
+        {
+            const int col = mw + 4 * MW * g;
+            const bool whole = rows >= C && values == MS;
+            if (a.pv) store_rows<float, C, MW>(pv + (int64_t)chunk * C * a.M, a.M, col, dv, a.scale, rows, there, whole, values - col, c);
+            else store_rows<T, C, MW>(gv + (int64_t)chunk * C * a.gv.sL, (int)a.gv.sL, col, dv, a.scale, rows, there, whole, values - col, c);
         }
+        x_end = inner(S);      // for the chunk before this one
         lds_barrier();
     }
+    if (first < stop && wave == NW - 2) decay_gradients(first);
 
     // rows behind the sequence
     const int64_t t0 = (int64_t)max(stop, first) * C, t1 = min((int64_t)last * C, (int64_t)a.L);
@@ -753,20 +832,20 @@ __global__ __launch_bounds__(64 * NW) void k_dsum_bwd(const DsumWalk a) {
         const int64_t t = i / E;
         const int e = i % E;
         if (e >= a.E) continue;
-        if (a.pq) a.pq[((((int64_t)(h % rq) * a.slices + slice) * a.N + n) * a.HQ + h / rq) * a.L * a.E + t * a.E + e] = 0.f;
-        else row<T>(a.gq, n, h, t)[e] = (T)0.f;
-        if (a.pk) a.pk[((((int64_t)(h % rk) * a.slices + slice) * a.N + n) * a.HK + h / rk) * a.L * a.E + t * a.E + e] = 0.f;
-        else row<T>(a.gk, n, h, t)[e] = (T)0.f;
+        if (a.pq) pq[t * a.E + e] = 0.f;
+        else gq[t * a.gq.sL + e] = (T)0.f;
+        if (a.pk) pk[t * a.E + e] = 0.f;
+        else gk[t * a.gk.sL + e] = (T)0.f;
     }
     for (int64_t i = t0 * MS + tid; i < t1 * MS; i += 64 * NW) {
         const int64_t t = i / MS;
         const int m = i % MS;
         if (m >= mcols) continue;
-        if (a.pv) a.pv[(((int64_t)(h % rv) * a.N + n) * a.HV + h / rv) * a.L * a.M + t * a.M + m0 + m] = 0.f;
-        else (row<T>(a.gv, n, h, t) + m0)[m] = (T)0.f;
+        if (a.pv) pv[t * a.M + m] = 0.f;
+        else gv[t * a.gv.sL + m] = (T)0.f;
     }
     if (a.sum_decay) {
-        if (wave == 0) {
+        if (wave == NW - 2) {
 #pragma unroll
             for (int off = 1; off < 64; off *= 2) all += __shfl_xor(all, off);
             if (lane == 0) a.gdecay[(head * a.slices + slice) * a.segments + seg] = all;
@@ -780,37 +859,47 @@ __global__ __launch_bounds__(64 * NW) void k_dsum_bwd(const DsumWalk a) {
 
 enum { kDsumForward, kDsumForwardEnds, kDsumBackward, kDsumBackwardEnds };
 
-// Launches one of the four for states of Ep keys and slices of MS value columns; false: there is no such kernel.
+// Launches one of the four for states of Ep keys and slices of MS value columns, or with `a` NULL only says how many of its workgroups a CU holds at once; 0: there
+// is no such kernel.
 template <typename T>
-bool dsum_launch(int which, const DsumWalk &a, int Ep, int MS, unsigned blocks, hipStream_t s);
+int dsum_launch(int which, const DsumWalk *a, int Ep, int MS, unsigned blocks, hipStream_t s);
 
 template <typename T, int NE, int NW, int MW>
-void dsum_launch_one(int which, const DsumWalk &a, unsigned blocks, hipStream_t s) {
+int dsum_launch_one(int which, const DsumWalk *a, unsigned blocks, hipStream_t s) {
+    using F = DsumForward<T, NE, NW, MW>;
+    using B = DsumBackward<T, NE, NW, MW>;
     const dim3 grid(blocks), block(64 * NW);
     switch (which) {
-        case kDsumForward: k_dsum_fwd<T, NE, NW, MW, false><<<grid, block, 0, s>>>(a); break;
-        case kDsumForwardEnds: k_dsum_fwd<T, NE, NW, MW, true><<<grid, block, 0, s>>>(a); break;
-        case kDsumBackward: k_dsum_bwd<T, NE, NW, MW><<<grid, block, 0, s>>>(a); break;
-        default: k_dsum_bwd_ends<T, NE, NW, MW><<<grid, block, 0, s>>>(a); break;
+        case kDsumForward:
+            if (a) k_dsum_fwd<T, NE, NW, MW, false><<<grid, block, 0, s>>>(*a);
+            return resident(sizeof(typename F::Shared), F::kWaves, NW);
+        case kDsumForwardEnds:
+            if (a) k_dsum_fwd<T, NE, NW, MW, true><<<grid, block, 0, s>>>(*a);
+            return resident(sizeof(typename F::Ends), F::kEndWaves, NW);
+        case kDsumBackward:
+            if (a) k_dsum_bwd<T, NE, NW, MW><<<grid, block, 0, s>>>(*a);
+            return resident(sizeof(typename B::Shared), B::kWaves, NW);
+        default:
+            if (a) k_dsum_bwd_ends<T, NE, NW, MW><<<grid, block, 0, s>>>(*a);
+            return resident(sizeof(typename B::Ends), B::kEndWaves, NW);
     }
 }
 
 template <typename T, int NE>
-bool dsum_launch_keys(int which, const DsumWalk &a, int MS, unsigned blocks, hipStream_t s) {
-    if (MS == 32) dsum_launch_one<T, NE, 2, 1>(which, a, blocks, s);
-    else if (MS == 64) dsum_launch_one<T, NE, 4, 1>(which, a, blocks, s);
-    else if (MS == 128) dsum_launch_one<T, NE, 8, 1>(which, a, blocks, s);
-    else return false;
-    return true;
+int dsum_launch_keys(int which, const DsumWalk *a, int MS, unsigned blocks, hipStream_t s) {
+    if (MS == 32) return dsum_launch_one<T, NE, 2, 1>(which, a, blocks, s);
+    if (MS == 64) return dsum_launch_one<T, NE, 4, 1>(which, a, blocks, s);
+    if (MS == 128) return dsum_launch_one<T, NE, 8, 1>(which, a, blocks, s);
+    return 0;
 }
 
-#define FWP_DSUM_INSTANCES(T)                                                                              \
-    template <>                                                                                            \
-    bool dsum_launch<T>(int which, const DsumWalk &a, int Ep, int MS, unsigned blocks, hipStream_t s) {    \
-        if (Ep == 32) return dsum_launch_keys<T, 2>(which, a, MS, blocks, s);                              \
-        if (Ep == 64) return dsum_launch_keys<T, 4>(which, a, MS, blocks, s);                              \
-        if (Ep == 128) return dsum_launch_keys<T, 8>(which, a, MS, blocks, s);                             \
-        return false;                                                                                      \
+#define FWP_DSUM_INSTANCES(T)                                                                            \
+    template <>                                                                                          \
+    int dsum_launch<T>(int which, const DsumWalk *a, int Ep, int MS, unsigned blocks, hipStream_t s) {   \
+        if (Ep == 32) return dsum_launch_keys<T, 2>(which, a, MS, blocks, s);                            \
+        if (Ep == 64) return dsum_launch_keys<T, 4>(which, a, MS, blocks, s);                            \
+        if (Ep == 128) return dsum_launch_keys<T, 8>(which, a, MS, blocks, s);                           \
+        return 0;                                                                                        \
     }
 
 }  // namespace fwp

@@ -48,45 +48,70 @@ __device__ __forceinline__ float lanes_sum(float x) {
     return x;
 }
 
-template <typename T, int K>
+// A lane's elements of a row: K runs of V, those of a group from `first` on.  Every lane loads, what lies beyond the group from the group's last elements: a branch
+// around a load would wait for it at its end.  ODD: groups that are no multiple of a run, of which the last one is then shifted; groups shorter than one are
+// read element by element.
+template <typename T, int K, bool ODD>
 struct Run {
     static constexpr int V = 16 / sizeof(T);
-    struct __attribute__((packed, aligned(sizeof(T)))) Vec { T x[V]; };
-    T x[K][V];
-    // the lane's elements at + (first + i * step) .., those before `end`
-    __device__ __forceinline__ void load(const T *at, int first, int step, int end) {
+    typedef uint32_t Words __attribute__((ext_vector_type(4)));
+    struct __attribute__((packed, aligned(sizeof(T)))) Anywhere { Words w; };
+    struct Elements { T x[V]; };
+    Words w[K];
+
+    __device__ __forceinline__ void load(const T *at, int first, int step, int size) {
 #pragma unroll
         for (int i = 0; i < K; i++) {
             const int c = first + i * step;
-            if (c + V <= end) {
-                const Vec v = *reinterpret_cast<const Vec *>(at + c);
+            if (!ODD || size >= V) {
+                w[i] = reinterpret_cast<const Anywhere *>(at + min(c, size - V))->w;
+            } else {
+                Elements few;
 #pragma unroll
-                for (int e = 0; e < V; e++) x[i][e] = v.x[e];
+                for (int e = 0; e < V; e++) few.x[e] = at[min(e, size - 1)];
+                w[i] = __builtin_bit_cast(Words, few);
+            }
+        }
+    }
+    // as fp32, zero beyond the group
+    __device__ __forceinline__ void get(float (&x)[K][V], int first, int step, int size) const {
+#pragma unroll
+        for (int i = 0; i < K; i++) {
+            const Elements few = __builtin_bit_cast(Elements, w[i]);
+            const int c = first + i * step;
+#pragma unroll
+            for (int e = 0; e < V; e++) x[i][e] = (float)few.x[e];
+            if constexpr (ODD) {
+                const int late = size >= V ? max(0, c - (size - V)) : 0;
+#pragma unroll
+                for (int b = 1; b < V; b *= 2)
+#pragma unroll
+                    for (int e = 0; e < V; e++) x[i][e] = late & b ? x[i][e + b < V ? e + b : e] : x[i][e];
+#pragma unroll
+                for (int e = 0; e < V; e++) x[i][e] = c + e < size ? x[i][e] : 0.f;
             } else {
 #pragma unroll
-                for (int e = 0; e < V; e++) x[i][e] = c + e < end ? at[c + e] : (T)0.f;
+                for (int e = 0; e < V; e++) x[i][e] = c < size ? x[i][e] : 0.f;
+            }
+        }
+    }
+    __device__ __forceinline__ static void store(const float (&x)[K][V], T *at, int first, int step, int size) {
+#pragma unroll
+        for (int i = 0; i < K; i++) {
+            const int c = first + i * step;
+            if (!ODD || c + V <= size) {
+                Elements few;
+#pragma unroll
+                for (int e = 0; e < V; e++) few.x[e] = (T)x[i][e];
+                if (c < size) reinterpret_cast<Anywhere *>(at + c)->w = __builtin_bit_cast(Words, few);
+            } else {
+#pragma unroll
+                for (int e = 0; e < V; e++)
+                    if (c + e < size) at[c + e] = (T)x[i][e];
             }
         }
     }
 };
-template <typename T, int K, int V>
-__device__ __forceinline__ void store_run(const float (&x)[K][V], T *at, int first, int step, int end) {
-    using Vec = typename Run<T, K>::Vec;
-#pragma unroll
-    for (int i = 0; i < K; i++) {
-        const int c = first + i * step;
-        if (c + V <= end) {
-            Vec v;
-#pragma unroll
-            for (int e = 0; e < V; e++) v.x[e] = (T)x[i][e];
-            *reinterpret_cast<Vec *>(at + c) = v;
-        } else {
-#pragma unroll
-            for (int e = 0; e < V; e++)
-                if (c + e < end) at[c + e] = (T)x[i][e];
-        }
-    }
-}
 
 __device__ __forceinline__ float act_of(float x, int act) {
     if (act == FWP_ACT_NONE) return x;
@@ -156,7 +181,7 @@ __device__ __forceinline__ void parameters(float (&to)[K][V], const float *p, fl
         }
 }
 
-template <typename T, int W, int K>
+template <typename T, int W, int K, bool ODD>
 __global__ __launch_bounds__(256) void k_group_norm_fwd(const NormWalk w) {
     using L = Lane<T, W, K>;
     constexpr int V = L::V, step = L::kStep;
@@ -169,17 +194,17 @@ __global__ __launch_bounds__(256) void k_group_norm_fwd(const NormWalk w) {
     float weight[K][V], bias[K][V];
     parameters(weight, w.weight ? w.weight + off : nullptr, 1.f, l.first, step, w.size);
     parameters(bias, w.bias ? w.bias + off : nullptr, 0.f, l.first, step, w.size);
-    Run<T, K> x, gate;
+    Run<T, K, ODD> x, gate;
+#pragma unroll
+    for (int i = 0; i < K; i++) gate.w[i] = 0;
     if (l.row0 < w.rows) {
         x.load(xs + l.row0 * width, l.first, step, w.size);
         if (gs) gate.load(gs + l.row0 * width, l.first, step, w.size);
     }
     for (int r = l.row0; r < w.rows; r += l.rows_step) {
         float h[K][V], g[K][V];
-#pragma unroll
-        for (int i = 0; i < K; i++)
-#pragma unroll
-            for (int e = 0; e < V; e++) h[i][e] = (float)x.x[i][e], g[i][e] = gs ? (float)gate.x[i][e] : 0.f;
+        x.get(h, l.first, step, w.size);
+        gate.get(g, l.first, step, w.size);
         if (r + l.rows_step < w.rows) {
             x.load(xs + (r + l.rows_step) * width, l.first, step, w.size);
             if (gs) gate.load(gs + (r + l.rows_step) * width, l.first, step, w.size);
@@ -192,11 +217,11 @@ __global__ __launch_bounds__(256) void k_group_norm_fwd(const NormWalk w) {
                 const float u = fmaf(h[i][e], weight[i][e], bias[i][e]);
                 h[i][e] = gs ? u * act_of(g[i][e], w.act) : act_of(u, w.act);
             }
-        store_run<T, K, V>(h, ys + r * width, l.first, step, w.size);
+        Run<T, K, ODD>::store(h, ys + r * width, l.first, step, w.size);
     }
 }
 
-template <typename T, int W, int K>
+template <typename T, int W, int K, bool ODD>
 __global__ __launch_bounds__(256) void k_group_norm_bwd(const NormWalk w) {
     using L = Lane<T, W, K>;
     constexpr int V = L::V, step = L::kStep;
@@ -212,19 +237,20 @@ __global__ __launch_bounds__(256) void k_group_norm_bwd(const NormWalk w) {
     for (int i = 0; i < K; i++)
 #pragma unroll
         for (int e = 0; e < V; e++) gw[i][e] = gb[i][e] = 0.f;
-    Run<T, K> x, gate, gy;
+    Run<T, K, ODD> x, gate, gy;
     const auto fetch = [&](int r) {
         x.load(xs + r * width, l.first, step, w.size);
         gy.load(ds + r * width, l.first, step, w.size);
         if (gs) gate.load(gs + r * width, l.first, step, w.size);
     };
+#pragma unroll
+    for (int i = 0; i < K; i++) gate.w[i] = 0;
     if (l.live && l.row0 < w.rows) fetch(l.row0);
     for (int r = l.row0; l.live && r < w.rows; r += l.rows_step) {
         float h[K][V], g[K][V], d[K][V];
-#pragma unroll
-        for (int i = 0; i < K; i++)
-#pragma unroll
-            for (int e = 0; e < V; e++) h[i][e] = (float)x.x[i][e], d[i][e] = (float)gy.x[i][e], g[i][e] = gs ? (float)gate.x[i][e] : 0.f;
+        x.get(h, l.first, step, w.size);
+        gy.get(d, l.first, step, w.size);
+        gate.get(g, l.first, step, w.size);
         if (r + l.rows_step < w.rows) fetch(r + l.rows_step);
         const float rstd = normalise<W>(h, l.first, step, w.size, w.eps, w.rms);
         float s0 = 0.f, s1 = 0.f;
@@ -249,8 +275,8 @@ __global__ __launch_bounds__(256) void k_group_norm_bwd(const NormWalk w) {
         for (int i = 0; i < K; i++)
 #pragma unroll
             for (int e = 0; e < V; e++) d[i][e] = rstd * (d[i][e] - fmaf(h[i][e], m1, m0));
-        store_run<T, K, V>(d, static_cast<T *>(w.gx) + off + r * width, l.first, step, w.size);
-        if (gs) store_run<T, K, V>(g, static_cast<T *>(w.ggate) + off + r * width, l.first, step, w.size);
+        Run<T, K, ODD>::store(d, static_cast<T *>(w.gx) + off + r * width, l.first, step, w.size);
+        if (gs) Run<T, K, ODD>::store(g, static_cast<T *>(w.ggate) + off + r * width, l.first, step, w.size);
     }
     if (!w.sums) return;
     const int lane = threadIdx.x % 64;
@@ -274,28 +300,28 @@ __global__ __launch_bounds__(256) void k_group_norm_bwd(const NormWalk w) {
         }
 }
 
-// The workgroups' sums added: 16 columns and 16 parts of the workgroups to a workgroup here
+// The workgroups' sums added: 8 columns and 32 parts of the workgroups to a workgroup here
 __global__ __launch_bounds__(256) void k_group_norm_sums(const float *sums, float *gweight, float *gbias, int blocks, int64_t width) {
-    __shared__ float part[16][17];
-    const int c = threadIdx.x % 16, y = threadIdx.x / 16;
-    const int64_t col = (int64_t)blockIdx.x * 16 + c;
+    __shared__ float part[32][9];
+    const int c = threadIdx.x % 8, y = threadIdx.x / 8;
+    const int64_t col = (int64_t)blockIdx.x * 8 + c;
     float s = 0.f;
     if (col < 2 * width) {
 #pragma unroll 8
-        for (int b = y; b < blocks; b += 16) s += sums[b * 2 * width + col];
+        for (int b = y; b < blocks; b += 32) s += sums[b * 2 * width + col];
     }
     part[y][c] = s;
     __syncthreads();
     if (y || col >= 2 * width) return;
     s = 0.f;
 #pragma unroll
-    for (int i = 0; i < 16; i++) s += part[i][c];
+    for (int i = 0; i < 32; i++) s += part[i][c];
     float *to = col < width ? gweight : gbias;
     if (to) to[col < width ? col : col - width] = s;
 }
 
-// The workgroups of a run of groups: eight to a CU over all runs, and no more than have rows
-int row_blocks(int rows, int runs) { return std::max(1, std::min((rows + 3) / 4, 256 * 8 / runs)); }
+// The workgroups of a run of groups: four to a CU over all runs, and no more than have rows
+int row_blocks(int rows, int runs) { return std::max(1, std::min((rows + 3) / 4, 256 * 4 / runs)); }
 int lanes_of(int type, int size) {
     const int V = type == FWP_F32 ? 4 : 8;
     int W = 1;
@@ -308,8 +334,14 @@ void launch(NormWalk w, hipStream_t s) {
     const int runs = (w.groups + 64 / W - 1) / (64 / W);
     w.blocks = row_blocks(w.rows, runs);
     const unsigned grid = (unsigned)(runs * w.blocks);
-    if constexpr (BACKWARD) k_group_norm_bwd<T, W, K><<<grid, 256, 0, s>>>(w);
-    else k_group_norm_fwd<T, W, K><<<grid, 256, 0, s>>>(w);
+    const bool odd = w.size % (16 / (int)sizeof(T)) != 0;
+    if constexpr (BACKWARD) {
+        if (odd) k_group_norm_bwd<T, W, K, true><<<grid, 256, 0, s>>>(w);
+        else k_group_norm_bwd<T, W, K, false><<<grid, 256, 0, s>>>(w);
+    } else {
+        if (odd) k_group_norm_fwd<T, W, K, true><<<grid, 256, 0, s>>>(w);
+        else k_group_norm_fwd<T, W, K, false><<<grid, 256, 0, s>>>(w);
+    }
 }
 template <typename T, bool BACKWARD>
 void by_size(const NormWalk &w, hipStream_t s) {
@@ -323,7 +355,7 @@ void by_size(const NormWalk &w, hipStream_t s) {
     else if (vecs <= 32) launch<T, 32, 1, BACKWARD>(w, s);
     else if (vecs <= 64) launch<T, 64, 1, BACKWARD>(w, s);
     else if (vecs <= 128) launch<T, 64, 2, BACKWARD>(w, s);
-    else launch<T, 64, 4, BACKWARD>(w, s);
+    else if constexpr (sizeof(T) == 4) launch<T, 64, 4, BACKWARD>(w, s);
 }
 
 NormWalk walk_of(const fwp_group_norm_args &a) {
@@ -356,7 +388,7 @@ int group_norm_bwd(const fwp_group_norm_args &a, const void *gy, void *gx, void 
     by_type(a.type, [&](auto t) { by_size<decltype(t), true>(w, s); });
     if (w.sums) {
         const int64_t width = (int64_t)a.groups * a.size;
-        k_group_norm_sums<<<(unsigned)((2 * width + 15) / 16), 256, 0, s>>>(workspace, gweight, gbias, blocks_of(a.type, a.rows, a.groups, a.size), width);
+        k_group_norm_sums<<<(unsigned)((2 * width + 7) / 8), 256, 0, s>>>(workspace, gweight, gbias, blocks_of(a.type, a.rows, a.groups, a.size), width);
     }
     return (int)hipGetLastError();
 }

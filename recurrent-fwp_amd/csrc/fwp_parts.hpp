@@ -23,32 +23,51 @@ typedef short v4h __attribute__((ext_vector_type(4)));
 // bfloat16 parts that hold a row element of this type whole
 template <typename T>
 constexpr int kPartsOf = std::is_same_v<T, bf16_t> ? 1 : std::is_same_v<T, half_t> ? 2 : 3;
+// In place of parts: fp32 numbers as they are, and v_mfma_f32_16x16x4_f32, eight for 32 summation indexes of the same fragments
+constexpr int kPlain = 0;
 
 template <int P>
 struct Frag {
     v8b p[P];
 };
+template <>
+struct Frag<kPlain> {
+    float x[8];
+};
 
-// x[i] as the sum of P parts: each takes what the ones before it left.  The rounding of a part to nearest is exact to 2^-9 of what was left.
+// Two numbers' next parts, rounded to nearest even, in one register; what they leave goes on in a and b.
+__device__ __forceinline__ uint32_t next_parts(float &a, float &b, bool last) {
+    typedef float v2f __attribute__((ext_vector_type(2)));
+    typedef __bf16 v2b __attribute__((ext_vector_type(2)));
+    const uint32_t u = __builtin_bit_cast(uint32_t, __builtin_convertvector((v2f{a, b}), v2b));
+    if (!last) a -= __uint_as_float(u << 16), b -= __uint_as_float(u & 0xffff0000u);
+    return u;
+}
+
+// x[i] as the sum of P parts: each takes what the ones before it left, which is exact.
 template <int P, int W, typename V>
 __device__ __forceinline__ void split(const float (&x)[W], V (&out)[P]) {
-    float left[W];
+    struct Words { uint32_t w[W / 2]; };
+    Words words[P];
 #pragma unroll
-    for (int i = 0; i < W; i++) left[i] = x[i];
+    for (int i = 0; i < W; i += 2) {
+        float a = x[i], b = x[i + 1];
 #pragma unroll
-    for (int p = 0; p < P; p++)
+        for (int p = 0; p < P; p++) words[p].w[i / 2] = next_parts(a, b, p + 1 == P);
+    }
 #pragma unroll
-        for (int i = 0; i < W; i++) {
-            const __bf16 part = (__bf16)left[i];
-            out[p][i] = part;
-            if (p + 1 < P) left[i] -= (float)part;
-        }
+    for (int p = 0; p < P; p++) out[p] = __builtin_bit_cast(V, words[p]);
 }
 
 template <int P>
 __device__ __forceinline__ Frag<P> split8(const float (&x)[8]) {
     Frag<P> f;
-    split<P, 8>(x, f.p);
+    if constexpr (P == kPlain) {
+#pragma unroll
+        for (int i = 0; i < 8; i++) f.x[i] = x[i];
+    } else {
+        split<P, 8>(x, f.p);
+    }
     return f;
 }
 
@@ -62,15 +81,24 @@ template <int P>
 __device__ __forceinline__ void join8(const Frag<P> &f, float (&x)[8]) {
 #pragma unroll
     for (int i = 0; i < 8; i++) {
-        x[i] = (float)f.p[P - 1][i];
+        if constexpr (P == kPlain) {
+            x[i] = f.x[i];
+        } else {
+            x[i] = (float)f.p[P - 1][i];
 #pragma unroll
-        for (int p = P - 2; p >= 0; p--) x[i] += (float)f.p[p][i];
+            for (int p = P - 2; p >= 0; p--) x[i] += (float)f.p[p][i];
+        }
     }
 }
 
 // acc + A B over 32 summation indexes, pairs of parts of orders below ORDERS
 template <int ORDERS, int PA, int PB>
 __device__ __forceinline__ v4f product(const Frag<PA> &a, const Frag<PB> &b, v4f acc) {
+    if constexpr (PA == kPlain) {
+#pragma unroll
+        for (int i = 0; i < 8; i++) acc = __builtin_amdgcn_mfma_f32_16x16x4f32(a.x[i], b.x[i], acc, 0, 0, 0);
+        return acc;
+    } else
 #pragma unroll
     for (int i = 0; i < PA; i++)
 #pragma unroll
@@ -89,7 +117,17 @@ struct alignas(16) Tile {
     __bf16 x[P * kPart];
 
     __device__ __forceinline__ void put(int p, int r, int col, const v8b &v) { *reinterpret_cast<v8b *>(&x[p * kPart + r * kStride + col]) = v; }
-    __device__ __forceinline__ void put4(int p, int r, int col, const v4b &v) { *reinterpret_cast<v4b *>(&x[p * kPart + r * kStride + col]) = v; }
+    __device__ __forceinline__ void put(int r, int col, const float (&f)[8]) {
+        const Frag<P> s = split8<P>(f);
+#pragma unroll
+        for (int p = 0; p < P; p++) put(p, r, col, s.p[p]);
+    }
+    __device__ __forceinline__ void put4(int r, int col, const float (&f)[4]) {
+        v4b s[P];
+        split<P, 4>(f, s);
+#pragma unroll
+        for (int p = 0; p < P; p++) *reinterpret_cast<v4b *>(&x[p * kPart + r * kStride + col]) = s[p];
+    }
 
     // rows r0 .. r0 + 15 against columns k0 .. k0 + 31 as they lie
     __device__ __forceinline__ Frag<P> rows(int r0, int k0, int g, int c) const {
@@ -126,47 +164,98 @@ struct alignas(16) Tile {
     }
 };
 
-// Eight elements of a row at any alignment: the hardware loads and stores 16 bytes at element addresses.
-template <typename T>
-struct alignas(sizeof(T)) Eight {
-    T x[8];
+template <int R, int W>
+struct alignas(16) Tile<R, W, kPlain> {
+    static constexpr int kStride = W + 4;
+    float x[R * kStride];
+
+    __device__ __forceinline__ void put(int r, int col, const float (&f)[8]) {
+        *reinterpret_cast<v4f *>(&x[r * kStride + col]) = v4f{f[0], f[1], f[2], f[3]};
+        *reinterpret_cast<v4f *>(&x[r * kStride + col + 4]) = v4f{f[4], f[5], f[6], f[7]};
+    }
+    __device__ __forceinline__ void put4(int r, int col, const float (&f)[4]) { *reinterpret_cast<v4f *>(&x[r * kStride + col]) = v4f{f[0], f[1], f[2], f[3]}; }
+    __device__ __forceinline__ Frag<kPlain> rows(int r0, int k0, int g, int c) const {
+        const v4f a = four(r0 + c, k0 + 8 * g), b = four(r0 + c, k0 + 8 * g + 4);
+        return {{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]}};
+    }
+    template <int TILES>
+    __device__ __forceinline__ Frag<kPlain> columns(int c0, int j, int k0, int g, int c) const {
+        Frag<kPlain> f;
+#pragma unroll
+        for (int i = 0; i < 8; i++) f.x[i] = x[(k0 + 8 * g + i) * kStride + c0 + place(TILES, c, j)];
+        return f;
+    }
+    __device__ __forceinline__ v4f four(int r, int col) const { return *reinterpret_cast<const v4f *>(&x[r * kStride + col]); }
 };
 
-// A block of R rows of up to W elements on its way from memory to a Tile: load() starts the loads, put() converts and writes what they brought.
-// Rows from `rows` on and columns from `cols` on are zero and not read.
+// Element i of memory that starts at an address all lanes share: a 32-bit offset of bytes, which costs no 64-bit sum
+template <typename T>
+__device__ __forceinline__ T *from(T *base, uint32_t i) {
+    using Byte = std::conditional_t<std::is_const_v<T>, const char, char>;
+    return reinterpret_cast<T *>(reinterpret_cast<Byte *>(base) + (uint32_t)(i * (uint32_t)sizeof(T)));
+}
+
+// A block of R rows of up to W elements on its way from memory to a Tile: load() starts the loads, put() converts and writes what they brought.  Rows from
+// `rows` on and columns from `cols` on are not read and become zero; at least one row is there.  Every lane loads 16 bytes at an element's address (the
+// hardware takes any), those beyond the block's rows the last row, those beyond its columns the last eight: a branch around a load would wait for
+// it at its end, and there would be no loads ahead.  put() zeroes and shifts what was read from elsewhere.
 template <typename T, int R, int W, int THREADS>
 struct Stage {
-    static constexpr int kRow = W / 8, kVecs = R * kRow, kPer = (kVecs + THREADS - 1) / THREADS;
-    T x[kPer][8];
+    typedef uint32_t v4u __attribute__((ext_vector_type(4)));
+    static constexpr int kRow = W / 8, kVecs = R * kRow, kPer = (kVecs + THREADS - 1) / THREADS, kRegs = sizeof(T) / 2;
+    struct Eight {
+        v4u x[kRegs];
+    };
+    struct __attribute__((packed, aligned(sizeof(T)))) Anywhere {
+        Eight e;
+    };
+    Eight x[kPer];
 
-    __device__ __forceinline__ void load(const T *base, int64_t stride, int rows, int cols, int tid) {
+    // base: the block's first row, the same for all lanes; R rows lie within 32 bits of bytes
+    __device__ __forceinline__ void load(const T *base, int stride, int rows, int cols, int tid) {
 #pragma unroll
         for (int i = 0; i < kPer; i++) {
-            const int v = tid + i * THREADS, r = v / kRow, col = v % kRow * 8;
-            const T *at = base + r * stride + col;
-            if (r < rows && col + 8 <= cols) {
-                struct __attribute__((packed, aligned(sizeof(T)))) Any { T x[8]; };
-                const Any a = *reinterpret_cast<const Any *>(at);
-#pragma unroll
-                for (int e = 0; e < 8; e++) x[i][e] = a.x[e];
+            const int v = tid + i * THREADS, r = min(v / kRow, rows - 1), col = v % kRow * 8;
+            if (cols >= 8) {
+                x[i] = reinterpret_cast<const Anywhere *>(from(base, (uint32_t)r * (uint32_t)stride + (uint32_t)min(col, cols - 8)))->e;
             } else {
+                struct { T e[8]; } few;
 #pragma unroll
-                for (int e = 0; e < 8; e++) x[i][e] = r < rows && col + e < cols ? at[e] : (T)0.f;
+                for (int e = 0; e < 8; e++) few.e[e] = *from(base, (uint32_t)r * (uint32_t)stride + (uint32_t)min(e, cols - 1));
+                x[i] = __builtin_bit_cast(Eight, few);
             }
         }
     }
     template <int P>
-    __device__ __forceinline__ void put(Tile<R, W, P> &t, int tid) const {
+    __device__ __forceinline__ void put(Tile<R, W, P> &t, int rows, int cols, int tid) const {
 #pragma unroll
         for (int i = 0; i < kPer; i++) {
             const int v = tid + i * THREADS, r = v / kRow, col = v % kRow * 8;
             if (kVecs % THREADS && v >= kVecs) continue;
+            const bool some = r < rows && col < cols;
+            if constexpr (P == 1)
+                if (cols % 8 == 0) {
+                    t.put(0, r, col, __builtin_bit_cast(v8b, some ? x[i].x[0] : v4u{0, 0, 0, 0}));
+                    continue;
+                }
+            struct Few { T e[8]; };
+            const Few few = __builtin_bit_cast(Few, x[i]);
             float f[8];
 #pragma unroll
-            for (int e = 0; e < 8; e++) f[e] = (float)x[i][e];
-            const Frag<P> s = split8<P>(f);
+            for (int e = 0; e < 8; e++) f[e] = some ? (float)few.e[e] : 0.f;
+            if (cols % 8) {
+                if (cols >= 8) {      // the last run of a row holds its last eight elements
+                    const int late = max(0, col - (cols - 8));
 #pragma unroll
-            for (int p = 0; p < P; p++) t.put(p, r, col, s.p[p]);
+                    for (int b = 1; b < 8; b *= 2)
+#pragma unroll
+                        for (int e = 0; e < 8; e++) f[e] = late & b ? (e + b < 8 ? f[e + b] : 0.f) : f[e];
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 8; e++) f[e] = e < cols ? f[e] : 0.f;
+                }
+            }
+            t.put(r, col, f);
         }
     }
 };

@@ -19,35 +19,43 @@ struct RotaryWalk {
 };
 
 template <typename T>
-struct __attribute__((packed, aligned(sizeof(T)))) Vec {
-    T x[16 / sizeof(T)];
+struct Run {
+    static constexpr int V = 16 / sizeof(T);
+    typedef uint32_t Words __attribute__((ext_vector_type(4)));
+    struct __attribute__((packed, aligned(sizeof(T)))) Anywhere { Words w; };
+    struct Elements { T x[V]; };
+    Words w;
+    // elements c .. of a row.  WHOLE: all V are there, and no branch makes a load wait for the one before it; else those from `end` on are zero.
+    template <bool WHOLE>
+    __device__ __forceinline__ void load(const T *at, int c, int end) {
+        if (WHOLE || c + V <= end) {
+            w = reinterpret_cast<const Anywhere *>(at + c)->w;
+        } else {
+            Elements few;
+#pragma unroll
+            for (int i = 0; i < V; i++) few.x[i] = c + i < end ? at[c + i] : (T)0.f;
+            w = __builtin_bit_cast(Words, few);
+        }
+    }
+    __device__ __forceinline__ void get(float (&x)[V]) const {
+        const Elements few = __builtin_bit_cast(Elements, w);
+#pragma unroll
+        for (int i = 0; i < V; i++) x[i] = (float)few.x[i];
+    }
+    template <bool WHOLE>
+    static __device__ __forceinline__ void store(const float (&x)[V], T *at, int c, int end) {
+        Elements few;
+#pragma unroll
+        for (int i = 0; i < V; i++) few.x[i] = (T)x[i];
+        if (WHOLE || c + V <= end) {
+            reinterpret_cast<Anywhere *>(at + c)->w = __builtin_bit_cast(Words, few);
+        } else {
+#pragma unroll
+            for (int i = 0; i < V; i++)
+                if (c + i < end) at[c + i] = few.x[i];
+        }
+    }
 };
-
-// elements [c, c + V) of a row, those below `end`
-template <typename T, int V>
-__device__ __forceinline__ void load_some(float (&x)[V], const T *at, int c, int end) {
-    if (c + V <= end) {
-        const Vec<T> v = *reinterpret_cast<const Vec<T> *>(at + c);
-#pragma unroll
-        for (int i = 0; i < V; i++) x[i] = (float)v.x[i];
-    } else {
-#pragma unroll
-        for (int i = 0; i < V; i++) x[i] = c + i < end ? (float)at[c + i] : 0.f;
-    }
-}
-template <typename T, int V>
-__device__ __forceinline__ void store_some(const float (&x)[V], T *at, int c, int end) {
-    if (c + V <= end) {
-        Vec<T> v;
-#pragma unroll
-        for (int i = 0; i < V; i++) v.x[i] = (T)x[i];
-        *reinterpret_cast<Vec<T> *>(at + c) = v;
-    } else {
-#pragma unroll
-        for (int i = 0; i < V; i++)
-            if (c + i < end) at[c + i] = (T)x[i];
-    }
-}
 
 __device__ __forceinline__ void sine_cosine(double angle, float &s, float &c) {
     const double quarters = angle * 0.63661977236758134308, whole = rint(quarters);
@@ -69,9 +77,10 @@ __device__ __forceinline__ void sine_cosine(double angle, float &s, float &c) {
 }
 
 // A thread has one unit of 2 V channels (V pairs, or as many of the channels that stay) of one step, for the heads of its group: those of q, then those of k.
-template <typename T>
+// WHOLE: all units have all of their channels.
+template <typename T, bool WHOLE>
 __global__ __launch_bounds__(256) void k_rotary(const RotaryWalk w) {
-    constexpr int V = 16 / sizeof(T);
+    constexpr int V = 16 / sizeof(T), kAhead = 4;
     const fwp_rotary_args &a = w.a;
     int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
     const int u = i % w.units;
@@ -87,46 +96,52 @@ __global__ __launch_bounds__(256) void k_rotary(const RotaryWalk w) {
     else if (a.interleaved) c0 = u * 2 * V, c1 = c0 + V, e0 = e1 = 2 * a.pairs;
     else c0 = u * V, c1 = a.pairs + c0, e0 = a.pairs, e1 = 2 * a.pairs;
     float sn[V], cs[V];
+#pragma unroll
+    for (int p = 0; p < V; p++) sn[p] = 0.f, cs[p] = 1.f;
     if (turns && counts) {
         int64_t at = t;
         if (a.positions) at = a.each_step ? a.positions[(int64_t)n * a.L + t] : a.positions[n] + t;
         const double position = (double)at;
 #pragma unroll
         for (int p = 0; p < V; p++) {
-            const int pair = u * V + p;
-            sine_cosine(pair < a.pairs ? position * a.frequencies[pair] : 0.0, sn[p], cs[p]);
+            sine_cosine(position * a.frequencies[min(u * V + p, a.pairs - 1)], sn[p], cs[p]);
             sn[p] *= a.inverse ? -a.scale : a.scale, cs[p] *= a.scale;
         }
     }
     const int last = min((group + 1) * w.per, a.HQ + a.HK);
-#pragma unroll 4
-    for (int h = group * w.per; h < last; h++) {
-        const bool key = h >= a.HQ;
-        const T *from = row<T>(key ? a.k : a.q, n, key ? h - a.HQ : h, t);
-        T *to = row<T>(key ? w.ok : w.oq, n, key ? h - a.HQ : h, t);
-        float x[V], y[V];
+    const auto source = [&](int h) { return h >= a.HQ ? row<T>(a.k, n, h - a.HQ, t) : row<T>(a.q, n, h, t); };
+    for (int h = group * w.per; h < last; h += kAhead) {
+        Run<T> x[kAhead], y[kAhead];
 #pragma unroll
-        for (int p = 0; p < V; p++) x[p] = y[p] = 0.f;
-        if (counts) load_some<T, V>(x, from, c0, e0), load_some<T, V>(y, from, c1, e1);
-        if (turns && counts) {
-            if (a.interleaved) {
-                float r[2 * V];
+        for (int j = 0; j < kAhead; j++) {
+            const T *from = source(min(h + j, last - 1));
+            x[j].template load<WHOLE>(from, c0, e0), y[j].template load<WHOLE>(from, c1, e1);
+        }
 #pragma unroll
-                for (int p = 0; p < V; p++) {
-                    const float p0 = p < V / 2 ? x[2 * p % V] : y[2 * p % V], p1 = p < V / 2 ? x[2 * p % V + 1] : y[2 * p % V + 1];
-                    r[2 * p] = fmaf(p0, cs[p], -(p1 * sn[p])), r[2 * p + 1] = fmaf(p0, sn[p], p1 * cs[p]);
+        for (int j = 0; j < kAhead; j++) {
+            if (h + j >= last) break;
+            T *to = h + j >= a.HQ ? row<T>(w.ok, n, h + j - a.HQ, t) : row<T>(w.oq, n, h + j, t);
+            float p0[V], p1[V], r0[V], r1[V];
+            x[j].get(p0), y[j].get(p1);
+            if (!turns) {
+#pragma unroll
+                for (int p = 0; p < V; p++) r0[p] = p0[p], r1[p] = p1[p];
+            } else if (a.interleaved) {
+#pragma unroll
+                for (int p = 0; p < V; p += 2) {
+                    r0[p] = fmaf(p0[p], cs[p / 2], -(p0[p + 1] * sn[p / 2])), r0[p + 1] = fmaf(p0[p], sn[p / 2], p0[p + 1] * cs[p / 2]);
+                    r1[p] = fmaf(p1[p], cs[(V + p) / 2], -(p1[p + 1] * sn[(V + p) / 2])), r1[p + 1] = fmaf(p1[p], sn[(V + p) / 2], p1[p + 1] * cs[(V + p) / 2]);
                 }
-#pragma unroll
-                for (int p = 0; p < V; p++) x[p] = r[p], y[p] = r[V + p];
             } else {
 #pragma unroll
-                for (int p = 0; p < V; p++) {
-                    const float p0 = x[p], p1 = y[p];
-                    x[p] = fmaf(p0, cs[p], -(p1 * sn[p])), y[p] = fmaf(p0, sn[p], p1 * cs[p]);
-                }
+                for (int p = 0; p < V; p++) r0[p] = fmaf(p0[p], cs[p], -(p1[p] * sn[p])), r1[p] = fmaf(p0[p], sn[p], p1[p] * cs[p]);
             }
+            if (!counts) {
+#pragma unroll
+                for (int p = 0; p < V; p++) r0[p] = r1[p] = 0.f;
+            }
+            Run<T>::template store<WHOLE>(r0, to, c0, e0), Run<T>::template store<WHOLE>(r1, to, c1, e1);
         }
-        store_some<T, V>(x, to, c0, e0), store_some<T, V>(y, to, c1, e1);
     }
 }
 
@@ -145,7 +160,11 @@ int rotary(const fwp_rotary_args &a, fwp_out_rows oq, fwp_out_rows ok, hipStream
     w.groups = (heads + w.per - 1) / w.per;
     const int64_t blocks = (rows * w.groups + 255) / 256;
     if (!fits_launch(blocks, 256)) return FWP_E_SHAPE;
-    by_type(a.type, [&](auto t) { k_rotary<decltype(t)><<<(unsigned)blocks, 256, 0, s>>>(w); });
+    const bool whole = a.pairs % V == 0 && (a.D - 2 * a.pairs) % (2 * V) == 0;
+    by_type(a.type, [&](auto t) {
+        if (whole) k_rotary<decltype(t), true><<<(unsigned)blocks, 256, 0, s>>>(w);
+        else k_rotary<decltype(t), false><<<(unsigned)blocks, 256, 0, s>>>(w);
+    });
     return (int)hipGetLastError();
 }
 
