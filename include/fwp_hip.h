@@ -515,9 +515,10 @@ int fwp_residual_norm_bwd(const fwp_norm_args *a, const float *stats, const void
  *   W[e][m] = exp(g) W[e][m] + k[e] v[m],  o[m] = scale sum_e q[e] W[e][m]
  * q [N,HQ,L,E], k [N,HK,L,E], v [N,HV,L,M], o [N,H,L,M]; HQ, HK and HV divide H, and head h takes the rows of head h / (H / HQ) and so on.  E <= 128.
  * g: fp32 at n dN + h dH + t dL, not positive; -inf empties the state.  per_head: g is of a head (dN and dL are 0), and so is its gradient.  lengths as
- * above.  W [N,H,E,M] fp32 in/out (NULL: from zeros, not kept).  saved: NULL, or fwp_decayed_sum_saved_floats, 16-byte aligned, for a backward pass;
+ * above.  Steps of a view lie at most FWP_DSUM_MAX_STEP elements apart.  W [N,H,E,M] fp32 in/out (NULL: from zeros, not kept).  saved: NULL, or fwp_decayed_sum_saved_floats, 16-byte aligned, for a backward pass;
  * workspace: fwp_decayed_sum_workspace(.., 0) floats, 16-byte aligned (NULL if that is 0).
  */
+#define FWP_DSUM_MAX_STEP (1 << 24)
 typedef struct fwp_dsum_args {
     fwp_rows q, k, v;
     const float *decay;
@@ -551,19 +552,21 @@ typedef struct fwp_rotary_args {
 int fwp_rotary(const fwp_rotary_args *a, fwp_out_rows oq, fwp_out_rows ok, void *stream);
 
 /*
- * Norm of groups of channels: every row's `groups` groups of `size` channels (size <= 1024, groups * size <= 65536), contiguous rows,
+ * Norm of groups of channels: every row's `groups` groups of `size` channels (size <= 1024, groups * size <= 65536); rows of x and of gate x_step and gate_step
+ * elements apart, those of everything else side by side,
  *   u = norm(group) weight + bias (either NULL: without it),  y = act(gate) u, or act(u) where gate is NULL
  * norm as above; act: FWP_ACT_*.  x, gate, y of `type`; weight, bias [groups * size].
  */
 typedef struct fwp_group_norm_args {
     const void *x, *gate;
+    int64_t x_step, gate_step;
     const float *weight, *bias;
     float eps;
     int type, rms, act, rows, groups, size;
 } fwp_group_norm_args;
 int fwp_group_norm_fwd(const fwp_group_norm_args *a, void *y, void *stream);
 
-/* Its adjoint: gx and ggate like x (ggate NULL without a gate), gweight and gbias [groups * size] or NULL.  workspace: fwp_group_norm_workspace floats. */
+/* Its adjoint: gx and ggate [rows, groups * size] (ggate NULL without a gate), gweight and gbias [groups * size] or NULL.  workspace: fwp_group_norm_workspace floats. */
 long long fwp_group_norm_workspace(int type, int rows, int groups, int size);
 int fwp_group_norm_bwd(const fwp_group_norm_args *a, const void *grad_y, void *gx, void *ggate, float *gweight, float *gbias, float *workspace,
                        void *stream);

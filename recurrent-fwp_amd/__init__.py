@@ -4,7 +4,8 @@ IDSIA/recurrent-fwp: ``fast_weight_delta``, ``rec_update_fwm_tanh``,
 in/out state tensors as in the reference's ``autograd.Function``s).  The
 arithmetic runs in hand-written HIP kernels for gfx950 reached through the C ABI
 of ``libfwp_hip.so``; there is no other implementation behind these names.  Beside them: the selective state space block
-(``causal_conv``, ``selective_scan``, ``residual_norm`` and their layers), which the reference does not have.
+(``causal_conv``, ``selective_scan``, ``residual_norm`` and their layers) and that of a decayed sum rule (``decayed_sum``, ``rotary``, ``group_norm`` and
+theirs), which the reference does not have.
 """
 from . import _lib
 from .fast_weight import DeltaFastWeight, fast_weight_delta
@@ -14,8 +15,8 @@ from .fast_weight_rnn_v2 import FastRNNv2, fast_rnn_v2
 from .rec_update_fwm_tanh import FastWeightRecUpdateTanh, rec_update_fwm_tanh
 from .selective_scan import causal_conv, residual_norm, selective_scan
 from .decayed_sum import decayed_sum, group_norm, rotary, rotary_frequencies
-from .layers import (DeltaNetDecoderLayer, DeltaNetLayer, DeltaNetPrep, PositionalEmbedding, PositionwiseFF, SelectiveScanDecoderLayer,
-                     SelectiveScanLayer)
+from .layers import (DecayedSumDecoderLayer, DecayedSumLayer, DeltaNetDecoderLayer, DeltaNetLayer, DeltaNetPrep, PositionalEmbedding,
+                     PositionwiseFF, SelectiveScanDecoderLayer, SelectiveScanLayer)
 from .lm import DeltaNetLM
 
 __all__ = ["DeltaFastWeight", "fast_weight_delta", "FastWeightSum", "fast_weight_sum", "FastRNNv2", "fast_rnn_v2",
@@ -23,4 +24,4 @@ __all__ = ["DeltaFastWeight", "fast_weight_delta", "FastWeightSum", "fast_weight
            "FastWeightRecUpdateTanh", "rec_update_fwm_tanh", "causal_conv", "selective_scan", "residual_norm", "decayed_sum", "rotary",
            "rotary_frequencies", "group_norm", "DeltaNetLayer", "DeltaNetPrep",
            "DeltaNetDecoderLayer", "PositionwiseFF", "PositionalEmbedding", "SelectiveScanLayer", "SelectiveScanDecoderLayer",
-           "DeltaNetLM"]
+           "DecayedSumLayer", "DecayedSumDecoderLayer", "DeltaNetLM"]

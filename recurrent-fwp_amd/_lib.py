@@ -71,8 +71,8 @@ class RotaryArgs(ctypes.Structure):
 
 class GroupNormArgs(ctypes.Structure):
     """struct fwp_group_norm_args."""
-    _fields_ = [(n, ctypes.c_void_p) for n in ("x", "gate", "weight", "bias")] + [("eps", ctypes.c_float)] + \
-               [(n, ctypes.c_int) for n in ("type", "rms", "act", "rows", "groups", "size")]
+    _fields_ = [("x", ctypes.c_void_p), ("gate", ctypes.c_void_p), ("x_step", ctypes.c_int64), ("gate_step", ctypes.c_int64), ("weight", ctypes.c_void_p),
+                ("bias", ctypes.c_void_p), ("eps", ctypes.c_float)] + [(n, ctypes.c_int) for n in ("type", "rms", "act", "rows", "groups", "size")]
 
 
 class FwpError(RuntimeError):

@@ -10,6 +10,11 @@ template <typename V>
 bool rows_ok(const V &v, int type) {
     return v.ptr && reinterpret_cast<uintptr_t>(v.ptr) % (type == FWP_F32 ? 4 : 2) == 0;
 }
+// sixty-four steps and a row lie within 32 bits of bytes
+template <typename V>
+bool step_ok(const V &v) {
+    return v.sL >= 0 && v.sL <= FWP_DSUM_MAX_STEP;
+}
 bool aligned16(const void *p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 bool divides(int part, int whole) { return part >= 1 && whole % part == 0; }
 
@@ -25,8 +30,10 @@ int dsum_check(const fwp_dsum_args *a) {
     if (!dims_ok(a->type, a->N, a->H, a->L, a->E, a->M) || !divides(a->HQ, a->H) || !divides(a->HK, a->H) || !divides(a->HV, a->H) ||
         (a->per_head && (a->dN || a->dL)))
         return FWP_E_SHAPE;
-    for (const fwp_rows *v : {&a->q, &a->k, &a->v})
+    for (const fwp_rows *v : {&a->q, &a->k, &a->v}) {
         if (!rows_ok(*v, a->type)) return FWP_E_NULL;
+        if (!step_ok(*v)) return FWP_E_SHAPE;
+    }
     return 0;
 }
 
@@ -54,6 +61,7 @@ long long fwp_decayed_sum_workspace(const fwp_dsum_args *a, int backward) {
 int fwp_decayed_sum_fwd(const fwp_dsum_args *a, float *W, fwp_out_rows out, float *saved, float *workspace, void *stream) {
     if (int rc = dsum_check(a)) return rc;
     if (!rows_ok(out, a->type) || !aligned16(saved) || !aligned16(workspace)) return FWP_E_NULL;
+    if (!step_ok(out)) return FWP_E_SHAPE;
     return dsum_fwd(*a, W, out, saved, workspace, (hipStream_t)stream);
 }
 
@@ -62,8 +70,11 @@ int fwp_decayed_sum_bwd(const fwp_dsum_args *a, const float *saved, fwp_rows gra
     if (int rc = dsum_check(a)) return rc;
     if (!saved || !aligned16(saved) || !gdecay || !aligned16(workspace) || (!workspace && dsum_workspace(*a, true)) || !rows_ok(grad_out, a->type))
         return FWP_E_NULL;
-    for (const fwp_out_rows *v : {&gq, &gk, &gv})
+    if (!step_ok(grad_out)) return FWP_E_SHAPE;
+    for (const fwp_out_rows *v : {&gq, &gk, &gv}) {
         if (!rows_ok(*v, a->type)) return FWP_E_NULL;
+        if (!step_ok(*v)) return FWP_E_SHAPE;
+    }
     return dsum_bwd(*a, saved, grad_out, gq, gk, gv, gdecay, workspace, (hipStream_t)stream);
 }
 

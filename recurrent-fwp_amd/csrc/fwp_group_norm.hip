@@ -19,6 +19,7 @@ namespace {
 
 struct NormWalk {
     const void *x, *gate, *gy;
+    int64_t x_step, gate_step;
     void *y, *gx, *ggate;
     const float *weight, *bias;
     float *sums;      // [blocks][2][groups * size]
@@ -198,16 +199,16 @@ __global__ __launch_bounds__(256) void k_group_norm_fwd(const NormWalk w) {
 #pragma unroll
     for (int i = 0; i < K; i++) gate.w[i] = 0;
     if (l.row0 < w.rows) {
-        x.load(xs + l.row0 * width, l.first, step, w.size);
-        if (gs) gate.load(gs + l.row0 * width, l.first, step, w.size);
+        x.load(xs + l.row0 * w.x_step, l.first, step, w.size);
+        if (gs) gate.load(gs + l.row0 * w.gate_step, l.first, step, w.size);
     }
     for (int r = l.row0; r < w.rows; r += l.rows_step) {
         float h[K][V], g[K][V];
         x.get(h, l.first, step, w.size);
         gate.get(g, l.first, step, w.size);
         if (r + l.rows_step < w.rows) {
-            x.load(xs + (r + l.rows_step) * width, l.first, step, w.size);
-            if (gs) gate.load(gs + (r + l.rows_step) * width, l.first, step, w.size);
+            x.load(xs + (r + l.rows_step) * w.x_step, l.first, step, w.size);
+            if (gs) gate.load(gs + (r + l.rows_step) * w.gate_step, l.first, step, w.size);
         }
         normalise<W>(h, l.first, step, w.size, w.eps, w.rms);
 #pragma unroll
@@ -239,9 +240,9 @@ __global__ __launch_bounds__(256) void k_group_norm_bwd(const NormWalk w) {
         for (int e = 0; e < V; e++) gw[i][e] = gb[i][e] = 0.f;
     Run<T, K, ODD> x, gate, gy;
     const auto fetch = [&](int r) {
-        x.load(xs + r * width, l.first, step, w.size);
+        x.load(xs + r * w.x_step, l.first, step, w.size);
         gy.load(ds + r * width, l.first, step, w.size);
-        if (gs) gate.load(gs + r * width, l.first, step, w.size);
+        if (gs) gate.load(gs + r * w.gate_step, l.first, step, w.size);
     };
 #pragma unroll
     for (int i = 0; i < K; i++) gate.w[i] = 0;
@@ -360,7 +361,7 @@ void by_size(const NormWalk &w, hipStream_t s) {
 
 NormWalk walk_of(const fwp_group_norm_args &a) {
     NormWalk w{};
-    w.x = a.x, w.gate = a.gate, w.weight = a.weight, w.bias = a.bias;
+    w.x = a.x, w.gate = a.gate, w.x_step = a.x_step, w.gate_step = a.gate_step, w.weight = a.weight, w.bias = a.bias;
     w.eps = a.eps, w.rms = a.rms, w.act = a.act, w.rows = a.rows, w.groups = a.groups, w.size = a.size;
     return w;
 }

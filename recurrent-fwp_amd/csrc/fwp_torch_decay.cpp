@@ -6,6 +6,8 @@ namespace {
 
 // ------------------------------------------------------------------ decayed sum rule
 
+constexpr int64_t kMost = FWP_DSUM_MAX_STEP;
+
 struct DecayedSumFn : torch::autograd::Function<DecayedSumFn> {
     static fwp_dsum_args args(const at::Tensor &q, const at::Tensor &k, const at::Tensor &v, const at::Tensor &decay, const at::Tensor &lengths,
                               double scale) {
@@ -45,8 +47,8 @@ struct DecayedSumFn : torch::autograd::Function<DecayedSumFn> {
             fail("W must be a contiguous fp32 [N,H,E,M] tensor");
         require_device(q_in);
         same_device(q_in, {k_in, v_in, decay_in, W, lengths});
-        const at::Tensor q = rows_of(q_in), k = rows_of(k_in), v = rows_of(v_in), decay = decay_in.is_neg() ? plain(decay_in) : decay_in,
-                         out = empty_rows(v, H);
+        const at::Tensor q = rows_of(q_in, kMost), k = rows_of(k_in, kMost), v = rows_of(v_in, kMost), decay = decay_in.is_neg() ? plain(decay_in) : decay_in,
+                         out = empty_rows(v, H, kMost);
         const fwp_dsum_args a = args(q, k, v, decay, lengths, scale);
         if (ctx) may_be_kept({q, k, v, decay, lengths});
         LaunchGuard guard(q);
@@ -67,11 +69,11 @@ struct DecayedSumFn : torch::autograd::Function<DecayedSumFn> {
         if (!grads[0].defined()) return res;
         once_only();
         const auto s = ctx->get_saved_variables();
-        const at::Tensor &q = s[0], &k = s[1], &v = s[2], &decay = s[3], &lengths = s[4], &saved = s[5], g = rows_of(grads[0]);
+        const at::Tensor &q = s[0], &k = s[1], &v = s[2], &decay = s[3], &lengths = s[4], &saved = s[5], g = rows_of(grads[0], kMost);
         const fwp_dsum_args a = args(q, k, v, decay, lengths, ctx->saved_data["scale"].toDouble());
         LaunchGuard guard(q);
         const at::Tensor work = scratch(fwp_decayed_sum_workspace(&a, 1), q);
-        res[0] = empty_rows(q), res[1] = empty_rows(k), res[2] = empty_rows(v), res[3] = at::empty(decay.sizes(), decay.options());
+        res[0] = empty_rows(q, 0, kMost), res[1] = empty_rows(k, 0, kMost), res[2] = empty_rows(v, 0, kMost), res[3] = at::empty(decay.sizes(), decay.options());
         check(fwp_decayed_sum_bwd(&a, floats(saved), view(g), out_view(res[0]), out_view(res[1]), out_view(res[2]), floats_out(res[3]),
                                   work.data_ptr<float>(), stream_of(q)),
               "fwp_decayed_sum_bwd");
@@ -172,11 +174,29 @@ std::pair<at::Tensor, Optional> rotary(const at::Tensor &q, const Optional &k, c
 // ------------------------------------------------------------------ norm of groups of channels
 
 struct GroupNormFn : torch::autograd::Function<GroupNormFn> {
+    // [..., channels] whose rows lie one step apart in memory, from the first to the last; a copy where they do not
+    static at::Tensor even_rows(const at::Tensor &t) {
+        if (!t.defined()) return t;
+        bool even = !t.is_neg() && (t.size(-1) == 1 || t.stride(-1) == 1);
+        int64_t inner = -1;      // the next axis inwards that has more than one row
+        for (int64_t i = t.dim() - 2; even && i >= 0; i--) {
+            if (t.size(i) == 1) continue;
+            if (inner >= 0) even = t.stride(i) == t.size(inner) * t.stride(inner);
+            inner = i;
+        }
+        return even ? t : t.resolve_neg().clone(at::MemoryFormat::Contiguous);
+    }
+    static int64_t step_of(const at::Tensor &t) {
+        for (int64_t i = t.dim() - 2; i >= 0; i--)
+            if (t.size(i) > 1) return t.stride(i);
+        return t.size(-1);
+    }
     static fwp_group_norm_args args(const at::Tensor &x, const at::Tensor &gate, const at::Tensor &w, const at::Tensor &b, int64_t groups, double eps, bool rms,
                                     int64_t act) {
         fwp_group_norm_args a{};
         a.x = x.const_data_ptr();
-        a.gate = gate.defined() ? gate.const_data_ptr() : nullptr;
+        a.x_step = step_of(x);
+        if (gate.defined()) a.gate = gate.const_data_ptr(), a.gate_step = step_of(gate);
         a.weight = floats(w), a.bias = floats(b);
         a.eps = (float)eps;
         a.type = type_of(x, "X");
@@ -199,7 +219,7 @@ struct GroupNormFn : torch::autograd::Function<GroupNormFn> {
         const at::Tensor w = parameter(given(w_in), {C}, "weight", "[channels]"), b = parameter(given(b_in), {C}, "bias", "[channels]");
         require_device(x_in);
         same_device(x_in, {g, w, b});
-        const at::Tensor x = plain(x_in), gate = plain(g), y = at::empty(x.sizes(), x.options());
+        const at::Tensor x = even_rows(x_in), gate = even_rows(g), y = at::empty(x.sizes(), x.options());
         if (ctx) may_be_kept({x, gate, w, b});
         LaunchGuard guard(x);
         const fwp_group_norm_args a = args(x, gate, w, b, groups, eps, rms, act);

@@ -66,13 +66,13 @@ inline fwp_out_rows out_view(const at::Tensor &t) {
 }
 
 // Do these rows lie with the steps outermost, as a layer's permuted views do?  Results take the order of the rows they belong to.
-inline bool steps_lead(const at::Tensor &t) {
+inline bool steps_lead(const at::Tensor &t, int64_t heads, int64_t most) {
     const int64_t N = t.size(0), H = t.size(1), L = t.size(2);
-    return L > 1 && (N > 1 || H > 1) && N * H * t.size(3) <= kMaxStep && (N == 1 || t.stride(2) > t.stride(0)) && (H == 1 || t.stride(2) > t.stride(1));
+    return L > 1 && (N > 1 || H > 1) && N * heads * t.size(3) <= most && (N == 1 || t.stride(2) > t.stride(0)) && (H == 1 || t.stride(2) > t.stride(1));
 }
-inline at::Tensor empty_rows(const at::Tensor &like, int64_t heads = 0) {
+inline at::Tensor empty_rows(const at::Tensor &like, int64_t heads = 0, int64_t most = kMaxStep) {
     const int64_t N = like.size(0), H = heads ? heads : like.size(1), L = like.size(2), D = like.size(3);
-    return steps_lead(like) ? at::empty({L, N, H, D}, like.options()).permute({1, 2, 0, 3}) : at::empty({N, H, L, D}, like.options());
+    return steps_lead(like, H, most) ? at::empty({L, N, H, D}, like.options()).permute({1, 2, 0, 3}) : at::empty({N, H, L, D}, like.options());
 }
 
 inline const float *floats(const at::Tensor &t) { return t.defined() ? t.const_data_ptr<float>() : nullptr; }

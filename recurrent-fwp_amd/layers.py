@@ -14,6 +14,7 @@ import torch.nn.functional as F
 from torch.utils._device import DeviceContext
 
 from . import _lib
+from .decayed_sum import decayed_sum, group_norm, rotary, rotary_frequencies
 from .fast_weight import _fwp_torch, fast_weight_delta
 from .selective_scan import causal_conv, residual_norm, selective_scan
 
@@ -395,18 +396,13 @@ class SelectiveScanLayer(nn.Module):
         return (out, (W, state)) if carry_over_fast_weight else out
 
 
-class SelectiveScanDecoderLayer(nn.Module):
-    """A :class:`SelectiveScanLayer` and the feed-forward block behind it on a residual stream: norm, mixer, norm and scale on its output, and
-    the same around the feed-forward block; :func:`residual_norm` is what lies between and behind the two, but for a norm that was replaced or
-    hooked to, which is called.  Constructor and call as :class:`DeltaNetDecoderLayer`'s, whose place it takes in :class:`DeltaNetLM`; heads do not
-    count here (q and k are shared by all channels), ``dropatt`` has nothing to drop, and norms come before a block whatever ``pre_lnorm``."""
+class _ResidualDecoderLayer(nn.Module):
+    """A mixer and the feed-forward block behind it on a residual stream: norm, mixer, norm and scale on its output, and the same around the
+    feed-forward block; :func:`residual_norm` is what lies between and behind the two, but for a norm that was replaced or hooked to, which is called."""
 
-    def __init__(self, n_head, d_model, d_head, d_inner, dropout=0.0, dropatt=0.0, pre_lnorm=True, layer_id=None, num_layer=None,
-                 fast_weight_op=None, n_state=16, taps=4):
+    def __init__(self, mixer, d_model, d_inner, dropout):
         super().__init__()
-        if fast_weight_op is not None:
-            raise ValueError("a selective scan layer has its own operator")
-        self.dec_attn = SelectiveScanLayer(d_model, n_state, taps, dropout=dropout)
+        self.dec_attn = mixer
         self.norm_in, self.norm_mid = nn.LayerNorm(d_model), nn.LayerNorm(d_model)
         self.norm_attn, self.norm_ff = nn.LayerNorm(d_model), nn.LayerNorm(d_model)
         self.scale_attn, self.scale_ff = nn.Parameter(torch.ones(d_model)), nn.Parameter(torch.ones(d_model))
@@ -418,6 +414,88 @@ class SelectiveScanDecoderLayer(nn.Module):
         r, n = _around(out, dec_inp, self.norm_attn, self.scale_attn, self.norm_mid)
         r, _ = _around(self.ff(n), r, self.norm_ff, self.scale_ff)
         return (r, mems) if carry_over_fast_weight else r
+
+
+class SelectiveScanDecoderLayer(_ResidualDecoderLayer):
+    """A :class:`SelectiveScanLayer` and the feed-forward block behind it on a residual stream.  Constructor and call as
+    :class:`DeltaNetDecoderLayer`'s, whose place it takes in :class:`DeltaNetLM`; heads do not count here (q and k are shared by all channels),
+    ``dropatt`` has nothing to drop, and norms come before a block whatever ``pre_lnorm``."""
+
+    def __init__(self, n_head, d_model, d_head, d_inner, dropout=0.0, dropatt=0.0, pre_lnorm=True, layer_id=None, num_layer=None,
+                 fast_weight_op=None, n_state=16, taps=4):
+        if fast_weight_op is not None:
+            raise ValueError("a selective scan layer has its own operator")
+        super().__init__(SelectiveScanLayer(d_model, n_state, taps, dropout=dropout), d_model, d_inner, dropout)
+
+
+class DecayedSumLayer(nn.Module):
+    """The mixer whose fast weights decay, beside :class:`DeltaNetLayer`: ``h`` is ``[len, bsz, d_model]``, one projection gives queries, keys and values of ``n_head``
+    heads and a gate, :func:`rotary` turns queries and keys, :func:`decayed_sum` writes and reads the fast weights, :func:`group_norm` normalises every
+    head and gates it, and a projection back follows.  No norm and no residual of the stream: those are the block's.
+
+    A head's decay is the sigmoid of a number of its own, from memories of 32 steps upwards; with ``token_decay`` the step adds to that number.  ``mems`` is the pair
+    (``W[bsz, n_head, d_head, d_head]``, the steps so far ``[bsz]``, int64); with ``carry_over_fast_weight`` the call returns ``(output, mems)``.  ``lengths`` (int64
+    ``[bsz]``) marks a padded batch.  No counterpart in the reference.
+    """
+
+    def __init__(self, n_head, d_model, d_head, dropout=0.0, token_decay=False):
+        super().__init__()
+        if d_head % 2:
+            raise ValueError("rotary positions turn pairs of channels: d_head must be even")
+        self.n_head, self.d_model, self.d_head, self.token_decay = n_head, d_model, d_head, token_decay
+        self.in_net = Linear(d_model, 4 * n_head * d_head + (n_head if token_decay else 0))
+        self.decay_logit = nn.Parameter(torch.empty(n_head))
+        self.norm_weight = nn.Parameter(torch.ones(n_head * d_head))
+        self.norm_bias = nn.Parameter(torch.zeros(n_head * d_head))
+        self.o_net = Linear(n_head * d_head, d_model)
+        self.drop = nn.Dropout(dropout)
+        self._frequencies = rotary_frequencies(d_head)[0]      # no buffer: a model in half precision keeps them in 64 bits
+        self.reset_decay_parameters()
+
+    def reset_decay_parameters(self):
+        """Memories of 32 steps for the first head, twice as long for each one behind it, up to 4096."""
+        with torch.no_grad():
+            steps = torch.exp2(5.0 + torch.arange(self.n_head, device=self.decay_logit.device).clamp(max=7))
+            self.decay_logit.copy_(torch.log(steps - 1))
+
+    def forward(self, h, attn_mask=None, mems=None, carry_over_fast_weight=False, lengths=None):
+        if mems is not None and not carry_over_fast_weight:
+            raise ValueError("mems are only meaningful with carry_over_fast_weight=True")
+        slen, bsz, _ = h.shape
+        H, D = self.n_head, self.d_head
+        x = self.in_net(h)
+        q, k, v, gate = (x[..., i * H * D:(i + 1) * H * D] for i in range(4))
+        rows = lambda t: t.unflatten(-1, (H, D)).permute(1, 2, 0, 3)        # [bsz, H, slen, D], the steps outermost in memory
+        logit = self.decay_logit.float()
+        if self.token_decay:
+            logit = (logit + x[..., 4 * H * D:].float()).permute(1, 2, 0)
+        W = position = None
+        if carry_over_fast_weight and mems is None:
+            W = torch.zeros(bsz, H, D, D, device=h.device, dtype=torch.float32)
+            position = torch.zeros(bsz, device=h.device, dtype=torch.int64)
+        elif carry_over_fast_weight:       # the last batch of an epoch may be smaller than the carried state
+            W, position = mems[0][:bsz].clone(), mems[1][:bsz]
+        if self._frequencies.device != h.device:
+            self._frequencies = self._frequencies.to(h.device)
+        q, k = rotary(rows(q), rows(k), self._frequencies, positions=position, lengths=lengths)
+        out = decayed_sum(q, k, rows(v), F.logsigmoid(logit), W, scale=D ** -0.5, lengths=lengths)
+        out = out.permute(2, 0, 1, 3).reshape(slen, bsz, H * D)
+        out = group_norm(out, H, self.norm_weight.float(), self.norm_bias.float(), gate=gate, activation="silu")
+        out = self.drop(self.o_net(out))
+        if not carry_over_fast_weight:
+            return out
+        return out, (W, position + (slen if lengths is None else lengths.clamp(0, slen)))
+
+
+class DecayedSumDecoderLayer(_ResidualDecoderLayer):
+    """A :class:`DecayedSumLayer` and the feed-forward block behind it on a residual stream.  Constructor and call as :class:`DeltaNetDecoderLayer`'s, whose place it
+    takes in :class:`DeltaNetLM`; ``dropatt`` has nothing to drop, and norms come before a block whatever ``pre_lnorm``."""
+
+    def __init__(self, n_head, d_model, d_head, d_inner, dropout=0.0, dropatt=0.0, pre_lnorm=True, layer_id=None, num_layer=None,
+                 fast_weight_op=None, token_decay=False):
+        if fast_weight_op is not None:
+            raise ValueError("a decayed sum layer has its own operator")
+        super().__init__(DecayedSumLayer(n_head, d_model, d_head, dropout, token_decay), d_model, d_inner, dropout)
 
 
 def _fuses(norm, cols):
