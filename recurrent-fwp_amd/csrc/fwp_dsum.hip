@@ -41,18 +41,35 @@ __global__ __launch_bounds__(256) void k_dsum_join(float *ends, const float *fac
     }
 }
 
-// rows [N,G,L,D] of type T as the sum of `parts` fp32 tensors of that shape, in their order
-template <typename T>
+// rows [N,G,L,D] of type T as the sum of `parts` fp32 tensors of that shape, in their order; K elements a thread, of one row, and the loads of eight parts at once
+template <typename T, int K>
 __global__ __launch_bounds__(256) void k_sum_parts(const float *x, fwp_out_rows out, int parts, int64_t total, int G, int L, int D) {
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
-        float s = 0.f;
-        for (int p = 0; p < parts; p++) s += x[p * total + i];
+    struct __attribute__((aligned(4 * K))) Run { float x[K]; };
+    struct __attribute__((packed, aligned(sizeof(T)))) Anywhere { T x[K]; };
+    for (int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * K; i < total; i += (int64_t)gridDim.x * 256 * K) {
+        float s[K] = {};
+#pragma unroll 8
+        for (int p = 0; p < parts; p++) {
+            const Run r = *reinterpret_cast<const Run *>(x + p * total + i);
+#pragma unroll
+            for (int k = 0; k < K; k++) s[k] += r.x[k];
+        }
         const int d = i % D;
         int64_t r = i / D;
         const int64_t t = r % L;
         r /= L;
-        store(row<T>(out, r / G, r % G, t) + d, s);
+        Anywhere a;
+#pragma unroll
+        for (int k = 0; k < K; k++) a.x[k] = (T)s[k];
+        *reinterpret_cast<Anywhere *>(row<T>(out, r / G, r % G, t) + d) = a;
     }
+}
+template <typename T>
+void sum_parts(const float *x, fwp_out_rows out, int parts, int N, int G, int L, int D, hipStream_t s) {
+    const int64_t total = (int64_t)N * G * L * D;
+    const auto blocks = [](int64_t n) { return (unsigned)std::min<int64_t>((n + 255) / 256, 8192); };
+    if (D % 4 == 0) k_sum_parts<T, 4><<<blocks(total / 4), 256, 0, s>>>(x, out, parts, total, G, L, D);
+    else k_sum_parts<T, 1><<<blocks(total), 256, 0, s>>>(x, out, parts, total, G, L, D);
 }
 
 // [H] = sums over n and the parts of each head of x [N,H,parts], one workgroup a head
@@ -205,7 +222,7 @@ DsumWalk walk_of(const fwp_dsum_args &a, const Plan &p) {
 
 int launch(int which, const fwp_dsum_args &a, const Plan &p, const DsumWalk &w, int segments, hipStream_t s) {
     const int64_t blocks = p.heads * p.slices * segments;
-    if (!fits_launch(blocks, 4 * p.MS) || !fits_launch(p.heads * (p.cells / 256), 256)) return FWP_E_SHAPE;
+    if (!fits_launch(blocks, 512) || !fits_launch(p.heads * (p.cells / 256), 256)) return FWP_E_SHAPE;
     bool done = false;
     by_type(a.type, [&](auto t) { done = dsum_launch<decltype(t)>(which, &w, p.Ep, p.MS, (unsigned)blocks, s) > 0; });
     return done ? 0 : FWP_E_SHAPE;
@@ -286,19 +303,17 @@ int dsum_bwd(const fwp_dsum_args &a, const float *saved, fwp_rows gout, fwp_out_
         k_dsum_join<true><<<(unsigned)(p.heads * (p.cells / 256)), 256, 0, s>>>(w.ends, w.factors, nullptr, a.E, a.M, p.Ep, p.Mp, p.segments);
     }
     if (int rc = launch(kDsumBackward, a, p, w, p.segments, s)) return rc;
-    const auto blocks = [](int64_t n) { return (unsigned)std::min<int64_t>((n + 255) / 256, 4096); };
     by_type(a.type, [&](auto t) {
         using T = decltype(t);
-        const int64_t nq = (int64_t)a.N * a.HQ * a.L * a.E, nk = (int64_t)a.N * a.HK * a.L * a.E, nv = (int64_t)a.N * a.HV * a.L * a.M;
-        if (w.pq) k_sum_parts<T><<<blocks(nq), 256, 0, s>>>(w.pq, gq, a.H / a.HQ * p.slices, nq, a.HQ, a.L, a.E);
-        if (w.pk) k_sum_parts<T><<<blocks(nk), 256, 0, s>>>(w.pk, gk, a.H / a.HK * p.slices, nk, a.HK, a.L, a.E);
-        if (w.pv) k_sum_parts<T><<<blocks(nv), 256, 0, s>>>(w.pv, gv, a.H / a.HV, nv, a.HV, a.L, a.M);
+        if (w.pq) sum_parts<T>(w.pq, gq, a.H / a.HQ * p.slices, a.N, a.HQ, a.L, a.E, s);
+        if (w.pk) sum_parts<T>(w.pk, gk, a.H / a.HK * p.slices, a.N, a.HK, a.L, a.E, s);
+        if (w.pv) sum_parts<T>(w.pv, gv, a.H / a.HV, a.N, a.HV, a.L, a.M, s);
     });
     if (a.per_head) {
         k_sum_heads<<<a.H, 256, 0, s>>>(parts, gdecay, a.N, a.H, p.slices * p.segments);
     } else if (parts) {
-        const int64_t n = p.heads * a.L;
-        k_sum_parts<float><<<blocks(n), 256, 0, s>>>(parts, fwp_out_rows{gdecay, (int64_t)a.H * a.L, a.L, 1}, p.slices, n, a.H, a.L, 1);
+        // its rows are those of the heads, L numbers each
+        sum_parts<float>(parts, fwp_out_rows{gdecay, (int64_t)a.H * a.L, a.L, 0}, p.slices, a.N, a.H, 1, a.L, s);
     }
     return (int)hipGetLastError();
 }

@@ -54,8 +54,8 @@ struct DsumWalk {
 
 // Workgroups b, b + 8, .. run on one XCD: neighbours in the order of the work get numbers that lie 8 apart.  Slices and heads come first in that order: they share
 // rows, or read rows that lie side by side where steps are outermost, at about the same time.
-__device__ __forceinline__ int64_t by_xcd(int64_t b, int64_t n) {
-    const int64_t whole = n / 8 * 8;
+__device__ __forceinline__ uint32_t by_xcd(uint32_t b, uint32_t n) {
+    const uint32_t whole = n / 8 * 8;
     return b < whole ? b % 8 * (n / 8) + b / 8 : b;
 }
 
@@ -139,24 +139,25 @@ __device__ __forceinline__ void store_whole(T *at, const float (&x)[W]) {
 #pragma unroll
     for (int i = 0; i < kWords / kStep; i++) reinterpret_cast<Anywhere *>(at)[i].w = split.w[i];
 }
-// A chunk's results, columns col .. of rows 16 I + c.  base: its first row, the same for all lanes; C rows lie within 32 bits of bytes.  live: the chunk's rows that count, the others become zero; there: those that are
-// there at all.  cols: this lane's columns that are there, of 4 J.
-template <typename T, int C, int J>
-__device__ __forceinline__ void store_rows(T *base, int stride, int col, const v4f (&acc)[C / 16][J], float scale, int live, int there, bool whole, int cols, int c) {
+// A chunk's results, columns col .. of rows 16 I + c.  base: its first row, the same for all lanes; C rows lie within 32 bits of bytes.  live: the chunk's rows that
+// count, the others become zero; there: those that are there at all.  cols: this lane's columns that are there, of 4 J (all where WHOLE).
+template <bool WHOLE, typename T, int C, int J>
+__device__ __forceinline__ void store_rows(T *base, int stride, int col, const v4f (&acc)[C / 16][J], float scale, int live, int there, int cols, int c) {
 #pragma unroll
     for (int I = 0; I < C / 16; I++) {
         float x[4 * J];
 #pragma unroll
         for (int j = 0; j < J; j++)
 #pragma unroll
-            for (int i = 0; i < 4; i++) x[4 * j + i] = acc[I][j][i] * scale;
+            for (int i = 0; i < 4; i++) x[4 * j + i] = 16 * I + c < live ? acc[I][j][i] * scale : 0.f;
         T *to = from(base, (uint32_t)(16 * I + c) * (uint32_t)stride + (uint32_t)col);
-        if (whole) {
+        if (16 * I + c >= there) continue;
+        if (WHOLE || cols >= 4 * J) {
             store_whole<T, 4 * J>(to, x);
-        } else if (16 * I + c < there) {
+        } else {
 #pragma unroll
             for (int i = 0; i < 4 * J; i++)
-                if (i < cols) to[i] = (T)(16 * I + c < live ? x[i] : 0.f);
+                if (i < cols) to[i] = (T)x[i];
         }
     }
 }
@@ -185,19 +186,19 @@ struct DsumForward {
 };
 
 // ENDS: the state that a segment leaves when it starts from zero, and the segment's whole decay; nothing else.
-template <typename T, int NE, int NW, int MW, bool ENDS>
+template <typename T, int NE, int NW, int MW, bool WHOLE, bool ENDS>
 __global__ __launch_bounds__(64 * NW, (ENDS ? DsumForward<T, NE, NW, MW>::kEndWaves : DsumForward<T, NE, NW, MW>::kWaves)) void k_dsum_fwd(const DsumWalk a) {
     using F = DsumForward<T, NE, NW, MW>;
     constexpr int C = F::C, P = F::P, O = F::O, X = F::X, E = F::E, MS = F::MS, NB = F::NB, SB = F::SB, TT = F::TT;
     __shared__ std::conditional_t<ENDS, typename F::Ends, typename F::Shared> sh;
     const int tid = threadIdx.x, lane = tid % 64, wave = tid / 64, g = lane / 16, c = lane % 16;
 
-    int64_t w = by_xcd(blockIdx.x, gridDim.x);
-    const int slice = w % a.slices;
-    w /= a.slices;
-    const int h = w % a.H;
-    w /= a.H;
-    const int n = w % a.N, seg = w / a.N;
+    uint32_t w = by_xcd(blockIdx.x, gridDim.x);
+    const int slice = w % (uint32_t)a.slices;
+    w /= (uint32_t)a.slices;
+    const int h = w % (uint32_t)a.H;
+    w /= (uint32_t)a.H;
+    const int n = w % (uint32_t)a.N, seg = w / (uint32_t)a.N;
 
     const int len = length_of(a.lengths, n, a.L), chunks = (a.L + C - 1) / C, live = (len + C - 1) / C;
     const int first = seg * a.per, last = min(first + a.per, chunks), stop = min(last, live);
@@ -233,8 +234,8 @@ __global__ __launch_bounds__(64 * NW, (ENDS ? DsumForward<T, NE, NW, MW>::kEndWa
         for (int i = tid; i < (int)(sizeof(sh.p) / 16); i += 64 * NW) reinterpret_cast<v4f *>(&sh.p)[i] = v4f{0, 0, 0, 0};
     }
 
-    Stage<T, C, E, 64 * NW> sq, sk;
-    Stage<T, C, MS, 64 * NW> sv;
+    Stage<T, C, E, 64 * NW, WHOLE> sq, sk;
+    Stage<T, C, MS, 64 * NW, WHOLE> sv;
     double total = 0;
     float gnext = 0;
     const auto fetch = [&](int chunk) {
@@ -354,7 +355,7 @@ __global__ __launch_bounds__(64 * NW, (ENDS ? DsumForward<T, NE, NW, MW>::kEndWa
         }
         if constexpr (!ENDS) {
             const int col = mw + 4 * MW * g;
-            store_rows<T, C, MW>(ob + (int64_t)chunk * C * a.out.sL, (int)a.out.sL, col, acc, a.scale, rows, a.L - chunk * C, rows >= C && values == MS, values - col, c);
+            store_rows<WHOLE, T, C, MW>(ob + (int64_t)chunk * C * a.out.sL, (int)a.out.sL, col, acc, a.scale, rows, a.L - chunk * C, values - col, c);
         }
         lds_barrier();
     }
@@ -396,40 +397,44 @@ __global__ __launch_bounds__(64 * NW, (ENDS ? DsumForward<T, NE, NW, MW>::kEndWa
 
 // ------------------------------------------------------------------ backward
 
+// A workgroup's waves share the walk back by what they own: KW key waves have EW tiles of 16 key rows each, the gradients of q and k there and the adjoint's
+// rows (all value columns, transposed); VW value waves have MW tiles of 16 value columns each, the gradient of v and the adjoint's columns, and make P and R.
+// The adjoint is held twice so that no product waits for another wave's share of it.
 template <typename T, int NE, int NW, int MW>
 struct DsumBackward {
-    static constexpr int C = kChunkOf<T>, P = Parts<T, NE>::P, O = Parts<T, NE>::O, X = Parts<T, NE>::X, E = 16 * NE, MS = 16 * MW * NW, kThreads = 64 * NW;
-    static constexpr int NB = NE / 2, SB = C / 32, TT = C / 16, MB = MW * NW / 2;      // an even number of waves
-    static constexpr int EW = NE >= NW ? NE / NW : 1;      // key tiles of a wave
+    static constexpr int C = kChunkOf<T>, P = Parts<T, NE>::P, O = Parts<T, NE>::O, X = Parts<T, NE>::X, E = 16 * NE, MS = 16 * MW * NW;
+    static constexpr int NB = NE / 2, SB = C / 32, TT = C / 16, MB = MS / 32;
+    static constexpr int KW = NE < 4 ? NE : 4, EW = NE / KW, VW = MS / 16 < 4 ? MS / 16 : 4, VM = MS / 16 / VW;
+    static constexpr bool kBoth = NE <= 4 && MS <= 64;      // every wave is of both kinds
+    static constexpr int kCount = kBoth ? (KW > VW ? KW : VW) : KW + VW, kThreads = 64 * kCount, kTileWaves = kBoth ? kCount : VW;
     struct Shared {
         Tile<C, E, P> q, k;
         Tile<C, MS, P> v, go;
-        Tile<C, C, O> p;
-        Tile<C, C, O> r;
+        Tile<C, C, O> p, r;
         Decays<C> d[2];
-        float sums[2][NW][C], within[2][TT + 1][C], inner[2][NW];
+        float sums[2][KW][C], within[2][TT + 1][C], inner[2][KW];
     };
     struct Ends {
         Tile<C, E, P> q;
         Tile<C, MS, P> go;
         Decays<C> d[2];
     };
-    static constexpr int kWaves = P == kPlain && NW <= 4 ? 3 : NE <= 4 || NW == 8 ? 2 : 1, kEndWaves = NE <= 4 ? 4 : 3;
+    static constexpr int kWaves = 2, kEndWaves = NE <= 4 ? 4 : 3;
 };
 
 // The adjoint of a segment's first state when that of its last one is zero, and the segment's whole decay.
-template <typename T, int NE, int NW, int MW>
+template <typename T, int NE, int NW, int MW, bool WHOLE>
 __global__ __launch_bounds__(64 * NW, (DsumBackward<T, NE, NW, MW>::kEndWaves)) void k_dsum_bwd_ends(const DsumWalk a) {
     using F = DsumBackward<T, NE, NW, MW>;
     constexpr int C = F::C, P = F::P, X = F::X, E = F::E, MS = F::MS, NB = F::NB, SB = F::SB;
     __shared__ typename F::Ends sh;
     const int tid = threadIdx.x, lane = tid % 64, wave = tid / 64, g = lane / 16, c = lane % 16;
-    int64_t w = by_xcd(blockIdx.x, gridDim.x);
-    const int slice = w % a.slices;
-    w /= a.slices;
-    const int h = w % a.H;
-    w /= a.H;
-    const int n = w % a.N, seg = w / a.N + 1;
+    uint32_t w = by_xcd(blockIdx.x, gridDim.x);
+    const int slice = w % (uint32_t)a.slices;
+    w /= (uint32_t)a.slices;
+    const int h = w % (uint32_t)a.H;
+    w /= (uint32_t)a.H;
+    const int n = w % (uint32_t)a.N, seg = w / (uint32_t)a.N + 1;
     const int len = length_of(a.lengths, n, a.L), chunks = (a.L + C - 1) / C, live = (len + C - 1) / C;
     const int first = seg * a.per, stop = min(min(first + a.per, chunks), live);
     const int hq = h / (a.H / a.HQ), m0 = slice * MS, mcols = min(a.M - m0, MS), mw = wave * 16 * MW;
@@ -443,8 +448,8 @@ __global__ __launch_bounds__(64 * NW, (DsumBackward<T, NE, NW, MW>::kEndWaves)) 
         for (int u = 0; u < 2; u++)
 #pragma unroll
             for (int j = 0; j < MW; j++) G[b][u][j] = v4f{0, 0, 0, 0};
-    Stage<T, C, E, 64 * NW> sq;
-    Stage<T, C, MS, 64 * NW> sd;
+    Stage<T, C, E, 64 * NW, WHOLE> sq;
+    Stage<T, C, MS, 64 * NW, WHOLE> sd;
     double total = 0;
     float gnext = 0;
     const auto fetch = [&](int chunk) {
@@ -515,67 +520,73 @@ __global__ __launch_bounds__(64 * NW, (DsumBackward<T, NE, NW, MW>::kEndWaves)) 
     if (tid == 64 * (NW - 1) && slice == 0) a.factors[head * a.segments + seg] = __builtin_amdgcn_exp2f((float)total);
 }
 
-template <typename T, int NE, int NW, int MW>
-__global__ __launch_bounds__(64 * NW, (DsumBackward<T, NE, NW, MW>::kWaves)) void k_dsum_bwd(const DsumWalk a) {
+// The walk of one kind of waves; `wave` counts them, `tid` all threads.
+template <bool KEYS, bool VALUES, typename T, int NE, int NW, int MW, bool WHOLE>
+__device__ __forceinline__ void dsum_walk_back(const DsumWalk &a, typename DsumBackward<T, NE, NW, MW>::Shared &sh, int wave, int tid) {
     using F = DsumBackward<T, NE, NW, MW>;
-    constexpr int C = F::C, P = F::P, O = F::O, X = F::X, E = F::E, MS = F::MS, NB = F::NB, SB = F::SB, TT = F::TT, MB = F::MB, EW = F::EW;
-    __shared__ typename F::Shared sh;
-    const int tid = threadIdx.x, lane = tid % 64, wave = tid / 64, g = lane / 16, c = lane % 16;
-    int64_t w = by_xcd(blockIdx.x, gridDim.x);
-    const int slice = w % a.slices;
-    w /= a.slices;
-    const int h = w % a.H;
-    w /= a.H;
-    const int n = w % a.N, seg = w / a.N;
+    constexpr int C = F::C, P = F::P, O = F::O, X = F::X, E = F::E, MS = F::MS, NB = F::NB, SB = F::SB, TT = F::TT, MB = F::MB, EW = F::EW, VM = F::VM,
+                  kThreads = F::kThreads;
+    const int lane = tid % 64, g = lane / 16, c = lane % 16;
+    uint32_t w = by_xcd(blockIdx.x, gridDim.x);
+    const int slice = w % (uint32_t)a.slices;
+    w /= (uint32_t)a.slices;
+    const int h = w % (uint32_t)a.H;
+    w /= (uint32_t)a.H;
+    const int n = w % (uint32_t)a.N, seg = w / (uint32_t)a.N;
     const int len = length_of(a.lengths, n, a.L), chunks = (a.L + C - 1) / C, live = (len + C - 1) / C;
     const int first = seg * a.per, last = min(first + a.per, chunks), stop = min(last, live);
-    const int rq = a.H / a.HQ, rk = a.H / a.HK, rv = a.H / a.HV, m0 = slice * MS, mcols = min(a.M - m0, MS), mw = wave * 16 * MW, ew = wave * 16 * EW;
-    const bool keys = ew < E;      // has this wave key rows of its own?
+    const int rq = a.H / a.HQ, rk = a.H / a.HK, rv = a.H / a.HV, m0 = slice * MS, mcols = min(a.M - m0, MS), mw = wave * 16 * VM, ew = wave * 16 * EW;
     const T *qb = row<T>(a.q, n, h / rq, 0), *kb = row<T>(a.k, n, h / rk, 0), *vb = row<T>(a.v, n, h / rv, 0) + m0, *db = row<T>(a.go, n, h, 0) + m0;
     const float *gb = a.decay + n * a.dN + h * a.dH;
     const int64_t head = (int64_t)n * a.H + h;
+    const bool sums_decay = VALUES && wave == F::kTileWaves - 1, grades_decay = VALUES && wave == F::kTileWaves - 2;
+    const bool keys = KEYS && wave < F::KW, values = VALUES && wave < F::VW;      // a wave of both kinds may be beyond the rows or columns there are
 
-    // where this head's gradients go: rows of their own, or its part of a sum
-    float *const pq = a.pq + ((((int64_t)(h % rq) * a.slices + slice) * a.N + n) * a.HQ + h / rq) * a.L * a.E;
-    float *const pk = a.pk + ((((int64_t)(h % rk) * a.slices + slice) * a.N + n) * a.HK + h / rk) * a.L * a.E;
-    float *const pv = a.pv + (((int64_t)(h % rv) * a.N + n) * a.HV + h / rv) * a.L * a.M + m0;
-    T *const gq = row<T>(a.gq, n, h, 0), *const gk = row<T>(a.gk, n, h, 0), *const gv = row<T>(a.gv, n, h, 0) + m0;
-
-    // G: all key rows of this wave's value columns.  H: the same numbers, all value columns of its key rows, transposed.
-    v4f G[NB][2][MW], H[MB][2][EW];
+    // the adjoint: key waves H, all value columns of their key rows, transposed; value waves G, all key rows of their value columns
+    v4f H[KEYS ? MB : 1][2][EW], G[VALUES ? NB : 1][2][VM];
     {
         const float *from = a.segments > 1 && seg + 1 < a.segments ? a.ends + (head * a.segments + seg) * E * a.Mp + m0 : nullptr;
+        if constexpr (KEYS) {
 #pragma unroll
-        for (int b = 0; b < NB; b++)
+            for (int b = 0; b < MB; b++)
 #pragma unroll
-            for (int u = 0; u < 2; u++)
+                for (int u = 0; u < 2; u++)
 #pragma unroll
-                for (int j = 0; j < MW; j++)
+                    for (int j = 0; j < EW; j++)
 #pragma unroll
-                    for (int i = 0; i < 4; i++) G[b][u][j][i] = from ? from[(32 * b + 8 * g + 4 * u + i) * a.Mp + mw + place(MW, c, j)] : 0.f;
+                        for (int i = 0; i < 4; i++) H[b][u][j][i] = from && keys ? from[(ew + place(EW, c, j)) * a.Mp + 32 * b + 8 * g + 4 * u + i] : 0.f;
+        }
+        if constexpr (VALUES) {
+#pragma unroll
+            for (int b = 0; b < NB; b++)
+#pragma unroll
+                for (int u = 0; u < 2; u++)
+#pragma unroll
+                    for (int j = 0; j < VM; j++)
+#pragma unroll
+                        for (int i = 0; i < 4; i++) G[b][u][j][i] = from && values ? from[(32 * b + 8 * g + 4 * u + i) * a.Mp + mw + place(VM, c, j)] : 0.f;
+        }
+    }
+#pragma unroll 1
+    for (int i = tid; i < (int)(sizeof(sh.p) / 16); i += kThreads) reinterpret_cast<v4f *>(&sh.p)[i] = v4f{0, 0, 0, 0};
+#pragma unroll 1
+    for (int i = tid; i < (int)(sizeof(sh.r) / 16); i += kThreads) reinterpret_cast<v4f *>(&sh.r)[i] = v4f{0, 0, 0, 0};
+
+    // a chunk's first state, as this key wave reads it
+    float S[KEYS ? MB : 1][EW][8];
+    const auto load_state = [&](int chunk) {
+        const float *base = a.saved + (head * chunks + chunk) * E * a.Mp + m0;
 #pragma unroll
         for (int b = 0; b < MB; b++)
 #pragma unroll
-            for (int u = 0; u < 2; u++)
-#pragma unroll
-                for (int j = 0; j < EW; j++)
-#pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        const int m = 32 * b + 8 * g + 4 * u + i;
-                        H[b][u][j][i] = from && keys ? from[(ew + place(EW, c, j)) * a.Mp + m] : 0.f;
-                    }
-    }
-    for (int i = tid; i < (int)(sizeof(sh.p) / 16); i += 64 * NW) reinterpret_cast<v4f *>(&sh.p)[i] = v4f{0, 0, 0, 0};
-    for (int i = tid; i < (int)(sizeof(sh.r) / 16); i += 64 * NW) reinterpret_cast<v4f *>(&sh.r)[i] = v4f{0, 0, 0, 0};
-
-    // what this wave reads of a chunk's first state, by key rows
-    const auto before = [&](int chunk, int b, int j, float (&x)[8]) {
-        const float *at = from((const float *)a.saved + (head * chunks + chunk) * E * a.Mp + m0, (uint32_t)((keys ? ew : 0) + place(EW, c, j)) * (uint32_t)a.Mp + 32 * b + 8 * g);
-        const float4 lo = *reinterpret_cast<const float4 *>(at), hi = *reinterpret_cast<const float4 *>(at + 4);
-        x[0] = lo.x, x[1] = lo.y, x[2] = lo.z, x[3] = lo.w, x[4] = hi.x, x[5] = hi.y, x[6] = hi.z, x[7] = hi.w;
+            for (int j = 0; j < EW; j++) {
+                const float *at = from(base, (uint32_t)((keys ? ew : 0) + place(EW, c, j)) * (uint32_t)a.Mp + 32 * b + 8 * g);
+                const float4 lo = *reinterpret_cast<const float4 *>(at), hi = *reinterpret_cast<const float4 *>(at + 4);
+                S[b][j][0] = lo.x, S[b][j][1] = lo.y, S[b][j][2] = lo.z, S[b][j][3] = lo.w, S[b][j][4] = hi.x, S[b][j][5] = hi.y, S[b][j][6] = hi.z, S[b][j][7] = hi.w;
+            }
     };
     // <H, S>, this wave's part
-    const auto inner = [&](const float(&S)[MB][EW][8]) {
+    const auto inner = [&] {
         float s = 0.f;
 #pragma unroll
         for (int b = 0; b < MB; b++)
@@ -586,43 +597,24 @@ __global__ __launch_bounds__(64 * NW, (DsumBackward<T, NE, NW, MW>::kWaves)) voi
         return over_groups(over_sixteen(s));
     };
 
-    Stage<T, C, E, 64 * NW> sq, sk;
-    Stage<T, C, MS, 64 * NW> sv, sd;
-    float gnext = 0, all = 0;
+    Stage<T, C, E, kThreads, WHOLE> sq, sk;
+    Stage<T, C, MS, kThreads, WHOLE> sv, sd;
+    float gnext = 0, all = 0, x_end = 0;
     const auto fetch = [&](int chunk) {
         const int64_t t0 = (int64_t)chunk * C;
-        const int rows = len - (int)t0;
-        sq.load(qb + t0 * a.q.sL, (int)a.q.sL, rows, a.E, tid);
-        sk.load(kb + t0 * a.k.sL, (int)a.k.sL, rows, a.E, tid);
-        sv.load(vb + t0 * a.v.sL, (int)a.v.sL, rows, mcols, tid);
-        sd.load(db + t0 * a.go.sL, (int)a.go.sL, rows, mcols, tid);
+        const int rows = len - (int)t0, wide = opaque(a.E), cols = opaque(mcols);
+        sq.load(qb + t0 * a.q.sL, (int)a.q.sL, rows, wide, tid);
+        sk.load(kb + t0 * a.k.sL, (int)a.k.sL, rows, wide, tid);
+        sv.load(vb + t0 * a.v.sL, (int)a.v.sL, rows, cols, tid);
+        sd.load(db + t0 * a.go.sL, (int)a.go.sL, rows, cols, tid);
     };
     const auto fetch_decay = [&](int chunk) { gnext = gb[min((int64_t)chunk * C + lane, (int64_t)len - 1) * a.dL]; };
     const auto sum_decay = [&](int chunk) { sh.d[chunk & 1].sum(lane < C && chunk * C + lane < len ? gnext : 0.f, lane); };
-    if (first < stop) {
-        if (wave == NW - 1) fetch_decay(stop - 1);
-        fetch(stop - 1);
-        if (wave == NW - 1) {
-            sum_decay(stop - 1);
-            if (stop - 1 > first) fetch_decay(stop - 2);
-        }
-    }
-    // the inner product at the segment's end, with the next segment's first state; behind the last chunk the adjoint is zero
-    float x_end = 0.f;
-    if (stop == last && stop < live) {
-        float S[MB][EW][8];
-#pragma unroll
-        for (int b = 0; b < MB; b++)
-#pragma unroll
-            for (int j = 0; j < EW; j++) before(stop, b, j, S[b][j]);
-        x_end = inner(S);
-    }
-
-    // the decays' gradients of the chunk behind this one, from what the waves have left in LDS
+    // the decays' gradients of a chunk, from what the waves have left in LDS
     const auto decay_gradients = [&](int chunk) {
         float s = 0.f, x = 0.f;
 #pragma unroll
-        for (int i = 0; i < NW; i++) s += sh.sums[chunk & 1][i][lane % C], x += sh.inner[chunk & 1][i];
+        for (int i = 0; i < F::KW; i++) s += sh.sums[chunk & 1][i][lane % C], x += sh.inner[chunk & 1][i];
 #pragma unroll
         for (int i = 0; i <= TT; i++) s += sh.within[chunk & 1][i][lane % C];
         if (lane >= C) s = 0.f;
@@ -636,144 +628,173 @@ __global__ __launch_bounds__(64 * NW, (DsumBackward<T, NE, NW, MW>::kWaves)) voi
         if (a.sum_decay) all += s;
         else if (lane < C && t < a.L) a.gdecay[(((int64_t)slice * a.N + n) * a.H + h) * a.L + t] = s;
     };
+    if (first < stop) {
+        if (sums_decay) fetch_decay(stop - 1);
+        fetch(stop - 1);
+        if (sums_decay) {
+            sum_decay(stop - 1);
+            if (stop - 1 > first) fetch_decay(stop - 2);
+        }
+        if constexpr (KEYS) {
+            // the inner product at the segment's end, with the next segment's first state; behind the last chunk the adjoint is zero
+            if (stop == last && stop < live) {
+                load_state(stop);
+                x_end = inner();
+            }
+            load_state(stop - 1);
+        }
+    }
 
     for (int chunk = stop - 1; chunk >= first; chunk--) {
-        const int rows = len - chunk * C, wide = opaque(a.E), values = opaque(mcols);
-        sq.put(sh.q, rows, wide, tid);
-        sk.put(sh.k, rows, wide, tid);
-        sv.put(sh.v, rows, values, tid);
-        sd.put(sh.go, rows, values, tid);
-        if (lane == 0) sh.inner[chunk & 1][wave] = x_end;
+        const int rows = len - chunk * C, there = a.L - chunk * C;
+        {
+            const int wide = opaque(a.E), cols = opaque(mcols);
+            sq.put(sh.q, rows, wide, tid);
+            sk.put(sh.k, rows, wide, tid);
+            sv.put(sh.v, rows, cols, tid);
+            sd.put(sh.go, rows, cols, tid);
+        }
+        if (keys && lane == 0) sh.inner[chunk & 1][wave] = x_end;
         lds_barrier();
         const Decays<C> &d = sh.d[chunk & 1];
-        float S[MB][EW][8];
-#pragma unroll
-        for (int b = 0; b < MB; b++)
-#pragma unroll
-            for (int j = 0; j < EW; j++) before(chunk, b, j, S[b][j]);
-        if (wave == NW - 1 && chunk > first) {
+        if (sums_decay && chunk > first) {
             sum_decay(chunk - 1);
             if (chunk - 1 > first) fetch_decay(chunk - 2);
         }
         if (chunk > first) fetch(chunk - 1);
-        if (wave == NW - 2 && chunk + 1 < stop) decay_gradients(chunk + 1);
+        if (grades_decay && chunk + 1 < stop) decay_gradients(chunk + 1);
 
-        for (int tile = wave; tile < TT * (TT + 1) / 2; tile += NW) {
-            int I = 0, J = tile;
-            while (J > I) J -= ++I;
-            v4f p = {0, 0, 0, 0}, r = {0, 0, 0, 0};
+        // P and R, a 16 x 16 tile of each at a time
+        if (VALUES)
+            for (int tile = wave; tile < TT * (TT + 1) / 2; tile += F::kTileWaves) {
+                int I = 0, J = tile;
+                while (J > I) J -= ++I;
+                v4f p = {0, 0, 0, 0}, r = {0, 0, 0, 0};
 #pragma unroll
-            for (int b = 0; b < NB; b++) p = product<X>(sh.k.rows(16 * J, 32 * b, g, c), sh.q.rows(16 * I, 32 * b, g, c), p);
+                for (int b = 0; b < NB; b++) p = product<X>(sh.k.rows(16 * J, 32 * b, g, c), sh.q.rows(16 * I, 32 * b, g, c), p);
 #pragma unroll
-            for (int b = 0; b < MB; b++) r = product<X>(sh.v.rows(16 * J, 32 * b, g, c), sh.go.rows(16 * I, 32 * b, g, c), r);
-            const int t = 16 * I + c, s = 16 * J + 4 * g;
-            const v4f f = d.between(t, s);
-            float x[4], y[4], u = 0.f, z[4];
+                for (int b = 0; b < MB; b++) r = product<X>(sh.v.rows(16 * J, 32 * b, g, c), sh.go.rows(16 * I, 32 * b, g, c), r);
+                const int t = 16 * I + c, s = 16 * J + 4 * g;
+                const v4f f = d.between(t, s);
+                float x[4], y[4], u = 0.f, z[4];
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                x[i] = s + i <= t ? p[i] * f[i] : 0.f, y[i] = s + i <= t ? r[i] * f[i] : 0.f;
-                z[i] = s + i < t ? x[i] * r[i] : 0.f;
-                u += z[i];
+                for (int i = 0; i < 4; i++) {
+                    x[i] = s + i <= t ? p[i] * f[i] : 0.f, y[i] = s + i <= t ? r[i] * f[i] : 0.f;
+                    z[i] = s + i < t ? x[i] * r[i] : 0.f;
+                    u += z[i];
+                }
+                // what step t reads of what step s wrote counts for the decays between them: sums over s for every t, and over t for every s
+                u = over_groups(u);
+#pragma unroll
+                for (int i = 0; i < 4; i++) z[i] = over_sixteen(z[i]);
+                if (g == 0) sh.within[chunk & 1][J][t] = u;
+                if (c == 0) *reinterpret_cast<v4f *>(&sh.within[chunk & 1][I == J ? TT : I][s]) = v4f{-z[0], -z[1], -z[2], -z[3]};
+                sh.p.put4(t, s, x);
+                sh.r.put4(t, s, y);
             }
-            // what step t reads of what step s wrote counts for the decays between them: sums over s for every t, and over t for every s
-            u = over_groups(u);
-#pragma unroll
-            for (int i = 0; i < 4; i++) z[i] = over_sixteen(z[i]);
-            if (g == 0) sh.within[chunk & 1][J][t] = u;
-            if (c == 0) *reinterpret_cast<v4f *>(&sh.within[chunk & 1][I == J ? TT : I][s]) = v4f{-z[0], -z[1], -z[2], -z[3]};
-            sh.p.put4(t, s, x);
-            sh.r.put4(t, s, y);
-        }
 
-        v4f dq[TT][EW], dk[TT][EW], dv[TT][MW];
-#pragma unroll
-        for (int I = 0; I < TT; I++) {
-#pragma unroll
-            for (int j = 0; j < EW; j++) dq[I][j] = dk[I][j] = v4f{0, 0, 0, 0};
-#pragma unroll
-            for (int j = 0; j < MW; j++) dv[I][j] = v4f{0, 0, 0, 0};
-        }
-        // through the states before and behind the chunk
+        v4f dq[TT][EW], dk[TT][EW], dv[TT][VM];
         if (keys) {
 #pragma unroll
-            for (int b = 0; b < MB; b++) {
-                Frag<X> s[EW], ht[EW];
+            for (int I = 0; I < TT; I++)
 #pragma unroll
-                for (int j = 0; j < EW; j++) {
-                    s[j] = split8<X>(S[b][j]);
-                    ht[j] = split8<X>(H[b][0][j], H[b][1][j]);
-                }
+                for (int j = 0; j < EW; j++) dq[I][j] = dk[I][j] = v4f{0, 0, 0, 0};
+            // through the states before and behind the chunk
+#pragma unroll
+            for (int b = 0; b < MB; b++) {
+                Frag<X> s[EW];
+#pragma unroll
+                for (int j = 0; j < EW; j++) s[j] = split8<X>(S[b][j]);
 #pragma unroll
                 for (int I = 0; I < TT; I++) {
-                    const Frag<P> go = sh.go.rows(16 * I, 32 * b, g, c), v = sh.v.rows(16 * I, 32 * b, g, c);
+                    const Frag<P> go = sh.go.rows(16 * I, 32 * b, g, c);
 #pragma unroll
-                    for (int j = 0; j < EW; j++) dq[I][j] = product<X>(s[j], go, dq[I][j]), dk[I][j] = product<X>(ht[j], v, dk[I][j]);
+                    for (int j = 0; j < EW; j++) dq[I][j] = product<X>(s[j], go, dq[I][j]);
+                }
+#pragma unroll
+                for (int j = 0; j < EW; j++) s[j] = split8<X>(H[b][0][j], H[b][1][j]);
+#pragma unroll
+                for (int I = 0; I < TT; I++) {
+                    const Frag<P> v = sh.v.rows(16 * I, 32 * b, g, c);
+#pragma unroll
+                    for (int j = 0; j < EW; j++) dk[I][j] = product<X>(s[j], v, dk[I][j]);
                 }
             }
-        }
-#pragma unroll
-        for (int b = 0; b < NB; b++) {
-            Frag<O> s[MW];
-#pragma unroll
-            for (int j = 0; j < MW; j++) s[j] = split8<O>(G[b][0][j], G[b][1][j]);
 #pragma unroll
             for (int I = 0; I < TT; I++) {
-                const Frag<P> k = sh.k.rows(16 * I, 32 * b, g, c);
+                const int r = 16 * I + c;
+                const float into = d.into[r], rest = d.rest[r];
+                float u = 0.f;
 #pragma unroll
-                for (int j = 0; j < MW; j++) dv[I][j] = product<O>(s[j], k, dv[I][j]);
-            }
-        }
-#pragma unroll
-        for (int I = 0; I < TT; I++) {
-            const int r = 16 * I + c;
-            const float into = d.into[r], rest = d.rest[r];
-            float u = 0.f;
-#pragma unroll
-            for (int j = 0; j < EW; j++) {
-                dq[I][j] *= into, dk[I][j] *= rest;
-                if (keys) {
+                for (int j = 0; j < EW; j++) {
+                    dq[I][j] *= into, dk[I][j] *= rest;
                     const v4f q = sh.q.four(r, ew + 4 * EW * g + 4 * j), k = sh.k.four(r, ew + 4 * EW * g + 4 * j);
 #pragma unroll
                     for (int i = 0; i < 4; i++) u = fmaf(q[i], dq[I][j][i], u), u = fmaf(-k[i], dk[I][j][i], u);
                 }
+                u = over_groups(u);
+                if (g == 0) sh.sums[chunk & 1][wave][r] = u;
             }
-            u = over_groups(u);
-            if (g == 0) sh.sums[chunk & 1][wave][r] = u;
+        }
+        if (values) {
 #pragma unroll
-            for (int j = 0; j < MW; j++) dv[I][j] *= rest;
+            for (int I = 0; I < TT; I++)
+#pragma unroll
+                for (int j = 0; j < VM; j++) dv[I][j] = v4f{0, 0, 0, 0};
+#pragma unroll
+            for (int b = 0; b < NB; b++) {
+                Frag<O> s[VM];
+#pragma unroll
+                for (int j = 0; j < VM; j++) s[j] = split8<O>(G[b][0][j], G[b][1][j]);
+#pragma unroll
+                for (int I = 0; I < TT; I++) {
+                    const Frag<P> k = sh.k.rows(16 * I, 32 * b, g, c);
+#pragma unroll
+                    for (int j = 0; j < VM; j++) dv[I][j] = product<O>(s[j], k, dv[I][j]);
+                }
+            }
+#pragma unroll
+            for (int I = 0; I < TT; I++) {
+                const float rest = d.rest[16 * I + c];
+#pragma unroll
+                for (int j = 0; j < VM; j++) dv[I][j] *= rest;
+            }
         }
         lds_barrier();
 
-        // within the chunk, and the adjoint of the state before it
+        if (keys) {
+            // within the chunk, and the adjoint of the state before it
 #pragma unroll
-        for (int b = 0; b < NB; b++)
+            for (int b = 0; b < MB; b++)
 #pragma unroll
-            for (int u = 0; u < 2; u++)
+                for (int u = 0; u < 2; u++)
 #pragma unroll
-                for (int j = 0; j < MW; j++) G[b][u][j] *= d.whole;
+                    for (int j = 0; j < EW; j++) H[b][u][j] *= d.whole;
 #pragma unroll
-        for (int b = 0; b < MB; b++)
-#pragma unroll
-            for (int u = 0; u < 2; u++)
-#pragma unroll
-                for (int j = 0; j < EW; j++) H[b][u][j] *= d.whole;
-#pragma unroll
-        for (int sb = 0; sb < SB; sb++) {
-            const v4f f0 = *reinterpret_cast<const v4f *>(&d.into[32 * sb + 8 * g]), f1 = *reinterpret_cast<const v4f *>(&d.into[32 * sb + 8 * g + 4]);
-            if (keys) {
+            for (int sb = 0; sb < SB; sb++) {
+                const v4f f0 = *reinterpret_cast<const v4f *>(&d.into[32 * sb + 8 * g]), f1 = *reinterpret_cast<const v4f *>(&d.into[32 * sb + 8 * g + 4]);
                 Frag<X> qs[EW];
+                Frag<P> q[EW], k[EW];
 #pragma unroll
                 for (int j = 0; j < EW; j++) {
-                    const Frag<P> k = sh.k.template columns<EW>(ew, j, 32 * sb, g, c), q = sh.q.template columns<EW>(ew, j, 32 * sb, g, c);
-#pragma unroll
-                    for (int I = 2 * sb; I < TT; I++) dq[I][j] = product<O>(k, sh.r.rows(16 * I, 32 * sb, g, c), dq[I][j]);
-#pragma unroll
-                    for (int I = 0; I < 2 * sb + 2; I++) dk[I][j] = product<O>(q, sh.r.template columns<1>(16 * I, 0, 32 * sb, g, c), dk[I][j]);
+                    k[j] = sh.k.template columns<EW>(ew, j, 32 * sb, g, c), q[j] = sh.q.template columns<EW>(ew, j, 32 * sb, g, c);
                     float x[8];
-                    join8(q, x);
+                    join8(q[j], x);
 #pragma unroll
                     for (int i = 0; i < 4; i++) x[i] *= f0[i], x[i + 4] *= f1[i];
                     qs[j] = split8<X>(x);
+                }
+#pragma unroll
+                for (int I = 2 * sb; I < TT; I++) {
+                    const Frag<O> r = sh.r.rows(16 * I, 32 * sb, g, c);
+#pragma unroll
+                    for (int j = 0; j < EW; j++) dq[I][j] = product<O>(k[j], r, dq[I][j]);
+                }
+#pragma unroll
+                for (int I = 0; I < 2 * sb + 2; I++) {
+                    const Frag<O> r = sh.r.template columns<1>(16 * I, 0, 32 * sb, g, c);
+#pragma unroll
+                    for (int j = 0; j < EW; j++) dk[I][j] = product<O>(q[j], r, dk[I][j]);
                 }
 #pragma unroll
                 for (int b = 0; b < MB; b++)
@@ -784,74 +805,119 @@ __global__ __launch_bounds__(64 * NW, (DsumBackward<T, NE, NW, MW>::kWaves)) voi
                         for (int j = 0; j < EW; j++) H[b][u][j] = product<X>(go, qs[j], H[b][u][j]);
                     }
             }
-            Frag<X> ds[MW];
-#pragma unroll
-            for (int j = 0; j < MW; j++) {
-                const Frag<P> go = sh.go.template columns<MW>(mw, j, 32 * sb, g, c);
-#pragma unroll
-                for (int I = 0; I < 2 * sb + 2; I++) dv[I][j] = product<O>(go, sh.p.template columns<1>(16 * I, 0, 32 * sb, g, c), dv[I][j]);
-                float x[8];
-                join8(go, x);
-#pragma unroll
-                for (int i = 0; i < 4; i++) x[i] *= f0[i], x[i + 4] *= f1[i];
-                ds[j] = split8<X>(x);
+            // for the chunk before this one; ahead of the stores, which the loads would else wait for
+            x_end = inner();
+            if (chunk > first) load_state(chunk - 1);
+            {
+                const int wide = opaque(a.E), col = ew + 4 * EW * g;
+                if (a.pq) {
+                    float *pq = a.pq + ((((int64_t)(h % rq) * a.slices + slice) * a.N + n) * a.HQ + h / rq) * a.L * wide;
+                    store_rows<WHOLE, float, C, EW>(pq + (int64_t)chunk * C * wide, wide, col, dq, a.scale, rows, there, wide - col, c);
+                } else {
+                    store_rows<WHOLE, T, C, EW>(row<T>(a.gq, n, h, (int64_t)chunk * C), (int)a.gq.sL, col, dq, a.scale, rows, there, wide - col, c);
+                }
+                if (a.pk) {
+                    float *pk = a.pk + ((((int64_t)(h % rk) * a.slices + slice) * a.N + n) * a.HK + h / rk) * a.L * wide;
+                    store_rows<WHOLE, float, C, EW>(pk + (int64_t)chunk * C * wide, wide, col, dk, a.scale, rows, there, wide - col, c);
+                } else {
+                    store_rows<WHOLE, T, C, EW>(row<T>(a.gk, n, h, (int64_t)chunk * C), (int)a.gk.sL, col, dk, a.scale, rows, there, wide - col, c);
+                }
             }
+        }
+        if (values) {
 #pragma unroll
             for (int b = 0; b < NB; b++)
 #pragma unroll
-                for (int u = 0; u < 2; u++) {
-                    const Frag<P> q = sh.q.template columns<2>(32 * b, u, 32 * sb, g, c);
+                for (int u = 0; u < 2; u++)
 #pragma unroll
-                    for (int j = 0; j < MW; j++) G[b][u][j] = product<X>(q, ds[j], G[b][u][j]);
+                    for (int j = 0; j < VM; j++) G[b][u][j] *= d.whole;
+#pragma unroll
+            for (int sb = 0; sb < SB; sb++) {
+                const v4f f0 = *reinterpret_cast<const v4f *>(&d.into[32 * sb + 8 * g]), f1 = *reinterpret_cast<const v4f *>(&d.into[32 * sb + 8 * g + 4]);
+                // this side of the adjoint ends in the gradient of v alone
+                Frag<O> ds[VM];
+                Frag<P> go[VM];
+#pragma unroll
+                for (int j = 0; j < VM; j++) {
+                    go[j] = sh.go.template columns<VM>(mw, j, 32 * sb, g, c);
+                    float x[8];
+                    join8(go[j], x);
+#pragma unroll
+                    for (int i = 0; i < 4; i++) x[i] *= f0[i], x[i + 4] *= f1[i];
+                    ds[j] = split8<O>(x);
                 }
+#pragma unroll
+                for (int I = 0; I < 2 * sb + 2; I++) {
+                    const Frag<O> p = sh.p.template columns<1>(16 * I, 0, 32 * sb, g, c);
+#pragma unroll
+                    for (int j = 0; j < VM; j++) dv[I][j] = product<O>(go[j], p, dv[I][j]);
+                }
+#pragma unroll
+                for (int b = 0; b < NB; b++)
+#pragma unroll
+                    for (int u = 0; u < 2; u++) {
+                        const Frag<P> q = sh.q.template columns<2>(32 * b, u, 32 * sb, g, c);
+#pragma unroll
+                        for (int j = 0; j < VM; j++) G[b][u][j] = product<O>(q, ds[j], G[b][u][j]);
+                    }
+            }
+            {
+                const int cols = opaque(mcols), col = mw + 4 * VM * g;
+                if (a.pv) {
+                    float *pv = a.pv + (((int64_t)(h % rv) * a.N + n) * a.HV + h / rv) * a.L * a.M + m0;
+                    store_rows<WHOLE, float, C, VM>(pv + (int64_t)chunk * C * a.M, a.M, col, dv, a.scale, rows, there, cols - col, c);
+                } else {
+                    store_rows<WHOLE, T, C, VM>(row<T>(a.gv, n, h, (int64_t)chunk * C) + m0, (int)a.gv.sL, col, dv, a.scale, rows, there, cols - col, c);
+                }
+            }
         }
-
-        const int there = a.L - chunk * C;
-        if (keys) {
-            const int col = ew + 4 * EW * g;
-            const bool whole = rows >= C && wide == E;
-            if (a.pq) store_rows<float, C, EW>(pq + (int64_t)chunk * C * wide, wide, col, dq, a.scale, rows, there, whole, wide - col, c);
-            else store_rows<T, C, EW>(gq + (int64_t)chunk * C * a.gq.sL, (int)a.gq.sL, col, dq, a.scale, rows, there, whole, wide - col, c);
-            if (a.pk) store_rows<float, C, EW>(pk + (int64_t)chunk * C * wide, wide, col, dk, a.scale, rows, there, whole, wide - col, c);
-            else store_rows<T, C, EW>(gk + (int64_t)chunk * C * a.gk.sL, (int)a.gk.sL, col, dk, a.scale, rows, there, whole, wide - col, c);
-        }
-        {
-            const int col = mw + 4 * MW * g;
-            const bool whole = rows >= C && values == MS;
-            if (a.pv) store_rows<float, C, MW>(pv + (int64_t)chunk * C * a.M, a.M, col, dv, a.scale, rows, there, whole, values - col, c);
-            else store_rows<T, C, MW>(gv + (int64_t)chunk * C * a.gv.sL, (int)a.gv.sL, col, dv, a.scale, rows, there, whole, values - col, c);
-        }
-        x_end = inner(S);      // for the chunk before this one
         lds_barrier();
     }
-    if (first < stop && wave == NW - 2) decay_gradients(first);
+    if (first < stop && grades_decay) decay_gradients(first);
 
     // rows behind the sequence
     const int64_t t0 = (int64_t)max(stop, first) * C, t1 = min((int64_t)last * C, (int64_t)a.L);
-    for (int64_t i = t0 * E + tid; i < t1 * E; i += 64 * NW) {
-        const int64_t t = i / E;
-        const int e = i % E;
-        if (e >= a.E) continue;
-        if (a.pq) pq[t * a.E + e] = 0.f;
-        else gq[t * a.gq.sL + e] = (T)0.f;
-        if (a.pk) pk[t * a.E + e] = 0.f;
-        else gk[t * a.gk.sL + e] = (T)0.f;
-    }
-    for (int64_t i = t0 * MS + tid; i < t1 * MS; i += 64 * NW) {
-        const int64_t t = i / MS;
-        const int m = i % MS;
-        if (m >= mcols) continue;
-        if (a.pv) pv[t * a.M + m] = 0.f;
-        else gv[t * a.gv.sL + m] = (T)0.f;
-    }
-    if (a.sum_decay) {
-        if (wave == NW - 2) {
-#pragma unroll
-            for (int off = 1; off < 64; off *= 2) all += __shfl_xor(all, off);
-            if (lane == 0) a.gdecay[(head * a.slices + slice) * a.segments + seg] = all;
+    if (t0 < t1) {
+        float *const pq = a.pq + ((((int64_t)(h % rq) * a.slices + slice) * a.N + n) * a.HQ + h / rq) * a.L * a.E;
+        float *const pk = a.pk + ((((int64_t)(h % rk) * a.slices + slice) * a.N + n) * a.HK + h / rk) * a.L * a.E;
+        float *const pv = a.pv + (((int64_t)(h % rv) * a.N + n) * a.HV + h / rv) * a.L * a.M + m0;
+#pragma unroll 1
+        for (int64_t i = t0 * E + tid; i < t1 * E; i += kThreads) {
+            const int64_t t = i / E;
+            const int e = i % E;
+            if (e >= a.E) continue;
+            if (a.pq) pq[t * a.E + e] = 0.f;
+            else row<T>(a.gq, n, h, t)[e] = (T)0.f;
+            if (a.pk) pk[t * a.E + e] = 0.f;
+            else row<T>(a.gk, n, h, t)[e] = (T)0.f;
         }
+#pragma unroll 1
+        for (int64_t i = t0 * MS + tid; i < t1 * MS; i += kThreads) {
+            const int64_t t = i / MS;
+            const int m = i % MS;
+            if (m >= mcols) continue;
+            if (a.pv) pv[t * a.M + m] = 0.f;
+            else row<T>(a.gv, n, h, t)[m0 + m] = (T)0.f;
+        }
+        if (!a.sum_decay)
+            for (int64_t t = t0 + tid; t < t1; t += kThreads) a.gdecay[(((int64_t)slice * a.N + n) * a.H + h) * a.L + t] = 0.f;
+    }
+    if (a.sum_decay && grades_decay) {
+        all = over_groups(over_sixteen(all));
+        if (lane == 0) a.gdecay[(head * a.slices + slice) * a.segments + seg] = all;
+    }
+}
+
+template <typename T, int NE, int NW, int MW, bool WHOLE>
+__global__ __launch_bounds__((DsumBackward<T, NE, NW, MW>::kThreads), (DsumBackward<T, NE, NW, MW>::kWaves)) void k_dsum_bwd(const DsumWalk a) {
+    using F = DsumBackward<T, NE, NW, MW>;
+    __shared__ typename F::Shared sh;
+    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid / 64);
+    if constexpr (F::kBoth) {
+        dsum_walk_back<true, true, T, NE, NW, MW, WHOLE>(a, sh, wave, tid);
     } else {
-        for (int64_t t = t0 + tid; t < t1; t += 64 * NW) a.gdecay[(((int64_t)slice * a.N + n) * a.H + h) * a.L + t] = 0.f;
+        if (wave < F::KW) dsum_walk_back<true, false, T, NE, NW, MW, WHOLE>(a, sh, wave, tid);
+        else dsum_walk_back<false, true, T, NE, NW, MW, WHOLE>(a, sh, wave - F::KW, tid);
     }
 }
 
@@ -864,32 +930,34 @@ enum { kDsumForward, kDsumForwardEnds, kDsumBackward, kDsumBackwardEnds };
 template <typename T>
 int dsum_launch(int which, const DsumWalk *a, int Ep, int MS, unsigned blocks, hipStream_t s);
 
-template <typename T, int NE, int NW, int MW>
+template <typename T, int NE, int NW, int MW, bool WHOLE>
 int dsum_launch_one(int which, const DsumWalk *a, unsigned blocks, hipStream_t s) {
     using F = DsumForward<T, NE, NW, MW>;
     using B = DsumBackward<T, NE, NW, MW>;
     const dim3 grid(blocks), block(64 * NW);
     switch (which) {
         case kDsumForward:
-            if (a) k_dsum_fwd<T, NE, NW, MW, false><<<grid, block, 0, s>>>(*a);
+            if (a) k_dsum_fwd<T, NE, NW, MW, WHOLE, false><<<grid, block, 0, s>>>(*a);
             return resident(sizeof(typename F::Shared), F::kWaves, NW);
         case kDsumForwardEnds:
-            if (a) k_dsum_fwd<T, NE, NW, MW, true><<<grid, block, 0, s>>>(*a);
+            if (a) k_dsum_fwd<T, NE, NW, MW, WHOLE, true><<<grid, block, 0, s>>>(*a);
             return resident(sizeof(typename F::Ends), F::kEndWaves, NW);
         case kDsumBackward:
-            if (a) k_dsum_bwd<T, NE, NW, MW><<<grid, block, 0, s>>>(*a);
-            return resident(sizeof(typename B::Shared), B::kWaves, NW);
+            if (a) k_dsum_bwd<T, NE, NW, MW, WHOLE><<<grid, dim3(B::kThreads), 0, s>>>(*a);
+            return resident(sizeof(typename B::Shared), B::kWaves, B::kCount);
         default:
-            if (a) k_dsum_bwd_ends<T, NE, NW, MW><<<grid, block, 0, s>>>(*a);
+            if (a) k_dsum_bwd_ends<T, NE, NW, MW, WHOLE><<<grid, block, 0, s>>>(*a);
             return resident(sizeof(typename B::Ends), B::kEndWaves, NW);
     }
 }
 
 template <typename T, int NE>
 int dsum_launch_keys(int which, const DsumWalk *a, int MS, unsigned blocks, hipStream_t s) {
-    if (MS == 32) return dsum_launch_one<T, NE, 2, 1>(which, a, blocks, s);
-    if (MS == 64) return dsum_launch_one<T, NE, 4, 1>(which, a, blocks, s);
-    if (MS == 128) return dsum_launch_one<T, NE, 8, 1>(which, a, blocks, s);
+    // all rows as wide as their tiles: nothing to cut off, and half the code
+    const bool whole = a && a->E == 16 * NE && a->M % MS == 0;
+    if (MS == 32) return whole ? dsum_launch_one<T, NE, 2, 1, true>(which, a, blocks, s) : dsum_launch_one<T, NE, 2, 1, false>(which, a, blocks, s);
+    if (MS == 64) return whole ? dsum_launch_one<T, NE, 4, 1, true>(which, a, blocks, s) : dsum_launch_one<T, NE, 4, 1, false>(which, a, blocks, s);
+    if (MS == 128) return whole ? dsum_launch_one<T, NE, 8, 1, true>(which, a, blocks, s) : dsum_launch_one<T, NE, 8, 1, false>(which, a, blocks, s);
     return 0;
 }
 

@@ -110,13 +110,23 @@ __device__ __forceinline__ v4f product(const Frag<PA> &a, const Frag<PB> &b, v4f
 // Row (or column) a of the j-th of `tiles` results that lie side by side: four consecutive numbers a lane, 4 * tiles in a row of them.
 __device__ __forceinline__ constexpr int place(int tiles, int a, int j) { return 4 * tiles * (a / 4) + 4 * j + a % 4; }
 
-// R rows of W elements as P parts; rows are 16 bytes longer than their elements, which spreads 16 rows over the banks.
+// R rows of W elements as P parts.  The 16-byte runs of a row lie in an order of its own: run q of row r is at q ^ key(r), so that every access below meets all banks evenly:
+// the same run of 16 rows, one run after another of a row, and four neighbouring runs of rows 4 i .. 4 i + 3.
 template <int R, int W, int P>
 struct alignas(16) Tile {
-    static constexpr int kStride = W + 8, kPart = R * kStride;
+    static_assert(W == 32 || W == 64 || W == 128, "row lengths that key() spreads");
+    static constexpr int kPart = R * W;
     __bf16 x[P * kPart];
 
-    __device__ __forceinline__ void put(int p, int r, int col, const v8b &v) { *reinterpret_cast<v8b *>(&x[p * kPart + r * kStride + col]) = v; }
+    // rows that share their banks' place (W / 32 of four, two or one) differ here, rows 4 i .. 4 i + 3 by whole groups of four runs
+    static __device__ __forceinline__ int key(int r) {
+        if constexpr (W == 32) return r / 4 % 4;
+        else if constexpr (W == 64) return r / 2 % 2 * 4 + r / 4 % 2 + r / 8 % 2 * 2;
+        else return r % 4 * 4 + r / 4 % 4;
+    }
+    static __device__ __forceinline__ int place_of(int r, int col) { return r * W + (((col >> 3) ^ key(r)) << 3) + (col & 7); }
+
+    __device__ __forceinline__ void put(int p, int r, int col, const v8b &v) { *reinterpret_cast<v8b *>(&x[p * kPart + place_of(r, col)]) = v; }
     __device__ __forceinline__ void put(int r, int col, const float (&f)[8]) {
         const Frag<P> s = split8<P>(f);
 #pragma unroll
@@ -126,27 +136,29 @@ struct alignas(16) Tile {
         v4b s[P];
         split<P, 4>(f, s);
 #pragma unroll
-        for (int p = 0; p < P; p++) *reinterpret_cast<v4b *>(&x[p * kPart + r * kStride + col]) = s[p];
+        for (int p = 0; p < P; p++) *reinterpret_cast<v4b *>(&x[p * kPart + place_of(r, col)]) = s[p];
     }
 
-    // rows r0 .. r0 + 15 against columns k0 .. k0 + 31 as they lie
+    // rows r0 .. r0 + 15 against columns k0 .. k0 + 31 as they lie; r0 is a multiple of 16, k0 of 32
     __device__ __forceinline__ Frag<P> rows(int r0, int k0, int g, int c) const {
+        const int at = c * W + (((g ^ key(c)) << 3) ^ k0) + r0 * W;
         Frag<P> f;
 #pragma unroll
-        for (int p = 0; p < P; p++) f.p[p] = *reinterpret_cast<const v8b *>(&x[p * kPart + (r0 + c) * kStride + k0 + 8 * g]);
+        for (int p = 0; p < P; p++) f.p[p] = *reinterpret_cast<const v8b *>(&x[p * kPart + at]);
         return f;
     }
-    // columns c0 + place(tiles, c, j) against rows k0 .. k0 + 31.  ds_read_b64_tr_b16: each lane names four elements, the 16 lanes of a group four
-    // rows of 16, and lane c of the group gets the four rows' c-th.
+    // columns c0 + place(TILES, c, j) against rows k0 .. k0 + 31; c0 is a multiple of 16 TILES, k0 of 32.  ds_read_b64_tr_b16: each lane names four elements, the 16 lanes of
+    // a group four rows of 16, and lane c of the group gets the four rows' c-th.
     template <int TILES>
     __device__ __forceinline__ Frag<P> columns(int c0, int j, int k0, int g, int c) const {
         typedef __attribute__((address_space(3))) v4h *lds4;
+        const int r = 8 * g + c / 4, col = 4 * TILES * (c % 4) + 4 * j;
+        const int lo = r * W + ((((col >> 3) ^ key(r)) << 3) ^ c0) + (col & 7) + k0 * W, hi = lo + 4 * W + ((((col >> 3) ^ key(r + 4)) << 3) ^ c0) - ((((col >> 3) ^ key(r)) << 3) ^ c0);
         Frag<P> f;
 #pragma unroll
         for (int p = 0; p < P; p++) {
-            const __bf16 *at = &x[p * kPart + (k0 + 8 * g + c / 4) * kStride + c0 + 4 * TILES * (c % 4) + 4 * j];
-            const v4h lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)at), hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(at + 4 * kStride));
-            const v4b l = __builtin_bit_cast(v4b, lo), h = __builtin_bit_cast(v4b, hi);
+            const v4h a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)&x[p * kPart + lo]), b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)&x[p * kPart + hi]);
+            const v4b l = __builtin_bit_cast(v4b, a), h = __builtin_bit_cast(v4b, b);
             f.p[p] = v8b{l[0], l[1], l[2], l[3], h[0], h[1], h[2], h[3]};
         }
         return f;
@@ -156,7 +168,7 @@ struct alignas(16) Tile {
         v4f s = {0, 0, 0, 0};
 #pragma unroll
         for (int p = P - 1; p >= 0; p--) {
-            const v4b v = *reinterpret_cast<const v4b *>(&x[p * kPart + r * kStride + col]);
+            const v4b v = *reinterpret_cast<const v4b *>(&x[p * kPart + place_of(r, col)]);
 #pragma unroll
             for (int i = 0; i < 4; i++) s[i] += (float)v[i];
         }
@@ -199,7 +211,7 @@ __device__ __forceinline__ T *from(T *base, uint32_t i) {
 // `rows` on and columns from `cols` on are not read and become zero; at least one row is there.  Every lane loads 16 bytes at an element's address (the
 // hardware takes any), those beyond the block's rows the last row, those beyond its columns the last eight: a branch around a load would wait for
 // it at its end, and there would be no loads ahead.  put() zeroes and shifts what was read from elsewhere.
-template <typename T, int R, int W, int THREADS>
+template <typename T, int R, int W, int THREADS, bool WHOLE>
 struct Stage {
     typedef uint32_t v4u __attribute__((ext_vector_type(4)));
     static constexpr int kRow = W / 8, kVecs = R * kRow, kPer = (kVecs + THREADS - 1) / THREADS, kRegs = sizeof(T) / 2;
@@ -216,7 +228,9 @@ struct Stage {
 #pragma unroll
         for (int i = 0; i < kPer; i++) {
             const int v = tid + i * THREADS, r = min(v / kRow, rows - 1), col = v % kRow * 8;
-            if (cols >= 8) {
+            if (WHOLE) {
+                x[i] = reinterpret_cast<const Anywhere *>(from(base, (uint32_t)r * (uint32_t)stride + (uint32_t)col))->e;
+            } else if (cols >= 8) {
                 x[i] = reinterpret_cast<const Anywhere *>(from(base, (uint32_t)r * (uint32_t)stride + (uint32_t)min(col, cols - 8)))->e;
             } else {
                 struct { T e[8]; } few;
@@ -232,9 +246,9 @@ struct Stage {
         for (int i = 0; i < kPer; i++) {
             const int v = tid + i * THREADS, r = v / kRow, col = v % kRow * 8;
             if (kVecs % THREADS && v >= kVecs) continue;
-            const bool some = r < rows && col < cols;
+            const bool some = r < rows && (WHOLE || col < cols);
             if constexpr (P == 1)
-                if (cols % 8 == 0) {
+                if (WHOLE || cols % 8 == 0) {
                     t.put(0, r, col, __builtin_bit_cast(v8b, some ? x[i].x[0] : v4u{0, 0, 0, 0}));
                     continue;
                 }
@@ -243,7 +257,7 @@ struct Stage {
             float f[8];
 #pragma unroll
             for (int e = 0; e < 8; e++) f[e] = some ? (float)few.e[e] : 0.f;
-            if (cols % 8) {
+            if (!WHOLE && cols % 8) {
                 if (cols >= 8) {      // the last run of a row holds its last eight elements
                     const int late = max(0, col - (cols - 8));
 #pragma unroll
