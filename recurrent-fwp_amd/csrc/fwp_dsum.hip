@@ -8,36 +8,39 @@ namespace fwp {
 namespace {
 
 // What the segments leave, joined in order: every segment's first state from the one before it.  Slot s of `ends` holds what segment s - 1 leaves when it
-// starts from zero, and then the state that segment s starts from; BACKWARD: of segment s + 1, from the last to the first.  One thread a number of the state;
-// the slots of eight segments are loaded at once.
-template <bool BACKWARD>
-__global__ __launch_bounds__(256) void k_dsum_join(float *ends, const float *factors, const float *from, int E, int M, int Ep, int Mp, int segments) {
-    const int cells = Ep * Mp, blocks = cells / 256, cell = blockIdx.x % blocks * 256 + threadIdx.x;      // at least 32 x 32 of them
+// starts from zero, and then the state that segment s starts from; BACKWARD: of segment s + 1, from the last to the first.  One thread a number of the state, so that
+// the chain of a long prompt's 80 segments is 80 additions long; the slots of kAhead segments are loaded at once (8 heads of 64 x 64, 86 segments: 7 us).
+template <bool BACKWARD, int kAhead>
+__global__ __launch_bounds__(64) void k_dsum_join(float *ends, const float *factors, const float *from, int E, int M, int Ep, int Mp, int segments) {
+    const int cells = Ep * Mp, blocks = cells / 64, cell = blockIdx.x % blocks * 64 + threadIdx.x;      // at least 32 x 32 of them
     const int64_t head = blockIdx.x / blocks;
     float *at = ends + head * segments * cells + cell;
     const float *f = factors + head * segments;
+    const auto slot_of = [&](int s) { return BACKWARD ? segments - 1 - s : s; };
     float cur = 0.f;
     if (!BACKWARD && from) {
         const int e = cell / Mp, m = cell % Mp;
         if (e < E && m < M) cur = from[(head * E + e) * M + m];
     }
-    at[(int64_t)(BACKWARD ? segments - 1 : 0) * cells] = cur;
-    for (int s0 = 1; s0 < segments; s0 += 8) {
-        float x[8], y[8];
+    float x[kAhead], y[kAhead];
+    const auto load = [&](int s0) {
 #pragma unroll
-        for (int i = 0; i < 8; i++)
-            if (s0 + i < segments) {
-                const int slot = BACKWARD ? segments - 1 - (s0 + i) : s0 + i;
-                x[i] = at[(int64_t)slot * cells];
-                y[i] = f[BACKWARD ? slot + 1 : slot - 1];
-            }
+        for (int i = 0; i < kAhead; i++) {
+            const int slot = slot_of(min(s0 + i, segments - 1));
+            x[i] = at[(int64_t)slot * cells];
+            y[i] = f[BACKWARD ? slot + 1 : slot - 1];
+        }
+    };
+    load(1);
+    at[(int64_t)slot_of(0) * cells] = cur;
+    for (int s0 = 1; s0 < segments; s0 += kAhead) {
+        float z[kAhead];
 #pragma unroll
-        for (int i = 0; i < 8; i++)
-            if (s0 + i < segments) {
-                const int slot = BACKWARD ? segments - 1 - (s0 + i) : s0 + i;
-                cur = fmaf(y[i], cur, x[i]);
-                at[(int64_t)slot * cells] = cur;
-            }
+        for (int i = 0; i < kAhead; i++) z[i] = cur = fmaf(y[i], cur, x[i]);
+        if (s0 + kAhead < segments) load(s0 + kAhead);
+#pragma unroll
+        for (int i = 0; i < kAhead; i++)
+            if (s0 + i < segments) at[(int64_t)slot_of(s0 + i) * cells] = z[i];
     }
 }
 
@@ -101,7 +104,7 @@ __global__ __launch_bounds__(256) void k_dsum_step(const DsumWalk a, int X, int 
                 if (m + i < a.M) out[m + i] = (T)0.f;
         return;
     }
-    struct __attribute__((packed, aligned(4))) Four { float x[4]; };
+    typedef float Quad __attribute__((ext_vector_type(4), aligned(4)));
     const float *from = a.from ? a.from + ((int64_t)n * a.H + h) * a.E * a.M : nullptr;
     const bool whole = m + 4 <= a.M;
     float S[R][4], kv[R], qv[R], vv[4], o[4] = {0.f, 0.f, 0.f, 0.f};
@@ -110,9 +113,9 @@ __global__ __launch_bounds__(256) void k_dsum_step(const DsumWalk a, int X, int 
         const int e = y + r * Y;
         kv[r] = e < a.E ? (float)k[e] : 0.f, qv[r] = e < a.E ? (float)q[e] : 0.f;
         if (from && e < a.E && whole) {
-            const Four s = *reinterpret_cast<const Four *>(from + (int64_t)e * a.M + m);
+            const Quad s = __builtin_nontemporal_load(reinterpret_cast<const Quad *>(from + (int64_t)e * a.M + m));
 #pragma unroll
-            for (int i = 0; i < 4; i++) S[r][i] = s.x[i];
+            for (int i = 0; i < 4; i++) S[r][i] = s[i];
         } else {
 #pragma unroll
             for (int i = 0; i < 4; i++) S[r][i] = from && e < a.E && m + i < a.M ? from[(int64_t)e * a.M + m + i] : 0.f;
@@ -124,18 +127,18 @@ __global__ __launch_bounds__(256) void k_dsum_step(const DsumWalk a, int X, int 
 #pragma unroll
     for (int r = 0; r < R; r++) {
         const int e = y + r * Y;
-        Four s;
+        Quad s;
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-            s.x[i] = fmaf(kv[r], vv[i], decay * S[r][i]);
-            if (e < a.E) o[i] = fmaf(qv[r], s.x[i], o[i]);
+            s[i] = fmaf(kv[r], vv[i], decay * S[r][i]);
+            if (e < a.E) o[i] = fmaf(qv[r], s[i], o[i]);
         }
         if (!a.to || e >= a.E) continue;
         float *to = a.to + (((int64_t)n * a.H + h) * a.E + e) * a.M + m;
-        if (whole) *reinterpret_cast<Four *>(to) = s;
+        if (whole) __builtin_nontemporal_store(s, reinterpret_cast<Quad *>(to));
         else
             for (int i = 0; i < 4; i++)
-                if (m + i < a.M) to[i] = s.x[i];
+                if (m + i < a.M) to[i] = s[i];
     }
 #pragma unroll
     for (int i = 0; i < 4; i++)
@@ -148,6 +151,13 @@ __global__ __launch_bounds__(256) void k_dsum_step(const DsumWalk a, int X, int 
     __syncthreads();
     if (tid < 4 * X && block * X * 4 + tid < a.M)
         store(out + block * X * 4 + tid, a.scale * ((part[0][tid] + part[1][tid]) + (part[2][tid] + part[3][tid])));
+}
+
+template <bool BACKWARD>
+void join(const DsumWalk &w, const float *from, int64_t heads, int Ep, hipStream_t s) {
+    const unsigned blocks = (unsigned)(heads * (Ep * w.Mp / 64));
+    if (w.segments > 9) k_dsum_join<BACKWARD, 16><<<blocks, 64, 0, s>>>(w.ends, w.factors, from, w.E, w.M, Ep, w.Mp, w.segments);
+    else k_dsum_join<BACKWARD, 4><<<blocks, 64, 0, s>>>(w.ends, w.factors, from, w.E, w.M, Ep, w.Mp, w.segments);
 }
 
 struct Plan {
@@ -222,7 +232,7 @@ DsumWalk walk_of(const fwp_dsum_args &a, const Plan &p) {
 
 int launch(int which, const fwp_dsum_args &a, const Plan &p, const DsumWalk &w, int segments, hipStream_t s) {
     const int64_t blocks = p.heads * p.slices * segments;
-    if (!fits_launch(blocks, 512) || !fits_launch(p.heads * (p.cells / 256), 256)) return FWP_E_SHAPE;
+    if (!fits_launch(blocks, 512) || !fits_launch(p.heads * (p.cells / 64), 64)) return FWP_E_SHAPE;
     bool done = false;
     by_type(a.type, [&](auto t) { done = dsum_launch<decltype(t)>(which, &w, p.Ep, p.MS, (unsigned)blocks, s) > 0; });
     return done ? 0 : FWP_E_SHAPE;
@@ -273,7 +283,7 @@ int dsum_fwd(const fwp_dsum_args &a, float *W, fwp_out_rows out, float *saved, f
         w.ends = workspace;
         w.factors = workspace + p.heads * p.segments * p.cells;
         if (int rc = launch(kDsumForwardEnds, a, p, w, p.segments - 1, s)) return rc;
-        k_dsum_join<false><<<(unsigned)(p.heads * (p.cells / 256)), 256, 0, s>>>(w.ends, w.factors, W, a.E, a.M, p.Ep, p.Mp, p.segments);
+        join<false>(w, W, p.heads, p.Ep, s);
     }
     if (int rc = launch(kDsumForward, a, p, w, p.segments, s)) return rc;
     return (int)hipGetLastError();
@@ -300,7 +310,7 @@ int dsum_bwd(const fwp_dsum_args &a, const float *saved, fwp_rows gout, fwp_out_
     w.gdecay = parts ? parts : gdecay;
     if (p.segments > 1) {
         if (int rc = launch(kDsumBackwardEnds, a, p, w, p.segments - 1, s)) return rc;
-        k_dsum_join<true><<<(unsigned)(p.heads * (p.cells / 256)), 256, 0, s>>>(w.ends, w.factors, nullptr, a.E, a.M, p.Ep, p.Mp, p.segments);
+        join<true>(w, nullptr, p.heads, p.Ep, s);
     }
     if (int rc = launch(kDsumBackward, a, p, w, p.segments, s)) return rc;
     by_type(a.type, [&](auto t) {

@@ -104,6 +104,17 @@ struct alignas(16) Decays {
     }
 };
 
+// A fragment times the steps' factors, split again
+template <int Q, int P>
+__device__ __forceinline__ Frag<Q> scaled(const Frag<P> &f, const float *factors, int sb, int g) {
+    const v4f r0 = *reinterpret_cast<const v4f *>(&factors[32 * sb + 8 * g]), r1 = *reinterpret_cast<const v4f *>(&factors[32 * sb + 8 * g + 4]);
+    float x[8];
+    join8(f, x);
+#pragma unroll
+    for (int i = 0; i < 4; i++) x[i] *= r0[i], x[i + 4] *= r1[i];
+    return split8<Q>(x);
+}
+
 // Sums over the four groups of 16 lanes, and over the lanes of a group, in every lane
 __device__ __forceinline__ float over_groups(float x) {
     float y = x;
@@ -119,48 +130,89 @@ __device__ __forceinline__ float over_sixteen(float x) {
     return x + dpp<kRowRor8>(x);
 }
 
-// A number that is the same all along, but not to the compiler: what follows from it is worked out where it is needed, instead of being kept in scalar registers that run out.
+// A number as it is, but one the compiler knows nothing of: what follows from it is worked out where it is needed, instead of being kept in scalar registers that
+// run out, or turned into addresses of their own for every row, which take vector registers and are advanced from chunk to chunk.
 __device__ __forceinline__ int opaque(int x) {
     asm volatile("" : "+s"(x));
     return x;
 }
 
-// W consecutive numbers of a row, in stores of up to 16 bytes at an element's address
+// W consecutive numbers of a row from element `at` of `base` on, in stores of up to 16 bytes at an element's address
 template <typename T, int W>
-__device__ __forceinline__ void store_whole(T *at, const float (&x)[W]) {
+__device__ __forceinline__ void store_whole(T *base, uint32_t at, const float (&x)[W]) {
     constexpr int kWords = sizeof(T) * W / 4, kStep = kWords < 4 ? kWords : 4;
     typedef uint32_t Words __attribute__((ext_vector_type(kStep)));
     struct __attribute__((packed, aligned(sizeof(T)))) Anywhere { Words w; };
-    struct Row { T x[W]; } row;
     struct Split { Words w[kWords / kStep]; };
+    Split split;
+    if constexpr (std::is_same_v<T, bf16_t>) {
+        struct { uint32_t w[kWords]; } words;
 #pragma unroll
-    for (int i = 0; i < W; i++) row.x[i] = (T)x[i];
-    const Split split = __builtin_bit_cast(Split, row);
+        for (int i = 0; i < kWords; i++) {
+            float a = x[2 * i], b = x[2 * i + 1];
+            words.w[i] = next_parts(a, b, true);
+        }
+        split = __builtin_bit_cast(Split, words);
+    } else {
+        struct { T x[W]; } row;
 #pragma unroll
-    for (int i = 0; i < kWords / kStep; i++) reinterpret_cast<Anywhere *>(at)[i].w = split.w[i];
+        for (int i = 0; i < W; i++) row.x[i] = (T)x[i];
+        split = __builtin_bit_cast(Split, row);
+    }
+    asm volatile("" : "+v"(at));      // made here, or the compiler keeps 64 bits of it for every row
+    Anywhere *to = reinterpret_cast<Anywhere *>(from(base, at));
+#pragma unroll
+    for (int i = 0; i < kWords / kStep; i++) to[i].w = split.w[i];
 }
 // A chunk's results, columns col .. of rows 16 I + c.  base: its first row, the same for all lanes; C rows lie within 32 bits of bytes.  live: the chunk's rows that
 // count, the others become zero; there: those that are there at all.  cols: this lane's columns that are there, of 4 J (all where WHOLE).
 template <bool WHOLE, typename T, int C, int J>
 __device__ __forceinline__ void store_rows(T *base, int stride, int col, const v4f (&acc)[C / 16][J], float scale, int live, int there, int cols, int c) {
-#pragma unroll
-    for (int I = 0; I < C / 16; I++) {
-        float x[4 * J];
+    const auto result = [&](int I, float (&x)[4 * J]) {
 #pragma unroll
         for (int j = 0; j < J; j++)
 #pragma unroll
-            for (int i = 0; i < 4; i++) x[4 * j + i] = 16 * I + c < live ? acc[I][j][i] * scale : 0.f;
-        T *to = from(base, (uint32_t)(16 * I + c) * (uint32_t)stride + (uint32_t)col);
+            for (int i = 0; i < 4; i++) x[4 * j + i] = acc[I][j][i] * scale;
+        return (uint32_t)(16 * I + c) * (uint32_t)stride + (uint32_t)col;
+    };
+    if (WHOLE && live >= C) {
+#pragma unroll
+        for (int I = 0; I < C / 16; I++) {
+            float x[4 * J];
+            const uint32_t at = result(I, x);
+            store_whole<T, 4 * J>(base, at, x);
+        }
+        return;
+    }
+#pragma unroll
+    for (int I = 0; I < C / 16; I++) {
+        float x[4 * J];
+        const uint32_t at = result(I, x);
         if (16 * I + c >= there) continue;
+#pragma unroll
+        for (int i = 0; i < 4 * J; i++) x[i] = 16 * I + c < live ? x[i] : 0.f;
         if (WHOLE || cols >= 4 * J) {
-            store_whole<T, 4 * J>(to, x);
+            store_whole<T, 4 * J>(base, at, x);
         } else {
+            T *to = from(base, at);
 #pragma unroll
             for (int i = 0; i < 4 * J; i++)
                 if (i < cols) to[i] = (T)x[i];
         }
     }
 }
+
+// The i-th of the pairs of a block of 32 steps s and a tile I of 16 steps t that meet on or below the diagonal: LOWER, t behind s (I >= 2 sb); else s in front of t (I < 2 sb + 2).
+template <int TT, bool LOWER>
+struct Pairs {
+    static constexpr int SB = TT / 2, kCount = SB * (SB + 1);
+    int sb, I;
+    __device__ __forceinline__ constexpr explicit Pairs(int i) : sb(0), I(0) {
+        int n = LOWER ? TT : 2;
+        while (i >= n) i -= n, sb++, n += LOWER ? -2 : 2;
+        I = LOWER ? 2 * sb + i : i;
+    }
+};
 
 // Workgroups of a kernel that a CU holds at once: 160 KB of LDS, and registers for `waves` on each of four SIMDs, which the kernel's launch bounds ask for
 constexpr int resident(size_t lds, int waves, int NW) { return (int)(160 * 1024 / lds) < 4 * waves / NW ? (int)(160 * 1024 / lds) : 4 * waves / NW; }
@@ -227,7 +279,8 @@ __global__ __launch_bounds__(64 * NW, (ENDS ? DsumForward<T, NE, NW, MW>::kEndWa
 #pragma unroll
                     for (int i = 0; i < 4; i++) {
                         const int e = 32 * b + 8 * g + 4 * u + i, m = m0 + mw + place(MW, c, j);
-                        S[b][u][j][i] = from && e < rows && m < cols ? from[e * stride + m] : 0.f;
+                        // arrived, as everything that is loaded ahead of the loop: a wait that its first round needs would be one of all rounds
+                        S[b][u][j][i] = pinned(from && e < rows && m < cols ? from[e * stride + m] : 0.f);
                     }
     }
     if constexpr (!ENDS) {      // tiles of P above the diagonal stay zero
@@ -239,7 +292,7 @@ __global__ __launch_bounds__(64 * NW, (ENDS ? DsumForward<T, NE, NW, MW>::kEndWa
     double total = 0;
     float gnext = 0;
     const auto fetch = [&](int chunk) {
-        const int64_t t0 = (int64_t)chunk * C;
+        const int64_t t0 = (int64_t)opaque(chunk) * C;
         const int rows = len - (int)t0;
         if constexpr (!ENDS) sq.load(qb + t0 * a.q.sL, (int)a.q.sL, rows, a.E, tid);
         sk.load(kb + t0 * a.k.sL, (int)a.k.sL, rows, a.E, tid);
@@ -255,6 +308,8 @@ __global__ __launch_bounds__(64 * NW, (ENDS ? DsumForward<T, NE, NW, MW>::kEndWa
             sum_decay(first);
             if (first + 1 < stop) fetch_decay(first + 1);
         }
+        if constexpr (!ENDS) sq.arrive();
+        sk.arrive(), sv.arrive();
     }
     for (int chunk = first; chunk < stop; chunk++) {
         const int rows = len - chunk * C, keys = opaque(a.E), values = opaque(mcols);
@@ -272,7 +327,7 @@ __global__ __launch_bounds__(64 * NW, (ENDS ? DsumForward<T, NE, NW, MW>::kEndWa
         v4f acc[TT][MW];
         if constexpr (!ENDS) {
             if (a.saved) {
-                float *at = a.saved + (head * chunks + chunk) * E * a.Mp + m0;
+                float *at = a.saved + (head * chunks + opaque(chunk)) * E * a.Mp + m0;
 #pragma unroll
                 for (int b = 0; b < NB; b++)
 #pragma unroll
@@ -286,9 +341,12 @@ __global__ __launch_bounds__(64 * NW, (ENDS ? DsumForward<T, NE, NW, MW>::kEndWa
             for (int tile = wave; tile < TT * (TT + 1) / 2; tile += NW) {
                 int I = 0, J = tile;
                 while (J > I) J -= ++I;
+                struct Frags {
+                    Frag<P> a, b;
+                };
                 v4f p = {0, 0, 0, 0};
-#pragma unroll
-                for (int b = 0; b < NB; b++) p = product<O>(sh.k.rows(16 * J, 32 * b, g, c), sh.q.rows(16 * I, 32 * b, g, c), p);
+                ahead<NB, kAhead<P>>([&](int b) { return Frags{sh.k.rows(16 * J, 32 * b, g, c), sh.q.rows(16 * I, 32 * b, g, c)}; },
+                                     [&](int, const Frags &f) { p = product<O>(f.a, f.b, p); });
                 const int t = 16 * I + c, s = 16 * J + 4 * g;
                 const v4f f = d.between(t, s);
                 float x[4];
@@ -301,18 +359,16 @@ __global__ __launch_bounds__(64 * NW, (ENDS ? DsumForward<T, NE, NW, MW>::kEndWa
             for (int I = 0; I < TT; I++)
 #pragma unroll
                 for (int j = 0; j < MW; j++) acc[I][j] = v4f{0, 0, 0, 0};
+            Frag<O> state[MW];
+            ahead<NB * TT, kAhead<P>>([&](int i) { return sh.q.rows(16 * (i % TT), 32 * (i / TT), g, c); },
+                                      [&](int i, const Frag<P> &q) {
+                                          const int b = i / TT, I = i % TT;
 #pragma unroll
-            for (int b = 0; b < NB; b++) {
-                Frag<O> s[MW];
-#pragma unroll
-                for (int j = 0; j < MW; j++) s[j] = split8<O>(S[b][0][j], S[b][1][j]);
-#pragma unroll
-                for (int I = 0; I < TT; I++) {
-                    const Frag<P> q = sh.q.rows(16 * I, 32 * b, g, c);
-#pragma unroll
-                    for (int j = 0; j < MW; j++) acc[I][j] = product<O>(s[j], q, acc[I][j]);
-                }
-            }
+                                          for (int j = 0; j < MW; j++) {
+                                              if (I == 0) state[j] = split8<O>(S[b][0][j], S[b][1][j]);
+                                              acc[I][j] = product<O>(state[j], q, acc[I][j]);
+                                          }
+                                      });
 #pragma unroll
             for (int I = 0; I < TT; I++) {
                 const float f = d.into[16 * I + c];
@@ -327,35 +383,34 @@ __global__ __launch_bounds__(64 * NW, (ENDS ? DsumForward<T, NE, NW, MW>::kEndWa
             for (int u = 0; u < 2; u++)
 #pragma unroll
                 for (int j = 0; j < MW; j++) S[b][u][j] *= d.whole;
+        Frag<P> v[SB][MW];
 #pragma unroll
-        for (int sb = 0; sb < SB; sb++) {
-            Frag<X> vs[MW];
-            const v4f r0 = *reinterpret_cast<const v4f *>(&d.rest[32 * sb + 8 * g]), r1 = *reinterpret_cast<const v4f *>(&d.rest[32 * sb + 8 * g + 4]);
+        for (int sb = 0; sb < SB; sb++)
 #pragma unroll
-            for (int j = 0; j < MW; j++) {
-                const Frag<P> v = sh.v.template columns<MW>(mw, j, 32 * sb, g, c);
-                if constexpr (!ENDS) {
-#pragma unroll
-                    for (int I = 2 * sb; I < TT; I++) acc[I][j] = product<O>(v, sh.p.rows(16 * I, 32 * sb, g, c), acc[I][j]);
-                }
-                float x[8];
-                join8(v, x);
-#pragma unroll
-                for (int i = 0; i < 4; i++) x[i] *= r0[i], x[i + 4] *= r1[i];
-                vs[j] = split8<X>(x);
-            }
-#pragma unroll
-            for (int b = 0; b < NB; b++)
-#pragma unroll
-                for (int u = 0; u < 2; u++) {
-                    const Frag<P> k = sh.k.template columns<2>(32 * b, u, 32 * sb, g, c);
-#pragma unroll
-                    for (int j = 0; j < MW; j++) S[b][u][j] = product<X>(k, vs[j], S[b][u][j]);
-                }
-        }
+            for (int j = 0; j < MW; j++) v[sb][j] = sh.v.template columns<MW>(mw, j, 32 * sb, g, c);
         if constexpr (!ENDS) {
+            using Below = Pairs<TT, true>;
+            ahead<Below::kCount, kAhead<O>>([&](int i) { return sh.p.rows(16 * Below(i).I, 32 * Below(i).sb, g, c); },
+                                            [&](int i, const Frag<O> &p) {
+#pragma unroll
+                                                for (int j = 0; j < MW; j++) acc[Below(i).I][j] = product<O>(v[Below(i).sb][j], p, acc[Below(i).I][j]);
+                                            });
+        }
+        Frag<X> vs[MW];
+        ahead<SB * NB * 2, kAhead<P>>([&](int i) { return sh.k.template columns<2>(32 * (i / 2 % NB), i % 2, 32 * (i / 2 / NB), g, c); },
+                                      [&](int i, const Frag<P> &k) {
+                                          const int sb = i / 2 / NB, b = i / 2 % NB, u = i % 2;
+#pragma unroll
+                                          for (int j = 0; j < MW; j++) {
+                                              if (b == 0 && u == 0) vs[j] = scaled<X>(v[sb][j], d.rest, sb, g);
+                                              S[b][u][j] = product<X>(k, vs[j], S[b][u][j]);
+                                          }
+                                      });
+        if constexpr (!ENDS) {
+            sq.arrive(), sk.arrive(), sv.arrive();
+            gnext = pinned(gnext);
             const int col = mw + 4 * MW * g;
-            store_rows<WHOLE, T, C, MW>(ob + (int64_t)chunk * C * a.out.sL, (int)a.out.sL, col, acc, a.scale, rows, a.L - chunk * C, values - col, c);
+            store_rows<WHOLE, T, C, MW>(ob + (int64_t)opaque(chunk) * C * a.out.sL, (int)a.out.sL, col, acc, a.scale, rows, a.L - chunk * C, values - col, c);
         }
         lds_barrier();
     }
@@ -453,7 +508,7 @@ __global__ __launch_bounds__(64 * NW, (DsumBackward<T, NE, NW, MW>::kEndWaves)) 
     double total = 0;
     float gnext = 0;
     const auto fetch = [&](int chunk) {
-        const int64_t t0 = (int64_t)chunk * C;
+        const int64_t t0 = (int64_t)opaque(chunk) * C;
         const int rows = len - (int)t0;
         sq.load(qb + t0 * a.q.sL, (int)a.q.sL, rows, a.E, tid);
         sd.load(db + t0 * a.go.sL, (int)a.go.sL, rows, mcols, tid);
@@ -485,27 +540,21 @@ __global__ __launch_bounds__(64 * NW, (DsumBackward<T, NE, NW, MW>::kEndWaves)) 
             for (int u = 0; u < 2; u++)
 #pragma unroll
                 for (int j = 0; j < MW; j++) G[b][u][j] *= d.whole;
+        Frag<P> go[SB][MW];
 #pragma unroll
-        for (int tb = 0; tb < SB; tb++) {
-            const v4f f0 = *reinterpret_cast<const v4f *>(&d.into[32 * tb + 8 * g]), f1 = *reinterpret_cast<const v4f *>(&d.into[32 * tb + 8 * g + 4]);
-            Frag<X> ds[MW];
+        for (int sb = 0; sb < SB; sb++)
 #pragma unroll
-            for (int j = 0; j < MW; j++) {
-                float x[8];
-                join8(sh.go.template columns<MW>(mw, j, 32 * tb, g, c), x);
+            for (int j = 0; j < MW; j++) go[sb][j] = sh.go.template columns<MW>(mw, j, 32 * sb, g, c);
+        Frag<X> ds[MW];
+        ahead<SB * NB * 2, kAhead<P>>([&](int i) { return sh.q.template columns<2>(32 * (i / 2 % NB), i % 2, 32 * (i / 2 / NB), g, c); },
+                                      [&](int i, const Frag<P> &q) {
+                                          const int sb = i / 2 / NB, b = i / 2 % NB, u = i % 2;
 #pragma unroll
-                for (int i = 0; i < 4; i++) x[i] *= f0[i], x[i + 4] *= f1[i];
-                ds[j] = split8<X>(x);
-            }
-#pragma unroll
-            for (int b = 0; b < NB; b++)
-#pragma unroll
-                for (int u = 0; u < 2; u++) {
-                    const Frag<P> q = sh.q.template columns<2>(32 * b, u, 32 * tb, g, c);
-#pragma unroll
-                    for (int j = 0; j < MW; j++) G[b][u][j] = product<X>(q, ds[j], G[b][u][j]);
-                }
-        }
+                                          for (int j = 0; j < MW; j++) {
+                                              if (b == 0 && u == 0) ds[j] = scaled<X>(go[sb][j], d.into, sb, g);
+                                              G[b][u][j] = product<X>(q, ds[j], G[b][u][j]);
+                                          }
+                                      });
         lds_barrier();
     }
     float *at = a.ends + (head * a.segments + seg - 1) * E * a.Mp + m0 + mw;
@@ -554,7 +603,7 @@ __device__ __forceinline__ void dsum_walk_back(const DsumWalk &a, typename DsumB
 #pragma unroll
                     for (int j = 0; j < EW; j++)
 #pragma unroll
-                        for (int i = 0; i < 4; i++) H[b][u][j][i] = from && keys ? from[(ew + place(EW, c, j)) * a.Mp + 32 * b + 8 * g + 4 * u + i] : 0.f;
+                        for (int i = 0; i < 4; i++) H[b][u][j][i] = pinned(from && keys ? from[(ew + place(EW, c, j)) * a.Mp + 32 * b + 8 * g + 4 * u + i] : 0.f);
         }
         if constexpr (VALUES) {
 #pragma unroll
@@ -564,7 +613,7 @@ __device__ __forceinline__ void dsum_walk_back(const DsumWalk &a, typename DsumB
 #pragma unroll
                     for (int j = 0; j < VM; j++)
 #pragma unroll
-                        for (int i = 0; i < 4; i++) G[b][u][j][i] = from && values ? from[(32 * b + 8 * g + 4 * u + i) * a.Mp + mw + place(VM, c, j)] : 0.f;
+                        for (int i = 0; i < 4; i++) G[b][u][j][i] = pinned(from && values ? from[(32 * b + 8 * g + 4 * u + i) * a.Mp + mw + place(VM, c, j)] : 0.f);
         }
     }
 #pragma unroll 1
@@ -575,7 +624,7 @@ __device__ __forceinline__ void dsum_walk_back(const DsumWalk &a, typename DsumB
     // a chunk's first state, as this key wave reads it
     float S[KEYS ? MB : 1][EW][8];
     const auto load_state = [&](int chunk) {
-        const float *base = a.saved + (head * chunks + chunk) * E * a.Mp + m0;
+        const float *base = a.saved + (head * chunks + opaque(chunk)) * E * a.Mp + m0;
 #pragma unroll
         for (int b = 0; b < MB; b++)
 #pragma unroll
@@ -584,6 +633,14 @@ __device__ __forceinline__ void dsum_walk_back(const DsumWalk &a, typename DsumB
                 const float4 lo = *reinterpret_cast<const float4 *>(at), hi = *reinterpret_cast<const float4 *>(at + 4);
                 S[b][j][0] = lo.x, S[b][j][1] = lo.y, S[b][j][2] = lo.z, S[b][j][3] = lo.w, S[b][j][4] = hi.x, S[b][j][5] = hi.y, S[b][j][6] = hi.z, S[b][j][7] = hi.w;
             }
+    };
+    const auto state_arrives = [&] {
+#pragma unroll
+        for (int b = 0; b < MB; b++)
+#pragma unroll
+            for (int j = 0; j < EW; j++)
+#pragma unroll
+                for (int i = 0; i < 8; i++) S[b][j][i] = pinned(S[b][j][i]);
     };
     // <H, S>, this wave's part
     const auto inner = [&] {
@@ -601,7 +658,7 @@ __device__ __forceinline__ void dsum_walk_back(const DsumWalk &a, typename DsumB
     Stage<T, C, MS, kThreads, WHOLE> sv, sd;
     float gnext = 0, all = 0, x_end = 0;
     const auto fetch = [&](int chunk) {
-        const int64_t t0 = (int64_t)chunk * C;
+        const int64_t t0 = (int64_t)opaque(chunk) * C;
         const int rows = len - (int)t0, wide = opaque(a.E), cols = opaque(mcols);
         sq.load(qb + t0 * a.q.sL, (int)a.q.sL, rows, wide, tid);
         sk.load(kb + t0 * a.k.sL, (int)a.k.sL, rows, wide, tid);
@@ -642,7 +699,9 @@ __device__ __forceinline__ void dsum_walk_back(const DsumWalk &a, typename DsumB
                 x_end = inner();
             }
             load_state(stop - 1);
+            state_arrives();
         }
+        sq.arrive(), sk.arrive(), sv.arrive(), sd.arrive();
     }
 
     for (int chunk = stop - 1; chunk >= first; chunk--) {
@@ -669,11 +728,18 @@ __device__ __forceinline__ void dsum_walk_back(const DsumWalk &a, typename DsumB
             for (int tile = wave; tile < TT * (TT + 1) / 2; tile += F::kTileWaves) {
                 int I = 0, J = tile;
                 while (J > I) J -= ++I;
+                struct Frags {
+                    Frag<P> a, b;
+                };
                 v4f p = {0, 0, 0, 0}, r = {0, 0, 0, 0};
-#pragma unroll
-                for (int b = 0; b < NB; b++) p = product<X>(sh.k.rows(16 * J, 32 * b, g, c), sh.q.rows(16 * I, 32 * b, g, c), p);
-#pragma unroll
-                for (int b = 0; b < MB; b++) r = product<X>(sh.v.rows(16 * J, 32 * b, g, c), sh.go.rows(16 * I, 32 * b, g, c), r);
+                ahead<NB + MB, kAhead<P>>([&](int i) {
+                                              return i < NB ? Frags{sh.k.rows(16 * J, 32 * i, g, c), sh.q.rows(16 * I, 32 * i, g, c)}
+                                                            : Frags{sh.v.rows(16 * J, 32 * (i - NB), g, c), sh.go.rows(16 * I, 32 * (i - NB), g, c)};
+                                          },
+                                          [&](int i, const Frags &f) {
+                                              if (i < NB) p = product<X>(f.a, f.b, p);
+                                              else r = product<X>(f.a, f.b, r);
+                                          });
                 const int t = 16 * I + c, s = 16 * J + 4 * g;
                 const v4f f = d.between(t, s);
                 float x[4], y[4], u = 0.f, z[4];
@@ -700,59 +766,57 @@ __device__ __forceinline__ void dsum_walk_back(const DsumWalk &a, typename DsumB
 #pragma unroll
                 for (int j = 0; j < EW; j++) dq[I][j] = dk[I][j] = v4f{0, 0, 0, 0};
             // through the states before and behind the chunk
+            Frag<X> state[EW];
+            ahead<MB * 2 * TT, kAhead<P>>(
+                [&](int i) { return i / TT % 2 ? sh.v.rows(16 * (i % TT), 32 * (i / TT / 2), g, c) : sh.go.rows(16 * (i % TT), 32 * (i / TT / 2), g, c); },
+                [&](int i, const Frag<P> &f) {
+                    const int b = i / TT / 2, I = i % TT;
+                    const bool adjoint = i / TT % 2;
 #pragma unroll
-            for (int b = 0; b < MB; b++) {
-                Frag<X> s[EW];
-#pragma unroll
-                for (int j = 0; j < EW; j++) s[j] = split8<X>(S[b][j]);
-#pragma unroll
-                for (int I = 0; I < TT; I++) {
-                    const Frag<P> go = sh.go.rows(16 * I, 32 * b, g, c);
-#pragma unroll
-                    for (int j = 0; j < EW; j++) dq[I][j] = product<X>(s[j], go, dq[I][j]);
-                }
-#pragma unroll
-                for (int j = 0; j < EW; j++) s[j] = split8<X>(H[b][0][j], H[b][1][j]);
-#pragma unroll
-                for (int I = 0; I < TT; I++) {
-                    const Frag<P> v = sh.v.rows(16 * I, 32 * b, g, c);
-#pragma unroll
-                    for (int j = 0; j < EW; j++) dk[I][j] = product<X>(s[j], v, dk[I][j]);
-                }
-            }
+                    for (int j = 0; j < EW; j++) {
+                        if (I == 0) state[j] = adjoint ? split8<X>(H[b][0][j], H[b][1][j]) : split8<X>(S[b][j]);
+                        if (adjoint) dk[I][j] = product<X>(state[j], f, dk[I][j]);
+                        else dq[I][j] = product<X>(state[j], f, dq[I][j]);
+                    }
+                });
+            // What the rows read of the state before the chunk, and wrote into what is read behind it, counts for the decays; and what was there before and is read by the
+            // chunk or behind it, for those of the chunk before: <G', S> = exp(b_C) <G, S> + the sum of what the rows read.
+            const float through = inner() * d.whole;
+            if (chunk > first) load_state(chunk - 1);
+            float read = 0.f;
 #pragma unroll
             for (int I = 0; I < TT; I++) {
                 const int r = 16 * I + c;
                 const float into = d.into[r], rest = d.rest[r];
-                float u = 0.f;
+                float u = 0.f, w = 0.f;
 #pragma unroll
                 for (int j = 0; j < EW; j++) {
                     dq[I][j] *= into, dk[I][j] *= rest;
                     const v4f q = sh.q.four(r, ew + 4 * EW * g + 4 * j), k = sh.k.four(r, ew + 4 * EW * g + 4 * j);
 #pragma unroll
-                    for (int i = 0; i < 4; i++) u = fmaf(q[i], dq[I][j][i], u), u = fmaf(-k[i], dk[I][j][i], u);
+                    for (int i = 0; i < 4; i++) u = fmaf(q[i], dq[I][j][i], u), w = fmaf(k[i], dk[I][j][i], w);
                 }
-                u = over_groups(u);
+                read += u;
+                u = over_groups(u - w);
                 if (g == 0) sh.sums[chunk & 1][wave][r] = u;
             }
+            x_end = through + over_groups(over_sixteen(read));
         }
         if (values) {
 #pragma unroll
             for (int I = 0; I < TT; I++)
 #pragma unroll
                 for (int j = 0; j < VM; j++) dv[I][j] = v4f{0, 0, 0, 0};
+            Frag<O> state[VM];
+            ahead<NB * TT, kAhead<P>>([&](int i) { return sh.k.rows(16 * (i % TT), 32 * (i / TT), g, c); },
+                                      [&](int i, const Frag<P> &k) {
+                                          const int b = i / TT, I = i % TT;
 #pragma unroll
-            for (int b = 0; b < NB; b++) {
-                Frag<O> s[VM];
-#pragma unroll
-                for (int j = 0; j < VM; j++) s[j] = split8<O>(G[b][0][j], G[b][1][j]);
-#pragma unroll
-                for (int I = 0; I < TT; I++) {
-                    const Frag<P> k = sh.k.rows(16 * I, 32 * b, g, c);
-#pragma unroll
-                    for (int j = 0; j < VM; j++) dv[I][j] = product<O>(s[j], k, dv[I][j]);
-                }
-            }
+                                          for (int j = 0; j < VM; j++) {
+                                              if (I == 0) state[j] = split8<O>(G[b][0][j], G[b][1][j]);
+                                              dv[I][j] = product<O>(state[j], k, dv[I][j]);
+                                          }
+                                      });
 #pragma unroll
             for (int I = 0; I < TT; I++) {
                 const float rest = d.rest[16 * I + c];
@@ -761,6 +825,7 @@ __device__ __forceinline__ void dsum_walk_back(const DsumWalk &a, typename DsumB
             }
         }
         lds_barrier();
+        gnext = pinned(gnext);
 
         if (keys) {
             // within the chunk, and the adjoint of the state before it
@@ -770,57 +835,48 @@ __device__ __forceinline__ void dsum_walk_back(const DsumWalk &a, typename DsumB
                 for (int u = 0; u < 2; u++)
 #pragma unroll
                     for (int j = 0; j < EW; j++) H[b][u][j] *= d.whole;
+            Frag<P> q[SB][EW], k[SB][EW];
 #pragma unroll
-            for (int sb = 0; sb < SB; sb++) {
-                const v4f f0 = *reinterpret_cast<const v4f *>(&d.into[32 * sb + 8 * g]), f1 = *reinterpret_cast<const v4f *>(&d.into[32 * sb + 8 * g + 4]);
-                Frag<X> qs[EW];
-                Frag<P> q[EW], k[EW];
+            for (int sb = 0; sb < SB; sb++)
 #pragma unroll
-                for (int j = 0; j < EW; j++) {
-                    k[j] = sh.k.template columns<EW>(ew, j, 32 * sb, g, c), q[j] = sh.q.template columns<EW>(ew, j, 32 * sb, g, c);
-                    float x[8];
-                    join8(q[j], x);
+                for (int j = 0; j < EW; j++) k[sb][j] = sh.k.template columns<EW>(ew, j, 32 * sb, g, c), q[sb][j] = sh.q.template columns<EW>(ew, j, 32 * sb, g, c);
+            using Below = Pairs<TT, true>;
+            using Above = Pairs<TT, false>;
+            ahead<Below::kCount, kAhead<O>>([&](int i) { return sh.r.rows(16 * Below(i).I, 32 * Below(i).sb, g, c); },
+                                            [&](int i, const Frag<O> &r) {
 #pragma unroll
-                    for (int i = 0; i < 4; i++) x[i] *= f0[i], x[i + 4] *= f1[i];
-                    qs[j] = split8<X>(x);
-                }
+                                                for (int j = 0; j < EW; j++) dq[Below(i).I][j] = product<O>(k[Below(i).sb][j], r, dq[Below(i).I][j]);
+                                            });
+            ahead<Above::kCount, kAhead<O>>([&](int i) { return sh.r.template columns<1>(16 * Above(i).I, 0, 32 * Above(i).sb, g, c); },
+                                            [&](int i, const Frag<O> &r) {
 #pragma unroll
-                for (int I = 2 * sb; I < TT; I++) {
-                    const Frag<O> r = sh.r.rows(16 * I, 32 * sb, g, c);
+                                                for (int j = 0; j < EW; j++) dk[Above(i).I][j] = product<O>(q[Above(i).sb][j], r, dk[Above(i).I][j]);
+                                            });
+            Frag<X> qs[EW];
+            ahead<SB * MB * 2, kAhead<P>>([&](int i) { return sh.go.template columns<2>(32 * (i / 2 % MB), i % 2, 32 * (i / 2 / MB), g, c); },
+                                          [&](int i, const Frag<P> &go) {
+                                              const int sb = i / 2 / MB, b = i / 2 % MB, u = i % 2;
 #pragma unroll
-                    for (int j = 0; j < EW; j++) dq[I][j] = product<O>(k[j], r, dq[I][j]);
-                }
-#pragma unroll
-                for (int I = 0; I < 2 * sb + 2; I++) {
-                    const Frag<O> r = sh.r.template columns<1>(16 * I, 0, 32 * sb, g, c);
-#pragma unroll
-                    for (int j = 0; j < EW; j++) dk[I][j] = product<O>(q[j], r, dk[I][j]);
-                }
-#pragma unroll
-                for (int b = 0; b < MB; b++)
-#pragma unroll
-                    for (int u = 0; u < 2; u++) {
-                        const Frag<P> go = sh.go.template columns<2>(32 * b, u, 32 * sb, g, c);
-#pragma unroll
-                        for (int j = 0; j < EW; j++) H[b][u][j] = product<X>(go, qs[j], H[b][u][j]);
-                    }
-            }
-            // for the chunk before this one; ahead of the stores, which the loads would else wait for
-            x_end = inner();
-            if (chunk > first) load_state(chunk - 1);
+                                              for (int j = 0; j < EW; j++) {
+                                                  if (b == 0 && u == 0) qs[j] = scaled<X>(q[sb][j], d.into, sb, g);
+                                                  H[b][u][j] = product<X>(go, qs[j], H[b][u][j]);
+                                              }
+                                          });
+            sq.arrive(), sk.arrive(), sv.arrive(), sd.arrive();
+            state_arrives();
             {
                 const int wide = opaque(a.E), col = ew + 4 * EW * g;
                 if (a.pq) {
                     float *pq = a.pq + ((((int64_t)(h % rq) * a.slices + slice) * a.N + n) * a.HQ + h / rq) * a.L * wide;
-                    store_rows<WHOLE, float, C, EW>(pq + (int64_t)chunk * C * wide, wide, col, dq, a.scale, rows, there, wide - col, c);
+                    store_rows<WHOLE, float, C, EW>(pq + (int64_t)opaque(chunk) * C * wide, wide, col, dq, a.scale, rows, there, wide - col, c);
                 } else {
-                    store_rows<WHOLE, T, C, EW>(row<T>(a.gq, n, h, (int64_t)chunk * C), (int)a.gq.sL, col, dq, a.scale, rows, there, wide - col, c);
+                    store_rows<WHOLE, T, C, EW>(row<T>(a.gq, n, h, (int64_t)opaque(chunk) * C), (int)a.gq.sL, col, dq, a.scale, rows, there, wide - col, c);
                 }
                 if (a.pk) {
                     float *pk = a.pk + ((((int64_t)(h % rk) * a.slices + slice) * a.N + n) * a.HK + h / rk) * a.L * wide;
-                    store_rows<WHOLE, float, C, EW>(pk + (int64_t)chunk * C * wide, wide, col, dk, a.scale, rows, there, wide - col, c);
+                    store_rows<WHOLE, float, C, EW>(pk + (int64_t)opaque(chunk) * C * wide, wide, col, dk, a.scale, rows, there, wide - col, c);
                 } else {
-                    store_rows<WHOLE, T, C, EW>(row<T>(a.gk, n, h, (int64_t)chunk * C), (int)a.gk.sL, col, dk, a.scale, rows, there, wide - col, c);
+                    store_rows<WHOLE, T, C, EW>(row<T>(a.gk, n, h, (int64_t)opaque(chunk) * C), (int)a.gk.sL, col, dk, a.scale, rows, there, wide - col, c);
                 }
             }
         }
@@ -831,43 +887,36 @@ __device__ __forceinline__ void dsum_walk_back(const DsumWalk &a, typename DsumB
                 for (int u = 0; u < 2; u++)
 #pragma unroll
                     for (int j = 0; j < VM; j++) G[b][u][j] *= d.whole;
+            Frag<P> go[SB][VM];
 #pragma unroll
-            for (int sb = 0; sb < SB; sb++) {
-                const v4f f0 = *reinterpret_cast<const v4f *>(&d.into[32 * sb + 8 * g]), f1 = *reinterpret_cast<const v4f *>(&d.into[32 * sb + 8 * g + 4]);
-                // this side of the adjoint ends in the gradient of v alone
-                Frag<O> ds[VM];
-                Frag<P> go[VM];
+            for (int sb = 0; sb < SB; sb++)
 #pragma unroll
-                for (int j = 0; j < VM; j++) {
-                    go[j] = sh.go.template columns<VM>(mw, j, 32 * sb, g, c);
-                    float x[8];
-                    join8(go[j], x);
+                for (int j = 0; j < VM; j++) go[sb][j] = sh.go.template columns<VM>(mw, j, 32 * sb, g, c);
+            using Above = Pairs<TT, false>;
+            ahead<Above::kCount, kAhead<O>>([&](int i) { return sh.p.template columns<1>(16 * Above(i).I, 0, 32 * Above(i).sb, g, c); },
+                                            [&](int i, const Frag<O> &p) {
 #pragma unroll
-                    for (int i = 0; i < 4; i++) x[i] *= f0[i], x[i + 4] *= f1[i];
-                    ds[j] = split8<O>(x);
-                }
+                                                for (int j = 0; j < VM; j++) dv[Above(i).I][j] = product<O>(go[Above(i).sb][j], p, dv[Above(i).I][j]);
+                                            });
+            // this side of the adjoint ends in the gradient of v alone
+            Frag<O> ds[VM];
+            ahead<SB * NB * 2, kAhead<P>>([&](int i) { return sh.q.template columns<2>(32 * (i / 2 % NB), i % 2, 32 * (i / 2 / NB), g, c); },
+                                          [&](int i, const Frag<P> &q) {
+                                              const int sb = i / 2 / NB, b = i / 2 % NB, u = i % 2;
 #pragma unroll
-                for (int I = 0; I < 2 * sb + 2; I++) {
-                    const Frag<O> p = sh.p.template columns<1>(16 * I, 0, 32 * sb, g, c);
-#pragma unroll
-                    for (int j = 0; j < VM; j++) dv[I][j] = product<O>(go[j], p, dv[I][j]);
-                }
-#pragma unroll
-                for (int b = 0; b < NB; b++)
-#pragma unroll
-                    for (int u = 0; u < 2; u++) {
-                        const Frag<P> q = sh.q.template columns<2>(32 * b, u, 32 * sb, g, c);
-#pragma unroll
-                        for (int j = 0; j < VM; j++) G[b][u][j] = product<O>(q, ds[j], G[b][u][j]);
-                    }
-            }
+                                              for (int j = 0; j < VM; j++) {
+                                                  if (b == 0 && u == 0) ds[j] = scaled<O>(go[sb][j], d.into, sb, g);
+                                                  G[b][u][j] = product<O>(q, ds[j], G[b][u][j]);
+                                              }
+                                          });
+            if (!KEYS) sq.arrive(), sk.arrive(), sv.arrive(), sd.arrive();
             {
                 const int cols = opaque(mcols), col = mw + 4 * VM * g;
                 if (a.pv) {
                     float *pv = a.pv + (((int64_t)(h % rv) * a.N + n) * a.HV + h / rv) * a.L * a.M + m0;
-                    store_rows<WHOLE, float, C, VM>(pv + (int64_t)chunk * C * a.M, a.M, col, dv, a.scale, rows, there, cols - col, c);
+                    store_rows<WHOLE, float, C, VM>(pv + (int64_t)opaque(chunk) * C * a.M, a.M, col, dv, a.scale, rows, there, cols - col, c);
                 } else {
-                    store_rows<WHOLE, T, C, VM>(row<T>(a.gv, n, h, (int64_t)chunk * C) + m0, (int)a.gv.sL, col, dv, a.scale, rows, there, cols - col, c);
+                    store_rows<WHOLE, T, C, VM>(row<T>(a.gv, n, h, (int64_t)opaque(chunk) * C) + m0, (int)a.gv.sL, col, dv, a.scale, rows, there, cols - col, c);
                 }
             }
         }

@@ -107,6 +107,24 @@ __device__ __forceinline__ v4f product(const Frag<PA> &a, const Frag<PB> &b, v4f
     return acc;
 }
 
+// N steps, each with what load(i) reads from LDS, whose reads are issued D steps ahead: left to itself the compiler puts a read right before its use and waits for it, some
+// 130 cycles for three products of 16.  The steps' numbers are constants.
+template <int N, int D, typename Load, typename Use>
+__device__ __forceinline__ void ahead(Load load, Use use) {
+    decltype(load(0)) f[D + 1];
+#pragma unroll
+    for (int i = 0; i < D && i < N; i++) f[i] = load(i);
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+        if (i + D < N) f[(i + D) % (D + 1)] = load(i + D);
+        __builtin_amdgcn_sched_barrier(0);
+        use(i, f[i % (D + 1)]);
+    }
+}
+// How far ahead: what P parts leave of the registers
+template <int P>
+constexpr int kAhead = P == 1 ? 3 : P == 2 ? 2 : P == kPlain ? 2 : 1;
+
 // Row (or column) a of the j-th of `tiles` results that lie side by side: four consecutive numbers a lane, 4 * tiles in a row of them.
 __device__ __forceinline__ constexpr int place(int tiles, int a, int j) { return 4 * tiles * (a / 4) + 4 * j + a % 4; }
 
@@ -239,6 +257,14 @@ struct Stage {
                 x[i] = __builtin_bit_cast(Eight, few);
             }
         }
+    }
+    // Waits for the loads.  The counter of outstanding accesses runs in order over loads and stores, and the compiler does not count over branches: a load that is still
+    // waited for behind a kernel's stores waits for them too, some 2 us.
+    __device__ __forceinline__ void arrive() {
+#pragma unroll
+        for (int i = 0; i < kPer; i++)
+#pragma unroll
+            for (int r = 0; r < kRegs; r++) asm volatile("" : "+v"(x[i].x[r]));
     }
     template <int P>
     __device__ __forceinline__ void put(Tile<R, W, P> &t, int rows, int cols, int tid) const {
