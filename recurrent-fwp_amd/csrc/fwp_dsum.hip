@@ -8,11 +8,13 @@ namespace fwp {
 namespace {
 
 // What the segments leave, joined in order: every segment's first state from the one before it.  Slot s of `ends` holds what segment s - 1 leaves when it
-// starts from zero, and then the state that segment s starts from; BACKWARD: of segment s + 1, from the last to the first.  One thread a number of the state, so that
-// the chain of a long prompt's 80 segments is 80 additions long; the slots of kAhead segments are loaded at once (8 heads of 64 x 64, 86 segments: 7 us).
-template <bool BACKWARD, int kAhead>
-__global__ __launch_bounds__(64) void k_dsum_join(float *ends, const float *factors, const float *from, int E, int M, int Ep, int Mp, int segments) {
-    const int cells = Ep * Mp, blocks = cells / 64, cell = blockIdx.x % blocks * 64 + threadIdx.x;      // at least 32 x 32 of them
+// starts from zero, and then the state that segment s starts from; BACKWARD: of segment s + 1, from the last to the first.  A lane has one number of the state, and
+// the slots of WAVES * K segments are loaded at once: the time is that of the loads' round trips.  Each of the WAVES waves folds the K slots that are its own from
+// zero, takes what the waves before it have come to, and folds again from there.
+template <bool BACKWARD, int WAVES, int K>
+__global__ __launch_bounds__(64 * WAVES) void k_dsum_join(float *ends, const float *factors, const float *from, int E, int M, int Ep, int Mp, int segments) {
+    __shared__ float left[WAVES][64], through[WAVES];
+    const int cells = Ep * Mp, blocks = cells / 64, lane = threadIdx.x % 64, wave = threadIdx.x / 64, cell = blockIdx.x % blocks * 64 + lane;      // at least 32 x 32
     const int64_t head = blockIdx.x / blocks;
     float *at = ends + head * segments * cells + cell;
     const float *f = factors + head * segments;
@@ -22,25 +24,37 @@ __global__ __launch_bounds__(64) void k_dsum_join(float *ends, const float *fact
         const int e = cell / Mp, m = cell % Mp;
         if (e < E && m < M) cur = from[(head * E + e) * M + m];
     }
-    float x[kAhead], y[kAhead];
-    const auto load = [&](int s0) {
+    if (wave == 0) at[(int64_t)slot_of(0) * cells] = cur;
+    for (int s0 = 1; s0 < segments; s0 += WAVES * K) {
+        const int mine = s0 + wave * K;
+        float x[K], y[K];
 #pragma unroll
-        for (int i = 0; i < kAhead; i++) {
-            const int slot = slot_of(min(s0 + i, segments - 1));
+        for (int i = 0; i < K; i++) {
+            const int slot = slot_of(min(mine + i, segments - 1));
             x[i] = at[(int64_t)slot * cells];
             y[i] = f[BACKWARD ? slot + 1 : slot - 1];
         }
-    };
-    load(1);
-    at[(int64_t)slot_of(0) * cells] = cur;
-    for (int s0 = 1; s0 < segments; s0 += kAhead) {
-        float z[kAhead];
+        float start = cur;
+        if (WAVES > 1) {
+            float z = 0.f, by = 1.f;
 #pragma unroll
-        for (int i = 0; i < kAhead; i++) z[i] = cur = fmaf(y[i], cur, x[i]);
-        if (s0 + kAhead < segments) load(s0 + kAhead);
+            for (int i = 0; i < K; i++) z = fmaf(y[i], z, x[i]), by *= y[i];
+            left[wave][lane] = z;
+            if (lane == 0) through[wave] = by;
+            __syncthreads();
 #pragma unroll
-        for (int i = 0; i < kAhead; i++)
-            if (s0 + i < segments) at[(int64_t)slot_of(s0 + i) * cells] = z[i];
+            for (int w = 0; w < WAVES; w++) {
+                cur = fmaf(through[w], cur, left[w][lane]);
+                if (w + 1 == wave) start = cur;
+            }
+            __syncthreads();
+        }
+#pragma unroll
+        for (int i = 0; i < K; i++) {
+            start = fmaf(y[i], start, x[i]);
+            if (mine + i < segments) at[(int64_t)slot_of(mine + i) * cells] = start;
+        }
+        if (WAVES == 1) cur = start;
     }
 }
 
@@ -156,8 +170,13 @@ __global__ __launch_bounds__(256) void k_dsum_step(const DsumWalk a, int X, int 
 template <bool BACKWARD>
 void join(const DsumWalk &w, const float *from, int64_t heads, int Ep, hipStream_t s) {
     const unsigned blocks = (unsigned)(heads * (Ep * w.Mp / 64));
-    if (w.segments > 9) k_dsum_join<BACKWARD, 16><<<blocks, 64, 0, s>>>(w.ends, w.factors, from, w.E, w.M, Ep, w.Mp, w.segments);
-    else k_dsum_join<BACKWARD, 4><<<blocks, 64, 0, s>>>(w.ends, w.factors, from, w.E, w.M, Ep, w.Mp, w.segments);
+    const auto launch = [&](auto waves, auto slots) {
+        k_dsum_join<BACKWARD, waves, slots><<<blocks, 64 * waves, 0, s>>>(w.ends, w.factors, from, w.E, w.M, Ep, w.Mp, w.segments);
+    };
+    using std::integral_constant;
+    if (w.segments <= 9) launch(integral_constant<int, 1>{}, integral_constant<int, 4>{});
+    else if (w.segments <= 33) launch(integral_constant<int, 8>{}, integral_constant<int, 4>{});
+    else launch(integral_constant<int, 8>{}, integral_constant<int, 16>{});
 }
 
 struct Plan {
@@ -232,7 +251,7 @@ DsumWalk walk_of(const fwp_dsum_args &a, const Plan &p) {
 
 int launch(int which, const fwp_dsum_args &a, const Plan &p, const DsumWalk &w, int segments, hipStream_t s) {
     const int64_t blocks = p.heads * p.slices * segments;
-    if (!fits_launch(blocks, 512) || !fits_launch(p.heads * (p.cells / 64), 64)) return FWP_E_SHAPE;
+    if (!fits_launch(blocks, 512) || !fits_launch(p.heads * (p.cells / 64), 512)) return FWP_E_SHAPE;
     bool done = false;
     by_type(a.type, [&](auto t) { done = dsum_launch<decltype(t)>(which, &w, p.Ep, p.MS, (unsigned)blocks, s) > 0; });
     return done ? 0 : FWP_E_SHAPE;
