@@ -387,7 +387,27 @@ __global__ __launch_bounds__(64 * NW, (ENDS ? DsumForward<T, NE, NW, MW>::kEndWa
         for (int sb = 0; sb < SB; sb++)
 #pragma unroll
             for (int j = 0; j < MW; j++) v[sb][j] = sh.v.template columns<MW>(mw, j, 32 * sb, g, c);
+        [[maybe_unused]] int bad[MW];      // the first step whose value in this lane's column is infinite or NaN; C: none
+        [[maybe_unused]] bool any_bad = false;
         if constexpr (!ENDS) {
+            // such a value must not reach the steps before it through the zeros of P: it is taken for zero, and results from its step on, and the state, are NaN
+            float x = 0.f;
+#pragma unroll
+            for (int sb = 0; sb < SB; sb++)
+#pragma unroll
+                for (int j = 0; j < MW; j++) x = unless_finite(v[sb][j], x);
+            any_bad = __any(x != 0.f);
+            if (any_bad) {
+#pragma unroll
+                for (int j = 0; j < MW; j++) {
+                    bad[j] = C;
+#pragma unroll
+                    for (int sb = 0; sb < SB; sb++)
+                        take_out(v[sb][j], [&](int i) { bad[j] = min(bad[j], 32 * sb + 8 * g + i); });
+                    bad[j] = min(bad[j], __shfl_xor(bad[j], 16));
+                    bad[j] = min(bad[j], __shfl_xor(bad[j], 32));
+                }
+            }
             using Below = Pairs<TT, true>;
             ahead<Below::kCount, kAhead<O>>([&](int i) { return sh.p.rows(16 * Below(i).I, 32 * Below(i).sb, g, c); },
                                             [&](int i, const Frag<O> &p) {
@@ -406,6 +426,23 @@ __global__ __launch_bounds__(64 * NW, (ENDS ? DsumForward<T, NE, NW, MW>::kEndWa
                                           }
                                       });
         if constexpr (!ENDS) {
+            if (any_bad) {
+                const float nan = __builtin_nanf("");
+#pragma unroll
+                for (int j = 0; j < MW; j++) {
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        // results lie with their columns along the groups of lanes, v with them along a group's lanes
+                        const int from_step = __shfl(bad[j], 4 * g + i);
+#pragma unroll
+                        for (int I = 0; I < TT; I++) acc[I][j][i] = 16 * I + c >= from_step ? nan : acc[I][j][i];
+                    }
+#pragma unroll
+                    for (int b = 0; b < NB; b++)
+#pragma unroll
+                        for (int u = 0; u < 2; u++) S[b][u][j] = bad[j] < C ? v4f{nan, nan, nan, nan} : S[b][u][j];
+                }
+            }
             sq.arrive(), sk.arrive(), sv.arrive();
             gnext = pinned(gnext);
             const int col = mw + 4 * MW * g;

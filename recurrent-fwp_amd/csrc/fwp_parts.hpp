@@ -91,6 +91,38 @@ __device__ __forceinline__ void join8(const Frag<P> &f, float (&x)[8]) {
     }
 }
 
+// Zero if the eight numbers are finite, else NaN
+template <int P>
+__device__ __forceinline__ float unless_finite(const Frag<P> &f, float acc) {
+    if constexpr (P == kPlain) {
+#pragma unroll
+        for (int i = 0; i < 8; i++) acc = fmaf(f.x[i], 0.f, acc);
+    } else {
+        typedef __bf16 v2b __attribute__((ext_vector_type(2)));
+        struct { v2b p[4]; } pairs = __builtin_bit_cast(decltype(pairs), f.p[0]);
+#pragma unroll
+        for (int i = 0; i < 4; i++) acc = __builtin_amdgcn_fdot2_f32_bf16(pairs.p[i], v2b{0, 0}, acc, false);
+    }
+    return acc;
+}
+
+// Takes what is not finite for zero; found(i) for each
+template <int P, typename Found>
+__device__ __forceinline__ void take_out(Frag<P> &f, Found found) {
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        if constexpr (P == kPlain) {
+            if (!(fmaf(f.x[i], 0.f, 0.f) == 0.f)) found(i), f.x[i] = 0.f;
+        } else {
+            if (!((float)f.p[0][i] * 0.f == 0.f)) {
+                found(i);
+#pragma unroll
+                for (int p = 0; p < P; p++) f.p[p][i] = (__bf16)0.f;
+            }
+        }
+    }
+}
+
 // acc + A B over 32 summation indexes, pairs of parts of orders below ORDERS
 template <int ORDERS, int PA, int PB>
 __device__ __forceinline__ v4f product(const Frag<PA> &a, const Frag<PB> &b, v4f acc) {

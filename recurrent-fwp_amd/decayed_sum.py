@@ -25,7 +25,8 @@ def decayed_sum(Q, K, V, log_decay, W=None, scale=1.0, lengths=None):
     state on entry and the one after the last step on return (``None``: zeros, not kept): a prompt and single tokens (L = 1) continue one another.  Returns ``[N,H,L,M]``;
     gradients flow to Q, K, V and log_decay.
 
-    A row that is not finite makes results of its own chunk infinite or NaN, up to 63 steps before it among them."""
+    A number that is not finite makes infinite or NaN what depends on it, and leaves the results of the steps before it as they are; gradients are NaN in its whole chunk,
+    up to 63 steps before and behind it."""
     return _native().decayed_sum(Q, K, V, log_decay, W, scale, lengths)
 
 
