@@ -277,7 +277,7 @@ struct Stage {
     __device__ __forceinline__ void load(const T *base, int stride, int rows, int cols, int tid) {
 #pragma unroll
         for (int i = 0; i < kPer; i++) {
-            const int v = tid + i * THREADS, r = min(v / kRow, rows - 1), col = v % kRow * 8;
+            const int v = tid + i * THREADS, r = min(v / kRow, min(rows, R) - 1), col = v % kRow * 8;
             if (WHOLE) {
                 x[i] = reinterpret_cast<const Anywhere *>(from(base, (uint32_t)r * (uint32_t)stride + (uint32_t)col))->e;
             } else if (cols >= 8) {
