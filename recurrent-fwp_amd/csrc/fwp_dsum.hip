@@ -11,8 +11,10 @@ namespace {
 // starts from zero, and then the state that segment s starts from; BACKWARD: of segment s + 1, from the last to the first.  A lane has one number of the state, and
 // the slots of WAVES * K segments are loaded at once: the time is that of the loads' round trips.  Each of the WAVES waves folds the K slots that are its own from
 // zero, takes what the waves before it have come to, and folds again from there.
-template <bool BACKWARD, int WAVES, int K>
-__global__ __launch_bounds__(64 * WAVES) void k_dsum_join(float *ends, const float *factors, const float *from, int E, int M, int Ep, int Mp, int segments) {
+constexpr int kJoinWaves = 8;
+template <bool BACKWARD, int K>
+__global__ __launch_bounds__(64 * kJoinWaves) void k_dsum_join(float *ends, const float *factors, const float *from, int E, int M, int Ep, int Mp, int segments) {
+    constexpr int WAVES = kJoinWaves;
     __shared__ float left[WAVES][64], through[WAVES];
     const int cells = Ep * Mp, blocks = cells / 64, lane = threadIdx.x % 64, wave = threadIdx.x / 64, cell = blockIdx.x % blocks * 64 + lane;      // at least 32 x 32
     const int64_t head = blockIdx.x / blocks;
@@ -34,27 +36,23 @@ __global__ __launch_bounds__(64 * WAVES) void k_dsum_join(float *ends, const flo
             x[i] = at[(int64_t)slot * cells];
             y[i] = f[BACKWARD ? slot + 1 : slot - 1];
         }
-        float start = cur;
-        if (WAVES > 1) {
-            float z = 0.f, by = 1.f;
+        float start = cur, z = 0.f, by = 1.f;
 #pragma unroll
-            for (int i = 0; i < K; i++) z = fmaf(y[i], z, x[i]), by *= y[i];
-            left[wave][lane] = z;
-            if (lane == 0) through[wave] = by;
-            __syncthreads();
+        for (int i = 0; i < K; i++) z = fmaf(y[i], z, x[i]), by *= y[i];
+        left[wave][lane] = z;
+        if (lane == 0) through[wave] = by;
+        __syncthreads();
 #pragma unroll
-            for (int w = 0; w < WAVES; w++) {
-                cur = fmaf(through[w], cur, left[w][lane]);
-                if (w + 1 == wave) start = cur;
-            }
-            __syncthreads();
+        for (int w = 0; w < WAVES; w++) {
+            cur = fmaf(through[w], cur, left[w][lane]);
+            if (w + 1 == wave) start = cur;
         }
+        __syncthreads();
 #pragma unroll
         for (int i = 0; i < K; i++) {
             start = fmaf(y[i], start, x[i]);
             if (mine + i < segments) at[(int64_t)slot_of(mine + i) * cells] = start;
         }
-        if (WAVES == 1) cur = start;
     }
 }
 
@@ -167,16 +165,15 @@ __global__ __launch_bounds__(256) void k_dsum_step(const DsumWalk a, int X, int 
         store(out + block * X * 4 + tid, a.scale * ((part[0][tid] + part[1][tid]) + (part[2][tid] + part[3][tid])));
 }
 
+// Up to so many segments, every workgroup of the walk joins what it starts from itself
+constexpr int kFewSegments = 9;
+
 template <bool BACKWARD>
 void join(const DsumWalk &w, const float *from, int64_t heads, int Ep, hipStream_t s) {
     const unsigned blocks = (unsigned)(heads * (Ep * w.Mp / 64));
-    const auto launch = [&](auto waves, auto slots) {
-        k_dsum_join<BACKWARD, waves, slots><<<blocks, 64 * waves, 0, s>>>(w.ends, w.factors, from, w.E, w.M, Ep, w.Mp, w.segments);
-    };
-    using std::integral_constant;
-    if (w.segments <= 9) launch(integral_constant<int, 1>{}, integral_constant<int, 4>{});
-    else if (w.segments <= 33) launch(integral_constant<int, 8>{}, integral_constant<int, 4>{});
-    else launch(integral_constant<int, 8>{}, integral_constant<int, 16>{});
+    const auto launch = [&](auto slots) { k_dsum_join<BACKWARD, slots><<<blocks, 64 * kJoinWaves, 0, s>>>(w.ends, w.factors, from, w.E, w.M, Ep, w.Mp, w.segments); };
+    if (w.segments <= 33) launch(std::integral_constant<int, 4>{});
+    else launch(std::integral_constant<int, 16>{});
 }
 
 struct Plan {
@@ -302,7 +299,8 @@ int dsum_fwd(const fwp_dsum_args &a, float *W, fwp_out_rows out, float *saved, f
         w.ends = workspace;
         w.factors = workspace + p.heads * p.segments * p.cells;
         if (int rc = launch(kDsumForwardEnds, a, p, w, p.segments - 1, s)) return rc;
-        join<false>(w, W, p.heads, p.Ep, s);
+        w.joined = p.segments > kFewSegments;
+        if (w.joined) join<false>(w, W, p.heads, p.Ep, s);
     }
     if (int rc = launch(kDsumForward, a, p, w, p.segments, s)) return rc;
     return (int)hipGetLastError();
@@ -329,7 +327,8 @@ int dsum_bwd(const fwp_dsum_args &a, const float *saved, fwp_rows gout, fwp_out_
     w.gdecay = parts ? parts : gdecay;
     if (p.segments > 1) {
         if (int rc = launch(kDsumBackwardEnds, a, p, w, p.segments - 1, s)) return rc;
-        join<true>(w, nullptr, p.heads, p.Ep, s);
+        w.joined = p.segments > kFewSegments;
+        if (w.joined) join<true>(w, nullptr, p.heads, p.Ep, s);
     }
     if (int rc = launch(kDsumBackward, a, p, w, p.segments, s)) return rc;
     by_type(a.type, [&](auto t) {

@@ -49,6 +49,7 @@ struct DsumWalk {
     float scale;
     int N, H, L, E, M, HQ, HK, HV, Mp, slices, segments, per;      // per: chunks of a segment
     int sum_decay;
+    int joined;                        // the segments' first states are in `ends`; else each workgroup joins those that it needs
 };
 
 // Workgroups b, b + 8, .. run on one XCD: neighbours in the order of the work get numbers that lie 8 apart.  Slices and heads come first in that order: they share
@@ -213,6 +214,35 @@ struct Pairs {
     }
 };
 
+// A first state from those that the segments leave, slots lo .. hi of `ends` one after another (backwards from lo down to hi where STEP is -1): S = factor S + what the
+// slot holds.  each(use) has use(number, four of the state's numbers, their offsets in a slot) called for all that the lane has; the loads of K slots go out together, as many as there are registers for.
+template <int STEP, int COUNT, typename Each>
+__device__ __forceinline__ void fold_segments(const float *ends, int64_t cells, const float *factors, int lo, int hi, bool joined, Each each) {
+    constexpr int K = COUNT <= 8 ? 4 : 2;
+#pragma unroll 1
+    for (int s0 = lo; STEP * s0 <= STEP * hi; s0 += STEP * K) {
+        v4f x[K][COUNT];
+        float y[K];
+#pragma unroll
+        for (int k = 0; k < K; k++) {
+            const int slot = STEP > 0 ? min(s0 + k, hi) : max(s0 - k, hi);
+            const float *at = ends + slot * cells;
+            y[k] = joined ? 0.f : factors[slot - STEP];
+            each([&](int n, v4f &, auto place) {
+#pragma unroll
+                for (int i = 0; i < 4; i++) x[k][n][i] = at[place(i)];
+            });
+        }
+#pragma unroll
+        for (int k = 0; k < K; k++)
+            if (STEP * (s0 + STEP * k) <= STEP * hi) each([&](int n, v4f &S, auto) { S = y[k] * S + x[k][n]; });
+    }
+}
+__device__ __forceinline__ void pin(v4f &x) {
+#pragma unroll
+    for (int i = 0; i < 4; i++) x[i] = pinned(x[i]);
+}
+
 // Workgroups of a kernel that a CU holds at once: 160 KB of LDS, and registers for `waves` on each of four SIMDs, which the kernel's launch bounds ask for
 constexpr int resident(size_t lds, int waves, int NW) { return (int)(160 * 1024 / lds) < 4 * waves / NW ? (int)(160 * 1024 / lds) : 4 * waves / NW; }
 
@@ -261,26 +291,35 @@ __global__ __launch_bounds__(64 * NW, (ENDS ? DsumForward<T, NE, NW, MW>::kEndWa
 
     v4f S[NB][2][MW];
     const int64_t head = (int64_t)n * a.H + h;
-    {
-        const float *from = nullptr;
-        int64_t stride = a.M;
-        int rows = a.E, cols = a.M;
-        if (!ENDS) {
-            if (a.segments > 1) from = a.ends + (head * a.segments + seg) * E * a.Mp, stride = a.Mp, rows = E, cols = a.Mp;
-            else if (a.from) from = a.from + head * a.E * a.M;
-        }
+    const auto each = [&](auto use) {
 #pragma unroll
         for (int b = 0; b < NB; b++)
 #pragma unroll
             for (int u = 0; u < 2; u++)
 #pragma unroll
                 for (int j = 0; j < MW; j++)
+                    use((b * 2 + u) * MW + j, S[b][u][j], [&](int i) { return (32 * b + 8 * g + 4 * u + i) * a.Mp + m0 + mw + place(MW, c, j); });
+    };
+    each([](int, v4f &x, auto) { x = v4f{0, 0, 0, 0}; });
+    if constexpr (!ENDS) {
+        if (a.from && !a.joined) {
+            const float *from = a.from + head * a.E * a.M;
 #pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        const int e = 32 * b + 8 * g + 4 * u + i, m = m0 + mw + place(MW, c, j);
-                        // arrived, as everything that is loaded ahead of the loop: a wait that its first round needs would be one of all rounds
-                        S[b][u][j][i] = pinned(from && e < rows && m < cols ? from[e * stride + m] : 0.f);
-                    }
+            for (int b = 0; b < NB; b++)
+#pragma unroll
+                for (int u = 0; u < 2; u++)
+#pragma unroll
+                    for (int j = 0; j < MW; j++)
+#pragma unroll
+                        for (int i = 0; i < 4; i++) {
+                            const int e = 32 * b + 8 * g + 4 * u + i, m = m0 + mw + place(MW, c, j);
+                            if (e < a.E && m < a.M) S[b][u][j][i] = from[(int64_t)e * a.M + m];
+                        }
+        }
+        if (a.segments > 1)
+            fold_segments<1, NB * 2 * MW>(a.ends + head * a.segments * E * a.Mp, (int64_t)E * a.Mp, a.factors + head * a.segments, a.joined ? seg : 1, seg, a.joined, each);
+        // arrived, as everything that is loaded ahead of the loop: a wait that its first round needs would be one of all rounds
+        each([](int, v4f &x, auto) { pin(x); });
     }
     if constexpr (!ENDS) {      // tiles of P above the diagonal stay zero
         for (int i = tid; i < (int)(sizeof(sh.p) / 16); i += 64 * NW) reinterpret_cast<v4f *>(&sh.p)[i] = v4f{0, 0, 0, 0};
@@ -629,8 +668,8 @@ __device__ __forceinline__ void dsum_walk_back(const DsumWalk &a, typename DsumB
 
     // the adjoint: key waves H, all value columns of their key rows, transposed; value waves G, all key rows of their value columns
     v4f H[KEYS ? MB : 1][2][EW], G[VALUES ? NB : 1][2][VM];
-    {
-        const float *from = a.segments > 1 && seg + 1 < a.segments ? a.ends + (head * a.segments + seg) * E * a.Mp + m0 : nullptr;
+    constexpr int kOfH = KEYS ? MB * 2 * EW : 0, kOfG = VALUES ? NB * 2 * VM : 0;
+    const auto each = [&](auto use) {
         if constexpr (KEYS) {
 #pragma unroll
             for (int b = 0; b < MB; b++)
@@ -638,8 +677,7 @@ __device__ __forceinline__ void dsum_walk_back(const DsumWalk &a, typename DsumB
                 for (int u = 0; u < 2; u++)
 #pragma unroll
                     for (int j = 0; j < EW; j++)
-#pragma unroll
-                        for (int i = 0; i < 4; i++) H[b][u][j][i] = pinned(from && keys ? from[(ew + place(EW, c, j)) * a.Mp + 32 * b + 8 * g + 4 * u + i] : 0.f);
+                        use((b * 2 + u) * EW + j, H[b][u][j], [&](int i) { return ((keys ? ew : 0) + place(EW, c, j)) * a.Mp + m0 + 32 * b + 8 * g + 4 * u + i; });
         }
         if constexpr (VALUES) {
 #pragma unroll
@@ -648,10 +686,13 @@ __device__ __forceinline__ void dsum_walk_back(const DsumWalk &a, typename DsumB
                 for (int u = 0; u < 2; u++)
 #pragma unroll
                     for (int j = 0; j < VM; j++)
-#pragma unroll
-                        for (int i = 0; i < 4; i++) G[b][u][j][i] = pinned(from && values ? from[(32 * b + 8 * g + 4 * u + i) * a.Mp + mw + place(VM, c, j)] : 0.f);
+                        use(kOfH + (b * 2 + u) * VM + j, G[b][u][j], [&](int i) { return (32 * b + 8 * g + 4 * u + i) * a.Mp + m0 + (values ? mw : 0) + place(VM, c, j); });
         }
-    }
+    };
+    each([](int, v4f &x, auto) { x = v4f{0, 0, 0, 0}; });
+    if (a.segments > 1)
+        fold_segments<-1, kOfH + kOfG>(a.ends + head * a.segments * E * a.Mp, (int64_t)E * a.Mp, a.factors + head * a.segments, a.joined ? seg : a.segments - 2, seg, a.joined, each);
+    each([](int, v4f &x, auto) { pin(x); });
 #pragma unroll 1
     for (int i = tid; i < (int)(sizeof(sh.p) / 16); i += kThreads) reinterpret_cast<v4f *>(&sh.p)[i] = v4f{0, 0, 0, 0};
 #pragma unroll 1
