@@ -530,6 +530,10 @@ __global__ __launch_bounds__(64 * NW, (ENDS ? DsumForward<T, NE, NW, MW>::kEndWa
 // A workgroup's waves share the walk back by what they own: KW key waves have EW tiles of 16 key rows each, the gradients of q and k there and the adjoint's
 // rows (all value columns, transposed); VW value waves have MW tiles of 16 value columns each, the gradient of v and the adjoint's columns, and make P and R.
 // The adjoint is held twice so that no product waits for another wave's share of it.
+// The walk back has fewer registers to spare
+template <int P>
+constexpr int kAheadBack = kAhead<P> < 2 ? kAhead<P> : 2;
+
 template <typename T, int NE, int NW, int MW>
 struct DsumBackward {
     static constexpr int C = kChunkOf<T>, P = Parts<T, NE>::P, O = Parts<T, NE>::O, X = Parts<T, NE>::X, E = 16 * NE, MS = 16 * MW * NW;
@@ -809,7 +813,7 @@ __device__ __forceinline__ void dsum_walk_back(const DsumWalk &a, typename DsumB
                     Frag<P> a, b;
                 };
                 v4f p = {0, 0, 0, 0}, r = {0, 0, 0, 0};
-                ahead<NB + MB, kAhead<P>>([&](int i) {
+                ahead<NB + MB, kAheadBack<P>>([&](int i) {
                                               return i < NB ? Frags{sh.k.rows(16 * J, 32 * i, g, c), sh.q.rows(16 * I, 32 * i, g, c)}
                                                             : Frags{sh.v.rows(16 * J, 32 * (i - NB), g, c), sh.go.rows(16 * I, 32 * (i - NB), g, c)};
                                           },
@@ -844,7 +848,7 @@ __device__ __forceinline__ void dsum_walk_back(const DsumWalk &a, typename DsumB
                 for (int j = 0; j < EW; j++) dq[I][j] = dk[I][j] = v4f{0, 0, 0, 0};
             // through the states before and behind the chunk
             Frag<X> state[EW];
-            ahead<MB * 2 * TT, kAhead<P>>(
+            ahead<MB * 2 * TT, kAheadBack<P>>(
                 [&](int i) { return i / TT % 2 ? sh.v.rows(16 * (i % TT), 32 * (i / TT / 2), g, c) : sh.go.rows(16 * (i % TT), 32 * (i / TT / 2), g, c); },
                 [&](int i, const Frag<P> &f) {
                     const int b = i / TT / 2, I = i % TT;
@@ -885,7 +889,7 @@ __device__ __forceinline__ void dsum_walk_back(const DsumWalk &a, typename DsumB
 #pragma unroll
                 for (int j = 0; j < VM; j++) dv[I][j] = v4f{0, 0, 0, 0};
             Frag<O> state[VM];
-            ahead<NB * TT, kAhead<P>>([&](int i) { return sh.k.rows(16 * (i % TT), 32 * (i / TT), g, c); },
+            ahead<NB * TT, kAheadBack<P>>([&](int i) { return sh.k.rows(16 * (i % TT), 32 * (i / TT), g, c); },
                                       [&](int i, const Frag<P> &k) {
                                           const int b = i / TT, I = i % TT;
 #pragma unroll
@@ -919,18 +923,18 @@ __device__ __forceinline__ void dsum_walk_back(const DsumWalk &a, typename DsumB
                 for (int j = 0; j < EW; j++) k[sb][j] = sh.k.template columns<EW>(ew, j, 32 * sb, g, c), q[sb][j] = sh.q.template columns<EW>(ew, j, 32 * sb, g, c);
             using Below = Pairs<TT, true>;
             using Above = Pairs<TT, false>;
-            ahead<Below::kCount, kAhead<O>>([&](int i) { return sh.r.rows(16 * Below(i).I, 32 * Below(i).sb, g, c); },
+            ahead<Below::kCount, kAheadBack<O>>([&](int i) { return sh.r.rows(16 * Below(i).I, 32 * Below(i).sb, g, c); },
                                             [&](int i, const Frag<O> &r) {
 #pragma unroll
                                                 for (int j = 0; j < EW; j++) dq[Below(i).I][j] = product<O>(k[Below(i).sb][j], r, dq[Below(i).I][j]);
                                             });
-            ahead<Above::kCount, kAhead<O>>([&](int i) { return sh.r.template columns<1>(16 * Above(i).I, 0, 32 * Above(i).sb, g, c); },
+            ahead<Above::kCount, kAheadBack<O>>([&](int i) { return sh.r.template columns<1>(16 * Above(i).I, 0, 32 * Above(i).sb, g, c); },
                                             [&](int i, const Frag<O> &r) {
 #pragma unroll
                                                 for (int j = 0; j < EW; j++) dk[Above(i).I][j] = product<O>(q[Above(i).sb][j], r, dk[Above(i).I][j]);
                                             });
             Frag<X> qs[EW];
-            ahead<SB * MB * 2, kAhead<P>>([&](int i) { return sh.go.template columns<2>(32 * (i / 2 % MB), i % 2, 32 * (i / 2 / MB), g, c); },
+            ahead<SB * MB * 2, kAheadBack<P>>([&](int i) { return sh.go.template columns<2>(32 * (i / 2 % MB), i % 2, 32 * (i / 2 / MB), g, c); },
                                           [&](int i, const Frag<P> &go) {
                                               const int sb = i / 2 / MB, b = i / 2 % MB, u = i % 2;
 #pragma unroll
@@ -970,14 +974,14 @@ __device__ __forceinline__ void dsum_walk_back(const DsumWalk &a, typename DsumB
 #pragma unroll
                 for (int j = 0; j < VM; j++) go[sb][j] = sh.go.template columns<VM>(mw, j, 32 * sb, g, c);
             using Above = Pairs<TT, false>;
-            ahead<Above::kCount, kAhead<O>>([&](int i) { return sh.p.template columns<1>(16 * Above(i).I, 0, 32 * Above(i).sb, g, c); },
+            ahead<Above::kCount, kAheadBack<O>>([&](int i) { return sh.p.template columns<1>(16 * Above(i).I, 0, 32 * Above(i).sb, g, c); },
                                             [&](int i, const Frag<O> &p) {
 #pragma unroll
                                                 for (int j = 0; j < VM; j++) dv[Above(i).I][j] = product<O>(go[Above(i).sb][j], p, dv[Above(i).I][j]);
                                             });
             // this side of the adjoint ends in the gradient of v alone
             Frag<O> ds[VM];
-            ahead<SB * NB * 2, kAhead<P>>([&](int i) { return sh.q.template columns<2>(32 * (i / 2 % NB), i % 2, 32 * (i / 2 / NB), g, c); },
+            ahead<SB * NB * 2, kAheadBack<P>>([&](int i) { return sh.q.template columns<2>(32 * (i / 2 % NB), i % 2, 32 * (i / 2 / NB), g, c); },
                                           [&](int i, const Frag<P> &q) {
                                               const int sb = i / 2 / NB, b = i / 2 % NB, u = i % 2;
 #pragma unroll
