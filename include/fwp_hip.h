@@ -552,8 +552,8 @@ typedef struct fwp_rotary_args {
 int fwp_rotary(const fwp_rotary_args *a, fwp_out_rows oq, fwp_out_rows ok, void *stream);
 
 /*
- * Norm of groups of channels: every row's `groups` groups of `size` channels (size <= 1024, groups * size <= 65536); rows of x and of gate x_step and gate_step
- * elements apart, those of everything else side by side,
+ * Norm of groups of channels: every row's `groups` groups of `size` channels (size <= 1024, groups * size <= 65536, at most 2^30 rows); rows of x and of gate
+ * x_step and gate_step elements apart, those of everything else side by side,
  *   u = norm(group) weight + bias (either NULL: without it),  y = act(gate) u, or act(u) where gate is NULL
  * norm as above; act: FWP_ACT_*.  x, gate, y of `type`; weight, bias [groups * size].
  */

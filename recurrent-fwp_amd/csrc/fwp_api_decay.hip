@@ -18,7 +18,7 @@ bool step_ok(const V &v) {
 bool aligned16(const void *p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 bool divides(int part, int whole) { return part >= 1 && whole % part == 0; }
 
-constexpr int kMaxKeys = 128, kMaxValues = 1 << 16, kMaxSteps = 1 << 30, kMaxWidth = 1 << 16, kMaxGroup = 1024;
+constexpr int kMaxKeys = 128, kMaxValues = 1 << 16, kMaxSteps = 1 << 30, kMaxWidth = 1 << 16, kMaxGroup = 1024, kMaxRows = 1 << 30;
 
 bool dims_ok(int type, int N, int H, int L, int E, int M) {
     return type_ok(type) && N >= 1 && H >= 1 && L >= 1 && L <= kMaxSteps && (int64_t)N * H < (int64_t(1) << 31) && E >= 1 && E <= kMaxKeys && M >= 1 &&
@@ -39,7 +39,7 @@ int dsum_check(const fwp_dsum_args *a) {
 
 int norm_check(const fwp_group_norm_args *a) {
     if (!a || !a->x) return FWP_E_NULL;
-    if (!type_ok(a->type) || a->rows < 1 || a->groups < 1 || a->size < 1 || a->size > kMaxGroup || (int64_t)a->groups * a->size > kMaxWidth ||
+    if (!type_ok(a->type) || a->rows < 1 || a->rows > kMaxRows || a->groups < 1 || a->size < 1 || a->size > kMaxGroup || (int64_t)a->groups * a->size > kMaxWidth ||
         (a->act != FWP_ACT_NONE && a->act != FWP_ACT_SIGMOID && a->act != FWP_ACT_SILU))
         return FWP_E_SHAPE;
     return 0;
@@ -93,7 +93,7 @@ int fwp_group_norm_fwd(const fwp_group_norm_args *a, void *y, void *stream) {
 }
 
 long long fwp_group_norm_workspace(int type, int rows, int groups, int size) {
-    return !type_ok(type) || rows < 1 || groups < 1 || size < 1 || size > kMaxGroup || (int64_t)groups * size > kMaxWidth
+    return !type_ok(type) || rows < 1 || rows > kMaxRows || groups < 1 || size < 1 || size > kMaxGroup || (int64_t)groups * size > kMaxWidth
                ? FWP_E_SHAPE
                : group_norm_workspace(type, rows, groups, size);
 }

@@ -9,7 +9,7 @@ namespace {
 
 // What the segments leave, joined in order: every segment's first state from the one before it.  Slot s of `ends` holds what segment s - 1 leaves when it
 // starts from zero, and then the state that segment s starts from; BACKWARD: of segment s + 1, from the last to the first.  A lane has one number of the state, and
-// the slots of WAVES * K segments are loaded at once: the time is that of the loads' round trips.  Each of the WAVES waves folds the K slots that are its own from
+// the slots of WAVES * K segments are loaded at once: the time is that of the loads' round trips (8 heads of 64 x 64, 86 segments: 6.3 us; one wave with 16 loads ahead 8.2).  Each of the WAVES waves folds the K slots that are its own from
 // zero, takes what the waves before it have come to, and folds again from there.
 constexpr int kJoinWaves = 8;
 template <bool BACKWARD, int K>
@@ -56,7 +56,8 @@ __global__ __launch_bounds__(64 * kJoinWaves) void k_dsum_join(float *ends, cons
     }
 }
 
-// rows [N,G,L,D] of type T as the sum of `parts` fp32 tensors of that shape, in their order; K elements a thread, of one row, and the loads of eight parts at once
+// rows [N,G,L,D] of type T as the sum of `parts` fp32 tensors of that shape, in their order; K elements a thread, of one row, and the loads of eight parts at once.  Bound by memory:
+// 32 parts of 4 x 4096 x 128 in 63 us, 4.2 TB/s (one element a thread: 127).
 template <typename T, int K>
 __global__ __launch_bounds__(256) void k_sum_parts(const float *x, fwp_out_rows out, int parts, int64_t total, int G, int L, int D) {
     struct __attribute__((aligned(4 * K))) Run { float x[K]; };
@@ -87,7 +88,7 @@ void sum_parts(const float *x, fwp_out_rows out, int parts, int N, int G, int L,
     else k_sum_parts<T, 1><<<blocks(total), 256, 0, s>>>(x, out, parts, total, G, L, D);
 }
 
-// [H] = sums over n and the parts of each head of x [N,H,parts], one workgroup a head
+// [H] = sums over n and the parts of each head of x [N,H,parts], one workgroup a head: a launch, 4.3 us
 __global__ __launch_bounds__(256) void k_sum_heads(const float *x, float *out, int N, int H, int parts) {
     __shared__ float part[4];
     const int h = blockIdx.x;
@@ -101,7 +102,8 @@ __global__ __launch_bounds__(256) void k_sum_heads(const float *x, float *out, i
 }
 
 // One step: S = exp(g) S + k (x) v, o = scale S^T q.  Bound by the state, which is read and written once: a lane holds four columns of R rows, all loaded before
-// any is used; X lanes lie side by side on a row.
+// any is used; X lanes lie side by side on a row.  No cache line of it is used again within a step: 256 x 16 states of 128 x 128 (0.54 GB) 127 us at 4.2 TB/s, 138 without saying so.
+// 32 x 8 states of 32 x 32: 4.4 us, a launch and two round trips.
 template <typename T, int R>
 __global__ __launch_bounds__(256) void k_dsum_step(const DsumWalk a, int X, int blocks) {
     __shared__ float part[4][128 + 4];
@@ -165,7 +167,8 @@ __global__ __launch_bounds__(256) void k_dsum_step(const DsumWalk a, int X, int 
         store(out + block * X * 4 + tid, a.scale * ((part[0][tid] + part[1][tid]) + (part[2][tid] + part[3][tid])));
 }
 
-// Up to so many segments, every workgroup of the walk joins what it starts from itself
+// Up to so many segments, every workgroup of the walk joins what it starts from itself: 8 x 16 sequences of 4096 steps, 64 x 64 bf16, six segments forward and four back, 357 us for both with
+// their walks, 370 with a kernel of its own for each; eight segments of 32 x 8 x 1024, 32 x 32 fp32, 170 and 174.  Many segments would read most of `ends` again and again.
 constexpr int kFewSegments = 9;
 
 template <bool BACKWARD>
@@ -189,8 +192,8 @@ int resident_of(int type, int which, int Ep, int MS) {
 
 // How a pass is cut.  Segments by a model of its time in chunks of the walk, which goes in rounds of as many workgroups as the GPU holds, each as long as its
 // chunks and the way into them.  Cutting sequences adds the walk that finds the segments' states: a chunk of it is 0.45 of a chunk forward and 0.3 backward where it
-// fills the GPU, and half of that at least; and joining them.  8 x 16 sequences of 64 chunks, 64 x 64 bf16: 6 segments forward 32 + 6 + 100 us, 8 are
-// 34 + 7 + 124; 4 segments backward 34 + 6 + 214, 8 are 36 + 7 + 228.
+// fills the GPU, and half of that at least; and joining them.  8 x 16 sequences of 64 chunks, 64 x 64 bf16, as measured when the two terms were set: 6 segments forward 32 + 6 + 100 us, 8 are 34 + 7 + 124;
+// 4 segments backward 34 + 6 + 214, 8 are 36 + 7 + 228.
 Plan plan_of(int type, int N, int H, int L, int E, int M, bool backward) {
     Plan p{};
     p.Ep = E <= 32 ? 32 : E <= 64 ? 64 : 128;
@@ -205,14 +208,17 @@ Plan plan_of(int type, int N, int H, int L, int E, int M, bool backward) {
                   ends = 256 * resident_of(type, backward ? kDsumBackwardEnds : kDsumForwardEnds, p.Ep, p.MS);
     const auto rounds = [](int64_t blocks, int64_t held) { return (double)((blocks + held - 1) / held); };
     double best = 0;
-    for (int64_t s = 1; s <= std::max(1, p.chunks / 2) && (s == 1 || units * (s - 1) < 4 * walks); s++) {
-        const int64_t per = (p.chunks + s - 1) / s, segments = (p.chunks + per - 1) / per;
+    // every length of a segment once, and the fewest segments that have it
+    for (int64_t s = 1, per; s <= std::max(1, p.chunks / 2) && (s == 1 || units * (s - 1) < 4 * walks); s = (p.chunks + per - 2) / (per - 1)) {
+        per = (p.chunks + s - 1) / s;
+        const int64_t segments = (p.chunks + per - 1) / per;
         double time = rounds(units * segments, walks) * (per + 0.6);
         if (segments > 1) {
             const double blocks = (double)units * (segments - 1);
             time += (per + 1) * (backward ? 0.3 : 0.45) * std::max(0.5 * rounds(units * (segments - 1), ends), blocks / ends) + 0.6 + 0.03 * segments;
         }
         if (s == 1 || time < best) best = time, p.per = (int)per, p.segments = (int)segments;
+        if (per == 1) break;
     }
     p.ends = p.segments > 1 ? p.heads * p.segments * (p.cells + 1) : 0;
     return p;

@@ -72,7 +72,7 @@ def group_norm(X, groups, weight=None, bias=None, gate=None, eps=1e-5, rms=False
     """Every row's channels in ``groups`` groups, each normalised by its own mean and variance (``rms``: divided by its root mean square), times ``weight`` plus ``bias``; then
     times ``act(gate)``, or ``act`` of it where there is no gate.
 
-    X, gate ``[..., channels]``, channels last; a row is normalised by itself, so that no step sees another.  weight, bias ``[channels]``; groups of up to 1024 channels.
+    X, gate ``[..., channels]``, channels last; a row is normalised by itself, so that no step sees another.  weight, bias ``[channels]``; groups of up to 1024 channels, at most 2^30 rows.
     ``activation``: ``None``, ``"sigmoid"`` or ``"silu"``.  Gradients flow to every tensor."""
     act = _ACTIVATIONS.get(activation)
     if act is None:

@@ -144,6 +144,33 @@ def test_c_entry_points_refuse_before_any_launch(fwp):
     assert lib.fwp_group_norm_workspace(0, 4, 4, 16) >= 2 * 64 and lib.fwp_group_norm_workspace(0, 0, 4, 16) == E_SHAPE
 
 
+def test_more_rows_than_a_walk_counts_are_refused(fwp):
+    """Rows go on in steps of up to 4096: the last ones below 2^31 have no next one in 32 bits"""
+    L = fwp._lib
+    lib, p = L.lib(), ctypes.c_void_p(4096)
+    norm = lambda rows: ctypes.byref(L.GroupNormArgs(x=4096, x_step=1, weight=4096, bias=4096, eps=1e-5, rows=rows, groups=1, size=1))
+    for rows in ((1 << 30) + 1, (1 << 31) - 1):
+        assert lib.fwp_group_norm_fwd(norm(rows), p, None) == -2
+        assert lib.fwp_group_norm_bwd(norm(rows), p, p, None, p, p, p, None) == -2
+        assert lib.fwp_group_norm_workspace(0, rows, 1, 1) == -2
+    assert lib.fwp_group_norm_workspace(0, 1 << 30, 1, 1) > 0
+
+
+def test_plans_of_long_sequences_are_quick(fwp):
+    """A call asks for its plan several times: those of one sequence of a million steps, which may have thousands of segments, within a millisecond each"""
+    import time
+    L = fwp._lib
+    lib = L.lib()
+    v = L.View(4096, 1 << 30, 1 << 30, 16)
+    a = ctypes.byref(L.DecayedSumArgs(q=v, k=v, v=v, decay=4096, dN=1 << 20, dH=1 << 20, dL=1, scale=1.0, N=1, H=1, L=1 << 20, E=16, M=16, HQ=1, HK=1, HV=1))
+    for backward in (0, 1):
+        assert lib.fwp_decayed_sum_workspace(a, backward) > 0
+        start = time.perf_counter()
+        for _ in range(100):
+            lib.fwp_decayed_sum_workspace(a, backward)
+        assert time.perf_counter() - start < 0.1
+
+
 @pytest.mark.parametrize("per_head", [True, False])
 def test_the_formulas_gradients_against_differences(per_head):
     g = torch.Generator().manual_seed(3)

@@ -145,3 +145,55 @@ def test_others_refuse_too(fwp, op):
         f = F.frequencies(8).cuda()
     with pytest.raises(fwp._lib.FwpError, match="inference"):
         fwp.rotary(x.clone().requires_grad_(), None, f) if op == "rotary" else fwp.group_norm(x.clone().requires_grad_(), 2, w)
+
+
+# ------------------------------------------------------------------ calls that the documentation allows
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("D,pairs", [(32, 16), (37, 12)])
+def test_rotary_in_place(fwp, D, pairs, interleaved, dtype):
+    """The C entry may write the rows that it reads"""
+    import ctypes
+    L = fwp._lib
+    g = torch.Generator().manual_seed(D)
+    q, k, f = rows(g, dtype, 2, 9, 33, D), rows(g, dtype, 2, 3, 33, D), F.frequencies(2 * pairs).cuda()
+    want = fwp.rotary(q, k, f, interleaved=interleaved, scale=0.7)
+    view = lambda t, kind: kind(t.data_ptr(), *t.stride()[:3])
+    a = L.RotaryArgs(q=view(q, L.View), k=view(k, L.View), frequencies=f.data_ptr(), scale=0.7, type=TYPES.index(dtype), interleaved=interleaved, N=2, HQ=9, HK=3, L=33, D=D, pairs=pairs)
+    assert L.lib().fwp_rotary(ctypes.byref(a), view(q, L.OutView), view(k, L.OutView), ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)) == 0
+    torch.cuda.synchronize()
+    assert torch.equal(q, want[0]) and torch.equal(k, want[1])
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_group_norm_of_any_dimensions_and_broadcast_rows(fwp, dtype):
+    g = torch.Generator().manual_seed(2)
+    x, w = randn(g, 3, 4, 5, 48).to(dtype).cuda(), randn(g, 48).cuda()
+    want = fwp.group_norm(x, 6, w, activation="silu")
+    assert torch.equal(fwp.group_norm(x.view(60, 48), 6, w, activation="silu").view_as(x), want)
+    assert torch.equal(fwp.group_norm(x[1, 2, 3], 6, w, activation="silu"), want[1, 2, 3])
+    one = randn(g, 1, 48).to(dtype).cuda().requires_grad_()
+    flat = x.view(60, 48)
+    y = fwp.group_norm(flat, 6, w, gate=one.expand(60, 48), activation="sigmoid")
+    dense = one.detach().expand(60, 48).contiguous().requires_grad_()
+    z = fwp.group_norm(flat, 6, w, gate=dense, activation="sigmoid")
+    assert torch.equal(y, z)
+    a, b = torch.autograd.grad(y, one, flat)[0], torch.autograd.grad(z, dense, flat)[0]
+    # 60 terms added in one order or another, in fp32 or more, and rounded once
+    exact = F.double(b).sum(0, keepdim=True)
+    assert float((F.double(a) - exact).abs().max()) <= 60 * F.EPS32 * float(F.double(b).abs().sum(0).max()) + F.half_step(dtype) * float(exact.abs().max())
+
+
+def test_broadcast_queries_and_decays(fwp):
+    g = torch.Generator().manual_seed(3)
+    q, d = randn(g, 1, 1, 70, 16).cuda().requires_grad_(), decays(g, 1, 1, 70, "token").requires_grad_()
+    k, v, go = rows(g, torch.float32, 3, 4, 70, 16), rows(g, torch.float32, 3, 4, 70, 20), rows(g, torch.float32, 3, 4, 70, 20)
+    out = fwp.decayed_sum(q.expand(3, 4, 70, 16), k, v, d.expand(3, 4, 70))
+    grads = torch.autograd.grad(out, (q, d), go)
+    full = [t.detach().expand(3, 4, *t.shape[2:]).contiguous().requires_grad_() for t in (q, d)]
+    same = fwp.decayed_sum(full[0], k, v, full[1])
+    assert torch.equal(out, same)
+    for a, b in zip(grads, torch.autograd.grad(same, full, go)):
+        b = F.double(b)
+        assert float((F.double(a) - b.sum((0, 1), keepdim=True)).abs().max()) <= 12 * F.EPS32 * float(b.abs().sum((0, 1)).max())
