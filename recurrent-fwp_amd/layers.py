@@ -475,8 +475,11 @@ class DecayedSumLayer(nn.Module):
             position = torch.zeros(bsz, device=h.device, dtype=torch.int64)
         elif carry_over_fast_weight:       # the last batch of an epoch may be smaller than the carried state
             W, position = mems[0][:bsz].clone(), mems[1][:bsz]
+            if position.is_inference() and not torch.is_inference_mode_enabled():       # autograd keeps no tensor of inference mode
+                position = position.clone()
         if self._frequencies.device != h.device:
-            self._frequencies = self._frequencies.to(h.device)
+            with torch.inference_mode(False):
+                self._frequencies = self._frequencies.to(h.device)
         q, k = rotary(rows(q), rows(k), self._frequencies, positions=position, lengths=lengths)
         out = decayed_sum(q, k, rows(v), F.logsigmoid(logit), W, scale=D ** -0.5, lengths=lengths)
         out = out.permute(2, 0, 1, 3).reshape(slen, bsz, H * D)

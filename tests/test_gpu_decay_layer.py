@@ -128,3 +128,22 @@ def test_a_language_model_of_them(fwp, token_decay):
         hid, mems = lm.hidden(data, carry_over_fast_weight=True)
         again, mems = lm.hidden(data[:1], mems, carry_over_fast_weight=True)
     assert torch.isfinite(again).all() and int(mems[0][1][0]) == 71
+
+
+@pytest.mark.parametrize("token_decay", [False, True])
+def test_training_after_inference_mode(fwp, token_decay):
+    """What a call under inference mode leaves, in the layer and as its state, is no obstacle to training"""
+    layer = build(fwp, token_decay=token_decay).cuda()
+    h = torch.randn(20, 2, 48).cuda()
+    with torch.inference_mode():
+        first, mems = layer(h[:12], carry_over_fast_weight=True)
+    y, _ = layer(h[12:], mems=mems, carry_over_fast_weight=True)
+    grads = torch.autograd.grad(y.square().sum(), list(layer.parameters()))
+    assert all(torch.isfinite(g).all() for g in grads)
+    with torch.no_grad():
+        want, state = layer(h[:12], carry_over_fast_weight=True)
+        assert torch.equal(first, want)
+    z, _ = layer(h[12:], mems=state, carry_over_fast_weight=True)
+    assert torch.equal(y, z)
+    for a, b in zip(grads, torch.autograd.grad(z.square().sum(), list(layer.parameters()))):
+        assert torch.equal(a, b)
