@@ -197,7 +197,9 @@ int resident_of(int type, int which, int Ep, int MS) {
 Plan plan_of(int type, int N, int H, int L, int E, int M, bool backward) {
     Plan p{};
     p.Ep = E <= 32 ? 32 : E <= 64 ? 64 : 128;
-    p.MS = M <= 32 ? 32 : M <= 64 ? 64 : 128;
+    // Slices of 128 columns make P once for twice as many (32 x 16 sequences of 1024 steps, 64 keys, 128 columns, fp16: 591 us for training, 869 in two of 64; 128 keys 1404 and 1430), but three of 64
+    // beat two of 128 (150 columns, training: 64 keys fp16 1274 for 1357, bf16 1137 for 1055, fp32 1552 for 1645; 128 keys 2255 for 3257, 2188 for 2882, 2740 for 4324).
+    p.MS = M <= 32 ? 32 : M <= 64 || (M > 128 && M <= 192) ? 64 : 128;
     p.slices = (M + p.MS - 1) / p.MS;
     p.Mp = p.slices * p.MS;
     by_type(type, [&](auto t) { p.chunk = kChunkOf<decltype(t)>; });
