@@ -190,10 +190,10 @@ int resident_of(int type, int which, int Ep, int MS) {
     return std::max(n, 1);
 }
 
-// How a pass is cut.  Segments by a model of its time in chunks of the walk, which goes in rounds of as many workgroups as the GPU holds, each as long as its
-// chunks and the way into them.  Cutting sequences adds the walk that finds the segments' states: a chunk of it is 0.45 of a chunk forward and 0.3 backward where it
-// fills the GPU, and half of that at least; and joining them.  8 x 16 sequences of 64 chunks, 64 x 64 bf16, as measured when the two terms were set: 6 segments forward 32 + 6 + 100 us, 8 are 34 + 7 + 124;
-// 4 segments backward 34 + 6 + 214, 8 are 36 + 7 + 228.
+// How a pass is cut.  Segments by a model of its time in chunks of the walk: workgroups go in rounds of as many as the GPU holds, each as long as its chunks and 2.5 for the way into them and out; a
+// last round of fewer to a CU is shorter, but not below half.  Cutting sequences adds the walk that finds the segments' states (a chunk of it is 0.45 of a chunk forward and 0.3 backward where it fills the
+// GPU, and half of that at least) and joining them.  Measured at 1 to 640 heads of 1024 to 16384 steps in up to 256 segments: the choice is within 7 % of the best one there is.  64 x 64 bf16: 8 x 16 sequences
+// of 64 chunks forward 203 us in one piece, 138, 99, 96 and 113 in 2, 4, 6 and 8 segments, backward 410, 264, 217, 254 and 265; 32 x 16 of 32 chunks forward 146 in one, 182 in two, 193 in four.
 Plan plan_of(int type, int N, int H, int L, int E, int M, bool backward) {
     Plan p{};
     p.Ep = E <= 32 ? 32 : E <= 64 ? 64 : 128;
@@ -209,15 +209,21 @@ Plan plan_of(int type, int N, int H, int L, int E, int M, bool backward) {
     const int64_t units = p.heads * p.slices, walks = 256 * resident_of(type, backward ? kDsumBackward : kDsumForward, p.Ep, p.MS),
                   ends = 256 * resident_of(type, backward ? kDsumBackwardEnds : kDsumForwardEnds, p.Ep, p.MS);
     const auto rounds = [](int64_t blocks, int64_t held) { return (double)((blocks + held - 1) / held); };
+    // rounds of workgroups of which a CU holds `held / 256`
+    const auto share = [](int64_t blocks, int64_t held) {
+        const int64_t rest = blocks % held;
+        return (double)(blocks / held) + (rest ? std::max(0.5, 0.2 + 0.8 * (double)((rest + 255) / 256 * 256) / held) : 0.0);
+    };
     double best = 0;
     // every length of a segment once, and the fewest segments that have it
     for (int64_t s = 1, per; s <= std::max(1, p.chunks / 2) && (s == 1 || units * (s - 1) < 4 * walks); s = (p.chunks + per - 2) / (per - 1)) {
         per = (p.chunks + s - 1) / s;
         const int64_t segments = (p.chunks + per - 1) / per;
-        double time = rounds(units * segments, walks) * (per + 0.6);
+        double time = share(units * segments, walks) * (per + 2.5);
         if (segments > 1) {
             const double blocks = (double)units * (segments - 1);
-            time += (per + 1) * (backward ? 0.3 : 0.45) * std::max(0.5 * rounds(units * (segments - 1), ends), blocks / ends) + 0.6 + 0.03 * segments;
+            time += (per + 1) * (backward ? 0.3 : 0.45) * std::max(0.5 * rounds(units * (segments - 1), ends), blocks / ends);
+            time += segments > kFewSegments ? 0.6 + 0.004 * segments : 0.3;
         }
         if (s == 1 || time < best) best = time, p.per = (int)per, p.segments = (int)segments;
         if (per == 1) break;
