@@ -273,7 +273,7 @@ struct DsumForward {
 
 // ENDS: the state that a segment leaves when it starts from zero, and the segment's whole decay; nothing else.
 // 8 x 16 sequences of 4096 steps, 64 x 64 bf16, six segments: ENDS 29 us at 4.2 TB/s, the walk 105 at 3.8 with the states it saves, a third of its bytes (24.5 without them for an eighth of the
-// sequences).  32 x 8 of 1024 steps, 32 x 32 fp32, eight segments: 14.5 and 47.
+// sequences).  32 x 8 of 1024 steps, 32 x 32 fp32, four segments: 14 and 39, 3.4 and 4.3 TB/s.
 template <typename T, int NE, int NW, int MW, bool WHOLE, bool ENDS>
 __global__ __launch_bounds__(64 * NW, (ENDS ? DsumForward<T, NE, NW, MW>::kEndWaves : DsumForward<T, NE, NW, MW>::kWaves)) void k_dsum_fwd(const DsumWalk a) {
     using F = DsumForward<T, NE, NW, MW>;
@@ -539,7 +539,7 @@ __global__ __launch_bounds__(64 * NW, (ENDS ? DsumForward<T, NE, NW, MW>::kEndWa
 // The adjoint is held twice so that no product waits for another wave's share of it.  Up to 64 keys and columns a wave is of both kinds, which leaves room for two workgroups of four waves on a
 // CU: 8 x 16 sequences of 4096 steps, 64 x 64 bf16, 213 us, 223 with eight waves of one kind each.  Wider ones have no registers for that: 4 x 32 heads, 128 x 64, queries and keys
 // shared, 8 waves of one kind 736 us for the training step, 4 of both 864; 8 key waves of one tile each 60 us more.  With LDS reads and loads ahead of their use (ahead, Stage::arrive) the walk is at
-// 180-190 us for the first of these (0.6 GB, 3.2 TB/s) and at 400 for the second (1 GB of which half are the heads' partial gradients).  Two kernels, one for the adjoints before every chunk and one that
+// 180-190 us for the first of these (0.6 GB, 3.2 TB/s) and at 383 for the second (1 GB of which half are the heads' partial gradients).  Two kernels, one for the adjoints before every chunk and one that
 // works on all chunks at once, take longer: 295 + 65 and 437 + 172 us.
 // The walk back has fewer registers to spare
 template <int P>
