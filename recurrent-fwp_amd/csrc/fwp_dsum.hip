@@ -312,8 +312,8 @@ int dsum_fwd(const fwp_dsum_args &a, float *W, fwp_out_rows out, float *saved, f
         if (!workspace) return FWP_E_NULL;
         w.ends = workspace;
         w.factors = workspace + p.heads * p.segments * p.cells;
-        if (int rc = launch(kDsumForwardEnds, a, p, w, p.segments - 1, s)) return rc;
         w.joined = p.segments > kFewSegments;
+        if (int rc = launch(kDsumForwardEnds, a, p, w, p.segments - 1, s)) return rc;
         if (w.joined) join<false>(w, W, p.heads, p.Ep, s);
     }
     if (int rc = launch(kDsumForward, a, p, w, p.segments, s)) return rc;

@@ -54,7 +54,7 @@ struct DsumWalk {
     float scale;
     int N, H, L, E, M, HQ, HK, HV, Mp, slices, segments, per;      // per: chunks of a segment
     int sum_decay;
-    int joined;                        // the segments' first states are in `ends`; else each workgroup joins those that it needs
+    int joined;                        // the segments' first states are in `ends`; else each workgroup joins those that it needs, and slot 0 is `from`
 };
 
 // Workgroups b, b + 8, .. run on one XCD: neighbours in the order of the work get numbers that lie 8 apart.  Slices and heads come first in that order: they share
@@ -219,10 +219,10 @@ struct Pairs {
     }
 };
 
-// A first state from those that the segments leave, slots lo .. hi of `ends` one after another (backwards from lo down to hi where STEP is -1): S = factor S + what the
+// A first state from those that the segments leave, slots lo .. hi of `ends` one after another (backwards from lo down to hi where STEP is -1): what slot lo holds, then S = factor S + what the
 // slot holds.  each(use) has use(number, four of the state's numbers, their offsets in a slot) called for all that the lane has; the loads of K slots go out together, as many as there are registers for.
 template <int STEP, int COUNT, typename Each>
-__device__ __forceinline__ void fold_segments(const float *ends, int64_t cells, const float *factors, int lo, int hi, bool joined, Each each) {
+__device__ __forceinline__ void fold_segments(const float *ends, int64_t cells, const float *factors, int lo, int hi, Each each) {
     constexpr int K = COUNT <= 8 ? 4 : 2;
 #pragma unroll 1
     for (int s0 = lo; STEP * s0 <= STEP * hi; s0 += STEP * K) {
@@ -232,7 +232,7 @@ __device__ __forceinline__ void fold_segments(const float *ends, int64_t cells, 
         for (int k = 0; k < K; k++) {
             const int slot = STEP > 0 ? min(s0 + k, hi) : max(s0 - k, hi);
             const float *at = ends + slot * cells;
-            y[k] = joined ? 0.f : factors[slot - STEP];
+            y[k] = slot == lo ? 0.f : factors[slot - STEP];
             each([&](int n, v4f &, auto place) {
 #pragma unroll
                 for (int i = 0; i < 4; i++) x[k][n][i] = at[place(i)];
@@ -271,7 +271,7 @@ struct DsumForward {
     static constexpr int kWaves = P == kPlain ? 4 : NE <= 4 ? 3 : 2, kEndWaves = NE <= 4 ? 4 : 3;
 };
 
-// ENDS: the state that a segment leaves when it starts from zero, and the segment's whole decay; nothing else.
+// ENDS: the state that a segment leaves when it starts from zero (the first from `from`, where nothing joins), and the segment's whole decay; nothing else.
 // 8 x 16 sequences of 4096 steps, 64 x 64 bf16, six segments: ENDS 29 us at 4.2 TB/s, the walk 105 at 3.8 with the states it saves, a third of its bytes (24.5 without them for an eighth of the
 // sequences).  32 x 8 of 1024 steps, 32 x 32 fp32, four segments: 14 and 39, 3.4 and 4.3 TB/s.
 template <typename T, int NE, int NW, int MW, bool WHOLE, bool ENDS>
@@ -308,23 +308,32 @@ __global__ __launch_bounds__(64 * NW, (ENDS ? DsumForward<T, NE, NW, MW>::kEndWa
                     use((b * 2 + u) * MW + j, S[b][u][j], [&](int i) { return (32 * b + 8 * g + 4 * u + i) * a.Mp + m0 + mw + place(MW, c, j); });
     };
     each([](int, v4f &x, auto) { x = v4f{0, 0, 0, 0}; });
-    if constexpr (!ENDS) {
-        if (a.from && !a.joined) {
-            const float *from = a.from + head * a.E * a.M;
+    // A walk in segments takes its first states from `ends` alone: the last segment's workgroup writes `to`, which is `from`, and may have done so before the other
+    // segments' have started.  Where nothing joins, the kernel that runs before starts the first segment from `from` and puts that into slot 0.
+    if (a.from && (ENDS ? seg == 0 && !a.joined : a.segments == 1)) {
+        const float *from = a.from + head * a.E * a.M;
 #pragma unroll
-            for (int b = 0; b < NB; b++)
+        for (int b = 0; b < NB; b++)
 #pragma unroll
-                for (int u = 0; u < 2; u++)
+            for (int u = 0; u < 2; u++)
 #pragma unroll
-                    for (int j = 0; j < MW; j++)
+                for (int j = 0; j < MW; j++)
 #pragma unroll
-                        for (int i = 0; i < 4; i++) {
-                            const int e = 32 * b + 8 * g + 4 * u + i, m = m0 + mw + place(MW, c, j);
-                            if (e < a.E && m < a.M) S[b][u][j][i] = from[(int64_t)e * a.M + m];
-                        }
+                    for (int i = 0; i < 4; i++) {
+                        const int e = 32 * b + 8 * g + 4 * u + i, m = m0 + mw + place(MW, c, j);
+                        if (e < a.E && m < a.M) S[b][u][j][i] = from[(int64_t)e * a.M + m];
+                    }
+        if constexpr (ENDS) {
+            float *at = a.ends + head * a.segments * E * a.Mp;
+            each([&](int, v4f &x, auto place) {
+#pragma unroll
+                for (int i = 0; i < 4; i++) at[place(i)] = x[i];
+            });
         }
-        if (a.segments > 1)
-            fold_segments<1, NB * 2 * MW>(a.ends + head * a.segments * E * a.Mp, (int64_t)E * a.Mp, a.factors + head * a.segments, a.joined ? seg : 1, seg, a.joined, each);
+    }
+    if constexpr (!ENDS) {
+        if (a.segments > 1 && (seg > 0 || a.from))
+            fold_segments<1, NB * 2 * MW>(a.ends + head * a.segments * E * a.Mp, (int64_t)E * a.Mp, a.factors + head * a.segments, a.joined ? seg : min(seg, 1), seg, each);
         // arrived, as everything that is loaded ahead of the loop: a wait that its first round needs would be one of all rounds
         each([](int, v4f &x, auto) { pin(x); });
     }
@@ -706,7 +715,7 @@ __device__ __forceinline__ void dsum_walk_back(const DsumWalk &a, typename DsumB
     };
     each([](int, v4f &x, auto) { x = v4f{0, 0, 0, 0}; });
     if (a.segments > 1)
-        fold_segments<-1, kOfH + kOfG>(a.ends + head * a.segments * E * a.Mp, (int64_t)E * a.Mp, a.factors + head * a.segments, a.joined ? seg : a.segments - 2, seg, a.joined, each);
+        fold_segments<-1, kOfH + kOfG>(a.ends + head * a.segments * E * a.Mp, (int64_t)E * a.Mp, a.factors + head * a.segments, a.joined ? seg : a.segments - 2, seg, each);
     each([](int, v4f &x, auto) { pin(x); });
 #pragma unroll 1
     for (int i = tid; i < (int)(sizeof(sh.p) / 16); i += kThreads) reinterpret_cast<v4f *>(&sh.p)[i] = v4f{0, 0, 0, 0};
