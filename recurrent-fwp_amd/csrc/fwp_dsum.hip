@@ -171,6 +171,7 @@ __global__ __launch_bounds__(256) void k_dsum_step(const DsumWalk a, int X, int 
 // their walks, 370 with a kernel of its own for each; eight segments of 32 x 8 x 1024, 32 x 32 fp32, 170 and 174.  Many segments would read most of `ends` again and again.
 constexpr int kFewSegments = 9;
 
+// A plan has more than kFewSegments segments only where heads times slices are fewer than half of what the GPU holds: its workgroups always fit a launch.
 template <bool BACKWARD>
 void join(const DsumWalk &w, const float *from, int64_t heads, int Ep, hipStream_t s) {
     const unsigned blocks = (unsigned)(heads * (Ep * w.Mp / 64));
@@ -262,7 +263,7 @@ DsumWalk walk_of(const fwp_dsum_args &a, const Plan &p) {
 
 int launch(int which, const fwp_dsum_args &a, const Plan &p, const DsumWalk &w, int segments, hipStream_t s) {
     const int64_t blocks = p.heads * p.slices * segments;
-    if (!fits_launch(blocks, 512) || !fits_launch(p.heads * (p.cells / 64), 512)) return FWP_E_SHAPE;
+    if (!fits_launch(blocks, 512)) return FWP_E_SHAPE;
     bool done = false;
     by_type(a.type, [&](auto t) { done = dsum_launch<decltype(t)>(which, &w, p.Ep, p.MS, (unsigned)blocks, s) > 0; });
     return done ? 0 : FWP_E_SHAPE;
