@@ -96,10 +96,19 @@ __global__ __launch_bounds__(256) void k_rotary(const RotaryWalk w) {
     if (!turns) c0 = 2 * a.pairs + (u - w.turning) * 2 * V, c1 = c0 + V, e0 = e1 = a.D;
     else if (a.interleaved) c0 = u * 2 * V, c1 = c0 + V, e0 = e1 = 2 * a.pairs;
     else c0 = u * V, c1 = a.pairs + c0, e0 = a.pairs, e1 = 2 * a.pairs;
+    if (!counts) {      // rows behind a sequence are not read: 8 x (32 + 8) heads of 4096 x 128, bf16, an eighth of them counting, 84 us, 127 where all do
+        const float none[V] = {};
+#pragma unroll 1
+        for (int h = group * w.per; h < min((group + 1) * w.per, a.HQ + a.HK); h++) {
+            T *to = h >= a.HQ ? row<T>(w.ok, n, h - a.HQ, t) : row<T>(w.oq, n, h, t);
+            Run<T>::template store<WHOLE>(none, to, c0, e0), Run<T>::template store<WHOLE>(none, to, c1, e1);
+        }
+        return;
+    }
     float sn[V], cs[V];
 #pragma unroll
     for (int p = 0; p < V; p++) sn[p] = 0.f, cs[p] = 1.f;
-    if (turns && counts) {
+    if (turns) {
         int64_t at = t;
         if (a.positions) at = a.each_step ? a.positions[(int64_t)n * a.L + t] : a.positions[n] + t;
         const double position = (double)at;
@@ -136,10 +145,6 @@ __global__ __launch_bounds__(256) void k_rotary(const RotaryWalk w) {
             } else {
 #pragma unroll
                 for (int p = 0; p < V; p++) r0[p] = fmaf(p0[p], cs[p], -(p1[p] * sn[p])), r1[p] = fmaf(p0[p], sn[p], p1[p] * cs[p]);
-            }
-            if (!counts) {
-#pragma unroll
-                for (int p = 0; p < V; p++) r0[p] = r1[p] = 0.f;
             }
             Run<T>::template store<WHOLE>(r0, to, c0, e0), Run<T>::template store<WHOLE>(r1, to, c1, e1);
         }
