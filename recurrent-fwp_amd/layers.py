@@ -449,7 +449,9 @@ class DecayedSumLayer(nn.Module):
         self.norm_bias = nn.Parameter(torch.zeros(n_head * d_head))
         self.o_net = Linear(n_head * d_head, d_model)
         self.drop = nn.Dropout(dropout)
-        self._frequencies = rotary_frequencies(d_head)[0]      # no buffer: a model in half precision keeps them in 64 bits
+        # no buffer: a model in half precision keeps them in 64 bits, and one that is built without memory has them all the same
+        device = self.decay_logit.device
+        self._frequencies = rotary_frequencies(d_head, device="cpu" if device.type == "meta" else device)[0]
         self.reset_decay_parameters()
 
     def reset_decay_parameters(self):
