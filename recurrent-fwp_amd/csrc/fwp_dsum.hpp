@@ -248,7 +248,8 @@ __device__ __forceinline__ void pin(v4f &x) {
     for (int i = 0; i < 4; i++) x[i] = pinned(x[i]);
 }
 
-// Workgroups of a kernel that a CU holds at once: 160 KB of LDS, and registers for `waves` on each of four SIMDs, which the kernel's launch bounds ask for
+// Workgroups of a kernel that a CU holds at once at the least: 160 KB of LDS, and registers for `waves` on each of four SIMDs, which the kernel's launch bounds ask for.  Where the compiler needs
+// fewer registers there may be up to twice as many, which plans do not count on.
 constexpr int resident(size_t lds, int waves, int NW) { return (int)(160 * 1024 / lds) < 4 * waves / NW ? (int)(160 * 1024 / lds) : 4 * waves / NW; }
 
 // ------------------------------------------------------------------ forward

@@ -26,7 +26,7 @@ def decayed_sum(Q, K, V, log_decay, W=None, scale=1.0, lengths=None):
     gradients flow to Q, K, V and log_decay.
 
     A number that is not finite makes infinite or NaN what depends on it, and leaves the results of the steps before it as they are; gradients are NaN in its whole chunk,
-    up to 63 steps before and behind it."""
+    up to 63 steps before and behind it.  fp32 numbers beyond 3.39e38 may count as infinite where there are more than 32 keys."""
     return _native().decayed_sum(Q, K, V, log_decay, W, scale, lengths)
 
 
